@@ -371,6 +371,110 @@ int msr_muon_each(const msr_muon_matrix *matrices, int32_t count, float beta, in
                   size_t workspace_bytes, msr_stream_t stream);
 
 /* ---------------------------------------------------------------------------
+ * The global norm of many gradients, and clipping by it.  No counterpart in the
+ * reference (a training loop calls torch.nn.utils.clip_grad_norm_ between
+ * backward and step).
+ *   N = (sum over every element of every item of |g|^p)^(1/p), p = 1, 2, or inf
+ *   c = min(1, max_norm / (N + 1e-6))       (fp32; NaN where N is NaN)
+ *   out[i] = round(f32(g[i]) * c)           (nearest even for a bf16 out)
+ * Sums are held in 64 bits, in a fixed order: squares of bf16 and fp32 values
+ * neither overflow nor vanish, and a list gives the same bits every time.
+ * items: HOST array, any count (empty tensors allowed).  out may be the item's
+ * own grad (same type; not written where c is 1); any other sharing of memory
+ * that is written is refused (MSR_ERR_OVERLAP).  norm_out: device fp32, the
+ * unclipped N.  workspace: msr_grad_norm_workspace_bytes of the same list,
+ * 8-byte aligned.  msr_grad_norm ignores out.
+ * ------------------------------------------------------------------------- */
+typedef struct msr_clip_item {
+    const void *grad;   /* bf16, or fp32 with MSR_CLIP_GRAD_F32, [n] */
+    void *out;          /* bf16, or fp32 with MSR_CLIP_OUT_F32 (fp32 grads only), [n] */
+    int64_t n;
+    int32_t flags;
+    int32_t reserved;   /* 0 */
+} msr_clip_item;
+#define MSR_CLIP_GRAD_F32 1
+#define MSR_CLIP_OUT_F32 2
+#define MSR_NORM_1 1
+#define MSR_NORM_2 2
+#define MSR_NORM_INF 3
+int msr_grad_norm_workspace_bytes(const msr_clip_item *items, int32_t count, size_t *bytes);
+int msr_grad_norm(const msr_clip_item *items, int32_t count, int32_t norm, float *norm_out, void *workspace,
+                  size_t workspace_bytes, msr_stream_t stream);
+int msr_clip_grads(const msr_clip_item *items, int32_t count, int32_t norm, float max_norm, float *norm_out,
+                   void *workspace, size_t workspace_bytes, msr_stream_t stream);
+
+/* ---------------------------------------------------------------------------
+ * Tokens sorted by expert and back, for mixture-of-experts layers.  No
+ * counterpart in the reference.
+ *
+ * msr_order_tokens: a stable counting sort of the tokens * k slots (t, j) by
+ * their expert ids[t][j] (int32, or int64 with ids_i64).  An id outside
+ * [0, experts) has no expert: the slot is dropped.
+ *   offsets  int32 [experts + 1]: expert e has the rows [offsets[e], offsets[e + 1])
+ *   position int32 [tokens][k]: the row of a slot, -1 for a dropped one
+ *   source   int32 [tokens * k]: the slot t * k + j of a row, -1 from row offsets[experts] on
+ * tokens * k < 2^30, experts <= MSR_EXPERTS_MAX.  workspace:
+ * msr_order_workspace_bytes, 4-byte aligned (may be NULL where that is 0).
+ *
+ * The four passes between tokens and rows, for elem = MSR_BF16 or MSR_F32
+ * activations of width d and n = tokens * k rows (a position outside [0, n) is
+ * taken as dropped; sums in fp32, one rounding to the stored type):
+ *   msr_dispatch        rows[position[t][j]] = x[t]; rows without a slot are 0
+ *   msr_dispatch_grad   dx[t] = sum_j drows[position[t][j]]
+ *   msr_combine         y[t] = sum_j w[t][j] rows[position[t][j]]
+ *   msr_combine_grad    drows[position[t][j]] = w[t][j] dy[t], 0 for rows without a slot;
+ *                       dw[t][j] = <dy[t], rows[position[t][j]]>, 0 for dropped slots
+ * offsets: as msr_order_tokens wrote it; `experts` is its index of the first row
+ * without a slot.  x, dy: rows of ldx / lddy elements; every other tensor is
+ * contiguous.  w and dw: welem.  drows or dw may be NULL (not wanted).
+ * Outputs must not overlap inputs.
+ * ------------------------------------------------------------------------- */
+#define MSR_BF16 0
+#define MSR_F32 1
+#define MSR_EXPERTS_MAX 1024
+int msr_order_workspace_bytes(int64_t tokens, int32_t k, int32_t experts, size_t *bytes);
+int msr_order_tokens(const void *ids, int32_t ids_i64, int64_t tokens, int32_t k, int32_t experts, int32_t *offsets,
+                     int32_t *position, int32_t *source, void *workspace, size_t workspace_bytes, msr_stream_t stream);
+int msr_dispatch(const void *x, int64_t ldx, void *rows, const int32_t *position, const int32_t *offsets,
+                 int32_t experts, int64_t tokens, int32_t k, int64_t d, int32_t elem, msr_stream_t stream);
+int msr_dispatch_grad(const void *drows, void *dx, const int32_t *position, int64_t tokens, int32_t k, int64_t d,
+                      int32_t elem, msr_stream_t stream);
+int msr_combine(const void *rows, const void *w, void *y, const int32_t *position, int64_t tokens, int32_t k, int64_t d,
+                int32_t elem, int32_t welem, msr_stream_t stream);
+int msr_combine_grad(const void *dy, int64_t lddy, const void *rows, const void *w, void *drows, void *dw,
+                     const int32_t *position, const int32_t *offsets, int32_t experts, int64_t tokens, int32_t k,
+                     int64_t d, int32_t elem, int32_t welem, msr_stream_t stream);
+
+/* ---------------------------------------------------------------------------
+ * The experts' products over rows sorted by expert (offsets: device int32
+ * [experts + 1], offsets[0] = 0, non-decreasing, as msr_order_tokens writes it;
+ * read on the GPU only, and clamped to [0, rows]).  No counterpart in the
+ * reference.  bf16 operands, fp32 accumulation, one rounding:
+ *   msr_experts_forward          y[r] = W[e] x[r]            for the rows r of expert e
+ *   msr_experts_dgrad            dx[r] = W[e]^T dy[r]
+ *   msr_experts_wgrad            dw[e] = sum_r dy[r] x[r]^T  (0 for an expert without rows)
+ *   msr_experts_wgrad_sr_accum   acc[e] <- SR(acc[e] + f32(bf16(dw[e]))): the arithmetic and noise
+ *                                of msr_sr_accum on the contiguous [experts][out][in] buffer, as
+ *                                msr_linear_wgrad_sr_accum does for one weight
+ * Rows from offsets[experts] on have no expert: their y and dx are 0, and dw does
+ * not see them.  x, dx: [rows][in] (x with row stride ldx), dy, y: [rows][out] (dy: lddy),
+ * W, dw, acc: [experts][out][in]; 16-byte aligned, in, out, ldx and lddy multiples
+ * of 8; rows < 2^30, in and out at most 2^20, experts <= MSR_EXPERTS_MAX; one expert's weights
+ * below 2 GiB.
+ * ------------------------------------------------------------------------- */
+int msr_experts_forward(const uint16_t *x, int64_t ldx, const uint16_t *w, uint16_t *y, const int32_t *offsets,
+                        int64_t rows, int32_t experts, int64_t in_features, int64_t out_features, msr_stream_t stream);
+int msr_experts_dgrad(const uint16_t *dy, int64_t lddy, const uint16_t *w, uint16_t *dx, const int32_t *offsets,
+                      int64_t rows, int32_t experts, int64_t in_features, int64_t out_features, msr_stream_t stream);
+int msr_experts_wgrad(uint16_t *dw, const uint16_t *x, int64_t ldx, const uint16_t *dy, int64_t lddy,
+                      const int32_t *offsets, int64_t rows, int32_t experts, int64_t in_features, int64_t out_features,
+                      msr_stream_t stream);
+int msr_experts_wgrad_sr_accum(uint16_t *acc, const uint16_t *x, int64_t ldx, const uint16_t *dy, int64_t lddy,
+                               const int32_t *offsets, int64_t rows, int32_t experts, int64_t in_features,
+                               int64_t out_features, uint32_t seed, int32_t zero_init, int32_t noise_mode,
+                               const uint16_t *inject, msr_stream_t stream);
+
+/* ---------------------------------------------------------------------------
  * Diagnostics (no counterpart in the reference; used by the parity tests).
  * ------------------------------------------------------------------------- */
 

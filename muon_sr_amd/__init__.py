@@ -12,6 +12,9 @@ from .adamw_8bit import TritonAdamW8bit, create_dynamic_map
 from .adamw import TritonAdamW, TritonSRAccumulator
 from .muon import TritonMuonSR, TritonMuonSRWithAuxAdam, newton_schulz
 from .linear import SRLinear, linear_wgrad_sr_accum
+from .clip import clip_grad_norm_, clip_grads, grad_norm
+from .experts import (SRExperts, TokenOrder, combine_tokens, dispatch_tokens, expert_linear, experts_wgrad_sr_accum,
+                      order_tokens)
 
 __all__ = [
     "TritonAdamW8bit",
@@ -19,4 +22,7 @@ __all__ = [
     "TritonMuonSR", "TritonMuonSRWithAuxAdam",
     "newton_schulz", "create_dynamic_map", "set_sr_noise", "get_sr_noise",
     "SRLinear", "linear_wgrad_sr_accum",
+    "clip_grad_norm_", "clip_grads", "grad_norm",
+    "TokenOrder", "order_tokens", "dispatch_tokens", "combine_tokens",
+    "SRExperts", "expert_linear", "experts_wgrad_sr_accum",
 ]

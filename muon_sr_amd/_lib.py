@@ -66,6 +66,19 @@ class MuonMatrix(ctypes.Structure):
                 ("apply_seed", ctypes.c_uint32), ("grad_f32", ctypes.c_int32), ("scale", ctypes.c_float)]
 
 
+class ClipItem(ctypes.Structure):
+    """msr_clip_item (include/muon_sr_amd.h)."""
+    _fields_ = [("grad", ctypes.c_void_p), ("out", ctypes.c_void_p), ("n", ctypes.c_int64), ("flags", ctypes.c_int32),
+                ("reserved", ctypes.c_int32)]
+
+
+CLIP_GRAD_F32 = 1
+CLIP_OUT_F32 = 2
+NORM_1, NORM_2, NORM_INF = 1, 2, 3
+BF16, F32 = 0, 1
+EXPERTS_MAX = 1024
+
+
 # name -> (restype, argtypes); mirrors include/muon_sr_amd.h
 SIGNATURES = {
     "msr_version": (ctypes.c_int, []),
@@ -93,6 +106,20 @@ SIGNATURES = {
                                             _P, ctypes.c_size_t, _P]),
     "msr_muon_each_workspace_bytes": (ctypes.c_int, [_P, _I32, _SIZE_P]),
     "msr_muon_each": (ctypes.c_int, [_P, _I32, _F, _I32, _I32, _F, _F, _F, _F, _F, _I32, _P, ctypes.c_size_t, _P]),
+    "msr_grad_norm_workspace_bytes": (ctypes.c_int, [_P, _I32, _SIZE_P]),
+    "msr_grad_norm": (ctypes.c_int, [_P, _I32, _I32, _P, _P, ctypes.c_size_t, _P]),
+    "msr_clip_grads": (ctypes.c_int, [_P, _I32, _I32, _F, _P, _P, ctypes.c_size_t, _P]),
+    "msr_order_workspace_bytes": (ctypes.c_int, [_I64, _I32, _I32, _SIZE_P]),
+    "msr_order_tokens": (ctypes.c_int, [_P, _I32, _I64, _I32, _I32, _P, _P, _P, _P, ctypes.c_size_t, _P]),
+    "msr_dispatch": (ctypes.c_int, [_P, _I64, _P, _P, _P, _I32, _I64, _I32, _I64, _I32, _P]),
+    "msr_dispatch_grad": (ctypes.c_int, [_P, _P, _P, _I64, _I32, _I64, _I32, _P]),
+    "msr_combine": (ctypes.c_int, [_P, _P, _P, _P, _I64, _I32, _I64, _I32, _I32, _P]),
+    "msr_combine_grad": (ctypes.c_int, [_P, _I64, _P, _P, _P, _P, _P, _P, _I32, _I64, _I32, _I64, _I32, _I32, _P]),
+    "msr_experts_forward": (ctypes.c_int, [_P, _I64, _P, _P, _P, _I64, _I32, _I64, _I64, _P]),
+    "msr_experts_dgrad": (ctypes.c_int, [_P, _I64, _P, _P, _P, _I64, _I32, _I64, _I64, _P]),
+    "msr_experts_wgrad": (ctypes.c_int, [_P, _P, _I64, _P, _I64, _P, _I64, _I32, _I64, _I64, _P]),
+    "msr_experts_wgrad_sr_accum": (ctypes.c_int, [_P, _P, _I64, _P, _I64, _P, _I64, _I32, _I64, _I64, _U32, _I32, _I32, _P,
+                                                  _P]),
     "msr_noise_fill": (ctypes.c_int, [_P, _I64, _I64, _U32, _U32, _I32, _P]),
     "msr_stream_probe8": (ctypes.c_int, [_P, _P, _P, _P, _P, _P, _I64, _I32, _I32, _P]),
     "msr_quantize": (ctypes.c_int, [_P, _P, _I64, _P, _I32, _P, _P]),

@@ -1,0 +1,503 @@
+// Tokens sorted by expert and back, for mixture-of-experts layers.
+//
+// Order: a stable counting sort of the n = tokens * k slots by expert.  Slot s of expert e
+// gets row  offsets[e] + #{s' < s : expert(s') = e}.  The slots are cut into one chunk per
+// work-group; count_kernel counts each chunk's slots per expert, and place_kernel adds the counts of
+// the chunks before its own, and of all chunks for the offsets (a few thousand numbers from
+// L2), then ranks its slots wave by wave.  A wave ranks 64 slots at a time by ballots, one
+// per bit of the expert number, so no order depends on atomics.  Dropped slots count as one
+// more expert, which gives the rows without a slot.  Bound by latency: two launches (one where a
+// single work-group takes all slots).
+//
+// The four passes between tokens and rows (see the header) move d elements per slot and do
+// next to nothing with them, so HBM bounds them.  All are written from the token's side: a
+// token's k rows are read or written by the same wave, so x and dy are read once, not k times, y
+// and dx are sums in registers, and nothing is added atomically.
+#include "common.hpp"
+#include "vecio.hpp"
+#include "../../include/muon_sr_amd.h"
+
+namespace msr {
+
+// ---------------------------------------------------------------------------
+// order
+// ---------------------------------------------------------------------------
+
+constexpr int ORD_THREADS = 1024, ORD_WAVES = ORD_THREADS / 64;
+constexpr int ORD_CHUNK = 2048;          // slots of a work-group, while there are at most ORD_MAXWG of them
+constexpr int ORD_MAXWG = 256;
+
+struct OrderArgs {
+    const void *ids;
+    int32_t *offsets, *position, *source;
+    int32_t *counts;                     // [work-groups][experts + 1]
+    int64_t n;                           // slots
+    int32_t experts, i64, chunk;
+};
+
+__device__ __forceinline__ int expert_of(const OrderArgs &a, int64_t s) {
+    if (a.i64) {
+        const int64_t e = static_cast<const int64_t *>(a.ids)[s];
+        return e >= 0 && e < a.experts ? (int)e : a.experts;
+    }
+    const int32_t e = static_cast<const int32_t *>(a.ids)[s];
+    return e >= 0 && e < a.experts ? e : a.experts;
+}
+
+__global__ __launch_bounds__(ORD_THREADS) void count_kernel(OrderArgs a) {
+    __shared__ int hist[MSR_EXPERTS_MAX + 1];
+    for (int e = threadIdx.x; e <= a.experts; e += ORD_THREADS) hist[e] = 0;
+    __syncthreads();
+    const int64_t s0 = (int64_t)blockIdx.x * a.chunk, s1 = min(s0 + a.chunk, a.n);
+    for (int64_t s = s0 + threadIdx.x; s < s1; s += ORD_THREADS) atomicAdd(&hist[expert_of(a, s)], 1);
+    __syncthreads();
+    for (int e = threadIdx.x; e <= a.experts; e += ORD_THREADS) a.counts[(int64_t)blockIdx.x * (a.experts + 1) + e] = hist[e];
+}
+
+// Inclusive sum over the lanes of a wave.
+__device__ __forceinline__ int wave_scan(int x) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int w = 1; w < 64; w <<= 1) {
+        const int y = __shfl_up(x, w);
+        x += lane >= w ? y : 0;
+    }
+    return x;
+}
+
+__global__ __launch_bounds__(ORD_THREADS) void place_kernel(OrderArgs a) {
+    extern __shared__ int wave_at[];                 // [ORD_WAVES][experts + 1]: counts, then the next row
+    __shared__ int wave_sum[ORD_WAVES];
+    const int E1 = a.experts + 1, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    for (int i = tid; i < ORD_WAVES * E1; i += ORD_THREADS) wave_at[i] = 0;
+    __syncthreads();
+    // each wave takes a run of the chunk's slots
+    const int run = a.chunk / ORD_WAVES;
+    const int64_t s0 = (int64_t)blockIdx.x * a.chunk + (int64_t)wave * run, s1 = min(s0 + run, a.n);
+    int *const mine = wave_at + wave * E1;
+    for (int64_t s = s0 + lane; s < s1; s += 64) atomicAdd(&mine[expert_of(a, s)], 1);
+    __syncthreads();
+    // Thread e: expert e's slots in the chunks before this one and in all; the sum over the
+    // experts before it gives its first row.  experts + 1 <= 1025 numbers: two rounds at most.
+    int carry = 0;
+    for (int e0 = 0; e0 < E1; e0 += ORD_THREADS) {
+        const int e = e0 + tid;
+        int before = 0, all = 0;
+        if (e < E1) {
+            if (gridDim.x == 1) {
+                for (int w = 0; w < ORD_WAVES; ++w) all += wave_at[w * E1 + e];
+            } else {
+                for (int b = 0; b < (int)gridDim.x; ++b) {
+                    const int c = a.counts[(int64_t)b * E1 + e];
+                    before += b < (int)blockIdx.x ? c : 0;
+                    all += c;
+                }
+            }
+        }
+        const int incl = wave_scan(all);
+        if (lane == 63) wave_sum[wave] = incl;
+        __syncthreads();
+        int first = carry + incl - all, total = 0;
+        for (int w = 0; w < ORD_WAVES; ++w) {
+            first += w < wave ? wave_sum[w] : 0;
+            total += wave_sum[w];
+        }
+        carry += total;
+        if (e < E1) {
+            if (blockIdx.x == 0) a.offsets[e] = first;   // expert `experts` is the dropped slots': their first row
+            int at = first + before;
+            for (int w = 0; w < ORD_WAVES; ++w) {
+                const int c = wave_at[w * E1 + e];
+                wave_at[w * E1 + e] = at;
+                at += c;
+            }
+        }
+        __syncthreads();
+    }
+    // Ranks: the lanes with this lane's expert, from one ballot per bit of its number.
+    const int bits = 32 - __clz(a.experts);
+    for (int64_t s = s0; s < s1; s += 64) {
+        const bool on = s + lane < s1;
+        const int e = on ? expert_of(a, s + lane) : 0;
+        uint64_t same = __ballot(on);
+        for (int b = 0; b < bits; ++b) {
+            const uint64_t m = __ballot((e >> b) & 1);
+            same &= (e >> b) & 1 ? m : ~m;
+        }
+        const int rank = __popcll(same & ((1ull << lane) - 1));
+        if (on) {
+            const int row = mine[e] + rank;
+            const bool kept = e < a.experts;
+            a.position[s + lane] = kept ? row : -1;
+            a.source[row] = kept ? (int)(s + lane) : -1;
+        }
+        // a wave's LDS accesses execute in order: every lane has read mine[e] before the last lane
+        // of an expert moves it on, and reads what that lane wrote in the next round
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        if (on && (same >> lane) == 1) mine[e] += rank + 1;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+}
+
+struct OrderPlan {
+    int wgs, chunk;
+};
+static OrderPlan order_plan(int64_t n) {
+    const int64_t wgs = std::min<int64_t>(std::max<int64_t>((n + ORD_CHUNK - 1) / ORD_CHUNK, 1), ORD_MAXWG);
+    const int64_t chunk = ((n + wgs - 1) / wgs + ORD_THREADS - 1) / ORD_THREADS * ORD_THREADS;   // whole waves' runs
+    return {(int)std::max<int64_t>((n + chunk - 1) / std::max<int64_t>(chunk, 1), 1), (int)std::max<int64_t>(chunk, ORD_THREADS)};
+}
+
+// ---------------------------------------------------------------------------
+// passes between tokens and rows
+// ---------------------------------------------------------------------------
+
+constexpr int MOVE_THREADS = 256, MOVE_WAVES = MOVE_THREADS / 64;
+constexpr int MOVE_GRID = 256 * 8;
+
+// 16 bytes of a row per lane (VEC), or one element.
+template <typename T, bool VEC>
+struct Pack {
+    static constexpr int N = VEC ? 16 / (int)sizeof(T) : 1;
+    float f[N];
+    __device__ __forceinline__ void load(const T *p) {
+        if constexpr (!VEC) {
+            if constexpr (sizeof(T) == 2) f[0] = bf16_to_f32(*p);
+            else f[0] = *p;
+        } else if constexpr (sizeof(T) == 2) {
+            const u32x4_t v = *reinterpret_cast<const u32x4_t *>(p);
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+            unpack8(w, f);
+        } else {
+            const f32x4_t v = *reinterpret_cast<const f32x4_t *>(p);
+            f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w;
+        }
+    }
+    __device__ __forceinline__ void store(T *p) const {
+        if constexpr (!VEC) {
+            if constexpr (sizeof(T) == 2) *p = (T)rne_bf16(f[0]);
+            else *p = f[0];
+        } else if constexpr (sizeof(T) == 2) {
+            *reinterpret_cast<u32x4_t *>(p) = u32x4_t{rne_bf16x2(f[0], f[1]), rne_bf16x2(f[2], f[3]),
+                                                      rne_bf16x2(f[4], f[5]), rne_bf16x2(f[6], f[7])};
+        } else {
+            *reinterpret_cast<f32x4_t *>(p) = f32x4_t{f[0], f[1], f[2], f[3]};
+        }
+    }
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int i = 0; i < N; ++i) f[i] = 0.0f;
+    }
+};
+
+struct MoveArgs {
+    const void *tok;             // x or dy: [tokens] rows of ldtok elements
+    int64_t ldtok;
+    const void *rows;            // [n][d], read
+    const void *w;               // [n] slot weights
+    void *out;                   // rows or dx, y, drows
+    void *dw;                    // [n]
+    const int32_t *position, *offsets;
+    int64_t tokens, n, d;
+    int32_t k, experts, w32;
+};
+
+__device__ __forceinline__ float weight_of(const MoveArgs &a, int64_t s) {
+    return a.w32 ? static_cast<const float *>(a.w)[s] : bf16_to_f32(static_cast<const uint16_t *>(a.w)[s]);
+}
+// The row of slot s, or -1.
+__device__ __forceinline__ int64_t row_of(const MoveArgs &a, int64_t s) {
+    const int64_t p = a.position[s];
+    return p < a.n ? p : -1;
+}
+
+// Rows without a slot, [offsets[experts], n), to zero: the waves of the launch in turn.
+template <typename T, bool VEC>
+__device__ __forceinline__ void zero_tail(const MoveArgs &a, int64_t wave, int64_t waves) {
+    constexpr int N = Pack<T, VEC>::N;
+    Pack<T, VEC> z;
+    z.zero();
+    for (int64_t r = max(0, a.offsets[a.experts]) + wave; r < a.n; r += waves)
+        for (int64_t c = (int64_t)(threadIdx.x & 63) * N; c < a.d; c += 64 * N) z.store(static_cast<T *>(a.out) + r * a.d + c);
+}
+
+__device__ __forceinline__ int64_t this_wave() {
+    return (int64_t)blockIdx.x * MOVE_WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+}
+
+// rows[position[t][j]] = x[t]
+template <typename T, bool VEC>
+__global__ __launch_bounds__(MOVE_THREADS) void dispatch_kernel(MoveArgs a) {
+    constexpr int N = Pack<T, VEC>::N;
+    const int64_t waves = (int64_t)gridDim.x * MOVE_WAVES;
+    for (int64_t t = this_wave(); t < a.tokens; t += waves) {
+        const T *x = static_cast<const T *>(a.tok) + t * a.ldtok;
+        for (int64_t c = (int64_t)(threadIdx.x & 63) * N; c < a.d; c += 64 * N) {
+            Pack<T, VEC> v;
+            v.load(x + c);
+            for (int j = 0; j < a.k; ++j) {
+                const int64_t p = row_of(a, t * a.k + j);
+                if (p >= 0) v.store(static_cast<T *>(a.out) + p * a.d + c);
+            }
+        }
+    }
+    zero_tail<T, VEC>(a, this_wave(), waves);
+}
+
+// out[t] = sum_j w[t][j] rows[position[t][j]], or without weights (WEIGHTED false)
+template <typename T, bool VEC, bool WEIGHTED>
+__global__ __launch_bounds__(MOVE_THREADS) void combine_kernel(MoveArgs a) {
+    constexpr int N = Pack<T, VEC>::N;
+    const int64_t waves = (int64_t)gridDim.x * MOVE_WAVES;
+    for (int64_t t = this_wave(); t < a.tokens; t += waves) {
+        for (int64_t c = (int64_t)(threadIdx.x & 63) * N; c < a.d; c += 64 * N) {
+            Pack<T, VEC> sum, v;
+            sum.zero();
+            for (int j = 0; j < a.k; ++j) {
+                const int64_t s = t * a.k + j, p = row_of(a, s);
+                if (p < 0) continue;
+                const float w = WEIGHTED ? weight_of(a, s) : 1.0f;
+                v.load(static_cast<const T *>(a.rows) + p * a.d + c);
+#pragma unroll
+                for (int i = 0; i < N; ++i) sum.f[i] = WEIGHTED ? __builtin_fmaf(w, v.f[i], sum.f[i]) : sum.f[i] + v.f[i];
+            }
+            sum.store(static_cast<T *>(a.out) + t * a.d + c);
+        }
+    }
+}
+
+// drows[position[t][j]] = w[t][j] dy[t];  dw[t][j] = <dy[t], rows[position[t][j]]>
+template <typename T, bool VEC>
+__global__ __launch_bounds__(MOVE_THREADS) void combine_grad_kernel(MoveArgs a) {
+    constexpr int N = Pack<T, VEC>::N;
+    const int lane = threadIdx.x & 63;
+    const int64_t waves = (int64_t)gridDim.x * MOVE_WAVES;
+    for (int64_t t = this_wave(); t < a.tokens; t += waves) {
+        const T *dy = static_cast<const T *>(a.tok) + t * a.ldtok;
+        for (int j = 0; j < a.k; ++j) {
+            const int64_t s = t * a.k + j, p = row_of(a, s);
+            float dot = 0.0f;
+            if (p >= 0) {
+                const float w = weight_of(a, s);
+                for (int64_t c = (int64_t)lane * N; c < a.d; c += 64 * N) {
+                    Pack<T, VEC> g, r;
+                    g.load(dy + c);
+                    if (a.dw) {
+                        r.load(static_cast<const T *>(a.rows) + p * a.d + c);
+#pragma unroll
+                        for (int i = 0; i < N; ++i) dot = __builtin_fmaf(g.f[i], r.f[i], dot);
+                    }
+                    if (a.out) {
+#pragma unroll
+                        for (int i = 0; i < N; ++i) g.f[i] = g.f[i] * w;
+                        g.store(static_cast<T *>(a.out) + p * a.d + c);
+                    }
+                }
+            }
+            if (a.dw) {
+#pragma unroll
+                for (int w = 32; w > 0; w >>= 1) dot += __shfl_xor(dot, w);
+                if (lane == 0) {
+                    if (a.w32) static_cast<float *>(a.dw)[s] = dot;
+                    else static_cast<uint16_t *>(a.dw)[s] = (uint16_t)rne_bf16(dot);
+                }
+            }
+        }
+    }
+    if (a.out) zero_tail<T, VEC>(a, this_wave(), waves);
+}
+
+// ---------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------
+
+static bool touch(const void *p, size_t np, const void *q, size_t nq) {
+    const uintptr_t u = (uintptr_t)p, v = (uintptr_t)q;
+    return p && q && np && nq && u < v + nq && v < u + np;
+}
+
+static int move_check(const char *name, const MoveArgs &a, int32_t elem, int32_t welem) {
+    if (a.tokens < 0 || a.k < 1 || a.d < 0 || a.tokens > (int64_t(1) << 30) / a.k || a.d > (int64_t(1) << 30) ||
+        (elem != MSR_BF16 && elem != MSR_F32) || (welem != MSR_BF16 && welem != MSR_F32)) {
+        set_error("%s: bad sizes or types (tokens %lld, k %d, d %lld)", name, (long long)a.tokens, (int)a.k, (long long)a.d);
+        return MSR_ERR_ARG;
+    }
+    return MSR_OK;
+}
+
+static unsigned move_grid(int64_t waves) {
+    return (unsigned)std::min<int64_t>(std::max<int64_t>((waves + MOVE_WAVES - 1) / MOVE_WAVES, 1), MOVE_GRID);
+}
+
+static bool move_vec(int64_t d, int64_t ld, size_t es, const void *p, const void *q, const void *r) {
+    const int64_t n = 16 / (int64_t)es;
+    return d % n == 0 && ld % n == 0 && aligned(p, 16) && aligned(q, 16) && aligned(r, 16);
+}
+
+#define MOVE_LAUNCH(KERNEL, ...)                                                                                     \
+    do {                                                                                                             \
+        if (elem == MSR_BF16) {                                                                                      \
+            if (vec) hipLaunchKernelGGL((KERNEL<uint16_t, true __VA_ARGS__>), grid, dim3(MOVE_THREADS), 0, s, a);    \
+            else hipLaunchKernelGGL((KERNEL<uint16_t, false __VA_ARGS__>), grid, dim3(MOVE_THREADS), 0, s, a);       \
+        } else {                                                                                                     \
+            if (vec) hipLaunchKernelGGL((KERNEL<float, true __VA_ARGS__>), grid, dim3(MOVE_THREADS), 0, s, a);       \
+            else hipLaunchKernelGGL((KERNEL<float, false __VA_ARGS__>), grid, dim3(MOVE_THREADS), 0, s, a);          \
+        }                                                                                                            \
+    } while (0)
+
+}  // namespace msr
+
+using namespace msr;
+
+extern "C" {
+
+int msr_order_workspace_bytes(int64_t tokens, int32_t k, int32_t experts, size_t *bytes) {
+    if (!bytes || tokens < 0 || k < 1 || experts < 1 || experts > MSR_EXPERTS_MAX || tokens >= (int64_t(1) << 30) / k) {
+        set_error("msr_order_workspace_bytes: bad arguments");
+        return MSR_ERR_ARG;
+    }
+    const OrderPlan p = order_plan(tokens * k);
+    *bytes = p.wgs > 1 ? (size_t)p.wgs * (size_t)(experts + 1) * 4 : 0;
+    return MSR_OK;
+}
+
+int msr_order_tokens(const void *ids, int32_t ids_i64, int64_t tokens, int32_t k, int32_t experts, int32_t *offsets,
+                     int32_t *position, int32_t *source, void *workspace, size_t workspace_bytes, msr_stream_t stream) {
+    size_t need = 0;
+    if (msr_order_workspace_bytes(tokens, k, experts, &need)) {
+        set_error("msr_order_tokens: need tokens * k < 2^30 and 1 to %d experts (got %lld x %d, %d experts)", MSR_EXPERTS_MAX,
+                  (long long)tokens, (int)k, (int)experts);
+        return MSR_ERR_ARG;
+    }
+    const int64_t n = tokens * k;
+    if (!offsets || (n > 0 && (!ids || !position || !source))) { set_error("msr_order_tokens: a pointer is NULL"); return MSR_ERR_ARG; }
+    if (!aligned(ids, ids_i64 ? 8 : 4) || !aligned(offsets, 4) || !aligned(position, 4) || !aligned(source, 4) || !aligned(workspace, 4)) {
+        set_error("msr_order_tokens: operands must be aligned to their types");
+        return MSR_ERR_ALIGN;
+    }
+    if (need && (!workspace || workspace_bytes < need)) {
+        set_error("msr_order_tokens: workspace of %zu bytes is smaller than the %zu required", workspace_bytes, need);
+        return MSR_ERR_WORKSPACE;
+    }
+    const void *ops[5] = {ids, offsets, position, source, workspace};
+    const size_t len[5] = {(size_t)n * (ids_i64 ? 8 : 4), ((size_t)experts + 1) * 4, (size_t)n * 4, (size_t)n * 4, need};
+    for (int i = 0; i < 5; ++i)
+        for (int j = i + 1; j < 5; ++j)
+            if (touch(ops[i], len[i], ops[j], len[j])) {
+                set_error("msr_order_tokens: operands %d and %d overlap", i, j);
+                return MSR_ERR_OVERLAP;
+            }
+    const OrderPlan p = order_plan(n);
+    OrderArgs a{ids, offsets, position, source, static_cast<int32_t *>(workspace), n, experts, ids_i64 != 0, p.chunk};
+    hipStream_t s = (hipStream_t)stream;
+    if (p.wgs > 1) {
+        hipLaunchKernelGGL(count_kernel, dim3(p.wgs), dim3(ORD_THREADS), 0, s, a);
+        const int rc = check_launch("count_kernel");
+        if (rc) return rc;
+    }
+    hipLaunchKernelGGL(place_kernel, dim3(p.wgs), dim3(ORD_THREADS), ORD_WAVES * (experts + 1) * 4, s, a);
+    return check_launch("place_kernel");
+}
+
+int msr_dispatch(const void *x, int64_t ldx, void *rows, const int32_t *position, const int32_t *offsets,
+                 int32_t experts, int64_t tokens, int32_t k, int64_t d, int32_t elem, msr_stream_t stream) {
+    MoveArgs a{};
+    a.tok = x; a.ldtok = ldx; a.out = rows; a.position = position; a.offsets = offsets;
+    a.tokens = tokens; a.d = d; a.k = k; a.experts = experts;
+    int rc = move_check("msr_dispatch", a, elem, MSR_F32);
+    if (rc) return rc;
+    a.n = tokens * k;
+    if (a.n == 0 || d == 0) return MSR_OK;
+    const size_t es = elem == MSR_BF16 ? 2 : 4;
+    if (!x || !rows || !position || !offsets || ldx < d || experts < 0) { set_error("msr_dispatch: bad arguments"); return MSR_ERR_ARG; }
+    if (!aligned(x, es) || !aligned(rows, es)) { set_error("msr_dispatch: operands must be aligned to their types"); return MSR_ERR_ALIGN; }
+    const size_t rb = (size_t)a.n * (size_t)d * es;
+    if (touch(rows, rb, x, ((size_t)(tokens - 1) * (size_t)ldx + (size_t)d) * es) || touch(rows, rb, position, (size_t)a.n * 4) ||
+        touch(rows, rb, offsets, ((size_t)experts + 1) * 4)) {
+        set_error("msr_dispatch: rows overlap an input");
+        return MSR_ERR_OVERLAP;
+    }
+    const bool vec = move_vec(d, ldx, es, x, rows, nullptr);
+    const dim3 grid(move_grid(tokens));
+    hipStream_t s = (hipStream_t)stream;
+    MOVE_LAUNCH(dispatch_kernel);
+    return check_launch("dispatch_kernel");
+}
+
+int msr_dispatch_grad(const void *drows, void *dx, const int32_t *position, int64_t tokens, int32_t k, int64_t d,
+                      int32_t elem, msr_stream_t stream) {
+    MoveArgs a{};
+    a.rows = drows; a.out = dx; a.position = position; a.tokens = tokens; a.d = d; a.k = k;
+    int rc = move_check("msr_dispatch_grad", a, elem, MSR_F32);
+    if (rc) return rc;
+    a.n = tokens * k;
+    if (a.n == 0 || d == 0) return MSR_OK;
+    const size_t es = elem == MSR_BF16 ? 2 : 4;
+    if (!drows || !dx || !position) { set_error("msr_dispatch_grad: a pointer is NULL"); return MSR_ERR_ARG; }
+    if (!aligned(drows, es) || !aligned(dx, es)) { set_error("msr_dispatch_grad: operands must be aligned to their types"); return MSR_ERR_ALIGN; }
+    const size_t rb = (size_t)a.n * (size_t)d * es, tb = (size_t)tokens * (size_t)d * es;
+    if (touch(dx, tb, drows, rb) || touch(dx, tb, position, (size_t)a.n * 4)) { set_error("msr_dispatch_grad: dx overlaps an input"); return MSR_ERR_OVERLAP; }
+    const bool vec = move_vec(d, d, es, drows, dx, nullptr);
+    const dim3 grid(move_grid(tokens));
+    hipStream_t s = (hipStream_t)stream;
+    MOVE_LAUNCH(combine_kernel, , false);
+    return check_launch("combine_kernel");
+}
+
+int msr_combine(const void *rows, const void *w, void *y, const int32_t *position, int64_t tokens, int32_t k, int64_t d,
+                int32_t elem, int32_t welem, msr_stream_t stream) {
+    MoveArgs a{};
+    a.rows = rows; a.w = w; a.out = y; a.position = position; a.tokens = tokens; a.d = d; a.k = k; a.w32 = welem == MSR_F32;
+    int rc = move_check("msr_combine", a, elem, welem);
+    if (rc) return rc;
+    a.n = tokens * k;
+    if (a.n == 0 || d == 0) return MSR_OK;
+    const size_t es = elem == MSR_BF16 ? 2 : 4, ws = welem == MSR_BF16 ? 2 : 4;
+    if (!rows || !w || !y || !position) { set_error("msr_combine: a pointer is NULL"); return MSR_ERR_ARG; }
+    if (!aligned(rows, es) || !aligned(y, es) || !aligned(w, ws)) { set_error("msr_combine: operands must be aligned to their types"); return MSR_ERR_ALIGN; }
+    const size_t rb = (size_t)a.n * (size_t)d * es, tb = (size_t)tokens * (size_t)d * es;
+    if (touch(y, tb, rows, rb) || touch(y, tb, w, (size_t)a.n * ws) || touch(y, tb, position, (size_t)a.n * 4)) {
+        set_error("msr_combine: y overlaps an input");
+        return MSR_ERR_OVERLAP;
+    }
+    const bool vec = move_vec(d, d, es, rows, y, nullptr);
+    const dim3 grid(move_grid(tokens));
+    hipStream_t s = (hipStream_t)stream;
+    MOVE_LAUNCH(combine_kernel, , true);
+    return check_launch("combine_kernel");
+}
+
+int msr_combine_grad(const void *dy, int64_t lddy, const void *rows, const void *w, void *drows, void *dw,
+                     const int32_t *position, const int32_t *offsets, int32_t experts, int64_t tokens, int32_t k,
+                     int64_t d, int32_t elem, int32_t welem, msr_stream_t stream) {
+    MoveArgs a{};
+    a.tok = dy; a.ldtok = lddy; a.rows = rows; a.w = w; a.out = drows; a.dw = dw; a.position = position; a.offsets = offsets;
+    a.tokens = tokens; a.d = d; a.k = k; a.experts = experts; a.w32 = welem == MSR_F32;
+    int rc = move_check("msr_combine_grad", a, elem, welem);
+    if (rc) return rc;
+    a.n = tokens * k;
+    if (a.n == 0 || (!drows && !dw)) return MSR_OK;
+    const size_t es = elem == MSR_BF16 ? 2 : 4, ws = welem == MSR_BF16 ? 2 : 4;
+    if ((d > 0 && !dy) || (d > 0 && dw && !rows) || !w || !position || (drows && !offsets) || lddy < d || experts < 0) {
+        set_error("msr_combine_grad: bad arguments");
+        return MSR_ERR_ARG;
+    }
+    if (!aligned(dy, es) || !aligned(rows, es) || !aligned(drows, es) || !aligned(w, ws) || !aligned(dw, ws)) {
+        set_error("msr_combine_grad: operands must be aligned to their types");
+        return MSR_ERR_ALIGN;
+    }
+    const size_t rb = (size_t)a.n * (size_t)d * es, tb = ((size_t)(tokens - 1) * (size_t)lddy + (size_t)d) * es;
+    const size_t wb = (size_t)a.n * ws, pb = (size_t)a.n * 4, ob = ((size_t)experts + 1) * 4;
+    const void *in[5] = {dy, rows, w, position, offsets};
+    const size_t ib[5] = {tb, rb, wb, pb, ob};
+    bool bad = touch(drows, rb, dw, wb);
+    for (int i = 0; i < 5; ++i) bad = bad || touch(drows, rb, in[i], ib[i]) || touch(dw, wb, in[i], ib[i]);
+    if (bad) { set_error("msr_combine_grad: an output overlaps another operand"); return MSR_ERR_OVERLAP; }
+    const bool vec = move_vec(d, lddy, es, dy, rows, drows);
+    const dim3 grid(move_grid(tokens));
+    hipStream_t s = (hipStream_t)stream;
+    MOVE_LAUNCH(combine_grad_kernel);
+    return check_launch("combine_grad_kernel");
+}
+
+}  // extern "C"
