@@ -459,8 +459,8 @@ int msr_combine_grad(const void *dy, int64_t lddy, const void *rows, const void 
  * Rows from offsets[experts] on have no expert: their y and dx are 0, and dw does
  * not see them.  x, dx: [rows][in] (x with row stride ldx), dy, y: [rows][out] (dy: lddy),
  * W, dw, acc: [experts][out][in]; 16-byte aligned, in, out, ldx and lddy multiples
- * of 8; rows < 2^30, in and out at most 2^20, experts <= MSR_EXPERTS_MAX; one expert's weights
- * below 2 GiB.
+ * of 8; rows < 2^30, in and out at most 2^20, ldx and lddy at most 2^21, experts <=
+ * MSR_EXPERTS_MAX; one expert's weights below 2 GiB.  An accumulator of an expert without rows is not touched.
  * ------------------------------------------------------------------------- */
 int msr_experts_forward(const uint16_t *x, int64_t ldx, const uint16_t *w, uint16_t *y, const int32_t *offsets,
                         int64_t rows, int32_t experts, int64_t in_features, int64_t out_features, msr_stream_t stream);
@@ -542,6 +542,10 @@ int msr_fastmath_check(int32_t kind, uint32_t bits_lo, uint32_t bits_hi, uint32_
 int msr_tile_gemm(int32_t product, int32_t tile, int32_t stages, const uint16_t *p, const uint16_t *q, uint16_t *d,
                   int64_t batch, int64_t m, int64_t n, int64_t k, float alpha, float beta, float diag,
                   const float *rvec, float *resid, uint32_t seed, int32_t noise_mode, msr_stream_t stream);
+
+/* Host only: the tile (64, 128 or 256) that an experts' product of these sizes takes; product 0 forward, 1 dgrad,
+ * 2 wgrad, 3 wgrad_sr_accum.  Test support. */
+int msr_experts_tile(int32_t product, int64_t rows, int32_t experts, int64_t in_features, int64_t out_features, int32_t *tile);
 
 /* Batched bf16 GEMM  D[b] = alpha * P[b] Q[b]^T + beta * C[b] + diag * I  (fp32 accumulate, RNE
  * bf16 out; the diag term is added where m == n).

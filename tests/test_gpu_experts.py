@@ -4,6 +4,7 @@ Bound.  bf16 products are exact in fp32; a sum of K of them in fp32, in any orde
 K 2^-24 sum|terms| of the exact one (first order), and storing as bf16 (8 significant bits) adds 2^-8 of the value:
 |got - exact| <= 2^-8 |exact| + 2 K 2^-24 sum|terms|.  The accumulation is compared bit for bit with
 the stored product followed by msr_sr_accum."""
+import ctypes
 import random
 
 import pytest
@@ -102,6 +103,32 @@ def test_products_of_ordinary_layers(L, counts, fout, fin):
     near(y, s, "y", fin)
     near(dx, s, "dx", fout)
     near(dw, s, "dw", max(counts))
+
+
+@pytest.mark.parametrize("counts,fout,fin,tiles", [([41, 0, 130, 29, 0, 99, 1], 264, 136, [64, 64, 64, 64]),
+                                                   ([1201, 0, 900, 7, 893], 1544, 2056, [128, 128, 128, 128]),
+                                                   ([1013, 987], 4096, 4096, [256, 256, 256, 256]),
+                                                   ([1500, 1, 1499], 2056, 4104, [128, 256, 256, 256])])
+def test_every_tile(L, counts, fout, fin, tiles):
+    """Each product in each of its tiles (features and groups that end inside them), the accumulation against
+    the stored product whatever its tile: the same products in the same order."""
+    from muon_sr_amd import _lib, experts_wgrad_sr_accum
+    s = make(counts, 9, fout, fin, 4)
+    rows, E, t = s["x"].shape[0], len(counts), ctypes.c_int32()
+    for product, tile in enumerate(tiles):
+        check(L, L.msr_experts_tile(product, rows, E, fin, fout, ctypes.byref(t)))
+        assert t.value == tile
+    y, dx, dw = passes(s)
+    near(y, s, "y", fin)
+    near(dx, s, "dx", fout)
+    near(dw, s, "dw", max(counts))
+    assert not y[rows - 9:].any() and not dx[rows - 9:].any()
+    w, want = torch.nn.Parameter(s["w"].clone()), torch.zeros_like(dw)
+    for micro in range(2):
+        experts_wgrad_sr_accum(w, s["x"], s["dy"], s["off"], seed=99 + micro)
+        check(L, L.msr_sr_accum(want.data_ptr(), dw.data_ptr(), 0, dw.numel(), 99 + micro, int(micro == 0), _lib.noise_mode(),
+                                None, stream()))
+        assert torch.equal(w.acc_grad, want)
 
 
 def test_no_rows(L):
