@@ -42,43 +42,47 @@ def _dense(t: torch.Tensor) -> bool:
 
 
 def _check(t: torch.Tensor, device, what: str):
-    if t.is_sparse:
+    if t.layout is not torch.strided:
         raise RuntimeError(f"{what} does not support sparse gradients")
     if t.dtype != torch.bfloat16 and t.dtype != torch.float32:
         raise ValueError(f"{what} supports bf16 or fp32 gradients, got {t.dtype}")
     if not t.is_cuda:
         _lib.require_gpu(t, what)
-    if device is not None and t.get_device() != device:
+    if t.get_device() != device:
         raise ValueError(f"{what} needs every gradient on one GPU")
 
 
 def _run(grads, outs, norm_type, max_norm, what):
     """The norm of ``grads`` and, with ``outs``, the clipped gradients written there."""
     code = _norm_code(norm_type)
-    f32 = torch.float32
-    items, keep, back, device = [], [], [], None
+    bf16, f32 = torch.bfloat16, torch.float32
+    items, keep, back, device = [], [], [], grads[0].get_device()
     for i, g in enumerate(grads):
+        o = None if outs is None else outs[i]
+        # the common case by as few calls as will do (host time bounds many small tensors: 73 tensors, out of
+        # place, 98 us with every check in order, 62 so)
+        if (g.dtype is bf16 and g.get_device() == device >= 0 and g.is_contiguous() and
+                (o is g or o is None or (o.dtype is bf16 and o.is_same_size(g) and o.get_device() == device and o.is_contiguous()))):
+            at = g.data_ptr()
+            items.append(_pack_item(at, at if o is g else 0 if o is None else o.data_ptr(), g.numel(), 0, 0))
+            continue
         _check(g, device, what)
-        device = g.get_device()
         flags = _lib.CLIP_GRAD_F32 if g.dtype is f32 else 0
-        src, dst = g, None
-        if outs is not None:
-            o = outs[i]
-            if o is not g:
-                _check(o, device, what)
-                if o.shape != g.shape:
-                    raise ValueError(f"{what}: out {i} has shape {tuple(o.shape)}, its gradient {tuple(g.shape)}")
-                if o.dtype is f32 and not flags:
-                    raise ValueError(f"{what}: out {i} is fp32, its gradient bf16")
+        src, dst = g, o
+        if o is not None:
+            _check(o, device, what)
+            if o.shape != g.shape:
+                raise ValueError(f"{what}: out {i} has shape {tuple(o.shape)}, its gradient {tuple(g.shape)}")
+            if o.dtype is f32 and not flags:
+                raise ValueError(f"{what}: out {i} is fp32, its gradient bf16")
             if o.dtype is f32:
                 flags |= _lib.CLIP_OUT_F32
-            dst = o
             # elements may be walked in memory order where both tensors have the same one
             if not (g.is_contiguous() and o.is_contiguous()) and not (g.stride() == o.stride() and _dense(g)):
                 src = g.contiguous()
                 dst = torch.empty(o.shape, dtype=o.dtype, device=o.device)
                 back.append((o, dst))
-        elif not g.is_contiguous() and not _dense(g):
+        elif not _dense(g):
             src = g.contiguous()
         if src is not g:
             keep.append(src)

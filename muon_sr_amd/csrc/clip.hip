@@ -26,10 +26,11 @@ constexpr int CLIP_MAXT = 112;                       // tensors of one launch (3
 constexpr int CLIP_THREADS = 256;
 constexpr int CLIP_UNROLL = 4;
 constexpr int CLIP_TILE = CLIP_THREADS * 8 * CLIP_UNROLL;   // elements of a work-group's step
-constexpr int CLIP_GRID = 256 * 8;                   // work-groups of a launch: 8 on each CU
+constexpr int CLIP_GRID = 256 * 4;                   // work-groups of a launch: 4 on each CU (of 1.3e9 bf16 elements,
+                                                     // both passes: 1313 us, 5.9 TB/s; with 8 1403, with 2 1533)
 constexpr float CLIP_EPS = 1e-6f;
 
-constexpr uint32_t CLIP_G32 = MSR_CLIP_GRAD_F32, CLIP_O32 = MSR_CLIP_OUT_F32, CLIP_VEC = 4u;
+constexpr uint32_t CLIP_G32 = MSR_CLIP_GRAD_F32, CLIP_O32 = MSR_CLIP_OUT_F32;
 
 struct ClipArgs {
     const void *g[CLIP_MAXT];
@@ -74,33 +75,77 @@ __device__ __forceinline__ float norm_root(double s) {
     else return __uint_as_float((uint32_t)s);
 }
 
-template <int P, bool G32, bool VEC>
-__device__ __forceinline__ void norm_tile(const void *g, int64_t at, int64_t n, double &s0, double &s1) {
-    const int64_t left = n - at;
-    if (VEC && left >= CLIP_TILE) {
-        float f[CLIP_UNROLL][8];
+// 8 elements from element o on, of `valid` (<= 8) that exist; the others are 0.  Tensors start where they like: 16
+// bytes go in one access at any alignment of the element type, which the hardware allows for global memory.
+typedef uint32_t u32x4_any_t __attribute__((ext_vector_type(4), aligned(2)));
+typedef float f32x4_any_t __attribute__((ext_vector_type(4), aligned(4)));
+template <bool F32>
+__device__ __forceinline__ void clip_load(const void *g, int64_t o, int valid, float f[8]) {
+    if constexpr (F32) {
+        const float *p = static_cast<const float *>(g) + o;
+        if (valid == 8) {
+            const f32x4_any_t x = __builtin_nontemporal_load(reinterpret_cast<const f32x4_any_t *>(p));
+            const f32x4_any_t y = __builtin_nontemporal_load(reinterpret_cast<const f32x4_any_t *>(p + 4));
+            f[0] = x.x; f[1] = x.y; f[2] = x.z; f[3] = x.w;
+            f[4] = y.x; f[5] = y.y; f[6] = y.z; f[7] = y.w;
+        } else {
 #pragma unroll
-        for (int u = 0; u < CLIP_UNROLL; ++u) {
-            const int64_t o = at + (int64_t)(u * CLIP_THREADS + (int)threadIdx.x) * 8;
-            if constexpr (G32) {
-                load_f32x8<true>(static_cast<const float *>(g), o, 8, f[u]);
-            } else {
-                uint32_t w[4];
-                load_bf16x8<true>(static_cast<const uint16_t *>(g), o, 8, w);
-                unpack8(w, f[u]);
-            }
+            for (int j = 0; j < 8; ++j) f[j] = j < valid ? p[j] : 0.0f;
         }
-#pragma unroll
-        for (int u = 0; u < CLIP_UNROLL; ++u)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) norm_add<P>(j & 1 ? s1 : s0, f[u][j]);
     } else {
-        const int m = left < CLIP_TILE ? (int)left : CLIP_TILE;
-        for (int i = threadIdx.x; i < m; i += CLIP_THREADS) {
-            const float x = G32 ? static_cast<const float *>(g)[at + i] : bf16_to_f32(static_cast<const uint16_t *>(g)[at + i]);
-            norm_add<P>(s0, x);
+        const uint16_t *p = static_cast<const uint16_t *>(g) + o;
+        if (valid == 8) {
+            const u32x4_any_t x = __builtin_nontemporal_load(reinterpret_cast<const u32x4_any_t *>(p));
+            const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+            unpack8(w, f);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) f[j] = j < valid ? bf16_to_f32(p[j]) : 0.0f;
         }
     }
+}
+template <bool F32>
+__device__ __forceinline__ void clip_store(void *out, int64_t o, int valid, const float f[8]) {
+    if constexpr (F32) {
+        float *p = static_cast<float *>(out) + o;
+        if (valid == 8) {
+            __builtin_nontemporal_store(f32x4_any_t{f[0], f[1], f[2], f[3]}, reinterpret_cast<f32x4_any_t *>(p));
+            __builtin_nontemporal_store(f32x4_any_t{f[4], f[5], f[6], f[7]}, reinterpret_cast<f32x4_any_t *>(p + 4));
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (j < valid) p[j] = f[j];
+        }
+    } else {
+        uint16_t *p = static_cast<uint16_t *>(out) + o;
+        if (valid == 8) {
+            __builtin_nontemporal_store(u32x4_any_t{rne_bf16x2(f[0], f[1]), rne_bf16x2(f[2], f[3]), rne_bf16x2(f[4], f[5]),
+                                                    rne_bf16x2(f[6], f[7])}, reinterpret_cast<u32x4_any_t *>(p));
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (j < valid) p[j] = (uint16_t)rne_bf16(f[j]);
+        }
+    }
+}
+
+// Chunk u of this thread in the tile at element `at`, and how many of its 8 elements exist.
+__device__ __forceinline__ int64_t chunk_of(int64_t at, int u) { return at + (int64_t)(u * CLIP_THREADS + (int)threadIdx.x) * 8; }
+
+template <int P, bool G32>
+__device__ __forceinline__ void norm_tile(const void *g, int64_t at, int64_t n, double &s0, double &s1) {
+    float f[CLIP_UNROLL][8];
+    if (n - at >= CLIP_TILE) {
+#pragma unroll
+        for (int u = 0; u < CLIP_UNROLL; ++u) clip_load<G32>(g, chunk_of(at, u), 8, f[u]);
+    } else {
+#pragma unroll
+        for (int u = 0; u < CLIP_UNROLL; ++u) clip_load<G32>(g, chunk_of(at, u), clamp_valid(n, chunk_of(at, u)), f[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < CLIP_UNROLL; ++u)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) norm_add<P>(j & 1 ? s1 : s0, f[u][j]);
 }
 
 template <int P>
@@ -112,13 +157,8 @@ __global__ __launch_bounds__(CLIP_THREADS) void norm_kernel(ClipArgs a, double *
         while (t >= a.start[i + 1]) ++i;
         const int64_t at = (int64_t)(t - a.start[i]) * CLIP_TILE;
         const uint32_t f = a.flags[i];
-        if (f & CLIP_G32) {
-            if (f & CLIP_VEC) norm_tile<P, true, true>(a.g[i], at, a.n[i], s0, s1);
-            else norm_tile<P, true, false>(a.g[i], at, a.n[i], s0, s1);
-        } else {
-            if (f & CLIP_VEC) norm_tile<P, false, true>(a.g[i], at, a.n[i], s0, s1);
-            else norm_tile<P, false, false>(a.g[i], at, a.n[i], s0, s1);
-        }
+        if (f & CLIP_G32) norm_tile<P, true>(a.g[i], at, a.n[i], s0, s1);
+        else norm_tile<P, false>(a.g[i], at, a.n[i], s0, s1);
     }
     const double s = norm_block<P>(norm_join<P>(s0, s1), red);
     if (threadIdx.x == 0) partial[blockIdx.x] = s;
@@ -139,45 +179,22 @@ __global__ __launch_bounds__(CLIP_THREADS) void norm_finish_kernel(const double 
     if (threadIdx.x == 0) *norm_out = norm;
 }
 
-template <bool G32, bool O32, bool VEC>
+template <bool G32, bool O32>
 __device__ __forceinline__ void clip_tile(const void *g, void *out, int64_t at, int64_t n, float c) {
-    const int64_t left = n - at;
-    if (VEC && left >= CLIP_TILE) {
-        float f[CLIP_UNROLL][8];
+    float f[CLIP_UNROLL][8];
+    const bool full = n - at >= CLIP_TILE;
+    if (full) {
 #pragma unroll
-        for (int u = 0; u < CLIP_UNROLL; ++u) {
-            const int64_t o = at + (int64_t)(u * CLIP_THREADS + (int)threadIdx.x) * 8;
-            if constexpr (G32) {
-                load_f32x8<true>(static_cast<const float *>(g), o, 8, f[u]);
-            } else {
-                uint32_t w[4];
-                load_bf16x8<true>(static_cast<const uint16_t *>(g), o, 8, w);
-                unpack8(w, f[u]);
-            }
-        }
-#pragma unroll
-        for (int u = 0; u < CLIP_UNROLL; ++u) {
-            const int64_t o = at + (int64_t)(u * CLIP_THREADS + (int)threadIdx.x) * 8;
-            float *x = f[u];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = x[j] * c;
-            if constexpr (O32) {
-                float *p = static_cast<float *>(out) + o;
-                __builtin_nontemporal_store(f32x4_t{x[0], x[1], x[2], x[3]}, reinterpret_cast<f32x4_t *>(p));
-                __builtin_nontemporal_store(f32x4_t{x[4], x[5], x[6], x[7]}, reinterpret_cast<f32x4_t *>(p + 4));
-            } else {
-                const uint32_t w[4] = {rne_bf16x2(x[0], x[1]), rne_bf16x2(x[2], x[3]), rne_bf16x2(x[4], x[5]),
-                                       rne_bf16x2(x[6], x[7])};
-                store_bf16x8<true>(static_cast<uint16_t *>(out), o, 8, w);
-            }
-        }
+        for (int u = 0; u < CLIP_UNROLL; ++u) clip_load<G32>(g, chunk_of(at, u), 8, f[u]);
     } else {
-        const int m = left < CLIP_TILE ? (int)left : CLIP_TILE;
-        for (int i = threadIdx.x; i < m; i += CLIP_THREADS) {
-            const float x = G32 ? static_cast<const float *>(g)[at + i] : bf16_to_f32(static_cast<const uint16_t *>(g)[at + i]);
-            if constexpr (O32) static_cast<float *>(out)[at + i] = x * c;
-            else static_cast<uint16_t *>(out)[at + i] = (uint16_t)rne_bf16(x * c);
-        }
+#pragma unroll
+        for (int u = 0; u < CLIP_UNROLL; ++u) clip_load<G32>(g, chunk_of(at, u), clamp_valid(n, chunk_of(at, u)), f[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < CLIP_UNROLL; ++u) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[u][j] = f[u][j] * c;
+        clip_store<O32>(out, chunk_of(at, u), full ? 8 : clamp_valid(n, chunk_of(at, u)), f[u]);
     }
 }
 
@@ -195,16 +212,9 @@ __global__ __launch_bounds__(CLIP_THREADS) void clip_kernel(ClipArgs a, const do
         if (c == 1.0f && a.out[i] == a.g[i]) continue;   // in place and nothing to cut
         const int64_t at = (int64_t)(t - a.start[i]) * CLIP_TILE, n = a.n[i];
         const uint32_t f = a.flags[i];
-        if (f & CLIP_O32) {
-            if (f & CLIP_VEC) clip_tile<true, true, true>(a.g[i], a.out[i], at, n, c);
-            else clip_tile<true, true, false>(a.g[i], a.out[i], at, n, c);
-        } else if (f & CLIP_G32) {
-            if (f & CLIP_VEC) clip_tile<true, false, true>(a.g[i], a.out[i], at, n, c);
-            else clip_tile<true, false, false>(a.g[i], a.out[i], at, n, c);
-        } else {
-            if (f & CLIP_VEC) clip_tile<false, false, true>(a.g[i], a.out[i], at, n, c);
-            else clip_tile<false, false, false>(a.g[i], a.out[i], at, n, c);
-        }
+        if (f & CLIP_O32) clip_tile<true, true>(a.g[i], a.out[i], at, n, c);
+        else if (f & CLIP_G32) clip_tile<true, false>(a.g[i], a.out[i], at, n, c);
+        else clip_tile<false, false>(a.g[i], a.out[i], at, n, c);
     }
 }
 
@@ -222,7 +232,7 @@ static unsigned clip_fill(ClipArgs &a, const msr_clip_item *items, int32_t count
         a.out[t] = outs ? x.out : nullptr;
         a.n[t] = x.n;
         a.start[t] = (int32_t)tiles;
-        a.flags[t] = (uint8_t)(x.flags | (aligned(x.grad, 16) && (!outs || aligned(x.out, 16)) ? CLIP_VEC : 0));
+        a.flags[t] = (uint8_t)x.flags;
         tiles += more;
     }
     a.start[a.count] = (int32_t)tiles;

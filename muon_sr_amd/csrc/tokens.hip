@@ -26,11 +26,12 @@ namespace msr {
 constexpr int ORD_THREADS = 1024, ORD_WAVES = ORD_THREADS / 64;
 constexpr int ORD_CHUNK = 2048;          // slots of a work-group, while there are at most ORD_MAXWG of them
 constexpr int ORD_MAXWG = 256;
+constexpr int ORD_AHEAD = 4;             // experts whose counts a wave loads at once
 
 struct OrderArgs {
     const void *ids;
     int32_t *offsets, *position, *source;
-    int32_t *counts;                     // [work-groups][experts + 1]
+    int32_t *counts;                     // [experts + 1][work-groups]
     int64_t n;                           // slots
     int32_t experts, i64, chunk;
 };
@@ -51,7 +52,7 @@ __global__ __launch_bounds__(ORD_THREADS) void count_kernel(OrderArgs a) {
     const int64_t s0 = (int64_t)blockIdx.x * a.chunk, s1 = min(s0 + a.chunk, a.n);
     for (int64_t s = s0 + threadIdx.x; s < s1; s += ORD_THREADS) atomicAdd(&hist[expert_of(a, s)], 1);
     __syncthreads();
-    for (int e = threadIdx.x; e <= a.experts; e += ORD_THREADS) a.counts[(int64_t)blockIdx.x * (a.experts + 1) + e] = hist[e];
+    for (int e = threadIdx.x; e <= a.experts; e += ORD_THREADS) a.counts[(int64_t)e * gridDim.x + blockIdx.x] = hist[e];
 }
 
 // Inclusive sum over the lanes of a wave.
@@ -67,7 +68,7 @@ __device__ __forceinline__ int wave_scan(int x) {
 
 __global__ __launch_bounds__(ORD_THREADS) void place_kernel(OrderArgs a) {
     extern __shared__ int wave_at[];                 // [ORD_WAVES][experts + 1]: counts, then the next row
-    __shared__ int wave_sum[ORD_WAVES];
+    __shared__ int wave_sum[ORD_WAVES], all[MSR_EXPERTS_MAX + 1], before[MSR_EXPERTS_MAX + 1];
     const int E1 = a.experts + 1, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     for (int i = tid; i < ORD_WAVES * E1; i += ORD_THREADS) wave_at[i] = 0;
     __syncthreads();
@@ -77,27 +78,57 @@ __global__ __launch_bounds__(ORD_THREADS) void place_kernel(OrderArgs a) {
     int *const mine = wave_at + wave * E1;
     for (int64_t s = s0 + lane; s < s1; s += 64) atomicAdd(&mine[expert_of(a, s)], 1);
     __syncthreads();
-    // Thread e: expert e's slots in the chunks before this one and in all; the sum over the
-    // experts before it gives its first row.  experts + 1 <= 1025 numbers: two rounds at most.
-    int carry = 0;
-    for (int e0 = 0; e0 < E1; e0 += ORD_THREADS) {
-        const int e = e0 + tid;
-        int before = 0, all = 0;
-        if (e < E1) {
-            if (gridDim.x == 1) {
-                for (int w = 0; w < ORD_WAVES; ++w) all += wave_at[w * E1 + e];
-            } else {
-                for (int b = 0; b < (int)gridDim.x; ++b) {
-                    const int c = a.counts[(int64_t)b * E1 + e];
-                    before += b < (int)blockIdx.x ? c : 0;
-                    all += c;
+    // Each expert's slots in all chunks and in those before this one: a wave per expert, its lanes over
+    // the chunks (one number per thread and chunk after the other took 38 us for 128 chunks and 128
+    // experts, this 7 us).
+    if (gridDim.x == 1) {
+        for (int e = tid; e < E1; e += ORD_THREADS) {
+            int n = 0;
+            for (int w = 0; w < ORD_WAVES; ++w) n += wave_at[w * E1 + e];
+            all[e] = n;
+            before[e] = 0;
+        }
+    } else {
+        for (int e0 = wave; e0 < E1; e0 += ORD_AHEAD * ORD_WAVES) {
+            int c[ORD_AHEAD][ORD_MAXWG / 64];
+#pragma unroll
+            for (int u = 0; u < ORD_AHEAD; ++u)
+#pragma unroll
+                for (int i = 0; i < ORD_MAXWG / 64; ++i) {
+                    const int e = e0 + u * ORD_WAVES, b = i * 64 + lane;
+                    c[u][i] = e < E1 && b < (int)gridDim.x ? a.counts[(int64_t)e * gridDim.x + b] : 0;
+                }
+#pragma unroll
+            for (int u = 0; u < ORD_AHEAD; ++u) {
+                const int e = e0 + u * ORD_WAVES;
+                int n = 0, m = 0;
+#pragma unroll
+                for (int i = 0; i < ORD_MAXWG / 64; ++i) {
+                    n += c[u][i];
+                    m += i * 64 + lane < (int)blockIdx.x ? c[u][i] : 0;
+                }
+#pragma unroll
+                for (int w = 32; w > 0; w >>= 1) {
+                    n += __shfl_xor(n, w);
+                    m += __shfl_xor(m, w);
+                }
+                if (lane == 0 && e < E1) {
+                    all[e] = n;
+                    before[e] = m;
                 }
             }
         }
-        const int incl = wave_scan(all);
+    }
+    __syncthreads();
+    // Thread e: the sum over the experts before e gives its first row.  experts + 1 <= 1025 numbers: two
+    // rounds at most.
+    int carry = 0;
+    for (int e0 = 0; e0 < E1; e0 += ORD_THREADS) {
+        const int e = e0 + tid, n = e < E1 ? all[e] : 0;
+        const int incl = wave_scan(n);
         if (lane == 63) wave_sum[wave] = incl;
         __syncthreads();
-        int first = carry + incl - all, total = 0;
+        int first = carry + incl - n, total = 0;
         for (int w = 0; w < ORD_WAVES; ++w) {
             first += w < wave ? wave_sum[w] : 0;
             total += wave_sum[w];
@@ -105,7 +136,7 @@ __global__ __launch_bounds__(ORD_THREADS) void place_kernel(OrderArgs a) {
         carry += total;
         if (e < E1) {
             if (blockIdx.x == 0) a.offsets[e] = first;   // expert `experts` is the dropped slots': their first row
-            int at = first + before;
+            int at = first + before[e];
             for (int w = 0; w < ORD_WAVES; ++w) {
                 const int c = wave_at[w * E1 + e];
                 wave_at[w * E1 + e] = at;
@@ -155,7 +186,9 @@ static OrderPlan order_plan(int64_t n) {
 constexpr int MOVE_THREADS = 256, MOVE_WAVES = MOVE_THREADS / 64;
 constexpr int MOVE_GRID = 256 * 8;
 
-// 16 bytes of a row per lane (VEC), or one element.
+// 16 bytes of a row per lane (VEC), or one element.  Stores are non-temporal: the four passes over 32768 tokens x 8
+// of width 2048 take 1120 us so (5.3 TB/s), 1172 with plain stores, and over 8192 x 2 76 and 101 us; loads are not,
+// as the rows were mostly written just before (non-temporal: 1102 and 96 us).
 template <typename T, bool VEC>
 struct Pack {
     static constexpr int N = VEC ? 16 / (int)sizeof(T) : 1;
@@ -178,10 +211,9 @@ struct Pack {
             if constexpr (sizeof(T) == 2) *p = (T)rne_bf16(f[0]);
             else *p = f[0];
         } else if constexpr (sizeof(T) == 2) {
-            *reinterpret_cast<u32x4_t *>(p) = u32x4_t{rne_bf16x2(f[0], f[1]), rne_bf16x2(f[2], f[3]),
-                                                      rne_bf16x2(f[4], f[5]), rne_bf16x2(f[6], f[7])};
+            st_nt4(p, u32x4_t{rne_bf16x2(f[0], f[1]), rne_bf16x2(f[2], f[3]), rne_bf16x2(f[4], f[5]), rne_bf16x2(f[6], f[7])});
         } else {
-            *reinterpret_cast<f32x4_t *>(p) = f32x4_t{f[0], f[1], f[2], f[3]};
+            __builtin_nontemporal_store(f32x4_t{f[0], f[1], f[2], f[3]}, reinterpret_cast<f32x4_t *>(p));
         }
     }
     __device__ __forceinline__ void zero() {
@@ -202,14 +234,52 @@ struct MoveArgs {
     int32_t k, experts, w32;
 };
 
-__device__ __forceinline__ float weight_of(const MoveArgs &a, int64_t s) {
-    return a.w32 ? static_cast<const float *>(a.w)[s] : bf16_to_f32(static_cast<const uint16_t *>(a.w)[s]);
-}
-// The row of slot s, or -1.
-__device__ __forceinline__ int64_t row_of(const MoveArgs &a, int64_t s) {
-    const int64_t p = a.position[s];
-    return p < a.n ? p : -1;
-}
+// A token's slots, 64 at a time: lane j holds the row (-1: none) and the weight of slot first + j, so that one
+// load of each fetches them all ahead of the rows.
+struct Slots {
+    int row;
+    float w;
+    __device__ __forceinline__ void load(const MoveArgs &a, int64_t first, int count) {
+        const int lane = threadIdx.x & 63;
+        row = -1;
+        w = 0.0f;
+        if (lane < count) {
+            row = a.position[first + lane];
+            if (row >= a.n) row = -1;
+            if (a.w) w = a.w32 ? static_cast<const float *>(a.w)[first + lane] : bf16_to_f32(static_cast<const uint16_t *>(a.w)[first + lane]);
+        }
+    }
+    __device__ __forceinline__ int row_of(int j) const { return __builtin_amdgcn_readlane(row, j); }
+    __device__ __forceinline__ float weight_of(int j) const {
+        return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(w), j));
+    }
+};
+// A wave's piece of a row: U packs per lane, 64 packs apart, from column c on.  Whole rows (or 4 KiB of
+// them) at a time: a wave that went through a token's rows 1 KiB at a time would return to each row's memory page
+// several times (combine of 32768 x 8 rows of 4 KiB 339 us so, 272 a whole row at a time).
+template <typename T, bool VEC, int U>
+struct Piece {
+    static constexpr int N = Pack<T, VEC>::N, WIDTH = 64 * N * U;
+    Pack<T, VEC> p[U];
+    static __device__ __forceinline__ int64_t col(int64_t c, int u) { return c + ((int64_t)u * 64 + (threadIdx.x & 63)) * N; }
+    __device__ __forceinline__ void load(const T *row, int64_t c, int64_t d) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (col(c, u) < d) p[u].load(row + col(c, u));
+            else p[u].zero();
+        }
+    }
+    __device__ __forceinline__ void store(T *row, int64_t c, int64_t d) const {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (col(c, u) < d) p[u].store(row + col(c, u));
+    }
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int u = 0; u < U; ++u) p[u].zero();
+    }
+};
+constexpr int MOVE_AHEAD = 2;   // rows whose loads are in flight together (1: 4 % slower, 4: 35 %, too few waves)
 
 // Rows without a slot, [offsets[experts], n), to zero: the waves of the launch in turn.
 template <typename T, bool VEC>
@@ -226,80 +296,122 @@ __device__ __forceinline__ int64_t this_wave() {
 }
 
 // rows[position[t][j]] = x[t]
-template <typename T, bool VEC>
+template <typename T, bool VEC, int U>
 __global__ __launch_bounds__(MOVE_THREADS) void dispatch_kernel(MoveArgs a) {
-    constexpr int N = Pack<T, VEC>::N;
+    using P = Piece<T, VEC, U>;
     const int64_t waves = (int64_t)gridDim.x * MOVE_WAVES;
     for (int64_t t = this_wave(); t < a.tokens; t += waves) {
         const T *x = static_cast<const T *>(a.tok) + t * a.ldtok;
-        for (int64_t c = (int64_t)(threadIdx.x & 63) * N; c < a.d; c += 64 * N) {
-            Pack<T, VEC> v;
-            v.load(x + c);
-            for (int j = 0; j < a.k; ++j) {
-                const int64_t p = row_of(a, t * a.k + j);
-                if (p >= 0) v.store(static_cast<T *>(a.out) + p * a.d + c);
+        for (int j0 = 0; j0 < a.k; j0 += 64) {
+            const int js = min(64, a.k - j0);
+            Slots s;
+            s.load(a, t * a.k + j0, js);
+            for (int64_t c = 0; c < a.d; c += P::WIDTH) {
+                P v;
+                v.load(x, c, a.d);
+                for (int j = 0; j < js; ++j) {
+                    const int p = s.row_of(j);
+                    if (p >= 0) v.store(static_cast<T *>(a.out) + (int64_t)p * a.d, c, a.d);
+                }
             }
         }
     }
     zero_tail<T, VEC>(a, this_wave(), waves);
 }
 
-// out[t] = sum_j w[t][j] rows[position[t][j]], or without weights (WEIGHTED false)
-template <typename T, bool VEC, bool WEIGHTED>
+// out[t] = sum_j w[t][j] rows[position[t][j]], or without weights (WEIGHTED false), j ascending
+template <typename T, bool VEC, int U, bool WEIGHTED>
 __global__ __launch_bounds__(MOVE_THREADS) void combine_kernel(MoveArgs a) {
-    constexpr int N = Pack<T, VEC>::N;
+    using P = Piece<T, VEC, U>;
     const int64_t waves = (int64_t)gridDim.x * MOVE_WAVES;
     for (int64_t t = this_wave(); t < a.tokens; t += waves) {
-        for (int64_t c = (int64_t)(threadIdx.x & 63) * N; c < a.d; c += 64 * N) {
-            Pack<T, VEC> sum, v;
+        Slots s;
+        s.load(a, t * a.k, min(64, a.k));
+        for (int64_t c = 0; c < a.d; c += P::WIDTH) {
+            P sum;
             sum.zero();
-            for (int j = 0; j < a.k; ++j) {
-                const int64_t s = t * a.k + j, p = row_of(a, s);
-                if (p < 0) continue;
-                const float w = WEIGHTED ? weight_of(a, s) : 1.0f;
-                v.load(static_cast<const T *>(a.rows) + p * a.d + c);
+            for (int j0 = 0; j0 < a.k; j0 += MOVE_AHEAD) {
+                if (a.k > 64 && (j0 & 63) == 0) s.load(a, t * a.k + j0, min(64, a.k - j0));
+                P v[MOVE_AHEAD];
 #pragma unroll
-                for (int i = 0; i < N; ++i) sum.f[i] = WEIGHTED ? __builtin_fmaf(w, v.f[i], sum.f[i]) : sum.f[i] + v.f[i];
+                for (int y = 0; y < MOVE_AHEAD; ++y) {
+                    const int p = j0 + y < a.k ? s.row_of((j0 + y) & 63) : -1;
+                    if (p >= 0) v[y].load(static_cast<const T *>(a.rows) + (int64_t)p * a.d, c, a.d);
+                }
+#pragma unroll
+                for (int y = 0; y < MOVE_AHEAD; ++y) {
+                    if (j0 + y >= a.k || s.row_of((j0 + y) & 63) < 0) continue;
+                    const float w = WEIGHTED ? s.weight_of((j0 + y) & 63) : 1.0f;
+#pragma unroll
+                    for (int u = 0; u < U; ++u)
+#pragma unroll
+                        for (int i = 0; i < P::N; ++i)
+                            sum.p[u].f[i] = WEIGHTED ? __builtin_fmaf(w, v[y].p[u].f[i], sum.p[u].f[i]) : sum.p[u].f[i] + v[y].p[u].f[i];
+                }
             }
-            sum.store(static_cast<T *>(a.out) + t * a.d + c);
+            sum.store(static_cast<T *>(a.out) + t * a.d, c, a.d);
         }
     }
 }
 
 // drows[position[t][j]] = w[t][j] dy[t];  dw[t][j] = <dy[t], rows[position[t][j]]>
-template <typename T, bool VEC>
+template <typename T, bool VEC, int U>
 __global__ __launch_bounds__(MOVE_THREADS) void combine_grad_kernel(MoveArgs a) {
-    constexpr int N = Pack<T, VEC>::N;
+    using P = Piece<T, VEC, U>;
     const int lane = threadIdx.x & 63;
     const int64_t waves = (int64_t)gridDim.x * MOVE_WAVES;
     for (int64_t t = this_wave(); t < a.tokens; t += waves) {
         const T *dy = static_cast<const T *>(a.tok) + t * a.ldtok;
-        for (int j = 0; j < a.k; ++j) {
-            const int64_t s = t * a.k + j, p = row_of(a, s);
-            float dot = 0.0f;
-            if (p >= 0) {
-                const float w = weight_of(a, s);
-                for (int64_t c = (int64_t)lane * N; c < a.d; c += 64 * N) {
-                    Pack<T, VEC> g, r;
-                    g.load(dy + c);
-                    if (a.dw) {
-                        r.load(static_cast<const T *>(a.rows) + p * a.d + c);
+        const bool whole = a.d <= P::WIDTH;      // dy[t] stays in registers
+        P g;
+        if (whole) g.load(dy, 0, a.d);
+        Slots s;
+        for (int j0 = 0; j0 < a.k; j0 += MOVE_AHEAD) {
+            if ((j0 & 63) == 0) s.load(a, t * a.k + j0, min(64, a.k - j0));
+            float dot[MOVE_AHEAD] = {};
+            for (int64_t c = 0; c < a.d; c += P::WIDTH) {
+                if (!whole) g.load(dy, c, a.d);
+                if (a.dw) {
+                    P r[MOVE_AHEAD];
 #pragma unroll
-                        for (int i = 0; i < N; ++i) dot = __builtin_fmaf(g.f[i], r.f[i], dot);
+                    for (int y = 0; y < MOVE_AHEAD; ++y) {
+                        const int p = j0 + y < a.k ? s.row_of((j0 + y) & 63) : -1;
+                        if (p >= 0) r[y].load(static_cast<const T *>(a.rows) + (int64_t)p * a.d, c, a.d);
                     }
-                    if (a.out) {
 #pragma unroll
-                        for (int i = 0; i < N; ++i) g.f[i] = g.f[i] * w;
-                        g.store(static_cast<T *>(a.out) + p * a.d + c);
+                    for (int y = 0; y < MOVE_AHEAD; ++y) {
+                        if (j0 + y >= a.k || s.row_of((j0 + y) & 63) < 0) continue;
+#pragma unroll
+                        for (int u = 0; u < U; ++u)
+#pragma unroll
+                            for (int i = 0; i < P::N; ++i) dot[y] = __builtin_fmaf(g.p[u].f[i], r[y].p[u].f[i], dot[y]);
+                    }
+                }
+                if (a.out) {
+#pragma unroll
+                    for (int y = 0; y < MOVE_AHEAD; ++y) {
+                        const int p = j0 + y < a.k ? s.row_of((j0 + y) & 63) : -1;
+                        if (p < 0) continue;
+                        const float w = s.weight_of((j0 + y) & 63);
+                        P o;
+#pragma unroll
+                        for (int u = 0; u < U; ++u)
+#pragma unroll
+                            for (int i = 0; i < P::N; ++i) o.p[u].f[i] = g.p[u].f[i] * w;
+                        o.store(static_cast<T *>(a.out) + (int64_t)p * a.d, c, a.d);
                     }
                 }
             }
             if (a.dw) {
 #pragma unroll
-                for (int w = 32; w > 0; w >>= 1) dot += __shfl_xor(dot, w);
-                if (lane == 0) {
-                    if (a.w32) static_cast<float *>(a.dw)[s] = dot;
-                    else static_cast<uint16_t *>(a.dw)[s] = (uint16_t)rne_bf16(dot);
+                for (int y = 0; y < MOVE_AHEAD; ++y) {
+#pragma unroll
+                    for (int w = 32; w > 0; w >>= 1) dot[y] += __shfl_xor(dot[y], w);
+                    if (lane == y && j0 + y < a.k) {
+                        const int64_t at = t * a.k + j0 + y;
+                        if (a.w32) static_cast<float *>(a.dw)[at] = dot[y];
+                        else static_cast<uint16_t *>(a.dw)[at] = (uint16_t)rne_bf16(dot[y]);
+                    }
                 }
             }
         }
@@ -334,14 +446,22 @@ static bool move_vec(int64_t d, int64_t ld, size_t es, const void *p, const void
     return d % n == 0 && ld % n == 0 && aligned(p, 16) && aligned(q, 16) && aligned(r, 16);
 }
 
+// U: the packs per lane that a row of d elements fills, at most 4.
+#define MOVE_LAUNCH_U(KERNEL, T, V, ...)                                                                             \
+    do {                                                                                                             \
+        const int64_t packs = (a.d + 64 * Pack<T, V>::N - 1) / (64 * Pack<T, V>::N);                                 \
+        if (packs > 2) hipLaunchKernelGGL((KERNEL<T, V, 4 __VA_ARGS__>), grid, dim3(MOVE_THREADS), 0, s, a);         \
+        else if (packs > 1) hipLaunchKernelGGL((KERNEL<T, V, 2 __VA_ARGS__>), grid, dim3(MOVE_THREADS), 0, s, a);    \
+        else hipLaunchKernelGGL((KERNEL<T, V, 1 __VA_ARGS__>), grid, dim3(MOVE_THREADS), 0, s, a);                   \
+    } while (0)
 #define MOVE_LAUNCH(KERNEL, ...)                                                                                     \
     do {                                                                                                             \
         if (elem == MSR_BF16) {                                                                                      \
-            if (vec) hipLaunchKernelGGL((KERNEL<uint16_t, true __VA_ARGS__>), grid, dim3(MOVE_THREADS), 0, s, a);    \
-            else hipLaunchKernelGGL((KERNEL<uint16_t, false __VA_ARGS__>), grid, dim3(MOVE_THREADS), 0, s, a);       \
+            if (vec) MOVE_LAUNCH_U(KERNEL, uint16_t, true, __VA_ARGS__);                                             \
+            else MOVE_LAUNCH_U(KERNEL, uint16_t, false, __VA_ARGS__);                                                \
         } else {                                                                                                     \
-            if (vec) hipLaunchKernelGGL((KERNEL<float, true __VA_ARGS__>), grid, dim3(MOVE_THREADS), 0, s, a);       \
-            else hipLaunchKernelGGL((KERNEL<float, false __VA_ARGS__>), grid, dim3(MOVE_THREADS), 0, s, a);          \
+            if (vec) MOVE_LAUNCH_U(KERNEL, float, true, __VA_ARGS__);                                                \
+            else MOVE_LAUNCH_U(KERNEL, float, false, __VA_ARGS__);                                                   \
         }                                                                                                            \
     } while (0)
 
