@@ -2,12 +2,12 @@
 //
 // Order: a stable counting sort of the n = tokens * k slots by expert.  Slot s of expert e
 // gets row  offsets[e] + #{s' < s : expert(s') = e}.  The slots are cut into one chunk per
-// work-group; count_kernel counts each chunk's slots per expert, and place_kernel adds the counts of
-// the chunks before its own, and of all chunks for the offsets (a few thousand numbers from
-// L2), then ranks its slots wave by wave.  A wave ranks 64 slots at a time by ballots, one
-// per bit of the expert number, so no order depends on atomics.  Dropped slots count as one
-// more expert, which gives the rows without a slot.  Bound by latency: two launches (one where a
-// single work-group takes all slots).
+// work-group.  place_kernel needs the slots per expert in the chunks before its own, and in all for the
+// offsets: up to ORD_SELF slots every work-group counts them all itself; beyond that count_kernel counts
+// each chunk, and the work-groups add its counts (a few thousand numbers from L2).  It then ranks its
+// slots wave by wave, 64 at a time by ballots, one per bit of the expert number: only the counts are
+// atomic, no order depends on them.  Dropped slots count as one more expert, which gives the rows without
+// a slot.  Bound by latency: one or two launches.
 //
 // The four passes between tokens and rows (see the header) move d elements per slot and do
 // next to nothing with them, so HBM bounds them.  All are written from the token's side: a
@@ -26,6 +26,7 @@ namespace msr {
 constexpr int ORD_THREADS = 1024, ORD_WAVES = ORD_THREADS / 64;
 constexpr int ORD_CHUNK = 2048;          // slots of a work-group, while there are at most ORD_MAXWG of them
 constexpr int ORD_MAXWG = 256;
+constexpr int ORD_SELF = 32768;          // slots that every work-group counts by itself
 constexpr int ORD_AHEAD = 4;             // experts whose counts a wave loads at once
 
 struct OrderArgs {
@@ -71,24 +72,33 @@ __global__ __launch_bounds__(ORD_THREADS) void place_kernel(OrderArgs a) {
     __shared__ int wave_sum[ORD_WAVES], all[MSR_EXPERTS_MAX + 1], before[MSR_EXPERTS_MAX + 1];
     const int E1 = a.experts + 1, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     for (int i = tid; i < ORD_WAVES * E1; i += ORD_THREADS) wave_at[i] = 0;
+    for (int e = tid; e < E1; e += ORD_THREADS) all[e] = before[e] = 0;
     __syncthreads();
     // each wave takes a run of the chunk's slots
     const int run = a.chunk / ORD_WAVES;
     const int64_t s0 = (int64_t)blockIdx.x * a.chunk + (int64_t)wave * run, s1 = min(s0 + run, a.n);
     int *const mine = wave_at + wave * E1;
-    for (int64_t s = s0 + lane; s < s1; s += 64) atomicAdd(&mine[expert_of(a, s)], 1);
-    __syncthreads();
-    // Each expert's slots in all chunks and in those before this one: a wave per expert, its lanes over
-    // the chunks (one number per thread and chunk after the other took 38 us for 128 chunks and 128
-    // experts, this 7 us).
-    if (gridDim.x == 1) {
-        for (int e = tid; e < E1; e += ORD_THREADS) {
-            int n = 0;
-            for (int w = 0; w < ORD_WAVES; ++w) n += wave_at[w * E1 + e];
-            all[e] = n;
-            before[e] = 0;
+    // Each expert's slots in all chunks and in those before this one.
+    if (!a.counts) {
+        // four loads in flight; a slot counts in `all`, and in `before` or its wave's count of this chunk
+        const int c0 = (int)blockIdx.x * a.chunk, n = (int)a.n;
+        for (int t = tid; t < n; t += 4 * ORD_THREADS) {
+            int e[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) e[u] = t + u * ORD_THREADS < n ? expert_of(a, t + u * ORD_THREADS) : -1;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                if (e[u] < 0) continue;
+                atomicAdd(&all[e[u]], 1);
+                const int at = t + u * ORD_THREADS - c0;
+                if (at < 0) atomicAdd(&before[e[u]], 1);
+                else if (at < a.chunk) atomicAdd(&wave_at[at / run * E1 + e[u]], 1);
+            }
         }
     } else {
+        for (int64_t s = s0 + lane; s < s1; s += 64) atomicAdd(&mine[expert_of(a, s)], 1);
+        // a wave per expert, its lanes over the chunks (one number per thread and chunk after the other took
+        // 38 us for 128 chunks and 128 experts, this 13 us)
         for (int e0 = wave; e0 < E1; e0 += ORD_AHEAD * ORD_WAVES) {
             int c[ORD_AHEAD][ORD_MAXWG / 64];
 #pragma unroll
@@ -136,11 +146,13 @@ __global__ __launch_bounds__(ORD_THREADS) void place_kernel(OrderArgs a) {
         carry += total;
         if (e < E1) {
             if (blockIdx.x == 0) a.offsets[e] = first;   // expert `experts` is the dropped slots': their first row
-            int at = first + before[e];
+            int at = first + before[e], c[ORD_WAVES];
+#pragma unroll
+            for (int w = 0; w < ORD_WAVES; ++w) c[w] = wave_at[w * E1 + e];
+#pragma unroll
             for (int w = 0; w < ORD_WAVES; ++w) {
-                const int c = wave_at[w * E1 + e];
                 wave_at[w * E1 + e] = at;
-                at += c;
+                at += c[w];
             }
         }
         __syncthreads();
@@ -446,12 +458,14 @@ static bool move_vec(int64_t d, int64_t ld, size_t es, const void *p, const void
     return d % n == 0 && ld % n == 0 && aligned(p, 16) && aligned(q, 16) && aligned(r, 16);
 }
 
-// U: the packs per lane that a row of d elements fills, at most 4.
+// U: the packs per lane of a piece, at most 4, as even as the row allows (6 packs: 2 pieces of 3).
 #define MOVE_LAUNCH_U(KERNEL, T, V, ...)                                                                             \
     do {                                                                                                             \
         const int64_t packs = (a.d + 64 * Pack<T, V>::N - 1) / (64 * Pack<T, V>::N);                                 \
-        if (packs > 2) hipLaunchKernelGGL((KERNEL<T, V, 4 __VA_ARGS__>), grid, dim3(MOVE_THREADS), 0, s, a);         \
-        else if (packs > 1) hipLaunchKernelGGL((KERNEL<T, V, 2 __VA_ARGS__>), grid, dim3(MOVE_THREADS), 0, s, a);    \
+        const int64_t u = (packs + (packs + 3) / 4 - 1) / ((packs + 3) / 4);                                         \
+        if (u > 3) hipLaunchKernelGGL((KERNEL<T, V, 4 __VA_ARGS__>), grid, dim3(MOVE_THREADS), 0, s, a);             \
+        else if (u > 2) hipLaunchKernelGGL((KERNEL<T, V, 3 __VA_ARGS__>), grid, dim3(MOVE_THREADS), 0, s, a);        \
+        else if (u > 1) hipLaunchKernelGGL((KERNEL<T, V, 2 __VA_ARGS__>), grid, dim3(MOVE_THREADS), 0, s, a);    \
         else hipLaunchKernelGGL((KERNEL<T, V, 1 __VA_ARGS__>), grid, dim3(MOVE_THREADS), 0, s, a);                   \
     } while (0)
 #define MOVE_LAUNCH(KERNEL, ...)                                                                                     \
@@ -477,7 +491,7 @@ int msr_order_workspace_bytes(int64_t tokens, int32_t k, int32_t experts, size_t
         return MSR_ERR_ARG;
     }
     const OrderPlan p = order_plan(tokens * k);
-    *bytes = p.wgs > 1 ? (size_t)p.wgs * (size_t)(experts + 1) * 4 : 0;
+    *bytes = tokens * k > ORD_SELF ? (size_t)p.wgs * (size_t)(experts + 1) * 4 : 0;
     return MSR_OK;
 }
 
@@ -508,9 +522,9 @@ int msr_order_tokens(const void *ids, int32_t ids_i64, int64_t tokens, int32_t k
                 return MSR_ERR_OVERLAP;
             }
     const OrderPlan p = order_plan(n);
-    OrderArgs a{ids, offsets, position, source, static_cast<int32_t *>(workspace), n, experts, ids_i64 != 0, p.chunk};
+    OrderArgs a{ids, offsets, position, source, need ? static_cast<int32_t *>(workspace) : nullptr, n, experts, ids_i64 != 0, p.chunk};
     hipStream_t s = (hipStream_t)stream;
-    if (p.wgs > 1) {
+    if (need) {
         hipLaunchKernelGGL(count_kernel, dim3(p.wgs), dim3(ORD_THREADS), 0, s, a);
         const int rc = check_launch("count_kernel");
         if (rc) return rc;
