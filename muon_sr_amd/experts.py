@@ -26,6 +26,7 @@ from . import _lib
 __all__ = ["TokenOrder", "order_tokens", "dispatch_tokens", "combine_tokens", "expert_linear",
            "experts_wgrad_sr_accum", "SRExperts"]
 
+MAX_ROW_STRIDE = 1 << 21   # of the experts' products
 _ELEM = {torch.bfloat16: _lib.BF16, torch.float32: _lib.F32}
 
 
@@ -48,11 +49,21 @@ def _elem(t: torch.Tensor, what: str) -> int:
     return code
 
 
-def _one_gpu(what: str, *tensors):
-    for t in tensors:
-        _lib.require_gpu(t, what)
-        if t.get_device() != tensors[0].get_device():
+def _one_gpu(what: str, first: torch.Tensor, *others):
+    device = first.get_device()
+    if device < 0:
+        _lib.require_gpu(first, what)
+    for t in others:
+        if t.get_device() != device:
+            _lib.require_gpu(t, what)
             raise ValueError(f"{what} needs every tensor on one GPU")
+
+
+def _once(backward):
+    """``once_differentiable`` where a graph of the backward pass is made (a second derivative raises); else
+    ``backward`` itself, which saves 12 us of host time per call."""
+    guarded = torch.autograd.function.once_differentiable(backward)
+    return lambda ctx, *grads: guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
 
 
 def order_tokens(ids: torch.Tensor, num_experts: int) -> TokenOrder:
@@ -85,10 +96,11 @@ def _check_order(what: str, order: TokenOrder):
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
-    """t [n, d] with unit column stride and, where 16 bytes divide a row, 16-byte aligned rows: a copy where
-    it has none (one pass over t, where unaligned kernels would take as long for each of a token's rows)."""
-    es, d = t.element_size(), t.shape[1]
-    if t.stride(1) != 1 or t.stride(0) < d or (d * es % 16 == 0 and (t.stride(0) * es % 16 or t.data_ptr() % 16)):
+    """t [n, d] with unit column stride, a row stride that the library takes and, where 16 bytes divide a row,
+    16-byte aligned rows: a copy where it has none (one pass over t, where unaligned kernels would take as
+    long for each of a token's rows)."""
+    es, d, ld = t.element_size(), t.shape[1], t.stride(0)
+    if t.stride(1) != 1 or ld < d or ld > MAX_ROW_STRIDE or (d * es % 16 == 0 and (ld * es % 16 or t.data_ptr() % 16)):
         t = t.clone(memory_format=torch.contiguous_format)
     return t
 
@@ -111,7 +123,7 @@ class _Dispatch(torch.autograd.Function):
         return rows
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, drows):
         tokens, k = ctx.order.position.shape
         drows = _contiguous(drows)
@@ -136,7 +148,7 @@ class _Combine(torch.autograd.Function):
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, dy):
         rows, weights = ctx.saved_tensors
         order = ctx.order
@@ -256,7 +268,7 @@ class _ExpertLinear(torch.autograd.Function):
         return _forward(x, weight, offsets)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, dy):
         x, weight, offsets = ctx.saved_tensors
         dy = _rows(dy)

@@ -195,6 +195,16 @@ def test_gradients_against_differences():
             assert abs(loss(t["x"], t["rows"], t["w"]) - base - grad.flatten()[i].item()) <= 1e-5
 
 
+def test_second_derivatives_are_refused():
+    from muon_sr_amd import combine_tokens, dispatch_tokens
+    s = make(9, 2, 3, 16, F32, F32, 9)
+    x, w = s["x"].requires_grad_(True), s["w"].requires_grad_(True)
+    y = combine_tokens(dispatch_tokens(x, s["order"]), w, s["order"])
+    (dx,) = torch.autograd.grad(y.square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        dx.sum().backward()
+
+
 def test_only_what_is_wanted():
     """Frozen weights, or frozen rows."""
     from muon_sr_amd import combine_tokens
