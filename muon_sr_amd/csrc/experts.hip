@@ -40,7 +40,9 @@ __device__ __forceinline__ int group_row(const ExpertArgs &a, int e) {
 
 constexpr uint32_t X_NONE = 0x80000000u;     // byte offset beyond every buffer resource
 constexpr int X_SORT = 512;                  // rows per expert from which the order of experts pays for finding it
-constexpr int X_GROUP = 4;                   // tile rows that share a walk over the columns
+// Tile rows that share a walk over the columns (forward, 16384 rows over 8 experts of 4096 x 4096, 256-wide tiles:
+// 555 us with 4, 531 with 8; the smaller tiles and the weight gradients lose 0 to 5 % with 8).
+constexpr int x_group(int kind, int T) { return kind != EX_WGRAD && T == 256 ? 8 : 4; }
 
 // 16 bytes per lane from byte `off` of a resource of `bytes` bytes at `base` (both wave-uniform; zeros from
 // beyond it) to 1 KiB of LDS.
@@ -141,7 +143,8 @@ __device__ __forceinline__ bool find_rows(const ExpertArgs &a, int v, int &e, in
     // tiles, whose operands its L2 shares
     const int per = total / NXCD;
     if (v < per * NXCD) v = (v % NXCD) * per + v / NXCD;
-    const int pg = X_GROUP * a.tiles_n, g = v / pg, first = X_GROUP * g, rows = min(X_GROUP, mt - first), r = v - g * pg;
+    constexpr int G = x_group(EX_FWD, T);
+    const int pg = G * a.tiles_n, g = v / pg, first = G * g, rows = min(G, mt - first), r = v - g * pg;
     int t = first + r % rows;
     nt = r / rows;
     for (int g0 = 0; g0 <= a.experts; g0 += 64) {
@@ -214,7 +217,8 @@ __global__ __launch_bounds__(64 * Shape<T>::NW, WGS) void experts_kernel(ExpertA
         e = a.by_size ? by_size(a, x / per) : x / per;
         const int v = (blockIdx.x % NXCD) * per + x % per;
         if (v >= tiles) return;
-        const int pg = X_GROUP * a.tiles_n, g = v / pg, first = X_GROUP * g, rows = min(X_GROUP, tiles_m - first), r = v - g * pg;
+        constexpr int G = x_group(EX_WGRAD, T);
+        const int pg = G * a.tiles_n, g = v / pg, first = G * g, rows = min(G, tiles_m - first), r = v - g * pg;
         m0 = (first + r % rows) * T;
         nt = r / rows;
         lo = __builtin_amdgcn_readfirstlane(group_row(a, e));
@@ -255,14 +259,14 @@ __global__ __launch_bounds__(64 * Shape<T>::NW, WGS) void experts_kernel(ExpertA
     // RPP y of a block, loaded ahead of the products
     constexpr int WC = S::TN / 8, RPP = 64 / WC, NP = 32 / RPP;   // chunks per row, rows per access, accesses per block
     constexpr int PRE = MODE >= 0 ? (FM < 2 ? FM : 2) : 0;
-    uint4 old[PRE ? PRE : 1][NP];
-    auto fetch = [&](uint4 (&c)[NP], int i, int ln) __attribute__((always_inline)) {
+    u32x4_t old[PRE ? PRE : 1][NP];
+    auto fetch = [&](u32x4_t (&c)[NP], int i, int ln) __attribute__((always_inline)) {
         const int n = n0 + wn * S::TN + 8 * (ln % WC);
 #pragma unroll
         for (int y = 0; y < NP; ++y) {
             const int m = m0 + wm * S::TM + 32 * i + ln / WC + RPP * y;
-            c[y] = make_uint4(0u, 0u, 0u, 0u);
-            if (m < M && n < a.N && !a.zero_init) c[y] = *reinterpret_cast<const uint4 *>(a.D + ((int64_t)e * M + m) * a.N + n);
+            c[y] = u32x4_t{0u, 0u, 0u, 0u};
+            if (m < M && n < a.N && !a.zero_init) c[y] = ld_nt4(a.D + ((int64_t)e * M + m) * a.N + n);
         }
     };
 
@@ -355,8 +359,11 @@ __global__ __launch_bounds__(64 * Shape<T>::NW, WGS) void experts_kernel(ExpertA
     }
 
     // ---------------- epilogue ----------------
-    // Each wave stages its sub-tile through LDS of its own, one 32-row block at a time (LDS accesses of one
-    // wave execute in order).  Lane l holds D[m = l % 32][n = 8 r + 4 (l / 32) + q] of each 32 x 32 block.
+    // Outputs and accumulators pass through once, non-temporal: kept out of the caches they leave room for the
+    // operands (weight gradients of 16411 rows over 64 experts of 1024 x 2048: 128 us with plain stores, 103 so;
+    // accumulated 171 and 154).  Each wave stages its sub-tile through LDS of its own, one 32-row block at a
+    // time (LDS accesses of one wave execute in order).  Lane l holds D[m = l % 32][n = 8 r + 4 (l / 32) + q] of each
+    // 32 x 32 block.
     constexpr int EP = S::TN + 8;                              // staging row pitch (16-byte rows)
     constexpr int PER = SP::BYTES / (32 * EP * 2);             // waves that stage in one variable
     static_assert(SP::BYTES == SQ::BYTES && PER > 0 && NW <= 4 * PER, "the staging fits the first two stages");
@@ -371,7 +378,7 @@ __global__ __launch_bounds__(64 * Shape<T>::NW, WGS) void experts_kernel(ExpertA
     const int n = n0 + wn * S::TN + 8 * cchk;
     wait_vm<0>();                                              // no load writes LDS any more
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    uint4 late[PRE && FM > PRE ? FM - PRE : 1][NP];
+    u32x4_t late[PRE && FM > PRE ? FM - PRE : 1][NP];
     if constexpr (PRE > 0 && FM > PRE) {
         fetch(late[0], 2, elane);
         fetch(late[1], 3, elane);
@@ -386,7 +393,7 @@ __global__ __launch_bounds__(64 * Shape<T>::NW, WGS) void experts_kernel(ExpertA
                     make_uint2(rne_bf16x2(acc[i][j][4 * r], acc[i][j][4 * r + 1]), rne_bf16x2(acc[i][j][4 * r + 2], acc[i][j][4 * r + 3]));
         const int mb = m0 + wm * S::TM + 32 * i + crow;
         if constexpr (MODE >= 0) {
-            uint4 (&c)[NP] = i < PRE ? old[i < PRE ? i : 0] : late[i < PRE ? 0 : i - PRE];
+            u32x4_t (&c)[NP] = i < PRE ? old[i < PRE ? i : 0] : late[i < PRE ? 0 : i - PRE];
 #pragma unroll
             for (int y = 0; y < NP; ++y) {
                 const int m = mb + RPP * y;
@@ -400,16 +407,16 @@ __global__ __launch_bounds__(64 * Shape<T>::NW, WGS) void experts_kernel(ExpertA
                     for (int q = 0; q < 4; ++q)
                         o[q] = pack2(sr_bf16(bf16_lo(cw[q]) + bf16_lo(gw[q]), rn[2 * q]),
                                      sr_bf16(bf16_hi(cw[q]) + bf16_hi(gw[q]), rn[2 * q + 1]));
-                    *reinterpret_cast<uint4 *>(a.D + o0) = make_uint4(o[0], o[1], o[2], o[3]);
+                    st_nt4(a.D + o0, u32x4_t{o[0], o[1], o[2], o[3]});
                 }
             }
         } else {
 #pragma unroll
             for (int y = 0; y < NP; ++y) {
                 const int m = mb + RPP * y;
-                const uint4 w = *reinterpret_cast<const uint4 *>(est(crow + RPP * y) + 8 * cchk);
+                const u32x4_t w = *reinterpret_cast<const u32x4_t *>(est(crow + RPP * y) + 8 * cchk);
                 const int64_t row = KIND == EX_WGRAD ? (int64_t)e * M + m : (int64_t)lo + m;
-                if (m < M && n < a.N) *reinterpret_cast<uint4 *>(a.D + row * a.N + n) = w;
+                if (m < M && n < a.N) st_nt4(a.D + row * a.N + n, w);
             }
         }
     };
