@@ -102,6 +102,7 @@ def _run(grads, outs, norm_type, max_norm, what):
     return norm
 
 
+@torch.no_grad()
 def grad_norm(grads, norm_type: float = 2.0) -> torch.Tensor:
     """The norm of all elements of ``grads`` (a tensor, or an iterable of bf16 and fp32 tensors on one
     GPU; ``norm_type`` 1, 2 or inf) as a 0-dim fp32 tensor on that GPU; 0 for an empty list."""
@@ -111,6 +112,7 @@ def grad_norm(grads, norm_type: float = 2.0) -> torch.Tensor:
     return _run(grads, None, norm_type, 0.0, "grad_norm")
 
 
+@torch.no_grad()
 def clip_grads(grads, max_norm: float, norm_type: float = 2.0, out=None) -> torch.Tensor:
     """Scales ``grads`` by min(1, max_norm / (norm + 1e-6)), in place or, with ``out`` (a tensor for each
     gradient: of its type, or bf16 for an fp32 one, say the ``.grad`` that an optimizer of bf16

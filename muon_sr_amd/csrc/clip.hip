@@ -266,29 +266,30 @@ static int clip_parts(const msr_clip_item *items, int32_t count) {
 }
 
 // Memory that one item writes may be touched by nothing else, but for its own gradient in place.
-static int clip_apart(const msr_clip_item *items, int32_t count, const float *norm_out, const void *ws, size_t ws_bytes) {
+static int clip_apart(const msr_clip_item *items, int32_t count, bool outs, const float *norm_out, const void *ws, size_t ws_bytes,
+                      const char *name) {
     std::vector<ItemRange> r;
     try {
         r.reserve(2 * (size_t)count + 2);
     } catch (const std::bad_alloc &) {
-        set_error("msr_clip_grads: out of host memory");
+        set_error("%s: out of host memory", name);
         return MSR_ERR_ARG;
     }
     for (int32_t i = 0; i < count; ++i) {
         const msr_clip_item &x = items[i];
         if (x.n == 0) continue;
         const size_t gb = (x.flags & MSR_CLIP_GRAD_F32 ? 4 : 2) * (size_t)x.n, ob = (x.flags & MSR_CLIP_OUT_F32 ? 4 : 2) * (size_t)x.n;
-        if (partial_overlap(x.grad, gb, x.out, ob)) {
-            set_error("msr_clip_grads: out of item %d overlaps its grad without being it", (int)i);
+        if (outs && partial_overlap(x.grad, gb, x.out, ob)) {
+            set_error("%s: out of item %d overlaps its grad without being it", name, (int)i);
             return MSR_ERR_OVERLAP;
         }
         r.push_back({(uintptr_t)x.grad, (uintptr_t)x.grad + gb, i, false});
-        r.push_back({(uintptr_t)x.out, (uintptr_t)x.out + ob, i, true});
+        if (outs) r.push_back({(uintptr_t)x.out, (uintptr_t)x.out + ob, i, true});
     }
     r.push_back({(uintptr_t)norm_out, (uintptr_t)norm_out + 4, count, true});
     r.push_back({(uintptr_t)ws, (uintptr_t)ws + ws_bytes, count + 1, true});
     if (ranges_conflict(r.data(), (int)r.size())) {
-        set_error("msr_clip_grads: an out (or the norm or the workspace) overlaps another item of the list");
+        set_error("%s: an out, the norm or the workspace overlaps another item of the list", name);
         return MSR_ERR_OVERLAP;
     }
     return MSR_OK;
@@ -338,7 +339,7 @@ static int clip_entry(const char *name, const msr_clip_item *items, int32_t coun
         set_error("%s: workspace of %zu bytes is smaller than the %zu required", name, workspace_bytes, need);
         return MSR_ERR_WORKSPACE;
     }
-    if (outs && (rc = clip_apart(items, count, norm_out, workspace, need))) return rc;
+    if ((rc = clip_apart(items, count, outs, norm_out, workspace, need, name))) return rc;
     double *const ws = static_cast<double *>(workspace);
     hipStream_t s = (hipStream_t)stream;
     if (norm == MSR_NORM_1) return clip_run<MSR_NORM_1>(items, count, outs, max_norm, norm_out, ws, s);

@@ -486,7 +486,7 @@ static int experts_launch(ExpertArgs a, const char *name, hipStream_t s) {
     // the rows fill
     const int64_t tiles = KIND == EX_WGRAD ? ((int64_t)((a.M + T - 1) / T) * a.tiles_n + NXCD - 1) / NXCD * NXCD * a.experts
                                            : ((int64_t)a.rows / T + a.experts + 1) * a.tiles_n;
-    if (tiles > INT32_MAX) { set_error("%s: too many tiles", name); return MSR_ERR_ARG; }
+    if (tiles > UINT32_MAX / (64 * Shape<256>::NW)) { set_error("%s: too many tiles for a launch (%lld)", name, (long long)tiles); return MSR_ERR_ARG; }
     if (T == 256) experts_launch_tile<KIND, MODE, 256>(a, (unsigned)tiles, s);
     else if (T == 128) experts_launch_tile<KIND, MODE, 128>(a, (unsigned)tiles, s);
     else experts_launch_tile<KIND, MODE, 64>(a, (unsigned)tiles, s);

@@ -487,7 +487,7 @@ extern "C" {
 
 int msr_order_workspace_bytes(int64_t tokens, int32_t k, int32_t experts, size_t *bytes) {
     if (!bytes || tokens < 0 || k < 1 || experts < 1 || experts > MSR_EXPERTS_MAX || tokens >= (int64_t(1) << 30) / k) {
-        set_error("msr_order_workspace_bytes: bad arguments");
+        set_error("msr_order_workspace_bytes: bad arguments (tokens %lld, k %d, %d experts)", (long long)tokens, (int)k, (int)experts);
         return MSR_ERR_ARG;
     }
     const OrderPlan p = order_plan(tokens * k);

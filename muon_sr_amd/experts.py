@@ -76,10 +76,10 @@ def order_tokens(ids: torch.Tensor, num_experts: int) -> TokenOrder:
         raise ValueError(f"order_tokens needs ids of shape [tokens, k], got {tuple(ids.shape)}")
     ids = ids.contiguous()
     tokens, k = ids.shape
-    made = lambda *shape: torch.empty(shape, dtype=torch.int32, device=ids.device)  # noqa: E731
-    order = TokenOrder(made(num_experts + 1), made(tokens, k), made(tokens * k))
     L, size = _lib.lib(), ctypes.c_size_t()
     _lib.check(L.msr_order_workspace_bytes(tokens, k, num_experts, ctypes.byref(size)), "msr_order_workspace_bytes")
+    made = lambda *shape: torch.empty(shape, dtype=torch.int32, device=ids.device)  # noqa: E731
+    order = TokenOrder(made(num_experts + 1), made(tokens, k), made(tokens * k))
     ws = made(size.value // 4) if size.value else None
     _lib.check(L.msr_order_tokens(ids.data_ptr(), int(ids.dtype == torch.int64), tokens, k, num_experts,
                                   order.offsets.data_ptr(), order.position.data_ptr(), order.source.data_ptr(),

@@ -221,5 +221,13 @@ def test_refusals():
         with pytest.raises(_lib.MuonSRLibraryError, match="overlap"):
             clip_grads(grads, 1e-3, out=out)
     same(g, kept)
+    sparse = torch.sparse_coo_tensor([[0, 2]], torch.ones(2, device=DEV, dtype=BF16), (4,))
+    for call in (lambda: grad_norm([sparse]), lambda: clip_grads([g, sparse], 1.0)):
+        with pytest.raises(RuntimeError):
+            call()
+    same(g, kept)
+    # gradients that require gradients themselves (a graph of the backward pass was made)
+    h = g.clone().requires_grad_(True)
+    assert clip_grads([h], 1e-3).item() == grad_norm([kept]).item() and not torch.equal(h, kept)
     # reading the same memory twice is no conflict
     assert abs(grad_norm([g, g]).item() - math.sqrt(2) * norm64([g], 2.0)) <= 2.0 ** -22 * norm64([g], 2.0)

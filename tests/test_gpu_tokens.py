@@ -109,7 +109,8 @@ def all_passes(s, x=None, rows=None, dy=None, drows=None):
 @pytest.mark.parametrize("wdtype", [BF16, F32], ids=["wbf16", "wfp32"])
 @pytest.mark.parametrize("tokens,k,E,d", [(1, 1, 1, 1), (1, 2, 4, 8), (7, 2, 8, 384), (33, 3, 5, 100), (130, 1, 64, 513),
                                           (64, 8, 16, 1400), (513, 5, 40, 2048), (5, 2, 3, 8200), (9000, 2, 16, 48),
-                                          (70, 11, 13, 264), (40, 4, 6, 4098)])
+                                          (70, 11, 13, 264), (40, 4, 6, 4098),
+                                          (21, 70, 90, 136), (5, 129, 40, 600)])
 def test_passes(tokens, k, E, d, dtype, wdtype):
     s = make(tokens, k, E, d, dtype, wdtype, tokens + d)
     o = s["order"]
@@ -245,6 +246,6 @@ def test_refusals():
                  lambda: dispatch_tokens(s["x"], (o.offsets.long(), o.position, o.source))):
         with pytest.raises(ValueError):
             call()
-    for experts in (0, 1025):
+    for experts in (-1, 0, 1025):
         with pytest.raises(_lib.MuonSRLibraryError, match="experts|bad arguments"):
             order_tokens(ids, experts)

@@ -41,6 +41,7 @@ def test_clip(lib):
     assert clip(lib, [(A, A, 100, 1)]) == OVERLAP                                     # fp32 grad, bf16 out in its place
     assert clip(lib, [(A, A, 100, 0), (A + 100, B, 100, 0)]) == OVERLAP               # an out in another's grad
     assert clip(lib, [(A, C, 100, 0), (B, C + 100, 100, 0)]) == OVERLAP
+    assert lib.msr_grad_norm(*items((A, 0, 100, 0)), 2, A + 40, W, 1 << 20, None) == OVERLAP
     assert clip(lib, [(A, B, 100, 0)], out=B + 8) == OVERLAP and clip(lib, [(A, W, 100, 0)]) == OVERLAP
 
 
@@ -86,6 +87,7 @@ def test_products(lib):
     assert fwd(rows=-1) == ARG and fwd(rows=1 << 30) == ARG and fwd(E_=0) == ARG and fwd(E_=1025) == ARG
     assert fwd(i=60, ldx=64) == ARG and fwd(o=33) == ARG and fwd(i=1 << 16, o=1 << 15, ldx=1 << 16) == ARG
     assert fwd(ldx=63) == ARG and fwd(ldx=1 << 22) == ARG and fwd(x=None) == ARG and fwd(off=None) == ARG
+    assert fwd(y=1 << 50, rows=(1 << 30) - 1, o=1 << 14) == ARG and b"tiles" in lib.msr_last_error()
     assert fwd(x=A + 8) == ALIGN and fwd(ldx=68) == ALIGN and fwd(off=D + 2) == ALIGN
     assert fwd(y=A + 128) == OVERLAP and fwd(y=B + 16) == OVERLAP and fwd(y=D - 64) == OVERLAP
     assert lib.msr_experts_dgrad(A, 31, B, C, D, 100, 4, 64, 32, None) == ARG
