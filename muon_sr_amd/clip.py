@@ -14,7 +14,9 @@ from __future__ import annotations
 
 import ctypes
 import math
+import operator
 import struct
+from array import array
 
 import torch
 
@@ -24,6 +26,7 @@ __all__ = ["grad_norm", "clip_grads", "clip_grad_norm_"]
 
 _NORMS = {1.0: _lib.NORM_1, 2.0: _lib.NORM_2, math.inf: _lib.NORM_INF}
 _pack_item = struct.Struct("=QQqii").pack   # msr_clip_item
+_T, _dtype = torch.Tensor, operator.attrgetter("dtype")
 
 
 def _norm_code(norm_type) -> int:
@@ -52,20 +55,33 @@ def _check(t: torch.Tensor, device, what: str):
         raise ValueError(f"{what} needs every gradient on one GPU")
 
 
-def _run(grads, outs, norm_type, max_norm, what):
-    """The norm of ``grads`` and, with ``outs``, the clipped gradients written there."""
-    code = _norm_code(norm_type)
-    bf16, f32 = torch.bfloat16, torch.float32
-    items, keep, back, device = [], [], [], grads[0].get_device()
+def _plain(tensors, device):
+    """Contiguous bf16 tensors on that GPU."""
+    return set(map(_T.get_device, tensors)) == {device} and set(map(_dtype, tensors)) == {torch.bfloat16} and \
+        all(map(_T.is_contiguous, tensors))
+
+
+def _items(grads, outs, device, what):
+    """The list's msr_clip_items, what has to live until they are used, and the outs to copy results to."""
+    # The common case by maps over the list: host time bounds many small tensors (73 gradients, out of place: 98 us
+    # a call with the loop below, 52 so).
+    if device >= 0 and _plain(grads, device) and (outs is None or outs is grads or (
+            _plain(outs, device) and all(map(_T.is_same_size, grads, outs)))):
+        a = array("q", bytes(32 * len(grads)))
+        a[0::4] = array("q", map(_T.data_ptr, grads))
+        if outs is not None:
+            a[1::4] = a[0::4] if outs is grads else array("q", map(_T.data_ptr, outs))
+        a[2::4] = array("q", map(_T.numel, grads))
+        return a.tobytes(), (), ()
+    with torch.no_grad():
+        return _mixed_items(grads, outs, device, what)
+
+
+def _mixed_items(grads, outs, device, what):
+    f32 = torch.float32
+    items, keep, back = [], [], []
     for i, g in enumerate(grads):
         o = None if outs is None else outs[i]
-        # the common case by as few calls as will do (host time bounds many small tensors: 73 tensors, out of
-        # place, 98 us with every check in order, 62 so)
-        if (g.dtype is bf16 and g.get_device() == device >= 0 and g.is_contiguous() and
-                (o is g or o is None or (o.dtype is bf16 and o.is_same_size(g) and o.get_device() == device and o.is_contiguous()))):
-            at = g.data_ptr()
-            items.append(_pack_item(at, at if o is g else 0 if o is None else o.data_ptr(), g.numel(), 0, 0))
-            continue
         _check(g, device, what)
         flags = _lib.CLIP_GRAD_F32 if g.dtype is f32 else 0
         src, dst = g, o
@@ -87,22 +103,30 @@ def _run(grads, outs, norm_type, max_norm, what):
         if src is not g:
             keep.append(src)
         items.append(_pack_item(src.data_ptr(), dst.data_ptr() if dst is not None else 0, src.numel(), flags, 0))
-    norm = torch.empty((), dtype=f32, device=torch.device("cuda", device))
-    L, arr, n, size = _lib.lib(), b"".join(items), len(items), ctypes.c_size_t()
-    _lib.check(L.msr_grad_norm_workspace_bytes(arr, n, ctypes.byref(size)), "msr_grad_norm_workspace_bytes")
+    return b"".join(items), keep, back
+
+
+def _run(grads, outs, norm_type, max_norm, what):
+    """The norm of ``grads`` and, with ``outs``, the clipped gradients written there."""
+    code, device, n = _norm_code(norm_type), grads[0].get_device(), len(grads)
+    items, keep, back = _items(grads, outs, device, what)
+    norm = torch.empty((), dtype=torch.float32, device=torch.device("cuda", device))
+    L, size = _lib.lib(), ctypes.c_size_t()
+    _lib.check(L.msr_grad_norm_workspace_bytes(items, n, ctypes.byref(size)), "msr_grad_norm_workspace_bytes")
     ws = torch.empty(max(8, size.value), dtype=torch.uint8, device=norm.device)
     stream = _lib.stream_of(norm)
     if outs is None:
-        _lib.check(L.msr_grad_norm(arr, n, code, norm.data_ptr(), ws.data_ptr(), ws.numel(), stream), "msr_grad_norm")
+        _lib.check(L.msr_grad_norm(items, n, code, norm.data_ptr(), ws.data_ptr(), ws.numel(), stream), "msr_grad_norm")
     else:
-        _lib.check(L.msr_clip_grads(arr, n, code, max_norm, norm.data_ptr(), ws.data_ptr(), ws.numel(), stream),
+        _lib.check(L.msr_clip_grads(items, n, code, max_norm, norm.data_ptr(), ws.data_ptr(), ws.numel(), stream),
                    "msr_clip_grads")
-    for o, dst in back:
-        o.copy_(dst)
+    if back:
+        with torch.no_grad():
+            for o, dst in back:
+                o.copy_(dst)
     return norm
 
 
-@torch.no_grad()
 def grad_norm(grads, norm_type: float = 2.0) -> torch.Tensor:
     """The norm of all elements of ``grads`` (a tensor, or an iterable of bf16 and fp32 tensors on one
     GPU; ``norm_type`` 1, 2 or inf) as a 0-dim fp32 tensor on that GPU; 0 for an empty list."""
@@ -112,7 +136,6 @@ def grad_norm(grads, norm_type: float = 2.0) -> torch.Tensor:
     return _run(grads, None, norm_type, 0.0, "grad_norm")
 
 
-@torch.no_grad()
 def clip_grads(grads, max_norm: float, norm_type: float = 2.0, out=None) -> torch.Tensor:
     """Scales ``grads`` by min(1, max_norm / (norm + 1e-6)), in place or, with ``out`` (a tensor for each
     gradient: of its type, or bf16 for an fp32 one, say the ``.grad`` that an optimizer of bf16
@@ -128,7 +151,6 @@ def clip_grads(grads, max_norm: float, norm_type: float = 2.0, out=None) -> torc
     return _run(grads, outs, norm_type, float(max_norm), "clip_grads")
 
 
-@torch.no_grad()
 def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_if_nonfinite: bool = False) -> torch.Tensor:
     """``torch.nn.utils.clip_grad_norm_`` for bf16 and fp32 gradients on one GPU: clips the ``.grad`` of
     ``parameters`` in place and returns their norm.  With ``error_if_nonfinite`` the norm is waited for, and
