@@ -449,7 +449,8 @@ int msr_combine_grad(const void *dy, int64_t lddy, const void *rows, const void 
  * The experts' products over rows sorted by expert (offsets: device int32
  * [experts + 1], offsets[0] = 0, non-decreasing, as msr_order_tokens writes it;
  * read on the GPU only, and clamped to [0, rows]).  No counterpart in the
- * reference.  bf16 operands, fp32 accumulation, one rounding:
+ * reference.  bf16 operands, fp32 accumulation, one rounding (the order of the sums, and so their last bits, may
+ * depend on the sizes of the call; the same call gives the same bits):
  *   msr_experts_forward          y[r] = W[e] x[r]            for the rows r of expert e
  *   msr_experts_dgrad            dx[r] = W[e]^T dy[r]
  *   msr_experts_wgrad            dw[e] = sum_r dy[r] x[r]^T  (0 for an expert without rows)
@@ -543,9 +544,10 @@ int msr_tile_gemm(int32_t product, int32_t tile, int32_t stages, const uint16_t 
                   int64_t batch, int64_t m, int64_t n, int64_t k, float alpha, float beta, float diag,
                   const float *rvec, float *resid, uint32_t seed, int32_t noise_mode, msr_stream_t stream);
 
-/* Host only: the tile (64, 128 or 256) that an experts' product of these sizes takes; product 0 forward, 1 dgrad,
- * 2 wgrad, 3 wgrad_sr_accum.  Test support. */
-int msr_experts_tile(int32_t product, int64_t rows, int32_t experts, int64_t in_features, int64_t out_features, int32_t *tile);
+/* Host only: the tile (64, 128 or 256) that an experts' product of these sizes takes, and whether it splits K
+ * between groups of waves; product 0 forward, 1 dgrad, 2 wgrad, 3 wgrad_sr_accum.  Test support. */
+int msr_experts_tile(int32_t product, int64_t rows, int32_t experts, int64_t in_features, int64_t out_features, int32_t *tile,
+                     int32_t *split);
 
 /* Batched bf16 GEMM  D[b] = alpha * P[b] Q[b]^T + beta * C[b] + diag * I  (fp32 accumulate, RNE
  * bf16 out; the diag term is added where m == n).

@@ -120,7 +120,7 @@ SIGNATURES = {
     "msr_experts_wgrad": (ctypes.c_int, [_P, _P, _I64, _P, _I64, _P, _I64, _I32, _I64, _I64, _P]),
     "msr_experts_wgrad_sr_accum": (ctypes.c_int, [_P, _P, _I64, _P, _I64, _P, _I64, _I32, _I64, _I64, _U32, _I32, _I32, _P,
                                                   _P]),
-    "msr_experts_tile": (ctypes.c_int, [_I32, _I64, _I32, _I64, _I64, ctypes.POINTER(_I32)]),
+    "msr_experts_tile": (ctypes.c_int, [_I32, _I64, _I32, _I64, _I64, ctypes.POINTER(_I32), ctypes.POINTER(_I32)]),
     "msr_noise_fill": (ctypes.c_int, [_P, _I64, _I64, _U32, _U32, _I32, _P]),
     "msr_stream_probe8": (ctypes.c_int, [_P, _P, _P, _P, _P, _P, _I64, _I32, _I32, _P]),
     "msr_quantize": (ctypes.c_int, [_P, _P, _I64, _P, _I32, _P, _P]),

@@ -191,8 +191,9 @@ struct Shape {
 };
 
 // BK: k per slab; S: LDS stages; WGS: work-groups per CU times waves per SIMD that the registers leave room for.
-template <int KIND, int MODE, int T, int BK, int S_, int WGS>
-__global__ __launch_bounds__(64 * Shape<T>::NW, WGS) void experts_kernel(ExpertArgs a) {
+// KG: groups of waves that take consecutive shares of K each, joined through LDS in their order at the end.
+template <int KIND, int MODE, int T, int BK, int S_, int WGS, int KG = 1>
+__global__ __launch_bounds__(64 * Shape<T>::NW * KG, WGS) void experts_kernel(ExpertArgs a) {
     using S = Shape<T>;
     constexpr int NW = S::NW, FM = S::FM, FN = S::FN;
     constexpr bool PK = KIND == EX_WGRAD, QK = KIND != EX_FWD;
@@ -201,12 +202,14 @@ __global__ __launch_bounds__(64 * Shape<T>::NW, WGS) void experts_kernel(ExpertA
     constexpr int NS = BK / 16, LPS = SP::LOADS + SQ::LOADS;   // substeps of a slab, a wave's loads for it
     // one variable per stage and operand, so that the compiler knows that fragment reads of one
     // stage do not alias the loads into the others
-    __shared__ __attribute__((aligned(1024))) char p_0[SP::BYTES], p_1[SP::BYTES], q_0[SQ::BYTES], q_1[SQ::BYTES];
-    __shared__ __attribute__((aligned(1024))) char p_2[S_ > 2 ? SP::BYTES : 16], q_2[S_ > 2 ? SQ::BYTES : 16];
-    __shared__ __attribute__((aligned(1024))) char p_3[S_ > 3 ? SP::BYTES : 16], q_3[S_ > 3 ? SQ::BYTES : 16];
+    constexpr int PB = SP::BYTES * KG, QB = SQ::BYTES * KG;
+    __shared__ __attribute__((aligned(1024))) char p_0[PB], p_1[PB], q_0[QB], q_1[QB];
+    __shared__ __attribute__((aligned(1024))) char p_2[S_ > 2 ? PB : 16], q_2[S_ > 2 ? QB : 16];
+    __shared__ __attribute__((aligned(1024))) char p_3[S_ > 3 ? PB : 16], q_3[S_ > 3 ? QB : 16];
 
     const int tid = threadIdx.x, lane = tid & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave / S::WN, wn = wave % S::WN;
+    const int wid = __builtin_amdgcn_readfirstlane(tid >> 6), kg = KG > 1 ? wid / NW : 0, wave = KG > 1 ? wid % NW : wid;
+    const int wm = wave / S::WN, wn = wave % S::WN;
     int e = 0, lo = 0, hi = 0, m0 = 0, nt = 0, M, K;
     if constexpr (KIND == EX_WGRAD) {
         // Consecutive work-groups go to the 8 XCDs in turn: each XCD takes a contiguous eighth of every
@@ -272,15 +275,17 @@ __global__ __launch_bounds__(64 * Shape<T>::NW, WGS) void experts_kernel(ExpertA
 
     auto lds_p = [&](auto ST) __attribute__((always_inline)) -> char * {
         constexpr int st = decltype(ST)::value;
-        return st == 0 ? p_0 : st == 1 ? p_1 : st == 2 ? p_2 : p_3;
+        return (st == 0 ? p_0 : st == 1 ? p_1 : st == 2 ? p_2 : p_3) + kg * SP::BYTES;
     };
     auto lds_q = [&](auto ST) __attribute__((always_inline)) -> char * {
         constexpr int st = decltype(ST)::value;
-        return st == 0 ? q_0 : st == 1 ? q_1 : st == 2 ? q_2 : q_3;
+        return (st == 0 ? q_0 : st == 1 ? q_1 : st == 2 ? q_2 : q_3) + kg * SQ::BYTES;
     };
+    // this group's share of K: `slabs` of them from kb on
+    const int slabs = ((K + BK - 1) / BK + KG - 1) / KG, kb = kg * slabs * BK, kend = min(K, kb + slabs * BK);
     auto load = [&](auto ST, int k0) __attribute__((always_inline)) {
-        sp.load(lds_p(ST), wave, P, a.ldp, mrows, M - m0, k0, K);
-        sq.load(lds_q(ST), wave, Q, a.ldq, nrows, a.N - n0, k0, K);
+        sp.load(lds_p(ST), wave, P, a.ldp, mrows, M - m0, kb + k0, kend);
+        sq.load(lds_q(ST), wave, Q, a.ldq, nrows, a.N - n0, kb + k0, kend);
     };
     bf16x8_t fp[2][FM], fq[2][FN];
     auto read = [&](auto ST, int ks, int b) __attribute__((always_inline)) {
@@ -321,7 +326,7 @@ __global__ __launch_bounds__(64 * Shape<T>::NW, WGS) void experts_kernel(ExpertA
     if constexpr (PRE > 1) fetch(old[1], 1, lane);
     if (K > 0) {
         // the first slab's stage is the one from which the last slab is in stage S - 1
-        const int KT = (K + BK - 1) / BK, r = KT % S_;
+        const int r = slabs % S_;
         auto begin = [&](auto ST) __attribute__((always_inline)) {
             constexpr int st = decltype(ST)::value;
             load(std::integral_constant<int, st>{}, 0);
@@ -350,7 +355,7 @@ __global__ __launch_bounds__(64 * Shape<T>::NW, WGS) void experts_kernel(ExpertA
         }
         if (r >= 1) { slab(std::integral_constant<int, S_ - 1>{}, k0); k0 += BK; }
 #pragma clang loop unroll(disable)
-        for (; k0 < K; k0 += S_ * BK) {
+        for (; k0 < slabs * BK; k0 += S_ * BK) {
             slab(I0{}, k0);
             slab(I1{}, k0 + BK);
             if constexpr (S_ > 2) slab(I2{}, k0 + 2 * BK);
@@ -365,10 +370,10 @@ __global__ __launch_bounds__(64 * Shape<T>::NW, WGS) void experts_kernel(ExpertA
     // time (LDS accesses of one wave execute in order).  Lane l holds D[m = l % 32][n = 8 r + 4 (l / 32) + q] of each
     // 32 x 32 block.
     constexpr int EP = S::TN + 8;                              // staging row pitch (16-byte rows)
-    constexpr int PER = SP::BYTES / (32 * EP * 2);             // waves that stage in one variable
+    constexpr int PER = PB / (32 * EP * 2);                    // waves that stage in one variable
     static_assert(SP::BYTES == SQ::BYTES && PER > 0 && NW <= 4 * PER, "the staging fits the first two stages");
     const int sv = wave / PER;
-    char *const wst = (sv == 0 ? p_0 : sv == 1 ? q_0 : sv == 2 ? p_1 : q_1) + (wave % PER) * (32 * EP * 2);
+    char *const wst = (KG > 1 ? p_1 : sv == 0 ? p_0 : sv == 1 ? q_0 : sv == 2 ? p_1 : q_1) + (wave % PER) * (32 * EP * 2);
     auto est = [&](int row) __attribute__((always_inline)) { return reinterpret_cast<uint16_t *>(wst + row * (EP * 2)); };
     // lane indices from an opaque copy of the thread index: the addresses are formed here, not kept
     // through the K loop
@@ -378,6 +383,25 @@ __global__ __launch_bounds__(64 * Shape<T>::NW, WGS) void experts_kernel(ExpertA
     const int n = n0 + wn * S::TN + 8 * cchk;
     wait_vm<0>();                                              // no load writes LDS any more
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if constexpr (KG > 1) {
+        // groups 1, 2, .. leave their sums in the first stage (16 floats per lane, 16 KiB per group), group 0 adds
+        // them in that order and stores
+        static_assert(T == 64 && PB >= KG * 8192 && PER >= NW, "the sums fit the first stage, the staging the second");
+        auto part = [&](int g, int i) __attribute__((always_inline)) {
+            char *const b = (g <= KG / 2 ? p_0 : q_0) + ((g - 1) % (KG / 2)) * 16384;
+            return reinterpret_cast<float *>(b) + (i * NW + wave) * 64 + lane;
+        };
+        if (kg > 0) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) *part(kg, i) = acc[0][0][i];
+        }
+        __syncthreads();
+        if (kg > 0) return;
+#pragma unroll
+        for (int g = 1; g < KG; ++g)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[0][0][i] = acc[0][0][i] + *part(g, i);
+    }
     u32x4_t late[PRE && FM > PRE ? FM - PRE : 1][NP];
     if constexpr (PRE > 0 && FM > PRE) {
         fetch(late[0], 2, elane);
@@ -429,7 +453,8 @@ __global__ __launch_bounds__(64 * Shape<T>::NW, WGS) void experts_kernel(ExpertA
 }
 
 // The slabs' k, the LDS stages and the work-groups per CU that a tile runs with.  Times of 8192 and 16384 rows
-// over 8 experts of 14336 x 4096 and 4096 x 4096, of 16411 and 32768 over 64 of 1024 and 1408 x 2048 (us):
+// over 8 experts of 14336 x 4096 and 4096 x 4096, of 16411 and 32768 over 64 of 1024 and 1408 x 2048 (us, with
+// outputs stored through the caches):
 //            256: (64, 2)  (32, 4)      128: (64, 2)  (32, 3)  (32, 4)
 //   forward   950 561 123 251   974 577 124 254     1127 640 122 271   1357 725 130 293   1309 720 131 294
 //   dgrad    1120 546 110 242  1070 527 110 238     1216 634 130 276   1420 688 125 286   1442 696 133 295
@@ -437,59 +462,87 @@ __global__ __launch_bounds__(64 * Shape<T>::NW, WGS) void experts_kernel(ExpertA
 //   accum    1130 542 188 378  1096 514 182 364     1356 664 198 438   1205 595 169 335   1286 622 182 378
 // Half-length slabs cost barriers and row-major reads of 64-byte rows, which the forward product pays most for;
 // more of them in flight hide the latency of operands that K-major products load in shorter pieces.
-template <int KIND, int T>
+// SPLIT: few tiles over a long K, a work-group to a CU: its time is the latency of one slab after the other, which
+// 2 groups with 4 stages (forward) or 4 groups with 2 (dgrad) shorten:
+//   rows x experts, out x in          forward: no split, (2, 4), (4, 2)      dgrad
+//   300 x 4,  1024 x 8192 (8192 x 1024)        62  26  34                    62  50  39
+//   1 x 1,    4096 x 4096                      32  15  18                    32  24  19
+//   64 x 8,   (4096 x 1024)                                                  34  28  23
+//   16 x 8,   4096 x 4096 (272 tiles)          35  36  41                    36  52  48
+template <int KIND, int T, bool SPLIT>
 struct Ring {
     static constexpr bool FINE = KIND != EX_FWD && T >= 128;
-    static constexpr int BK = FINE ? 32 : 64, S = FINE ? (T == 256 ? 4 : 3) : 2, WGS = FINE && T == 128 ? 3 : 2;
+    static constexpr int KG = !SPLIT ? 1 : KIND == EX_FWD ? 2 : 4;
+    static constexpr int BK = FINE ? 32 : 64, S = KG == 2 ? 4 : FINE ? (T == 256 ? 4 : 3) : 2;
+    static constexpr int WGS = KG == 4 ? 4 : FINE && T == 128 ? 3 : 2;
 };
 
 // Estimated time (us) of a call in tiles of T, from times per slab of 64 k of a tile: p with every CU busy, u for a
-// tile that has its CU to itself; and o for its start and end.  Fitted to the times above and of fewer rows:
+// tile that has its CU to itself; and o for its start and end.  Fitted to the forward and dgrad times above and to
+// (stored and accumulated weight gradients with non-temporal outputs):
 //   rows x experts, weights      forward 256 128 64   dgrad 256 128 64   wgrad 256 128 64   accum 256 128 64
-//   8192 x 8,    1536 x 384            17  20  27           33  20  23         44  27  25         51  31  26
-//   4096 x 128,   768 x 2048          126 108 107          116  96  96         99 101 155        194 159 206
-//   512 x 64,    1024 x 2048           49  41  40           48  44  42         61  43  73        124 100 128
+//   8192 x 8,    1536 x 384            17  20  27           33  20  23         39  25  23         47  29  25
+//   4096 x 128,   768 x 2048          126 108 107          116  96  96         83  71 114        193 147 206
+//   512 x 64,    1024 x 2048           49  41  40           48  44  42         54  42  67        131  96 131
 //   61 x 8,       512 x 256           9.1 5.8 4.7         13.6 7.9 5.7        6.2 4.0 4.0       13.0 6.6 4.2
-//   16 x 8,      4096 x 4096           72  45  36           72  40  36         50  45  69         98  83  94
+//   16411 x 64,  1024 x 2048                                                  101  98 154        165 155 214
+//   65536 x 64,  1024 x 2048          307 355 533          305 380 584        282 329 587        343 372 623
 // A group is taken to end in the middle of its last tile, and the largest expert to have twice the average rows.
-static float experts_cost(int kind, bool accum, int T, const ExpertArgs &a) {
+static float experts_cost(int kind, bool accum, int T, bool split, const ExpertArgs &a) {
     const int i = T == 256 ? 2 : T == 128 ? 1 : 0;
     constexpr float ROWS_P[3] = {0.25f, 0.62f, 1.9f}, U[3] = {0.5f, 0.75f, 1.2f}, ROWS_O[3] = {1.5f, 3.0f, 5.0f};
-    constexpr float W_P[3] = {0.215f, 0.54f, 1.75f}, W_O[3] = {0.6f, 1.9f, 8.0f}, ACC_O[3] = {1.0f, 3.1f, 15.0f};
+    constexpr float W_P[3] = {0.215f, 0.54f, 1.75f}, W_O[3] = {0.4f, 0.8f, 5.0f}, ACC_O[3] = {0.9f, 2.45f, 13.0f};
     const float tn = (float)((a.N + T - 1) / T);
     if (kind == EX_WGRAD) {
         const float n = (float)((a.M + T - 1) / T) * tn * (float)a.experts / 256.0f;   // tiles per CU
         const float ks = (float)a.rows / (float)a.experts / 64.0f + 0.5f, o = accum ? ACC_O[i] : W_O[i];
         return std::max(n * (ks * W_P[i] + o), 2.0f * ks * U[i] + o);
     }
-    const float n = ((float)a.rows / (float)T + 0.5f * (float)std::min(a.experts, a.rows)) * tn / 256.0f;
-    return (float)a.K / 64.0f * std::max(n * ROWS_P[i], U[i]) + std::max(n, 1.0f) * ROWS_O[i];
+    const float n = ((float)a.rows / (float)T + 0.5f * (float)std::min(a.experts, a.rows)) * tn / 256.0f, ks = (float)a.K / 64.0f;
+    if (split) return ceilf(n) * (ks * (kind == EX_FWD ? 0.22f : 0.33f) + 4.0f);
+    return ks * std::max(n * ROWS_P[i], U[i]) + std::max(n, 1.0f) * ROWS_O[i];
 }
 
-static int experts_tile(int kind, bool accum, const ExpertArgs &a) {
-    const float c64 = experts_cost(kind, accum, 64, a), c128 = experts_cost(kind, accum, 128, a), c256 = experts_cost(kind, accum, 256, a);
-    return c256 <= c128 && c256 <= c64 ? 256 : c128 <= c64 ? 128 : 64;
+struct ExpertPlan {
+    int tile;
+    bool split;
+};
+static ExpertPlan experts_plan(int kind, bool accum, const ExpertArgs &a) {
+    ExpertPlan best{64, false};
+    float least = experts_cost(kind, accum, 64, false, a);
+    for (const ExpertPlan p : {ExpertPlan{128, false}, ExpertPlan{256, false}, ExpertPlan{64, true}}) {
+        if (p.split && kind == EX_WGRAD) continue;
+        const float c = experts_cost(kind, accum, p.tile, p.split, a);
+        if (c < least) {
+            least = c;
+            best = p;
+        }
+    }
+    return best;
 }
 
-template <int KIND, int MODE, int T>
+template <int KIND, int MODE, int T, bool SPLIT>
 static void experts_launch_tile(const ExpertArgs &a, unsigned grid, hipStream_t s) {
-    using R = Ring<KIND, T>;
-    hipLaunchKernelGGL((experts_kernel<KIND, MODE, T, R::BK, R::S, R::WGS>), dim3(grid), dim3(64 * Shape<T>::NW), 0, s, a);
+    using R = Ring<KIND, T, SPLIT>;
+    hipLaunchKernelGGL((experts_kernel<KIND, MODE, T, R::BK, R::S, R::WGS, R::KG>), dim3(grid), dim3(64 * Shape<T>::NW * R::KG), 0, s, a);
 }
 
 template <int KIND, int MODE>
 static int experts_launch(ExpertArgs a, const char *name, hipStream_t s) {
-    const int T = experts_tile(KIND, MODE >= 0, a);
+    const ExpertPlan plan = experts_plan(KIND, MODE >= 0, a);
+    const int T = plan.tile;
     a.tiles_n = (a.N + T - 1) / T;
     a.by_size = a.experts <= 64 && a.rows / a.experts >= X_SORT;
     // wgrad: 8 shares of every expert's tiles; the row products: at most one part tile per group more than
     // the rows fill
     const int64_t tiles = KIND == EX_WGRAD ? ((int64_t)((a.M + T - 1) / T) * a.tiles_n + NXCD - 1) / NXCD * NXCD * a.experts
                                            : ((int64_t)a.rows / T + a.experts + 1) * a.tiles_n;
-    if (tiles > UINT32_MAX / (64 * Shape<256>::NW)) { set_error("%s: too many tiles for a launch (%lld)", name, (long long)tiles); return MSR_ERR_ARG; }
-    if (T == 256) experts_launch_tile<KIND, MODE, 256>(a, (unsigned)tiles, s);
-    else if (T == 128) experts_launch_tile<KIND, MODE, 128>(a, (unsigned)tiles, s);
-    else experts_launch_tile<KIND, MODE, 64>(a, (unsigned)tiles, s);
+    constexpr int MOST = 64 * Shape<64>::NW * 4;   // threads of a work-group; a launch has fewer than 2^32
+    if (tiles > UINT32_MAX / MOST) { set_error("%s: too many tiles for a launch (%lld)", name, (long long)tiles); return MSR_ERR_ARG; }
+    if (T == 256) experts_launch_tile<KIND, MODE, 256, false>(a, (unsigned)tiles, s);
+    else if (T == 128) experts_launch_tile<KIND, MODE, 128, false>(a, (unsigned)tiles, s);
+    else if (!plan.split) experts_launch_tile<KIND, MODE, 64, false>(a, (unsigned)tiles, s);
+    else if constexpr (KIND != EX_WGRAD) experts_launch_tile<KIND, MODE, 64, true>(a, (unsigned)tiles, s);
     return check_launch(name);
 }
 
@@ -571,16 +624,19 @@ using namespace msr;
 
 extern "C" {
 
-int msr_experts_tile(int32_t product, int64_t rows, int32_t experts, int64_t in_features, int64_t out_features, int32_t *tile) {
+int msr_experts_tile(int32_t product, int64_t rows, int32_t experts, int64_t in_features, int64_t out_features, int32_t *tile,
+                     int32_t *split) {
     const int rc = experts_check("msr_experts_tile", rows, experts, in_features, out_features);
     if (rc) return rc;
-    if (product < 0 || product > 3 || !tile) { set_error("msr_experts_tile: bad arguments"); return MSR_ERR_ARG; }
+    if (product < 0 || product > 3 || !tile || !split) { set_error("msr_experts_tile: bad arguments"); return MSR_ERR_ARG; }
     ExpertArgs a{};
     a.rows = (int)rows; a.experts = experts;
     a.M = (int)out_features;
     a.N = (int)(product == EX_FWD ? out_features : in_features);
     a.K = (int)(product == EX_FWD ? in_features : out_features);
-    *tile = experts_tile(std::min(product, (int32_t)EX_WGRAD), product == 3, a);
+    const ExpertPlan p = experts_plan(std::min(product, (int32_t)EX_WGRAD), product == 3, a);
+    *tile = p.tile;
+    *split = p.split;
     return MSR_OK;
 }
 

@@ -108,16 +108,20 @@ def test_products_of_ordinary_layers(L, counts, fout, fin):
 @pytest.mark.parametrize("counts,fout,fin,tiles", [([41, 0, 130, 29, 0, 99, 1], 264, 136, [64, 64, 64, 64]),
                                                    ([1201, 0, 900, 7, 893], 1544, 2056, [128, 128, 128, 128]),
                                                    ([1013, 987], 4096, 4096, [256, 256, 256, 256]),
-                                                   ([1500, 1, 1499], 2056, 4104, [128, 256, 256, 256])])
+                                                   ([1500, 1, 1499], 2056, 4104, [128, 256, 256, 128]),
+                                                   ([70, 0, 133], 136, 4104, [63, 64, 64, 64]),
+                                                   ([70, 0, 133], 4168, 136, [64, 63, 64, 64]),
+                                                   ([1], 4168, 8200, [63, 63, 128, 128])])
 def test_every_tile(L, counts, fout, fin, tiles):
-    """Each product in each of its tiles (features and groups that end inside them), the accumulation against
+    """Each product in each of its tiles (63: 64 with K split; features and groups that end inside them), the
+    accumulation against
     the stored product whatever its tile: the same products in the same order."""
     from muon_sr_amd import _lib, experts_wgrad_sr_accum
     s = make(counts, 9, fout, fin, 4)
-    rows, E, t = s["x"].shape[0], len(counts), ctypes.c_int32()
+    rows, E, t, split = s["x"].shape[0], len(counts), ctypes.c_int32(), ctypes.c_int32()
     for product, tile in enumerate(tiles):
-        check(L, L.msr_experts_tile(product, rows, E, fin, fout, ctypes.byref(t)))
-        assert t.value == tile
+        check(L, L.msr_experts_tile(product, rows, E, fin, fout, ctypes.byref(t), ctypes.byref(split)))
+        assert t.value - split.value == tile
     y, dx, dw = passes(s)
     near(y, s, "y", fin)
     near(dx, s, "dx", fout)

@@ -95,11 +95,12 @@ def test_products(lib):
     assert lib.msr_experts_wgrad(A, A, 64, B, 32, D, 100, 4, 64, 32, None) == OVERLAP
     acc = lambda mode, inject=None: lib.msr_experts_wgrad_sr_accum(C, A, 64, B, 32, D, 100, 4, 64, 32, 7, 0, mode, inject, None)  # noqa: E731
     assert acc(3) == ARG and acc(-1) == ARG and acc(2) == ARG
-    t = ctypes.c_int32()
-    assert lib.msr_experts_tile(4, 100, 4, 64, 32, ctypes.byref(t)) == ARG
+    t, split = ctypes.c_int32(), ctypes.c_int32()
+    assert lib.msr_experts_tile(4, 100, 4, 64, 32, ctypes.byref(t), ctypes.byref(split)) == ARG
     for product in range(4):
         for rows, E_, i, o in ((1, 1, 8, 8), (61, 8, 256, 512), (32768, 8, 4096, 14336), (1 << 29, 1024, 1024, 1 << 19)):
-            assert lib.msr_experts_tile(product, rows, E_, i, o, ctypes.byref(t)) == 0 and t.value in (64, 128, 256)
+            assert lib.msr_experts_tile(product, rows, E_, i, o, ctypes.byref(t), ctypes.byref(split)) == 0
+            assert t.value in (64, 128, 256) and split.value in (0, 1)
 
 
 def test_python_needs_a_gpu_and_fitting_arguments(lib):
