@@ -461,7 +461,7 @@ static bool move_vec(int64_t d, int64_t ld, size_t es, const void *p, const void
 // U: the packs per lane of a piece, at most 4, as even as the row allows (6 packs: 2 pieces of 3).
 #define MOVE_LAUNCH_U(KERNEL, T, V, ...)                                                                             \
     do {                                                                                                             \
-        const int64_t packs = (a.d + 64 * Pack<T, V>::N - 1) / (64 * Pack<T, V>::N);                                 \
+        const int64_t packs = std::max<int64_t>((a.d + 64 * Pack<T, V>::N - 1) / (64 * Pack<T, V>::N), 1);           \
         const int64_t u = (packs + (packs + 3) / 4 - 1) / ((packs + 3) / 4);                                         \
         if (u > 3) hipLaunchKernelGGL((KERNEL<T, V, 4 __VA_ARGS__>), grid, dim3(MOVE_THREADS), 0, s, a);             \
         else if (u > 2) hipLaunchKernelGGL((KERNEL<T, V, 3 __VA_ARGS__>), grid, dim3(MOVE_THREADS), 0, s, a);        \

@@ -77,6 +77,7 @@ COUNTS = {
     "one_has_all": [0] * 20 + [900] + [0] * 10,
     "many_small": [i * 7 % 23 for i in range(200)],
     "uneven": [700, 3, 0, 41, 1200, 17],
+    "most_experts": [i * 5 % 7 for i in range(1024)],
 }
 
 

@@ -69,6 +69,18 @@ def test_order_extremes():
     check_order(ids, 16)
 
 
+def test_no_tokens_and_no_width():
+    from muon_sr_amd import combine_tokens, dispatch_tokens, order_tokens
+    order = order_tokens(torch.zeros((0, 2), dtype=torch.int64, device=DEV), 3)
+    x, w = torch.zeros((0, 16), device=DEV, requires_grad=True), torch.zeros((0, 2), device=DEV, requires_grad=True)
+    y = combine_tokens(dispatch_tokens(x, order), w, order)
+    dx, dw = torch.autograd.grad(y, (x, w), torch.zeros((0, 16), device=DEV))
+    assert y.shape == dx.shape == (0, 16) and dw.shape == (0, 2)
+    s = make(5, 2, 3, 0, BF16, F32, 1)
+    moved, y, dx, dr, dw = all_passes(s)
+    assert moved.shape == dr.shape == (10, 0) and y.shape == dx.shape == (5, 0) and dw.shape == (5, 2) and not dw.any()
+
+
 def test_order_of_strided_ids():
     from muon_sr_amd import order_tokens
     ids = torch.randint(0, 9, (100, 12), generator=gen(1), device=DEV)
