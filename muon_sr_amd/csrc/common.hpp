@@ -470,6 +470,17 @@ __device__ __forceinline__ void group_max2(float &a, float &b) {
     }
 }
 
+// Inclusive sum over the lanes of a wave.
+__device__ __forceinline__ int wave_scan(int x) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int w = 1; w < 64; w <<= 1) {
+        const int y = __shfl_up(x, w);
+        x += lane >= w ? y : 0;
+    }
+    return x;
+}
+
 inline bool aligned(const void *p, uintptr_t a) { return ((uintptr_t)p & (a - 1)) == 0; }
 
 // Host-side race check: the byte ranges [a, a + na) and [b, b + nb) overlap

@@ -121,17 +121,6 @@ struct Frags {
     }
 };
 
-// Inclusive sum over the lanes of a wave.
-__device__ __forceinline__ int wave_sum_to(int x) {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int w = 1; w < 64; w <<= 1) {
-        const int y = __shfl_up(x, w);
-        x += lane >= w ? y : 0;
-    }
-    return x;
-}
-
 // The group, first row and column of tile v, over the E + 1 groups' tile rows (false: no such tile).  Every wave finds
 // it by itself: lane l adds the tile rows of c consecutive groups, a sum over the lanes gives the number of all and the lane
 // that holds the tile, and, where c > 1, the lanes then take that lane's groups one each.  Numbering the tiles without
@@ -148,7 +137,7 @@ __device__ __forceinline__ bool find_rows(const ExpertArgs &a, int v, int &e, in
         n += tiles(at, next);
         at = next;
     }
-    int to = wave_sum_to(n);
+    int to = wave_scan(n);
     const int mt = __builtin_amdgcn_readlane(to, 63), total = mt * a.tiles_n;
     if (v >= total) return false;
     // Consecutive work-groups go to the 8 XCDs in turn: each XCD takes a contiguous eighth of the
@@ -164,7 +153,7 @@ __device__ __forceinline__ bool find_rows(const ExpertArgs &a, int v, int &e, in
     e = l * c;
     if (c > 1) {
         n = lane < c ? tiles(group_row(a, e + lane), group_row(a, e + lane + 1)) : 0;
-        to = wave_sum_to(n);
+        to = wave_scan(n);
         l = __builtin_ctzll(__ballot(to > t) | 1ull << 63);
         t -= __builtin_amdgcn_readlane(to - n, l);
         e += l;

@@ -49,7 +49,7 @@ def check_order(ids, E, dtype=torch.int64):
 @pytest.mark.parametrize("dtype", [torch.int32, torch.int64], ids=["int32", "int64"])
 @pytest.mark.parametrize("tokens,k,E", [(1, 1, 1), (7, 2, 8), (64, 1, 3), (65, 3, 64), (1000, 2, 65), (1024, 2, 255),
                                         (2049, 1, 256), (683, 3, 1023), (5000, 8, 1024), (70001, 4, 130),
-                                        (300000, 2, 7)])
+                                        (300000, 2, 7), (40000, 2, 1000), (66000, 8, 500)])
 def test_order(tokens, k, E, dtype):
     rng = np.random.default_rng(tokens + E)
     check_order(rng.integers(0, E, (tokens, k)), E, dtype)
