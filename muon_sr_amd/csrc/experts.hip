@@ -254,7 +254,7 @@ __global__ __launch_bounds__(64 * Shape<T>::NW * KG, WPS) void experts_kernel(Ex
     // The accumulator's first PRE row blocks of the wave, as its epilogue takes them: 16 bytes at row crow +
     // RPP y of a block, loaded ahead of the products
     constexpr int WC = S::TN / 8, RPP = 64 / WC, NP = 32 / RPP;   // chunks per row, rows per access, accesses per block
-    constexpr int PRE = MODE >= 0 ? (FM < 2 ? FM : 2) : 0;
+    constexpr int PRE = MODE >= 0 ? FM < 4 ? 1 : 2 : 0;
     u32x4_t old[PRE ? PRE : 1][NP];
     auto fetch = [&](u32x4_t (&c)[NP], int i, int ln) __attribute__((always_inline)) {
         const int n = n0 + wn * S::TN + 8 * (ln % WC);
@@ -397,8 +397,8 @@ __global__ __launch_bounds__(64 * Shape<T>::NW * KG, WPS) void experts_kernel(Ex
     }
     u32x4_t late[PRE && FM > PRE ? FM - PRE : 1][NP];
     if constexpr (PRE > 0 && FM > PRE) {
-        fetch(late[0], 2, elane);
-        fetch(late[1], 3, elane);
+        fetch(late[0], PRE, elane);
+        if constexpr (FM > PRE + 1) fetch(late[1], PRE + 1, elane);
     }
     auto block = [&](auto I) __attribute__((always_inline)) {
         constexpr int i = decltype(I)::value;
@@ -462,34 +462,37 @@ __global__ __launch_bounds__(64 * Shape<T>::NW * KG, WPS) void experts_kernel(Ex
 //   1 x 1,    4096 x 4096                      32  15  18                    32  24  19
 //   64 x 8,   (4096 x 1024)                                                  34  28  23
 //   16 x 8,   4096 x 4096 (272 tiles)          35  36  41                    36  52  48
-template <int KIND, int T, bool SPLIT>
+// ACC, 128: the accumulation has its noise to compute and its accumulators to wait for, which a fourth work-group per CU
+// hides better than a third stage (16411 x 64, 1024 x 2048: 145 us with 2 stages and 4 waves per SIMD, one row block
+// of accumulators fetched ahead; 149 with 3 and 3; 156 with 3, 3 and two blocks ahead).
+template <int KIND, bool ACC, int T, bool SPLIT>
 struct Ring {
     static constexpr bool FINE = KIND != EX_FWD && T >= 128;
     static constexpr int KG = !SPLIT ? 1 : KIND == EX_FWD ? 2 : 4;
-    static constexpr int BK = FINE ? 32 : 64, S = KG == 2 ? 4 : FINE ? (T == 256 ? 4 : 3) : 2;
-    static constexpr int WPS = KG == 4 ? 4 : FINE && T == 128 ? 3 : 2;
+    static constexpr int BK = FINE ? 32 : 64, S = KG == 2 ? 4 : FINE ? (T == 256 ? 4 : ACC ? 2 : 3) : 2;
+    static constexpr int WPS = KG == 4 ? 4 : FINE && T == 128 ? (ACC ? 4 : 3) : 2;
 };
 
 // Estimated time (us) of a call in tiles of T, from times per slab of 64 k of a tile: p with every CU busy, u for a
 // tile that has its CU to itself; and o for its start and end.  Fitted to the forward and dgrad times above and to
 // (stored and accumulated weight gradients with non-temporal outputs):
 //   rows x experts, weights      forward 256 128 64   dgrad 256 128 64   wgrad 256 128 64   accum 256 128 64
-//   8192 x 8,    1536 x 384            17  20  27           33  20  23         39  25  23         47  29  25
+//   8192 x 8,    1536 x 384            17  20  27           33  20  23         39  25  23         47  42  25
 //   4096 x 128,   768 x 2048          126 108 107          116  96  96         83  71 114        193 147 206
 //   512 x 64,    1024 x 2048           49  41  40           48  44  42         54  42  67        131  96 131
 //   61 x 8,       512 x 256           9.1 5.8 4.7         13.6 7.9 5.7        6.2 4.0 4.0       13.0 6.6 4.2
-//   16411 x 64,  1024 x 2048                                                  101  98 154        165 155 214
+//   16411 x 64,  1024 x 2048                                                  101  98 154        165 145 214
 //   65536 x 64,  1024 x 2048          307 355 533          305 380 584        282 329 587        343 372 623
 // A group is taken to end in the middle of its last tile, and the largest expert to have twice the average rows.
 static float experts_cost(int kind, bool accum, int T, bool split, const ExpertArgs &a) {
     const int i = T == 256 ? 2 : T == 128 ? 1 : 0;
     constexpr float ROWS_P[3] = {0.25f, 0.62f, 1.9f}, U[3] = {0.5f, 0.75f, 1.2f}, ROWS_O[3] = {1.5f, 3.0f, 5.0f};
-    constexpr float W_P[3] = {0.215f, 0.54f, 1.75f}, W_O[3] = {0.4f, 0.8f, 5.0f}, ACC_O[3] = {0.9f, 2.45f, 13.0f};
+    constexpr float W_P[3] = {0.215f, 0.54f, 1.75f}, W_O[3] = {0.4f, 0.8f, 5.0f}, ACC_O[3] = {0.9f, 2.3f, 13.0f};
     const float tn = (float)((a.N + T - 1) / T);
     if (kind == EX_WGRAD) {
         const float n = (float)((a.M + T - 1) / T) * tn * (float)a.experts / 256.0f;   // tiles per CU
         const float ks = (float)a.rows / (float)a.experts / 64.0f + 0.5f, o = accum ? ACC_O[i] : W_O[i];
-        return std::max(n * (ks * W_P[i] + o), 2.0f * ks * U[i] + o);
+        return std::max(n * (ks * W_P[i] + o), 2.0f * ks * (accum && T == 128 ? 1.15f : U[i]) + o);   // its two stages alone: 42 us for 1536 x 384
     }
     const float n = ((float)a.rows / (float)T + 0.5f * (float)std::min(a.experts, a.rows)) * tn / 256.0f, ks = (float)a.K / 64.0f;
     if (split) return ceilf(n) * (ks * (kind == EX_FWD ? 0.22f : 0.33f) + 4.0f);
@@ -516,7 +519,7 @@ static ExpertPlan experts_plan(int kind, bool accum, const ExpertArgs &a) {
 
 template <int KIND, int MODE, int T, bool SPLIT>
 static void experts_launch_tile(const ExpertArgs &a, unsigned grid, hipStream_t s) {
-    using R = Ring<KIND, T, SPLIT>;
+    using R = Ring<KIND, (MODE >= 0), T, SPLIT>;
     hipLaunchKernelGGL((experts_kernel<KIND, MODE, T, R::BK, R::S, R::WPS, R::KG>), dim3(grid), dim3(64 * Shape<T>::NW * R::KG), 0, s, a);
 }
 
