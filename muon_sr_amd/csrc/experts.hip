@@ -139,7 +139,7 @@ __device__ __forceinline__ bool find_rows(const ExpertArgs &a, int v, int &e, in
     }
     int to = wave_scan(n);
     const int mt = __builtin_amdgcn_readlane(to, 63), total = mt * a.tiles_n;
-    if (v >= total) return false;
+    if (v >= total || mt > a.rows / T + a.experts + 1) return false;   // (offsets that do not ascend: too many)
     // Consecutive work-groups go to the 8 XCDs in turn: each XCD takes a contiguous eighth of the
     // tiles, whose operands its L2 shares
     const int per = total / NXCD;
@@ -161,7 +161,7 @@ __device__ __forceinline__ bool find_rows(const ExpertArgs &a, int v, int &e, in
     lo = __builtin_amdgcn_readfirstlane(group_row(a, e));
     hi = __builtin_amdgcn_readfirstlane(group_row(a, e + 1));
     m0 = t * T;
-    return t >= 0 && (int64_t)t * T < hi - lo;   // offsets that do not ascend: no tile outside a group
+    return t >= 0 && (int64_t)t * T < hi - lo;   // (and no tile outside a group)
 }
 
 // The expert with the q-th most rows (at most 64 experts): the last tiles to run are then short ones.

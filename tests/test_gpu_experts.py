@@ -236,6 +236,16 @@ def test_offsets_are_clamped_to_the_rows(L):
     assert all(torch.equal(a, b) for a, b in zip(want, passes(s)))
 
 
+def test_offsets_that_do_not_ascend_stay_inside(L):
+    """Not a valid order: the results mean nothing, but every row and weight that is read or written is the call's."""
+    s = make([50, 30, 20], 0, 72, 136, 18)
+    for bad in ([0, 90, 10, 100], [0, -5, 1000, 60], [7, 100, 0, 100], [0, 100, 100, -3]):
+        s["off"] = torch.tensor(bad, dtype=torch.int32, device=DEV)
+        y, dx, dw = passes(s)
+        assert y.shape == (100, 72) and dx.shape == (100, 136) and dw.shape == (3, 72, 136)
+    torch.cuda.synchronize()
+
+
 def test_gradients_against_differences(L):
     """The products are linear in each operand, so differences at unit steps on small whole numbers (exact in
     bf16 and fp32) are the gradients, exactly."""
