@@ -10,9 +10,11 @@
 // a slot.  Bound by latency: one or two launches.
 //
 // The four passes between tokens and rows (see the header) move d elements per slot and do
-// next to nothing with them, so HBM bounds them.  All are written from the token's side: a
-// token's k rows are read or written by the same wave, so x and dy are read once, not k times, y
+// next to nothing with them, so HBM bounds them.  All are written from the token's side: a piece of a
+// token's k rows is read or written by the same wave, so x and dy are read once, not k times, y
 // and dx are sums in registers, and nothing is added atomically.
+#include <type_traits>
+
 #include "common.hpp"
 #include "vecio.hpp"
 #include "../../include/muon_sr_amd.h"
@@ -175,41 +177,45 @@ static OrderPlan order_plan(int64_t n) {
 // ---------------------------------------------------------------------------
 
 constexpr int MOVE_THREADS = 256, MOVE_WAVES = MOVE_THREADS / 64;
-constexpr int MOVE_GRID = 256 * 8;
+// Work-groups at most: four times what the card holds (combine's gradient of 32768 x 4 of width 256 26 us so, 29 with
+// 8 per CU).
+constexpr int MOVE_GRID = 256 * 32;
 
-// 16 bytes of a row per lane (VEC), or one element.  Stores are non-temporal: the four passes over 32768 tokens x 8
-// of width 2048 take 1120 us so (5.3 TB/s), 1172 with plain stores, and over 8192 x 2 76 and 101 us; loads are not,
-// as the rows were mostly written just before (non-temporal: 1102 and 96 us).
+// 16 bytes of a row per lane (VEC), or one element, as they lie in memory: converted where they are used, so that the
+// loads of several rows are in flight together.  Stores are non-temporal: the four passes over 32768 tokens x 8
+// of width 2048 take 1100 us so (5.4 TB/s), 1166 with plain stores, and over 8192 x 2 73 and 77 us; loads are not,
+// as the rows were mostly written just before.
 template <typename T, bool VEC>
 struct Pack {
     static constexpr int N = VEC ? 16 / (int)sizeof(T) : 1;
-    float f[N];
-    __device__ __forceinline__ void load(const T *p) {
+    using V = std::conditional_t<!VEC, T, std::conditional_t<sizeof(T) == 2, u32x4_t, f32x4_t>>;
+    V v;
+    __device__ __forceinline__ void load(const T *p) { v = *reinterpret_cast<const V *>(p); }
+    __device__ __forceinline__ void store(T *p) const {
+        if constexpr (VEC) __builtin_nontemporal_store(v, reinterpret_cast<V *>(p));
+        else *p = v;
+    }
+    __device__ __forceinline__ void zero() { v = V{}; }
+    __device__ __forceinline__ void get(float (&f)[N]) const {
         if constexpr (!VEC) {
-            if constexpr (sizeof(T) == 2) f[0] = bf16_to_f32(*p);
-            else f[0] = *p;
+            if constexpr (sizeof(T) == 2) f[0] = bf16_to_f32(v);
+            else f[0] = v;
         } else if constexpr (sizeof(T) == 2) {
-            const u32x4_t v = *reinterpret_cast<const u32x4_t *>(p);
             const uint32_t w[4] = {v.x, v.y, v.z, v.w};
             unpack8(w, f);
         } else {
-            const f32x4_t v = *reinterpret_cast<const f32x4_t *>(p);
             f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w;
         }
     }
-    __device__ __forceinline__ void store(T *p) const {
+    __device__ __forceinline__ void set(const float (&f)[N]) {
         if constexpr (!VEC) {
-            if constexpr (sizeof(T) == 2) *p = (T)rne_bf16(f[0]);
-            else *p = f[0];
+            if constexpr (sizeof(T) == 2) v = (T)rne_bf16(f[0]);
+            else v = f[0];
         } else if constexpr (sizeof(T) == 2) {
-            st_nt4(p, u32x4_t{rne_bf16x2(f[0], f[1]), rne_bf16x2(f[2], f[3]), rne_bf16x2(f[4], f[5]), rne_bf16x2(f[6], f[7])});
+            v = u32x4_t{rne_bf16x2(f[0], f[1]), rne_bf16x2(f[2], f[3]), rne_bf16x2(f[4], f[5]), rne_bf16x2(f[6], f[7])};
         } else {
-            __builtin_nontemporal_store(f32x4_t{f[0], f[1], f[2], f[3]}, reinterpret_cast<f32x4_t *>(p));
+            v = f32x4_t{f[0], f[1], f[2], f[3]};
         }
-    }
-    __device__ __forceinline__ void zero() {
-#pragma unroll
-        for (int i = 0; i < N; ++i) f[i] = 0.0f;
     }
 };
 
@@ -223,6 +229,7 @@ struct MoveArgs {
     const int32_t *position, *offsets;
     int64_t tokens, n, d;
     int32_t k, experts, w32;
+    int32_t pieces, share;       // of a row; 2^share waves of a work-group take them in turn (set by the launch)
 };
 
 // A token's slots, 64 at a time: lane j holds the row (-1: none) and the weight of slot first + j, so that one
@@ -247,7 +254,7 @@ struct Slots {
 };
 // A wave's piece of a row: U packs per lane, 64 packs apart, from column c on.  Whole rows (or 4 KiB of
 // them) at a time: a wave that went through a token's rows 1 KiB at a time would return to each row's memory page
-// several times (combine of 32768 x 8 rows of 4 KiB 339 us so, 272 a whole row at a time).
+// several times (combine of 32768 x 8 rows of 4 KiB 231 us so, 221 a whole row at a time).
 template <typename T, bool VEC, int U>
 struct Piece {
     static constexpr int N = Pack<T, VEC>::N, WIDTH = 64 * N * U;
@@ -270,7 +277,9 @@ struct Piece {
         for (int u = 0; u < U; ++u) p[u].zero();
     }
 };
-constexpr int MOVE_AHEAD = 2;   // rows whose loads are in flight together (1: 4 % slower, 4: 35 %, too few waves)
+// Rows whose loads are in flight together (32768 x 8 of width 2048: combine 221 us, 227 with two; 300 x 8 of
+// width 7168: 7.5 and 7.9).
+constexpr int MOVE_AHEAD = 4;
 
 // Rows without a slot, [offsets[experts], n), to zero: the waves of the launch in turn.
 template <typename T, bool VEC>
@@ -291,15 +300,15 @@ template <typename T, bool VEC, int U>
 __global__ __launch_bounds__(MOVE_THREADS) void dispatch_kernel(MoveArgs a) {
     using P = Piece<T, VEC, U>;
     const int64_t waves = (int64_t)gridDim.x * MOVE_WAVES;
-    for (int64_t t = this_wave(); t < a.tokens; t += waves) {
-        const T *x = static_cast<const T *>(a.tok) + t * a.ldtok;
-        for (int j0 = 0; j0 < a.k; j0 += 64) {
-            const int js = min(64, a.k - j0);
-            Slots s;
-            s.load(a, t * a.k + j0, js);
-            for (int64_t c = 0; c < a.d; c += P::WIDTH) {
-                P v;
-                v.load(x, c, a.d);
+    for (int64_t i = this_wave(); i >> a.share < a.tokens; i += waves) {
+        const int64_t t = i >> a.share;
+        for (int64_t c = (i & ((1 << a.share) - 1)) * P::WIDTH; c < a.d; c += (int64_t)P::WIDTH << a.share) {
+            P v;
+            v.load(static_cast<const T *>(a.tok) + t * a.ldtok, c, a.d);
+            for (int j0 = 0; j0 < a.k; j0 += 64) {
+                const int js = min(64, a.k - j0);
+                Slots s;
+                s.load(a, t * a.k + j0, js);
                 for (int j = 0; j < js; ++j) {
                     const int p = s.row_of(j);
                     if (p >= 0) v.store(static_cast<T *>(a.out) + (int64_t)p * a.d, c, a.d);
@@ -314,100 +323,151 @@ __global__ __launch_bounds__(MOVE_THREADS) void dispatch_kernel(MoveArgs a) {
 template <typename T, bool VEC, int U, bool WEIGHTED>
 __global__ __launch_bounds__(MOVE_THREADS) void combine_kernel(MoveArgs a) {
     using P = Piece<T, VEC, U>;
-    const int64_t waves = (int64_t)gridDim.x * MOVE_WAVES;
-    for (int64_t t = this_wave(); t < a.tokens; t += waves) {
+    constexpr int A = MOVE_AHEAD;
+    for (int64_t i = this_wave(); i >> a.share < a.tokens; i += (int64_t)gridDim.x * MOVE_WAVES) {
+        const int64_t t = i >> a.share;
         Slots s;
         s.load(a, t * a.k, min(64, a.k));
-        for (int64_t c = 0; c < a.d; c += P::WIDTH) {
-            P sum;
-            sum.zero();
-            for (int j0 = 0; j0 < a.k; j0 += MOVE_AHEAD) {
+        for (int64_t c = (i & ((1 << a.share) - 1)) * P::WIDTH; c < a.d; c += (int64_t)P::WIDTH << a.share) {
+            float sum[U][P::N] = {};
+            for (int j0 = 0; j0 < a.k; j0 += A) {
                 if (a.k > 64 && (j0 & 63) == 0) s.load(a, t * a.k + j0, min(64, a.k - j0));
-                P v[MOVE_AHEAD];
+                P v[A];
 #pragma unroll
-                for (int y = 0; y < MOVE_AHEAD; ++y) {
+                for (int y = 0; y < A; ++y) {
                     const int p = j0 + y < a.k ? s.row_of((j0 + y) & 63) : -1;
                     if (p >= 0) v[y].load(static_cast<const T *>(a.rows) + (int64_t)p * a.d, c, a.d);
                 }
 #pragma unroll
-                for (int y = 0; y < MOVE_AHEAD; ++y) {
+                for (int y = 0; y < A; ++y) {
                     if (j0 + y >= a.k || s.row_of((j0 + y) & 63) < 0) continue;
                     const float w = WEIGHTED ? s.weight_of((j0 + y) & 63) : 1.0f;
 #pragma unroll
-                    for (int u = 0; u < U; ++u)
+                    for (int u = 0; u < U; ++u) {
+                        float f[P::N];
+                        v[y].p[u].get(f);
 #pragma unroll
-                        for (int i = 0; i < P::N; ++i)
-                            sum.p[u].f[i] = WEIGHTED ? __builtin_fmaf(w, v[y].p[u].f[i], sum.p[u].f[i]) : sum.p[u].f[i] + v[y].p[u].f[i];
+                        for (int x = 0; x < P::N; ++x) sum[u][x] = WEIGHTED ? __builtin_fmaf(w, f[x], sum[u][x]) : sum[u][x] + f[x];
+                    }
                 }
             }
-            sum.store(static_cast<T *>(a.out) + t * a.d, c, a.d);
+            P out;
+#pragma unroll
+            for (int u = 0; u < U; ++u) out.p[u].set(sum[u]);
+            out.store(static_cast<T *>(a.out) + t * a.d, c, a.d);
         }
     }
 }
 
-// drows[position[t][j]] = w[t][j] dy[t];  dw[t][j] = <dy[t], rows[position[t][j]]>
-template <typename T, bool VEC, int U>
+// The sums of x and of y over the wave, in registers: lanes 0 to 31 add up x, the others y.
+struct Sums2 {
+    float v;
+    __device__ __forceinline__ Sums2(float x, float y) {
+        const auto h = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(y), false, false);
+        v = __uint_as_float(h[0]) + __uint_as_float(h[1]);
+        const auto q = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = __uint_as_float(q[0]) + __uint_as_float(q[1]);
+        v = turned<0x128>(turned<0x124>(turned<0x122>(turned<0x121>(v))));
+    }
+    template <int CTRL>   // row_ror: 1, 2, 4, 8 lanes within 16
+    static __device__ __forceinline__ float turned(float x) {
+        return x + __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(x), CTRL, 0xf, 0xf, true));
+    }
+    __device__ __forceinline__ float of(int y) const { return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(v), y * 32)); }
+};
+
+// drows[position[t][j]] = w[t][j] dy[t];  dw[t][j] = <dy[t], rows[position[t][j]]>: the parts of the waves that
+// share a token are added in their order
+template <typename T, bool VEC, int U, bool SHARED>
 __global__ __launch_bounds__(MOVE_THREADS) void combine_grad_kernel(MoveArgs a) {
     using P = Piece<T, VEC, U>;
-    const int lane = threadIdx.x & 63;
-    const int64_t waves = (int64_t)gridDim.x * MOVE_WAVES;
-    for (int64_t t = this_wave(); t < a.tokens; t += waves) {
+    constexpr int A = MOVE_AHEAD;
+    static_assert(A % 2 == 0, "dw is summed in pairs");
+    __shared__ float part[SHARED ? MOVE_WAVES : 1][64];
+    const int share = SHARED ? a.share : 0;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w0 = wave & ((1 << share) - 1);
+    const int64_t c0 = (int64_t)w0 * P::WIDTH;
+    const bool whole = a.pieces <= 1 << share;     // the wave's part of dy[t] stays in registers
+    // every wave of the work-group makes the same rounds (barriers)
+    for (int64_t i0 = (int64_t)blockIdx.x * MOVE_WAVES; i0 >> share < a.tokens; i0 += (int64_t)gridDim.x * MOVE_WAVES) {
+        const int64_t t = (i0 + wave) >> share;
+        const bool on = t < a.tokens;
         const T *dy = static_cast<const T *>(a.tok) + t * a.ldtok;
-        const bool whole = a.d <= P::WIDTH;      // dy[t] stays in registers
         P g;
-        if (whole) g.load(dy, 0, a.d);
-        Slots s;
-        for (int j0 = 0; j0 < a.k; j0 += MOVE_AHEAD) {
-            if ((j0 & 63) == 0) s.load(a, t * a.k + j0, min(64, a.k - j0));
-            float dot[MOVE_AHEAD] = {};
-            for (int64_t c = 0; c < a.d; c += P::WIDTH) {
-                if (!whole) g.load(dy, c, a.d);
-                if (a.dw) {
-                    P r[MOVE_AHEAD];
+        if (whole && on) g.load(dy, c0, a.d);
+        for (int j1 = 0; j1 < a.k; j1 += 64) {
+            const int js = on ? min(64, a.k - j1) : 0;
+            Slots s;
+            s.load(a, t * a.k + j1, js);
+            float mine = 0.0f;                       // lane j: the dot product of slot j1 + j
+            for (int j0 = 0; j0 < js; j0 += A) {
+                float dot[A] = {};
+                for (int64_t c = c0; c < a.d; c += (int64_t)P::WIDTH << share) {
+                    if (!whole) g.load(dy, c, a.d);
+                    if (a.dw) {
+                        P r[A];
 #pragma unroll
-                    for (int y = 0; y < MOVE_AHEAD; ++y) {
-                        const int p = j0 + y < a.k ? s.row_of((j0 + y) & 63) : -1;
-                        if (p >= 0) r[y].load(static_cast<const T *>(a.rows) + (int64_t)p * a.d, c, a.d);
+                        for (int y = 0; y < A; ++y) {
+                            const int p = j0 + y < js ? s.row_of(j0 + y) : -1;
+                            if (p >= 0) r[y].load(static_cast<const T *>(a.rows) + (int64_t)p * a.d, c, a.d);
+                        }
+#pragma unroll
+                        for (int y = 0; y < A; ++y) {
+                            if (j0 + y >= js || s.row_of(j0 + y) < 0) continue;
+#pragma unroll
+                            for (int u = 0; u < U; ++u) {
+                                float f[P::N], h[P::N];
+                                g.p[u].get(f);
+                                r[y].p[u].get(h);
+#pragma unroll
+                                for (int x = 0; x < P::N; ++x) dot[y] = __builtin_fmaf(f[x], h[x], dot[y]);
+                            }
+                        }
                     }
+                    if (a.out) {
 #pragma unroll
-                    for (int y = 0; y < MOVE_AHEAD; ++y) {
-                        if (j0 + y >= a.k || s.row_of((j0 + y) & 63) < 0) continue;
+                        for (int y = 0; y < A; ++y) {
+                            const int p = j0 + y < js ? s.row_of(j0 + y) : -1;
+                            if (p < 0) continue;
+                            const float w = s.weight_of(j0 + y);
+                            P o;
 #pragma unroll
-                        for (int u = 0; u < U; ++u)
+                            for (int u = 0; u < U; ++u) {
+                                float f[P::N];
+                                g.p[u].get(f);
 #pragma unroll
-                            for (int i = 0; i < P::N; ++i) dot[y] = __builtin_fmaf(g.p[u].f[i], r[y].p[u].f[i], dot[y]);
+                                for (int x = 0; x < P::N; ++x) f[x] *= w;
+                                o.p[u].set(f);
+                            }
+                            o.store(static_cast<T *>(a.out) + (int64_t)p * a.d, c, a.d);
+                        }
                     }
                 }
-                if (a.out) {
+                if (a.dw) {
 #pragma unroll
-                    for (int y = 0; y < MOVE_AHEAD; ++y) {
-                        const int p = j0 + y < a.k ? s.row_of((j0 + y) & 63) : -1;
-                        if (p < 0) continue;
-                        const float w = s.weight_of((j0 + y) & 63);
-                        P o;
-#pragma unroll
-                        for (int u = 0; u < U; ++u)
-#pragma unroll
-                            for (int i = 0; i < P::N; ++i) o.p[u].f[i] = g.p[u].f[i] * w;
-                        o.store(static_cast<T *>(a.out) + (int64_t)p * a.d, c, a.d);
+                    for (int y = 0; y < A; y += 2) {
+                        const Sums2 sums(dot[y], dot[y + 1]);
+                        mine = lane == j0 + y ? sums.of(0) : lane == j0 + y + 1 ? sums.of(1) : mine;
                     }
                 }
             }
             if (a.dw) {
-#pragma unroll
-                for (int y = 0; y < MOVE_AHEAD; ++y) {
-#pragma unroll
-                    for (int w = 32; w > 0; w >>= 1) dot[y] += __shfl_xor(dot[y], w);
-                    if (lane == y && j0 + y < a.k) {
-                        const int64_t at = t * a.k + j0 + y;
-                        if (a.w32) static_cast<float *>(a.dw)[at] = dot[y];
-                        else static_cast<uint16_t *>(a.dw)[at] = (uint16_t)rne_bf16(dot[y]);
-                    }
+                if constexpr (SHARED) {
+                    part[wave][lane] = mine;
+                    __syncthreads();
+                    mine = part[wave - w0][lane];
+                    for (int w = 1; w < 1 << share; ++w) mine = mine + part[wave - w0 + w][lane];
+                    __syncthreads();
+                }
+                if (w0 == 0 && lane < js) {
+                    const int64_t at = t * a.k + j1 + lane;
+                    if (a.w32) static_cast<float *>(a.dw)[at] = mine;
+                    else static_cast<uint16_t *>(a.dw)[at] = (uint16_t)rne_bf16(mine);
                 }
             }
         }
     }
-    if (a.out) zero_tail<T, VEC>(a, this_wave(), waves);
+    if (a.out) zero_tail<T, VEC>(a, this_wave(), (int64_t)gridDim.x * MOVE_WAVES);
 }
 
 // ---------------------------------------------------------------------------
@@ -428,35 +488,51 @@ static int move_check(const char *name, const MoveArgs &a, int32_t elem, int32_t
     return MSR_OK;
 }
 
-static unsigned move_grid(int64_t waves) {
-    return (unsigned)std::min<int64_t>(std::max<int64_t>((waves + MOVE_WAVES - 1) / MOVE_WAVES, 1), MOVE_GRID);
-}
-
 static bool move_vec(int64_t d, int64_t ld, size_t es, const void *p, const void *q, const void *r) {
     const int64_t n = 16 / (int64_t)es;
     return d % n == 0 && ld % n == 0 && aligned(p, 16) && aligned(q, 16) && aligned(r, 16);
 }
 
-// U: the packs per lane of a piece, at most 4, as even as the row allows (6 packs: 2 pieces of 3).
-#define MOVE_LAUNCH_U(KERNEL, T, V, ...)                                                                             \
-    do {                                                                                                             \
-        const int64_t packs = std::max<int64_t>((a.d + 64 * Pack<T, V>::N - 1) / (64 * Pack<T, V>::N), 1);           \
-        const int64_t u = (packs + (packs + 3) / 4 - 1) / ((packs + 3) / 4);                                         \
-        if (u > 3) hipLaunchKernelGGL((KERNEL<T, V, 4 __VA_ARGS__>), grid, dim3(MOVE_THREADS), 0, s, a);             \
-        else if (u > 2) hipLaunchKernelGGL((KERNEL<T, V, 3 __VA_ARGS__>), grid, dim3(MOVE_THREADS), 0, s, a);        \
-        else if (u > 1) hipLaunchKernelGGL((KERNEL<T, V, 2 __VA_ARGS__>), grid, dim3(MOVE_THREADS), 0, s, a);    \
-        else hipLaunchKernelGGL((KERNEL<T, V, 1 __VA_ARGS__>), grid, dim3(MOVE_THREADS), 0, s, a);                   \
-    } while (0)
-#define MOVE_LAUNCH(KERNEL, ...)                                                                                     \
-    do {                                                                                                             \
-        if (elem == MSR_BF16) {                                                                                      \
-            if (vec) MOVE_LAUNCH_U(KERNEL, uint16_t, true, __VA_ARGS__);                                             \
-            else MOVE_LAUNCH_U(KERNEL, uint16_t, false, __VA_ARGS__);                                                \
-        } else {                                                                                                     \
-            if (vec) MOVE_LAUNCH_U(KERNEL, float, true, __VA_ARGS__);                                                \
-            else MOVE_LAUNCH_U(KERNEL, float, false, __VA_ARGS__);                                                   \
-        }                                                                                                            \
-    } while (0)
+// Sets the pieces of a pass's rows; returns their packs per lane: at most 4, and as even as the row allows (6 packs: 2
+// pieces of 3).  Up to 4 waves share a token's pieces, so that few tokens of wide rows have waves too: 300 x 8 of width
+// 7168 take 8, 8, 15 and 8 us (dispatch, combine, its gradient, dispatch's), with a wave per token 8, 19, 36 and 19; of
+// 32768 x 2 of width 4096 119, 146, 264, 145 and 122, 154, 286, 154.  Rows moved by single elements gain only while
+// tokens are few (width 1001: 2048 x 2 5.2, 5.5, 9.3, 5.1 us shared, 5.7, 6.5, 9.9, 6.1 not; 8192 x 2 10.6, 13.2, 26.8,
+// 12.5 and 10.1, 11.2, 22.7, 11.3).
+static int move_plan(MoveArgs &a, int32_t elem, bool vec) {
+    const int64_t pack = 64 * (!vec ? 1 : elem == MSR_BF16 ? 8 : 4), packs = std::max<int64_t>((a.d + pack - 1) / pack, 1);
+    const int64_t u = (packs + (packs + 3) / 4 - 1) / ((packs + 3) / 4);
+    a.pieces = (int32_t)((packs + u - 1) / u);
+    a.share = !vec && a.tokens > 4096 ? 0 : a.pieces > 2 ? 2 : a.pieces - 1;
+    return (int)u;
+}
+// launch(type, VEC, U): the pass's kernel
+template <typename T, typename V, typename F>
+static void move_packs(int u, F launch) {
+    if (u > 3) launch(T{}, V{}, std::integral_constant<int, 4>{});
+    else if (u > 2) launch(T{}, V{}, std::integral_constant<int, 3>{});
+    else if (u > 1) launch(T{}, V{}, std::integral_constant<int, 2>{});
+    else launch(T{}, V{}, std::integral_constant<int, 1>{});
+}
+template <typename F>
+static void move_launch(int32_t elem, bool vec, int u, F launch) {
+    if (elem == MSR_BF16) {
+        if (vec) move_packs<uint16_t, std::true_type>(u, launch);
+        else move_packs<uint16_t, std::false_type>(u, launch);
+    } else {
+        if (vec) move_packs<float, std::true_type>(u, launch);
+        else move_packs<float, std::false_type>(u, launch);
+    }
+}
+static dim3 move_grid(const MoveArgs &a) {
+    const int64_t wgs = ((a.tokens << a.share) + MOVE_WAVES - 1) / MOVE_WAVES;
+    return dim3((unsigned)std::min<int64_t>(std::max<int64_t>(wgs, 1), MOVE_GRID));
+}
+#define MOVE_LAUNCH(KERNEL, ...)                                                                                       \
+    move_launch(elem, vec, packs, [&](auto t, auto v, auto u) {                                                              \
+        hipLaunchKernelGGL((KERNEL<decltype(t), decltype(v)::value, decltype(u)::value __VA_OPT__(, ) __VA_ARGS__>),         \
+                           move_grid(a), dim3(MOVE_THREADS), 0, (hipStream_t)stream, a);                               \
+    })
 
 }  // namespace msr
 
@@ -531,8 +607,7 @@ int msr_dispatch(const void *x, int64_t ldx, void *rows, const int32_t *position
         return MSR_ERR_OVERLAP;
     }
     const bool vec = move_vec(d, ldx, es, x, rows, nullptr);
-    const dim3 grid(move_grid(tokens));
-    hipStream_t s = (hipStream_t)stream;
+    const int packs = move_plan(a, elem, vec);
     MOVE_LAUNCH(dispatch_kernel);
     return check_launch("dispatch_kernel");
 }
@@ -551,9 +626,8 @@ int msr_dispatch_grad(const void *drows, void *dx, const int32_t *position, int6
     const size_t rb = (size_t)a.n * (size_t)d * es, tb = (size_t)tokens * (size_t)d * es;
     if (touch(dx, tb, drows, rb) || touch(dx, tb, position, (size_t)a.n * 4)) { set_error("msr_dispatch_grad: dx overlaps an input"); return MSR_ERR_OVERLAP; }
     const bool vec = move_vec(d, d, es, drows, dx, nullptr);
-    const dim3 grid(move_grid(tokens));
-    hipStream_t s = (hipStream_t)stream;
-    MOVE_LAUNCH(combine_kernel, , false);
+    const int packs = move_plan(a, elem, vec);
+    MOVE_LAUNCH(combine_kernel, false);
     return check_launch("combine_kernel");
 }
 
@@ -574,9 +648,8 @@ int msr_combine(const void *rows, const void *w, void *y, const int32_t *positio
         return MSR_ERR_OVERLAP;
     }
     const bool vec = move_vec(d, d, es, rows, y, nullptr);
-    const dim3 grid(move_grid(tokens));
-    hipStream_t s = (hipStream_t)stream;
-    MOVE_LAUNCH(combine_kernel, , true);
+    const int packs = move_plan(a, elem, vec);
+    MOVE_LAUNCH(combine_kernel, true);
     return check_launch("combine_kernel");
 }
 
@@ -607,9 +680,9 @@ int msr_combine_grad(const void *dy, int64_t lddy, const void *rows, const void 
     for (int i = 0; i < 5; ++i) bad = bad || touch(drows, rb, in[i], ib[i]) || touch(dw, wb, in[i], ib[i]);
     if (bad) { set_error("msr_combine_grad: an output overlaps another operand"); return MSR_ERR_OVERLAP; }
     const bool vec = move_vec(d, lddy, es, dy, rows, drows);
-    const dim3 grid(move_grid(tokens));
-    hipStream_t s = (hipStream_t)stream;
-    MOVE_LAUNCH(combine_grad_kernel);
+    const int packs = move_plan(a, elem, vec);
+    if (a.share) MOVE_LAUNCH(combine_grad_kernel, true);
+    else MOVE_LAUNCH(combine_grad_kernel, false);
     return check_launch("combine_grad_kernel");
 }
 

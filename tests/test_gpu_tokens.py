@@ -153,6 +153,14 @@ def test_passes(tokens, k, E, d, dtype, wdtype):
     assert all(torch.equal(a, b) for a, b in zip((moved, y, dx, dr, dw), all_passes(s)))
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("tokens,k,E,d", [(1, 2, 3, 2056), (5, 70, 9, 4104), (3, 3, 5, 9000), (6, 2, 5, 9003), (4099, 1, 4, 270),
+                                          (20011, 2, 4, 1032)])
+def test_rows_of_several_pieces(tokens, k, E, d, dtype):
+    """Rows that several waves share, more of them than one round of the launch, and slots beyond a wave's lanes."""
+    test_passes(tokens, k, E, d, dtype, F32)
+
+
 def test_strides_and_alignment():
     """x and dy with row strides, unaligned starts, transposed: the same bits as contiguous ones."""
     s = make(77, 2, 6, 96, BF16, F32, 1)
