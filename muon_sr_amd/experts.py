@@ -264,7 +264,9 @@ class _ExpertLinear(torch.autograd.Function):
     def forward(ctx, x, weight, offsets, accumulate):
         x = _rows(x)
         ctx.save_for_backward(x, weight, offsets)
-        ctx.accumulate = accumulate
+        # the tensor that holds acc_grad: saved-tensor hooks (activation checkpointing, offloading) unpack another one.  A
+        # weight that is computed (a parametrization) holds nothing that lasts, so its gradient goes to autograd.
+        ctx.owner = weight if accumulate and weight.is_leaf else None
         return _forward(x, weight, offsets)
 
     @staticmethod
@@ -275,8 +277,8 @@ class _ExpertLinear(torch.autograd.Function):
         dx = _dgrad(dy, weight, offsets) if ctx.needs_input_grad[0] else None
         dw = None
         if ctx.needs_input_grad[1]:
-            if ctx.accumulate:
-                experts_wgrad_sr_accum(weight, x, dy, offsets)
+            if ctx.owner is not None:
+                experts_wgrad_sr_accum(ctx.owner, x, dy, offsets)
             else:
                 dw = _wgrad(weight, x, dy, offsets)
         return dx, dw, None, None
@@ -296,7 +298,8 @@ class SRExperts(torch.nn.Module):
     accumulated into ``weight.acc_grad`` with stochastic rounding inside the weight-gradient product (for
     training with ``TritonSRAccumulator``: ``reassign_grad_buffer`` then moves ``acc_grad`` to ``grad``
     as for every other parameter).  ``weight`` is [experts, out, in], initialised as ``nn.Linear``'s; the
-    Muon classes orthogonalise each expert's matrix by itself."""
+    Muon classes orthogonalise each expert's matrix by itself.  The accumulator is the parameter's under activation
+    checkpointing and other saved-tensor hooks too; a parametrized weight's gradient goes to autograd."""
 
     def __init__(self, num_experts: int, in_features: int, out_features: int, device=None, dtype=torch.bfloat16):
         super().__init__()
