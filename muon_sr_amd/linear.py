@@ -74,6 +74,9 @@ class _SRLinearFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias):
         ctx.save_for_backward(x, weight)
+        # the tensor that holds acc_grad: saved-tensor hooks (activation checkpointing, offloading) unpack another one.  A
+        # weight that is computed (a parametrization) holds nothing that lasts, so its gradient goes to autograd.
+        ctx.owner = weight if weight.is_leaf else None
         ctx.has_bias = bias is not None
         return torch.nn.functional.linear(x, weight, bias)
 
@@ -90,7 +93,7 @@ class _SRLinearFunction(torch.autograd.Function):
                 x2 = x2.contiguous()
             if dy2.stride(1) != 1:
                 dy2 = dy2.contiguous()
-            if not linear_wgrad_sr_accum(weight, x2, dy2):
+            if ctx.owner is None or not linear_wgrad_sr_accum(ctx.owner, x2, dy2):
                 dw = dy2.t() @ x2
         if ctx.has_bias and ctx.needs_input_grad[2]:
             db = dy2.sum(0)
@@ -101,7 +104,9 @@ class SRLinear(torch.nn.Linear):
     """``nn.Linear`` whose weight gradient is accumulated into ``weight.acc_grad``
     with stochastic rounding inside the weight-gradient GEMM (for training with
     ``TritonSRAccumulator``: ``reassign_grad_buffer`` then moves ``acc_grad`` to
-    ``grad`` as for every other parameter)."""
+    ``grad`` as for every other parameter).  The accumulator is the parameter's
+    under activation checkpointing and other saved-tensor hooks too; a
+    parametrized weight's gradient goes to autograd."""
 
     def forward(self, x):
         return _SRLinearFunction.apply(x, self.weight, self.bias)

@@ -79,7 +79,7 @@ def on_cpu(f, x):
         return f(x)
 
 
-MAKERS = [make_experts]
+MAKERS = [make_experts, make_linear]
 WAYS = [plain, checkpoint, reentrant, hooks, on_cpu]
 named = pytest.mark.parametrize("make", MAKERS, ids=lambda f: f.__name__)
 

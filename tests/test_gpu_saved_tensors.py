@@ -67,3 +67,12 @@ def test_experts_accumulate(way):
     offsets = torch.tensor([0, 100, 100, 160, 187], dtype=torch.int32, device=DEV)
     f = lambda x: layer(x, offsets)  # noqa: E731
     assert all(torch.equal(a, b) for a, b in zip(accumulated(layer, f, direct), accumulated(layer, f, way)))
+
+
+@HOOKS
+def test_linear_accumulates(way):
+    from muon_sr_amd import SRLinear
+    layer = SRLinear(256, 512, bias=False, device=DEV, dtype=BF16)
+    f = lambda x: layer(torch.cat([x, x[:67]]))  # noqa: E731   (256 tokens)
+    cut = lambda x: f(x)[:189]  # noqa: E731
+    assert all(torch.equal(a, b) for a, b in zip(accumulated(layer, cut, direct), accumulated(layer, cut, way)))
