@@ -223,3 +223,11 @@ def noise_mode() -> int:
 def require_gpu(t: torch.Tensor, what: str, exc=ValueError) -> None:
     if not t.is_cuda:
         raise exc(f"{what} requires tensors on a ROCm GPU (got device {t.device})")
+
+
+def check_accumulator(weight: torch.Tensor, what: str) -> None:
+    """``weight.acc_grad`` is what a kernel that accumulates into it by its address takes."""
+    acc = weight.acc_grad
+    if not isinstance(acc, torch.Tensor) or acc.dtype != torch.bfloat16 or acc.shape != weight.shape or \
+            acc.device != weight.device or not acc.is_contiguous():
+        raise ValueError(f"{what} needs an acc_grad that is contiguous bf16 of its weight's shape and device")

@@ -243,12 +243,14 @@ def experts_wgrad_sr_accum(weight: torch.Tensor, x: torch.Tensor, dy: torch.Tens
     """``weight.acc_grad[e] <- SR(weight.acc_grad[e] + bf16(dy_e^T x_e))`` for every expert in one kernel: the
     counterpart of ``linear_wgrad_sr_accum`` for ``weight`` [experts, out, in] and rows sorted by expert.
     ``x``: bf16 [rows, in], ``dy``: bf16 [rows, out].  The buffer is created (as zeros) on the first
-    call; ``seed``: 32 bits, drawn from ``random`` if not given, as the accumulator's hook draws it."""
+    call, and one that is there has to be like it (ValueError); ``seed``: 32 bits, drawn from ``random`` if not given, as the accumulator's hook draws it."""
     _check_products("experts_wgrad_sr_accum", weight, offsets, x, dy)
     x, dy = _rows(x), _rows(dy)
+    first = not hasattr(weight, "acc_grad")
+    if not first:
+        _lib.check_accumulator(weight, "experts_wgrad_sr_accum")
     if seed is None:
         seed = random.getrandbits(32)
-    first = not hasattr(weight, "acc_grad")
     if first:
         weight.acc_grad = torch.empty_like(weight, memory_format=torch.contiguous_format)
     acc = weight.acc_grad

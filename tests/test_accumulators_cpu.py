@@ -109,3 +109,30 @@ def test_a_weight_that_is_computed_returns_its_gradient(library, make):
     f(x).backward(torch.ones(5, 24, dtype=BF16))
     grad = layer.parametrizations.weight.original.grad
     assert library.calls == [] and torch.equal(grad.view(24, 16), 2 * (torch.ones(24, 5, dtype=BF16) @ x))
+
+
+def accumulate_experts(weight, seed=5):
+    from muon_sr_amd import experts_wgrad_sr_accum
+    x, dy = torch.zeros(5, 16, dtype=BF16), torch.zeros(5, 24, dtype=BF16)
+    experts_wgrad_sr_accum(weight, x, dy, torch.tensor([0, 5], dtype=torch.int32), seed=seed)
+
+
+CALLS = [(accumulate_experts, (1, 24, 16))]
+called = pytest.mark.parametrize("call,shape", CALLS, ids=[c.__name__ for c, _ in CALLS])
+
+
+@called
+def test_a_buffer_that_is_no_accumulator_is_refused(library, call, shape):
+    """Another type, order, size or device than the kernel writes."""
+    weight = torch.nn.Parameter(torch.zeros(shape, dtype=BF16))
+    turned = torch.zeros(shape, dtype=BF16).transpose(-1, -2).contiguous().transpose(-1, -2)
+    smaller = torch.zeros(shape, dtype=BF16)[..., :8].contiguous()
+    for buffer in (torch.zeros(shape), turned, smaller, torch.zeros(24 * 16, dtype=BF16),
+                   torch.zeros(shape, dtype=BF16, device="meta"), None):
+        weight.acc_grad = buffer
+        with pytest.raises(ValueError, match="acc_grad"):
+            call(weight)
+        assert library.calls == [] and weight.acc_grad is buffer
+    weight.acc_grad = torch.zeros(shape, dtype=BF16)
+    call(weight)
+    assert library.calls == [0]

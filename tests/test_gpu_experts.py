@@ -308,3 +308,16 @@ def test_refusals(L):
     assert L.msr_experts_dgrad(dy.data_ptr() + 2, 16, w.data_ptr(), x.data_ptr(), off.data_ptr(), 8, 2, 24, 16, stream()) == 1002
     assert _lib.lib().msr_experts_wgrad(w.data_ptr(), x.data_ptr(), 23, dy.data_ptr(), 16, off.data_ptr(), 8, 2, 24, 16,
                                         stream()) == 1001
+
+
+def test_accumulators_of_another_kind_are_refused(L):
+    """A buffer of another type, order or size is refused and stays as it was."""
+    from muon_sr_amd import experts_wgrad_sr_accum
+    s = make([4, 4], 0, 16, 24, 18)
+    w = torch.nn.Parameter(s["w"])
+    for buffer in (torch.zeros(2, 16, 24, device=DEV), torch.zeros(2, 24, 16, dtype=BF16, device=DEV).transpose(1, 2),
+                   torch.zeros(2, 16, 16, dtype=BF16, device=DEV), torch.zeros(2, 16, 24, dtype=BF16)):
+        w.acc_grad = buffer
+        with pytest.raises(ValueError, match="acc_grad"):
+            experts_wgrad_sr_accum(w, s["x"], s["dy"], s["off"])
+        assert w.acc_grad is buffer and not buffer.any()
