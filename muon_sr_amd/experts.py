@@ -251,14 +251,14 @@ def experts_wgrad_sr_accum(weight: torch.Tensor, x: torch.Tensor, dy: torch.Tens
         _lib.check_accumulator(weight, "experts_wgrad_sr_accum")
     if seed is None:
         seed = random.getrandbits(32)
-    if first:
-        weight.acc_grad = torch.empty_like(weight, memory_format=torch.contiguous_format)
-    acc = weight.acc_grad
+    acc = torch.empty_like(weight, memory_format=torch.contiguous_format) if first else weight.acc_grad
     E, o, i = weight.shape
     rc = _lib.lib().msr_experts_wgrad_sr_accum(acc.data_ptr(), x.data_ptr(), x.stride(0), dy.data_ptr(), dy.stride(0),
                                                offsets.data_ptr(), x.shape[0], E, i, o, seed, int(first),
                                                _lib.noise_mode(), None, _lib.stream_of(acc))
     _lib.check(rc, "msr_experts_wgrad_sr_accum")
+    if first:
+        weight.acc_grad = acc
 
 
 class _ExpertLinear(torch.autograd.Function):

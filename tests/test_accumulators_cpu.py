@@ -136,3 +136,17 @@ def test_a_buffer_that_is_no_accumulator_is_refused(library, call, shape):
     weight.acc_grad = torch.zeros(shape, dtype=BF16)
     call(weight)
     assert library.calls == [0]
+
+
+@called
+def test_a_refused_first_call_leaves_no_accumulator(library, call, shape):
+    from muon_sr_amd import _lib
+    weight = torch.nn.Parameter(torch.zeros(shape, dtype=BF16))
+    library.status = 1005
+    with pytest.raises(_lib.MuonSRLibraryError, match="refused"):
+        call(weight)
+    assert not hasattr(weight, "acc_grad")
+    library.status = 0
+    call(weight)
+    call(weight)
+    assert library.calls == [1, 1, 0] and weight.acc_grad.shape == shape

@@ -321,3 +321,15 @@ def test_accumulators_of_another_kind_are_refused(L):
         with pytest.raises(ValueError, match="acc_grad"):
             experts_wgrad_sr_accum(w, s["x"], s["dy"], s["off"])
         assert w.acc_grad is buffer and not buffer.any()
+
+
+def test_a_refused_first_accumulation_leaves_no_buffer(L):
+    from muon_sr_amd import experts_wgrad_sr_accum
+    s = make([4, 4], 0, 16, 24, 19)
+    w, fresh = torch.nn.Parameter(s["w"]), torch.nn.Parameter(s["w"].clone())
+    with pytest.raises(ctypes.ArgumentError):
+        experts_wgrad_sr_accum(w, s["x"], s["dy"], s["off"], seed="7")
+    assert not hasattr(w, "acc_grad")
+    for weight in (w, fresh):
+        experts_wgrad_sr_accum(weight, s["x"], s["dy"], s["off"], seed=7)
+    assert torch.equal(w.acc_grad, fresh.acc_grad)
