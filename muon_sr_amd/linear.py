@@ -50,15 +50,17 @@ def linear_wgrad_sr_accum(weight: torch.Tensor, x2: torch.Tensor, dy2: torch.Ten
     """``weight.acc_grad <- SR(weight.acc_grad + bf16(dy2^T x2))`` in one kernel.
 
     x2: bf16 [tokens, in], dy2: bf16 [tokens, out] (unit column stride), weight:
-    [out, in].  The buffer is created (as zeros) on the first call.  Returns
-    False, with nothing done, when the shapes or dtypes do not fit the fused
-    kernel.
+    [out, in].  The buffer is created (as zeros) on the first call, and one that
+    is there has to be like it (ValueError).  Returns False, with nothing
+    done, when the shapes or dtypes do not fit the fused kernel.
     """
     if not _fits(weight, x2, dy2):
         return False
+    first = not hasattr(weight, "acc_grad")
+    if not first:
+        _lib.check_accumulator(weight, "linear_wgrad_sr_accum")
     if seed is None:
         seed = random.getrandbits(32)
-    first = not hasattr(weight, "acc_grad")
     if first:
         weight.acc_grad = torch.empty_like(weight, dtype=torch.bfloat16, memory_format=torch.contiguous_format)
     acc = weight.acc_grad

@@ -117,7 +117,12 @@ def accumulate_experts(weight, seed=5):
     experts_wgrad_sr_accum(weight, x, dy, torch.tensor([0, 5], dtype=torch.int32), seed=seed)
 
 
-CALLS = [(accumulate_experts, (1, 24, 16))]
+def accumulate_linear(weight, seed=5):
+    from muon_sr_amd import linear_wgrad_sr_accum
+    assert linear_wgrad_sr_accum(weight, torch.zeros(5, 16, dtype=BF16), torch.zeros(5, 24, dtype=BF16), seed=seed)
+
+
+CALLS = [(accumulate_experts, (1, 24, 16)), (accumulate_linear, (24, 16))]
 called = pytest.mark.parametrize("call,shape", CALLS, ids=[c.__name__ for c, _ in CALLS])
 
 
@@ -138,7 +143,7 @@ def test_a_buffer_that_is_no_accumulator_is_refused(library, call, shape):
     assert library.calls == [0]
 
 
-@called
+@pytest.mark.parametrize("call,shape", CALLS[:1], ids=["accumulate_experts"])
 def test_a_refused_first_call_leaves_no_accumulator(library, call, shape):
     from muon_sr_amd import _lib
     weight = torch.nn.Parameter(torch.zeros(shape, dtype=BF16))
