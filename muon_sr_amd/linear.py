@@ -61,14 +61,14 @@ def linear_wgrad_sr_accum(weight: torch.Tensor, x2: torch.Tensor, dy2: torch.Ten
         _lib.check_accumulator(weight, "linear_wgrad_sr_accum")
     if seed is None:
         seed = random.getrandbits(32)
-    if first:
-        weight.acc_grad = torch.empty_like(weight, dtype=torch.bfloat16, memory_format=torch.contiguous_format)
-    acc = weight.acc_grad
+    acc = torch.empty_like(weight, dtype=torch.bfloat16, memory_format=torch.contiguous_format) if first else weight.acc_grad
     out_f, in_f = weight.shape
     rc = _lib.lib().msr_linear_wgrad_sr_accum(acc.data_ptr(), x2.data_ptr(), x2.stride(0), dy2.data_ptr(),
                                               dy2.stride(0), x2.shape[0], in_f, out_f, seed, int(first),
                                               _lib.noise_mode(), None, _lib.stream_of(acc))
     _lib.check(rc, "msr_linear_wgrad_sr_accum")
+    if first:
+        weight.acc_grad = acc
     return True
 
 

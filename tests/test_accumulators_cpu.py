@@ -143,7 +143,7 @@ def test_a_buffer_that_is_no_accumulator_is_refused(library, call, shape):
     assert library.calls == [0]
 
 
-@pytest.mark.parametrize("call,shape", CALLS[:1], ids=["accumulate_experts"])
+@called
 def test_a_refused_first_call_leaves_no_accumulator(library, call, shape):
     from muon_sr_amd import _lib
     weight = torch.nn.Parameter(torch.zeros(shape, dtype=BF16))
