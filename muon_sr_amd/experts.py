@@ -150,7 +150,8 @@ class _Combine(torch.autograd.Function):
     @staticmethod
     @_once
     def backward(ctx, dy):
-        rows, weights = ctx.saved_tensors
+        rows, weights = ctx.saved_tensors     # saved-tensor hooks may have changed their strides
+        rows, weights = _contiguous(rows), weights.contiguous()
         order = ctx.order
         tokens, k = order.position.shape
         d = rows.shape[1]
@@ -274,8 +275,8 @@ class _ExpertLinear(torch.autograd.Function):
     @staticmethod
     @_once
     def backward(ctx, dy):
-        x, weight, offsets = ctx.saved_tensors
-        dy = _rows(dy)
+        x, weight, offsets = ctx.saved_tensors     # saved-tensor hooks may have changed their strides
+        x, weight, offsets, dy = _rows(x), weight.contiguous(), offsets.contiguous(), _rows(dy)
         dx = _dgrad(dy, weight, offsets) if ctx.needs_input_grad[0] else None
         dw = None
         if ctx.needs_input_grad[1]:

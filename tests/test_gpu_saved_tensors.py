@@ -76,3 +76,32 @@ def test_linear_accumulates(way):
     f = lambda x: layer(torch.cat([x, x[:67]]))  # noqa: E731   (256 tokens)
     cut = lambda x: f(x)[:189]  # noqa: E731
     assert all(torch.equal(a, b) for a, b in zip(accumulated(layer, cut, direct), accumulated(layer, cut, way)))
+
+
+def turned(f, *args):
+    """Tensors come back with their last dimension of the largest stride, vectors with gaps."""
+    def columns(t):
+        return torch.stack([t, t], 1)[:, 0] if t.dim() == 1 else t.transpose(-1, -2).contiguous().transpose(-1, -2)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, columns):
+        return f(*args)
+
+
+@pytest.mark.parametrize("way", [checkpointed, offloaded, hooked, turned], ids=lambda f: f.__name__)
+def test_layer_of_operators(way):
+    """dispatch, the experts' products and combine: every input's gradient."""
+    from muon_sr_amd import combine_tokens, dispatch_tokens, expert_linear, order_tokens
+    ids = torch.randint(-1, 5, (301, 2), generator=gen(1), device=DEV)
+    tensors = [randn((301, 72), 2), torch.rand((301, 2), generator=gen(3), device=DEV), randn((5, 136, 72), 4), randn((5, 72, 136), 5)]
+    dy = randn((301, 72), 6)
+
+    def layer(x, w, up, down):
+        order = order_tokens(ids, 5)
+        rows = expert_linear(dispatch_tokens(x, order), up, order.offsets)
+        return combine_tokens(expert_linear(rows, down, order.offsets), w, order)
+
+    results = []
+    for how in (direct, way):
+        leaves = [t.clone().requires_grad_(True) for t in tensors]
+        y = how(layer, *leaves)
+        results.append([y, *torch.autograd.grad(y, leaves, dy)])
+    assert all(torch.equal(a, b) for a, b in zip(*results))
