@@ -5,10 +5,13 @@
 // gradients are the least: 2 (or 4) bytes read, then as many read and 2 (or 4) written per
 // element.  Both are bound by HBM.  Each pass takes many tensors per launch (a table in the
 // kernel arguments):
-//   1. norm_kernel   work-groups over tiles of all tensors, one partial sum each
-//   2. clip_kernel   every work-group first adds the partial sums itself (at most a few
-//                    thousand numbers, from L2, in the same order everywhere), which saves
-//                    a launch and its gap between the two passes
+//   1. norm_kernel   work-groups over tiles of all tensors, one partial sum each, to which the
+//                    work-groups of the same number in later launches add theirs, so that a list of
+//                    any length has at most CLIP_GRID of them (clipping 9000 tensors of 2^17: 1.90 ms,
+//                    with new partial sums from each launch, which every work-group reads, 4.78)
+//   2. clip_kernel   every work-group first adds the partial sums itself (8 KiB at most, from L2,
+//                    in the same order everywhere), which saves a launch and its gap between the
+//                    two passes
 // Squares and their sums are held in 64 bits: bf16 and fp32 gradients have the same
 // exponents, and the square of 1e20 does not fit 32 bits, nor does that of 1e-23.
 #include <math.h>
@@ -148,10 +151,11 @@ __device__ __forceinline__ void norm_tile(const void *g, int64_t at, int64_t n, 
         for (int j = 0; j < 8; ++j) norm_add<P>(j & 1 ? s1 : s0, f[u][j]);
 }
 
+// have: partial sums that earlier launches wrote
 template <int P>
-__global__ __launch_bounds__(CLIP_THREADS) void norm_kernel(ClipArgs a, double *partial) {
+__global__ __launch_bounds__(CLIP_THREADS) void norm_kernel(ClipArgs a, double *partial, int have) {
     __shared__ double red[CLIP_THREADS / 64];
-    double s0 = 0.0, s1 = 0.0;
+    double s0 = threadIdx.x == 0 && (int)blockIdx.x < have ? partial[blockIdx.x] : 0.0, s1 = 0.0;
     int i = 0;
     for (int t = blockIdx.x; t < a.start[a.count]; t += gridDim.x) {
         while (t >= a.start[i + 1]) ++i;
@@ -257,11 +261,11 @@ static int clip_check(const msr_clip_item *items, int32_t count, bool outs, cons
     return MSR_OK;
 }
 
-// The partial sums of a list: one per work-group of its norm launches.
+// The partial sums of a list: one per work-group of its largest norm launch.
 static int clip_parts(const msr_clip_item *items, int32_t count) {
     ClipArgs a;
     int parts = 0;
-    for (int32_t i = 0; i < count;) parts += (int)clip_fill(a, items, count, i, false);
+    for (int32_t i = 0; i < count;) parts = std::max(parts, (int)clip_fill(a, items, count, i, false));
     return parts;
 }
 
@@ -303,9 +307,9 @@ static int clip_run(const msr_clip_item *items, int32_t count, bool outs, float 
     for (int32_t i = 0; i < count;) {
         const unsigned grid = clip_fill(a, items, count, i, false);
         if (!grid) break;
-        hipLaunchKernelGGL((norm_kernel<P>), dim3(grid), dim3(CLIP_THREADS), 0, s, a, partial + parts);
+        hipLaunchKernelGGL((norm_kernel<P>), dim3(grid), dim3(CLIP_THREADS), 0, s, a, partial, parts);
         if ((rc = check_launch("norm_kernel"))) return rc;
-        parts += (int)grid;
+        parts = std::max(parts, (int)grid);
     }
     if (!outs || !parts) {
         hipLaunchKernelGGL((norm_finish_kernel<P>), dim3(1), dim3(CLIP_THREADS), 0, s, partial, parts, norm_out);

@@ -231,3 +231,20 @@ def test_refusals():
     assert clip_grads([h], 1e-3).item() == grad_norm([kept]).item() and not torch.equal(h, kept)
     # reading the same memory twice is no conflict
     assert abs(grad_norm([g, g]).item() - math.sqrt(2) * norm64([g], 2.0)) <= 2.0 ** -22 * norm64([g], 2.0)
+
+
+@pytest.mark.parametrize("p", [1.0, 2.0, math.inf])
+@pytest.mark.parametrize("where", [None, 3, 150, 400])
+def test_lists_of_several_launches(where, p):
+    """Launches of few, many, and few work-groups again, whose partial sums join; a NaN in any of them reaches the norm."""
+    from muon_sr_amd import clip_grads, grad_norm
+    grads = [randn(n, BF16, 20 + i, 1e-2 * (1 + i % 5)) for i, n in enumerate([5] * 112 + [90001] * 112 + [9, 3000] * 100)]
+    ref = norm64(grads, p)
+    if where is not None:
+        grads[where][-1] = math.nan
+    got, kept = grad_norm(grads, p), [g.clone() for g in grads]
+    assert math.isnan(got.item()) if where is not None else abs(got.item() - ref) <= 2.0 ** -23 * ref
+    norm = clip_grads(grads, 0.37 * ref, p)
+    same(norm.view(1), got.view(1))
+    for g, k in zip(grads, kept):
+        same(g, expect(k, norm, 0.37 * ref, BF16))

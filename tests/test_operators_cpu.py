@@ -116,3 +116,12 @@ def test_python_needs_a_gpu_and_fitting_arguments(lib):
     assert layer.weight.abs().max() <= 1 / math.sqrt(16)
     with pytest.raises(ValueError, match="GPU"):
         layer(torch.zeros((2, 16), dtype=torch.bfloat16), torch.zeros(4, dtype=torch.int32))
+
+
+def test_the_norms_workspace_does_not_grow_with_the_list(lib):
+    """Every work-group of a clip launch adds up all partial sums: they stay at one per work-group of a launch."""
+    size = ctypes.c_size_t()
+    for tensors in (1, 113, 1000, 9000):
+        assert lib.msr_grad_norm_workspace_bytes(*items(*[(A + (i << 24), 0, 1 << 22, 0) for i in range(tensors)]),
+                                                 ctypes.byref(size)) == 0
+        assert 8 <= size.value <= 8 * 4096
