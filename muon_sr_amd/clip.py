@@ -6,9 +6,10 @@
     opt.step()
 
 ``clip_grad_norm_`` takes the place of ``torch.nn.utils.clip_grad_norm_`` (the reference's
-training loops would call that one): the same arguments, result and treatment of non-finite
-norms, many tensors per kernel launch, and sums in 64 bits.  Nothing synchronises with the
-host, except for ``error_if_nonfinite``.
+training loops would call that one): the same arguments and treatment of non-finite norms, for
+bf16 and fp32 gradients on one GPU and the norms 1, 2 and inf (others are refused); many tensors
+per kernel launch, sums in 64 bits, and a norm in fp32 whatever the gradients' type.  Nothing
+synchronises with the host, except for ``error_if_nonfinite``.
 """
 from __future__ import annotations
 
@@ -151,10 +152,12 @@ def clip_grads(grads, max_norm: float, norm_type: float = 2.0, out=None) -> torc
     return _run(grads, outs, norm_type, float(max_norm), "clip_grads")
 
 
-def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_if_nonfinite: bool = False) -> torch.Tensor:
-    """``torch.nn.utils.clip_grad_norm_`` for bf16 and fp32 gradients on one GPU: clips the ``.grad`` of
-    ``parameters`` in place and returns their norm.  With ``error_if_nonfinite`` the norm is waited for, and
-    a non-finite one raises RuntimeError with the gradients as they were."""
+def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_if_nonfinite: bool = False,
+                    foreach: bool = None) -> torch.Tensor:
+    """``torch.nn.utils.clip_grad_norm_`` for bf16 and fp32 gradients on one GPU and norms 1, 2 and inf: clips
+    the ``.grad`` of ``parameters`` in place and returns their norm (fp32).  With ``error_if_nonfinite`` the norm is
+    waited for, and a non-finite one raises RuntimeError with the gradients as they were.  ``foreach``, which
+    chooses an implementation in torch, changes nothing."""
     parameters = [parameters] if isinstance(parameters, torch.Tensor) else parameters
     grads = [p.grad for p in parameters if p.grad is not None]
     if not grads:

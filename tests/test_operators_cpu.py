@@ -125,3 +125,11 @@ def test_the_norms_workspace_does_not_grow_with_the_list(lib):
         assert lib.msr_grad_norm_workspace_bytes(*items(*[(A + (i << 24), 0, 1 << 22, 0) for i in range(tensors)]),
                                                  ctypes.byref(size)) == 0
         assert 8 <= size.value <= 8 * 4096
+
+
+def test_clip_grad_norm_takes_the_arguments_of_torchs():
+    import inspect
+    import muon_sr_amd as M
+    want, got = (list(inspect.signature(f).parameters.values()) for f in (torch.nn.utils.clip_grad_norm_, M.clip_grad_norm_))
+    assert [(p.name, p.default) for p in got] == [(p.name, p.default) for p in want]
+    assert M.clip_grad_norm_([], 1.0, foreach=True).item() == 0.0
