@@ -142,7 +142,8 @@ def clip_grads(grads, max_norm: float, norm_type: float = 2.0, out=None) -> torc
     gradient: of its type, or bf16 for an fp32 one, say the ``.grad`` that an optimizer of bf16
     parameters will read), into ``out``.  Returns the norm before clipping, as ``grad_norm`` does.
     The product is formed in fp32 and rounded once.  A NaN norm makes every gradient NaN, an infinite one
-    makes the finite gradients 0, as in torch.  Tensors that share memory are refused."""
+    makes the finite gradients 0, as in torch.  Tensors that share memory are refused, except that sharing is
+    not noticed between tensors with gaps between their elements, which go through copies."""
     grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
     outs = grads if out is None else [out] if isinstance(out, torch.Tensor) else list(out)
     if len(outs) != len(grads):
