@@ -17,6 +17,7 @@ import argparse
 import glob
 import os
 import sys
+import sysconfig
 
 import torch
 import torch.nn as nn
@@ -80,13 +81,16 @@ def param_groups(model):
             dict(params=rest, lr=2e-3, betas=(0.9, 0.95), eps=1e-10, weight_decay=0.0, use_muon=False)]
 
 
-def corpus(limit=4 << 20):
-    text = b""
-    for name in sorted(glob.glob("/usr/lib/python3*/*.py")):
+def corpus(folder=None, limit=4 << 20):
+    """The text of a folder's Python files (default: the running interpreter's standard library), as bytes."""
+    folder, text = folder or sysconfig.get_paths()["stdlib"], b""
+    for name in sorted(glob.glob(os.path.join(folder, "*.py"))):
         with open(name, "rb") as f:
             text += f.read()
         if len(text) >= limit:
             break
+    if len(text) < 1 << 16:
+        raise RuntimeError(f"{folder} has only {len(text)} bytes of Python files to train on; 65536 are the least")
     return torch.frombuffer(bytearray(text[:limit]), dtype=torch.uint8).long()
 
 
