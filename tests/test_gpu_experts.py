@@ -333,3 +333,42 @@ def test_a_refused_first_accumulation_leaves_no_buffer(L):
     for weight in (w, fresh):
         experts_wgrad_sr_accum(weight, s["x"], s["dy"], s["off"], seed=7)
     assert torch.equal(w.acc_grad, fresh.acc_grad)
+
+
+def guarded(rows, cols, ld, fill, seed=None):
+    """A [rows, cols] view of row stride ld, 64 elements into a buffer of `fill` that is longer by 4096; random
+    values with a seed."""
+    buffer = torch.full((rows * ld + 64 + 4096,), fill, dtype=BF16, device=DEV)
+    view = buffer[64:64 + rows * ld].view(rows, ld)[:, :cols]
+    if seed is not None:
+        view.copy_(torch.randn((rows, cols), generator=gen(seed), device=DEV))
+    return buffer, view
+
+
+@pytest.mark.parametrize("pad", [0, 24])
+@pytest.mark.parametrize("E,rows,fout,fin", [(3, 100, 72, 136), (63, 700, 72, 136), (64, 700, 72, 136), (65, 700, 136, 264),
+                                             (1024, 2000, 24, 40), (1000, 300, 8, 8), (65, 9000, 520, 776), (5, 6000, 1544, 2056),
+                                             (2, 3, 136, 4104), (2, 3, 4104, 136), (5, 9000, 2056, 3080)])
+def test_no_offsets_reach_outside_the_operands(L, E, rows, fout, fin, pad):
+    """Offsets that ascend and offsets that do not: with NaN around the inputs every output is finite, and what
+    lies around the outputs is as it was."""
+    g = torch.Generator().manual_seed(E + rows)
+    _, x = guarded(rows, fin, fin + pad, float("nan"), 1)
+    _, dy = guarded(rows, fout, fout + pad, float("nan"), 2)
+    _, w = guarded(E * fout, fin, fin, float("nan"), 3)
+    ascending = torch.randint(0, rows + 1, (E + 1,), generator=g).sort().values
+    ascending[0] = 0
+    for offsets in (ascending, ascending.flip(0), torch.randint(-50, rows + 50, (E + 1,), generator=g),
+                    torch.where(torch.arange(E + 1) % 2 == 0, 0, rows), torch.full((E + 1,), -(1 << 31)),
+                    torch.where(torch.arange(E + 1) % 2 == 0, -(1 << 31), (1 << 31) - 1)):
+        off = offsets.to(torch.int32).to(DEV)
+        outs = [guarded(n, c, c, 7.0) for n, c in ((rows, fout), (rows, fin), (E * fout, fin), (E * fout, fin))]
+        y, dx, dw, acc = (v.data_ptr() for _, v in outs)
+        op = (x.data_ptr(), fin + pad, dy.data_ptr(), fout + pad, off.data_ptr(), rows, E, fin, fout)
+        check(L, L.msr_experts_forward(op[0], op[1], w.data_ptr(), y, *op[4:], stream()))
+        check(L, L.msr_experts_dgrad(op[2], op[3], w.data_ptr(), dx, *op[4:], stream()))
+        check(L, L.msr_experts_wgrad(dw, *op, stream()))
+        check(L, L.msr_experts_wgrad_sr_accum(acc, *op, 9, 0, 1, None, stream()))
+        for buffer, view in outs:
+            assert bool(torch.isfinite(view).all())
+            assert bool((buffer[:64] == 7.0).all()) and bool((buffer[64 + view.numel():] == 7.0).all())
