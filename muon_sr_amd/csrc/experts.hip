@@ -463,8 +463,14 @@ __global__ __launch_bounds__(64 * Shape<T>::NW * KG, WPS) void experts_kernel(Ex
 //   64 x 8,   (4096 x 1024)                                                  34  28  23
 //   16 x 8,   4096 x 4096 (272 tiles)          35  36  41                    36  52  48
 // ACC, 128: the accumulation has its noise to compute and its accumulators to wait for, which a fourth work-group per CU
-// hides better than a third stage (16411 x 64, 1024 x 2048: 145 us with 2 stages and 4 waves per SIMD, one row block
-// of accumulators fetched ahead; 149 with 3 and 3; 156 with 3, 3 and two blocks ahead).
+// hides better than a third stage.  us with 2 stages and 4 waves per SIMD (so); 3 and 3; 3, 3 and two row blocks of
+// accumulators fetched ahead instead of one, on one card, the same tensors every time and four sets of them in turn (no
+// operand left in the last-level cache):
+//   16411 x 64, 1024 x 2048   148 153 155   161 162 161
+//   32768 x 64, 1408 x 2048   303 311 311   327 331 330
+//   8192 x 32,  1024 x 2048    78  79  83    78  79  82
+//   16384 x 128, 768 x 2048   176 182 184   189 193 191
+//   4096 x 8,   1536 x 1536    37  37  36    40  37  37
 template <int KIND, bool ACC, int T, bool SPLIT>
 struct Ring {
     static constexpr bool FINE = KIND != EX_FWD && T >= 128;

@@ -7,7 +7,8 @@
 // each chunk, and the work-groups add its counts (a few thousand numbers from L2).  It then ranks its
 // slots wave by wave, 64 at a time by ballots, one per bit of the expert number: only the counts are
 // atomic, no order depends on them.  Dropped slots count as one more expert, which gives the rows without
-// a slot.  Bound by latency: one or two launches.
+// a slot.  One or two launches of some 4 (14 slots) to 18 us (262144 of them), far above what their bytes take; how much
+// of that is latency and how much the LDS atomics, two per slot up to ORD_SELF, was not told apart.
 //
 // The four passes between tokens and rows (see the header) move d elements per slot and do
 // next to nothing with them, so HBM bounds them.  All are written from the token's side: a piece of a
