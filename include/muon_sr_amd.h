@@ -476,6 +476,104 @@ int msr_experts_wgrad_sr_accum(uint16_t *acc, const uint16_t *x, int64_t ldx, co
                                const uint16_t *inject, msr_stream_t stream);
 
 /* ---------------------------------------------------------------------------
+ * A language model's head with its softmax cross entropy, in pieces of the
+ * vocabulary: the logits are never in memory.  No counterpart in the reference.
+ *   S[n][v] = <x[n], W[v]>,  l[n] = log sum_v exp S[n][v],  loss[n] = l[n] - S[n][t[n]]
+ *   G[n][v] = g[n] (exp(S[n][v] - l[n]) - [v = t[n]]),  dx = G W,  dW = G^T x
+ * x: bf16, rows of ldx elements, any 2-byte alignment; W: bf16 [vocab][d],
+ * 16-byte aligned; target: int32, or int64 with target_i64.  Rows whose target is
+ * ignore_index have loss 0 and gradient 0, and what they hold reaches nothing; any
+ * other target outside [0, vocab) makes its loss NaN, and with it the gradients.
+ * reduction: MSR_LOSS_NONE (loss [rows]), _SUM or _MEAN over the rows that are not
+ * ignored (loss [1]; 0 where there are none).  Products are of bf16 operands with
+ * fp32 accumulation (G rounded to bf16), dx and dW rounded once.
+ *
+ * msr_head_forward also writes what the backward pass reads: packed (bf16
+ * [rows][d], 16-byte aligned: the rows that are not ignored, one after the other), kept
+ * (int32 [3 * rows + 1]: their number, their places in x, their targets, and every
+ * row's place in packed, or -1) and lse (fp32 [rows], packed order).
+ * msr_head_backward: dloss fp32 [rows] with MSR_LOSS_NONE, else [1].  dx [rows][d]
+ * or dw [vocab][d] may be NULL (not wanted).  noise_mode -1 stores dw; a noise mode
+ * accumulates dw <- SR(dw + f32(bf16(dW))) with the arithmetic and noise of
+ * msr_sr_accum on [vocab][d] (seed, zero_init and inject as there).
+ * rows and vocab below 2^24, rows * vocab below 2^40, d a multiple of 8 up to 2^16.
+ * workspaces: msr_head_workspace_bytes, 16-byte aligned.  The order of the sums, and so
+ * their last bits, may depend on the sizes of the call; the same call gives the same bits.
+ * ------------------------------------------------------------------------- */
+#define MSR_LOSS_NONE 0
+#define MSR_LOSS_SUM 1
+#define MSR_LOSS_MEAN 2
+int msr_head_workspace_bytes(int64_t rows, int64_t vocab, int64_t d, size_t *forward, size_t *backward);
+int msr_head_forward(const uint16_t *x, int64_t ldx, const uint16_t *w, const void *target, int32_t target_i64,
+                     int64_t ignore_index, int64_t rows, int64_t vocab, int64_t d, int32_t reduction, uint16_t *packed,
+                     int32_t *kept, float *lse, float *loss, void *workspace, size_t workspace_bytes, msr_stream_t stream);
+int msr_head_backward(const uint16_t *packed, const uint16_t *w, const int32_t *kept, const float *lse, const float *dloss,
+                      int64_t rows, int64_t vocab, int64_t d, int32_t reduction, uint16_t *dx, uint16_t *dw,
+                      int32_t noise_mode, uint32_t seed, int32_t zero_init, const uint16_t *inject, void *workspace,
+                      size_t workspace_bytes, msr_stream_t stream);
+
+/* ---------------------------------------------------------------------------
+ * Embedding, and its gradient by sorted tokens.  No counterpart in the reference.
+ *   msr_embedding                 y[i] = round(scale * W[ids[i]]), 0 for an id outside [0, vocab)
+ *   msr_embedding_grad            dw[v] = round(scale * sum_{i: ids[i] = v} dy[i]), 0 without a token
+ *   msr_embedding_grad_sr_accum   acc[v] <- SR(acc[v] + f32(bf16(dw[v]))) with the arithmetic and noise of
+ *                                 msr_sr_accum on [vocab][d]; words without a token are not touched (with
+ *                                 zero_init they are set to 0)
+ * Sums in fp32, tokens in order (in parts of up to 32).  Ids outside [0, vocab) and the id
+ * `padding` (negative: none) give no gradient.  ids: int32, or int64 with ids_i64; W, y, dy, dw: elem
+ * (MSR_BF16 or MSR_F32), contiguous but for dy's row stride lddy; aligned to their
+ * types.  Fewer than 2^28 tokens and 2^27 words.  workspace:
+ * msr_embedding_workspace_bytes, 8-byte aligned.
+ * ------------------------------------------------------------------------- */
+int msr_embedding(const void *ids, int32_t ids_i64, int64_t n, const void *w, int64_t vocab, int64_t d, float scale, void *y,
+                  int32_t elem, msr_stream_t stream);
+int msr_embedding_workspace_bytes(int64_t n, int64_t vocab, int64_t d, size_t *bytes);
+int msr_embedding_grad(const void *ids, int32_t ids_i64, int64_t n, const void *dy, int64_t lddy, int64_t vocab, int64_t d,
+                       float scale, int64_t padding, void *dw, int32_t elem, void *workspace, size_t workspace_bytes,
+                       msr_stream_t stream);
+int msr_embedding_grad_sr_accum(const void *ids, int32_t ids_i64, int64_t n, const uint16_t *dy, int64_t lddy, int64_t vocab,
+                                int64_t d, float scale, int64_t padding, uint16_t *acc, uint32_t seed, int32_t zero_init,
+                                int32_t noise_mode, const uint16_t *inject, void *workspace, size_t workspace_bytes,
+                                msr_stream_t stream);
+
+/* ---------------------------------------------------------------------------
+ * Layer norm over rows of d elements, and its gradient.  No counterpart in the
+ * reference.
+ *   mean = mean(x), rstd = 1 / sqrt(mean((x - mean)^2) + eps), h = (x - mean) rstd, y = h w + b
+ *   q = dy w, dx = rstd (q - mean(q) - h mean(q h)), dw = sum_n dy h, db = sum_n dy
+ * x, y, dy, dx: elem, x and dy with row strides ldx and lddy; w (NULL: 1), b (NULL: 0), dw, db:
+ * welem.  Statistics and sums in fp32, one rounding.  mean and rstd (fp32 [rows]) are
+ * written by the forward pass and read by the other.  dx, dw, db may be NULL (not
+ * wanted).  Aligned to their types.  workspace: msr_layer_norm_workspace_bytes (dw or
+ * db wanted).  dw and db are sums in an order that depends on the sizes alone.
+ * ------------------------------------------------------------------------- */
+int msr_layer_norm(const void *x, int64_t ldx, const void *w, const void *b, float eps, int64_t rows, int64_t d, void *y,
+                   float *mean, float *rstd, int32_t elem, int32_t welem, msr_stream_t stream);
+int msr_layer_norm_workspace_bytes(int64_t rows, int64_t d, int32_t elem, size_t *bytes);
+int msr_layer_norm_grad(const void *dy, int64_t lddy, const void *x, int64_t ldx, const void *w, const float *mean,
+                        const float *rstd, int64_t rows, int64_t d, void *dx, void *dw, void *db, int32_t elem,
+                        int32_t welem, void *workspace, size_t workspace_bytes, msr_stream_t stream);
+
+/* ---------------------------------------------------------------------------
+ * A router's balance loss.  No counterpart in the reference.  For the n tokens whose
+ * mask (one byte each; NULL: all) is not 0,
+ *   p[t] = softmax(logits[t]), counts[e] = their slots (t, j) with ids[t][j] = e, f[e] = counts[e] / (n k)
+ *   loss = experts / n * sum_e f[e] sum_t p[t][e]      (0 where n is 0)
+ *   dlogits[t][e] = dloss p[t][e] (u[e] - sum_j u[j] p[t][j]), u[e] = experts / n f[e]; 0 for the other tokens
+ * ids outside [0, experts) are dropped slots.  Logits of -inf have probability 0 (a token without any
+ * other: 0 everywhere).  logits: elem, row stride ld; ids: int32, or int64 with ids_i64,
+ * contiguous [tokens][k]; counts int32 [experts]; lse (fp32 [tokens]) and slope (u, fp32
+ * [experts]) are written for the gradient.  tokens * k < 2^30, experts <= MSR_EXPERTS_MAX.
+ * workspace: msr_balance_workspace_bytes.
+ * ------------------------------------------------------------------------- */
+int msr_balance_workspace_bytes(int64_t tokens, int32_t experts, size_t *bytes);
+int msr_balance_loss(const void *logits, int64_t ld, const void *ids, int32_t ids_i64, const uint8_t *mask, int64_t tokens,
+                     int32_t experts, int32_t k, float *loss, int32_t *counts, float *lse, float *slope, int32_t elem,
+                     void *workspace, size_t workspace_bytes, msr_stream_t stream);
+int msr_balance_grad(const void *logits, int64_t ld, const uint8_t *mask, const float *lse, const float *slope,
+                     const float *dloss, int64_t tokens, int32_t experts, void *dlogits, int32_t elem, msr_stream_t stream);
+
+/* ---------------------------------------------------------------------------
  * Diagnostics (no counterpart in the reference; used by the parity tests).
  * ------------------------------------------------------------------------- */
 
@@ -548,6 +646,10 @@ int msr_tile_gemm(int32_t product, int32_t tile, int32_t stages, const uint16_t 
  * between groups of waves; product 0 forward, 1 dgrad, 2 wgrad, 3 wgrad_sr_accum.  Test support. */
 int msr_experts_tile(int32_t product, int64_t rows, int32_t experts, int64_t in_features, int64_t out_features, int32_t *tile,
                      int32_t *split);
+
+/* Host only: how a head of these sizes is computed: plan[7] = the tiles of the loss's logits, of the gradient's, of dx
+ * and its splits of the vocabulary, of dW and its splits of the rows, and the words of a piece.  Test support. */
+int msr_head_plan(int64_t rows, int64_t vocab, int64_t d, int32_t *plan);
 
 /* Batched bf16 GEMM  D[b] = alpha * P[b] Q[b]^T + beta * C[b] + diag * I  (fp32 accumulate, RNE
  * bf16 out; the diag term is added where m == n).

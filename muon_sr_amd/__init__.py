@@ -15,6 +15,10 @@ from .linear import SRLinear, linear_wgrad_sr_accum
 from .clip import clip_grad_norm_, clip_grads, grad_norm
 from .experts import (SRExperts, TokenOrder, combine_tokens, dispatch_tokens, expert_linear, experts_wgrad_sr_accum,
                       order_tokens)
+from .balance import balance_loss
+from .embedding import SREmbedding, embedding, embedding_grad_sr_accum
+from .head import SRHead, linear_cross_entropy
+from .norm import LayerNorm, layer_norm
 
 __all__ = [
     "TritonAdamW8bit",
@@ -25,4 +29,8 @@ __all__ = [
     "clip_grad_norm_", "clip_grads", "grad_norm",
     "TokenOrder", "order_tokens", "dispatch_tokens", "combine_tokens",
     "SRExperts", "expert_linear", "experts_wgrad_sr_accum",
+    "balance_loss",
+    "SREmbedding", "embedding", "embedding_grad_sr_accum",
+    "SRHead", "linear_cross_entropy",
+    "LayerNorm", "layer_norm",
 ]

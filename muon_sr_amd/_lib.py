@@ -121,6 +121,24 @@ SIGNATURES = {
     "msr_experts_wgrad_sr_accum": (ctypes.c_int, [_P, _P, _I64, _P, _I64, _P, _I64, _I32, _I64, _I64, _U32, _I32, _I32, _P,
                                                   _P]),
     "msr_experts_tile": (ctypes.c_int, [_I32, _I64, _I32, _I64, _I64, ctypes.POINTER(_I32), ctypes.POINTER(_I32)]),
+    "msr_head_workspace_bytes": (ctypes.c_int, [_I64, _I64, _I64, _SIZE_P, _SIZE_P]),
+    "msr_head_plan": (ctypes.c_int, [_I64, _I64, _I64, ctypes.POINTER(_I32)]),
+    "msr_head_forward": (ctypes.c_int, [_P, _I64, _P, _P, _I32, _I64, _I64, _I64, _I64, _I32, _P, _P, _P, _P, _P, ctypes.c_size_t,
+                                        _P]),
+    "msr_head_backward": (ctypes.c_int, [_P, _P, _P, _P, _P, _I64, _I64, _I64, _I32, _P, _P, _I32, _U32, _I32, _P, _P,
+                                         ctypes.c_size_t, _P]),
+    "msr_embedding": (ctypes.c_int, [_P, _I32, _I64, _P, _I64, _I64, _F, _P, _I32, _P]),
+    "msr_embedding_workspace_bytes": (ctypes.c_int, [_I64, _I64, _I64, _SIZE_P]),
+    "msr_embedding_grad": (ctypes.c_int, [_P, _I32, _I64, _P, _I64, _I64, _I64, _F, _I64, _P, _I32, _P, ctypes.c_size_t, _P]),
+    "msr_embedding_grad_sr_accum": (ctypes.c_int, [_P, _I32, _I64, _P, _I64, _I64, _I64, _F, _I64, _P, _U32, _I32, _I32, _P, _P,
+                                                   ctypes.c_size_t, _P]),
+    "msr_layer_norm": (ctypes.c_int, [_P, _I64, _P, _P, _F, _I64, _I64, _P, _P, _P, _I32, _I32, _P]),
+    "msr_layer_norm_workspace_bytes": (ctypes.c_int, [_I64, _I64, _I32, _SIZE_P]),
+    "msr_layer_norm_grad": (ctypes.c_int, [_P, _I64, _P, _I64, _P, _P, _P, _I64, _I64, _P, _P, _P, _I32, _I32, _P,
+                                           ctypes.c_size_t, _P]),
+    "msr_balance_workspace_bytes": (ctypes.c_int, [_I64, _I32, _SIZE_P]),
+    "msr_balance_loss": (ctypes.c_int, [_P, _I64, _P, _I32, _P, _I64, _I32, _I32, _P, _P, _P, _P, _I32, _P, ctypes.c_size_t, _P]),
+    "msr_balance_grad": (ctypes.c_int, [_P, _I64, _P, _P, _P, _P, _I64, _I32, _P, _I32, _P]),
     "msr_noise_fill": (ctypes.c_int, [_P, _I64, _I64, _U32, _U32, _I32, _P]),
     "msr_stream_probe8": (ctypes.c_int, [_P, _P, _P, _P, _P, _P, _I64, _I32, _I32, _P]),
     "msr_quantize": (ctypes.c_int, [_P, _P, _I64, _P, _I32, _P, _P]),
@@ -183,6 +201,26 @@ def stream_of(t: torch.Tensor):
     if _raw_stream is not None:
         return _raw_stream(t.get_device())
     return torch.cuda.current_stream(t.device).cuda_stream
+
+
+def call(t: torch.Tensor, name: str, *args) -> None:
+    """The entry point `name` on t's device and that device's current stream, which is its last argument."""
+    fn, device = getattr(lib(), name), t.get_device()
+    if device == torch.cuda.current_device():
+        rc = fn(*args, stream_of(t))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, stream_of(t))
+    check(rc, name)
+
+
+def workspace(t: torch.Tensor, size: int):
+    """Scratch memory of a call on t's device (None for none)."""
+    return torch.empty(size, dtype=torch.uint8, device=t.device) if size else None
+
+
+def ptr(t):
+    return None if t is None else t.data_ptr()
 
 
 def ptr_array(ptrs, ctype=ctypes.c_void_p):

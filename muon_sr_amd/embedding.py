@@ -1,0 +1,138 @@
+"""Embedding with scaling, and its gradient by sorted tokens.
+
+    y = embedding(ids, weight, scale=scale)      # scale * weight[ids]
+
+``SREmbedding`` is to ``nn.Embedding`` what ``SRLinear`` is to ``nn.Linear``: its gradient is added to
+``weight.acc_grad`` with stochastic rounding, with the arithmetic, seeds and noise of ``TritonSRAccumulator``'s hook
+(muon_sr/triton_adamw.py:206-229, 252-265), row by row of the words that the tokens hit, where the hook
+reads a whole gradient and accumulator.  Sums are formed in fp32 in a fixed order: the same call gives the
+same bits.  The reference's training loops call torch's embedding.
+"""
+from __future__ import annotations
+
+import ctypes
+import random
+
+import torch
+
+from . import _lib
+from .experts import _ELEM, _elem, _once, _one_gpu
+from .head import _flat_rows
+
+__all__ = ["embedding", "embedding_grad_sr_accum", "SREmbedding"]
+
+
+def _check(what, ids, weight, padding_idx):
+    _one_gpu(what, weight, ids)
+    _elem(weight, f"{what}: weight")
+    if weight.dim() != 2 or not weight.is_contiguous():
+        raise ValueError(f"{what} needs a contiguous weight [vocab, d], got {tuple(weight.shape)}")
+    if ids.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"{what} needs int32 or int64 ids, got {ids.dtype}")
+    vocab = weight.shape[0]
+    if vocab == 0:
+        raise ValueError(f"{what} needs words, got {tuple(weight.shape)}")
+    if padding_idx is None:
+        return -1
+    if not -vocab <= padding_idx < vocab:
+        raise ValueError(f"{what}: padding_idx {padding_idx} is outside the {vocab} words")
+    return padding_idx % vocab
+
+
+def _grad_args(ids, dy, vocab, d, scale, padding):
+    """The entry points' first arguments, the tensors that they point to, and the workspace."""
+    ids = ids.contiguous()
+    dy, ld = _flat_rows(dy, d)
+    size = ctypes.c_size_t()
+    _lib.check(_lib.lib().msr_embedding_workspace_bytes(ids.numel(), vocab, d, ctypes.byref(size)), "msr_embedding_workspace_bytes")
+    ws = _lib.workspace(dy, size.value)
+    return (ids.data_ptr(), int(ids.dtype == torch.int64), ids.numel(), dy.data_ptr(), ld, vocab, d, scale, padding), (ids, dy), ws, size.value
+
+
+def _grad(weight, ids, dy, scale, padding):
+    vocab, d = weight.shape
+    dw = torch.empty_like(weight, memory_format=torch.contiguous_format)
+    args, keep, ws, size = _grad_args(ids, dy, vocab, d, scale, padding)
+    _lib.call(weight, "msr_embedding_grad", *args, dw.data_ptr(), _ELEM[weight.dtype], _lib.ptr(ws), size)
+    return dw
+
+
+def _accumulate(weight, ids, dy, scale, padding, seed):
+    vocab, d = weight.shape
+    first = not hasattr(weight, "acc_grad")
+    if not first:
+        _lib.check_accumulator(weight, "embedding_grad_sr_accum")
+    if seed is None:
+        seed = random.getrandbits(32)
+    acc = torch.empty_like(weight, memory_format=torch.contiguous_format) if first else weight.acc_grad
+    args, keep, ws, size = _grad_args(ids, dy, vocab, d, scale, padding)
+    _lib.call(weight, "msr_embedding_grad_sr_accum", *args, acc.data_ptr(), seed, int(first), _lib.noise_mode(), None, _lib.ptr(ws), size)
+    if first:
+        weight.acc_grad = acc
+
+
+class _Embedding(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, ids, weight, scale, padding, accumulate):
+        vocab, d = weight.shape
+        ids = ids.contiguous()
+        y = torch.empty((*ids.shape, d), dtype=weight.dtype, device=weight.device)
+        _lib.call(weight, "msr_embedding", ids.data_ptr(), int(ids.dtype == torch.int64), ids.numel(), weight.data_ptr(), vocab, d, scale,
+                  y.data_ptr(), _ELEM[weight.dtype])
+        ctx.save_for_backward(ids, weight)
+        ctx.scale, ctx.padding = scale, padding
+        # the tensor that holds acc_grad: saved-tensor hooks unpack another one.  A weight that is computed (a
+        # parametrization) holds nothing that lasts, and one that is not bf16 has no accumulator: autograd gets the gradient.
+        ctx.owner = weight if accumulate and weight.is_leaf and weight.dtype == torch.bfloat16 else None
+        return y
+
+    @staticmethod
+    @_once
+    def backward(ctx, dy):
+        ids, weight = ctx.saved_tensors
+        if ctx.owner is None:
+            return None, _grad(weight, ids, dy, ctx.scale, ctx.padding), None, None, None
+        _accumulate(ctx.owner, ids, dy, ctx.scale, ctx.padding, None)
+        return None, None, None, None, None
+
+
+def embedding(ids: torch.Tensor, weight: torch.Tensor, padding_idx: int = None, scale: float = 1.0) -> torch.Tensor:
+    """``scale * weight[ids]``, rounded once, as [*ids.shape, d].  ``weight``: bf16 or fp32 [vocab, d]; ``ids``: int32 or int64; one
+    outside [0, vocab) has no word: its row is 0 and gives no gradient.  ``padding_idx`` gives none either (its row is
+    looked up as any other).  The gradient goes to autograd, whole; ``SREmbedding`` adds it to its accumulator."""
+    padding = _check("embedding", ids, weight, padding_idx)
+    return _Embedding.apply(ids, weight, float(scale), padding, False)
+
+
+def embedding_grad_sr_accum(weight: torch.Tensor, ids: torch.Tensor, dy: torch.Tensor, padding_idx: int = None,
+                            scale: float = 1.0, seed: int = None) -> None:
+    """``weight.acc_grad[v] <- SR(weight.acc_grad[v] + bf16(scale * sum of dy's rows of word v))`` for the words of ``ids``; the
+    other rows are not touched.  ``weight``: bf16 [vocab, d], ``dy``: bf16 [*ids.shape, d].  The buffer is created (as
+    zeros) on the first call, and one that is there has to be like it (ValueError); ``seed``: 32 bits, drawn from ``random``
+    if not given, as the accumulator's hook draws it."""
+    padding = _check("embedding_grad_sr_accum", ids, weight, padding_idx)
+    _one_gpu("embedding_grad_sr_accum", weight, dy)
+    if weight.dtype != torch.bfloat16 or dy.dtype != torch.bfloat16:
+        raise ValueError(f"embedding_grad_sr_accum needs bf16 tensors, got {weight.dtype} and {dy.dtype}")
+    if dy.shape != (*ids.shape, weight.shape[1]):
+        raise ValueError(f"embedding_grad_sr_accum needs dy of shape {(*ids.shape, weight.shape[1])}, got {tuple(dy.shape)}")
+    _accumulate(weight, ids, dy, float(scale), padding, seed)
+
+
+class SREmbedding(torch.nn.Embedding):
+    """``nn.Embedding`` (its rows scaled by ``scale``) whose gradient is added to ``weight.acc_grad`` with stochastic
+    rounding (for training with ``TritonSRAccumulator``: ``reassign_grad_buffer`` then moves ``acc_grad`` to
+    ``grad`` as for every other parameter).  The accumulator is the parameter's under activation checkpointing and other
+    saved-tensor hooks too; the gradient of a parametrized weight, or of one that is not bf16, goes to autograd."""
+
+    def __init__(self, num_embeddings: int, embedding_dim: int, padding_idx: int = None, scale: float = 1.0, device=None,
+                 dtype=torch.bfloat16):
+        super().__init__(num_embeddings, embedding_dim, padding_idx=padding_idx, device=device, dtype=dtype)
+        self.scale = float(scale)
+
+    def forward(self, ids: torch.Tensor) -> torch.Tensor:
+        padding = _check("SREmbedding", ids, self.weight, self.padding_idx)
+        return _Embedding.apply(ids, self.weight, self.scale, padding, True)
+
+    def extra_repr(self):
+        return super().extra_repr() + (f", scale={self.scale}" if self.scale != 1.0 else "")

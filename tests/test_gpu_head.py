@@ -1,0 +1,296 @@
+"""The head's loss and gradients against 64-bit evaluations of their definition on the same bf16 operands.
+
+Bounds, with u = 2^-24 (an fp32 rounding) and h = 2^-8 (a bf16 one).  A logit S formed in fp32 from d products is off by at
+most eS = 2 (d + 1) u sum|x w| (the factor 2: any order of the sums, and what higher terms add).  exp of an argument
+a costs 4 u (|a| + 1): the difference, its product with log2 e, that constant and the function.  The sum behind l has at most depth =
+64 + vocab / 64 additions one after the other (32 in a lane, the waves', and a share of the tiles), so l is off by at most
+el = max eS + 2 depth u + 8 u (|l| + 1), and the loss by eS + el + u |loss|.
+G = g (p - [target]) is off by eG = g (p (eS + el + 4 u (|S - l| + 1)) + 2 u), then h |G| by its rounding; a product over
+K terms adds 2 (K + 16) u sum|terms| and the stored value's rounding h |value|.  Values below the smallest normal
+number may vanish: 2^-126 per term."""
+import ctypes
+import math
+import random
+
+import pytest
+import torch
+
+from _gpu import DEV, check, need_gpu, stream
+
+pytestmark = pytest.mark.gpu
+
+BF16 = torch.bfloat16
+U, H = 2.0 ** -24, 2.0 ** -8
+REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
+
+
+@pytest.fixture(scope="module", autouse=True)
+def L():
+    return need_gpu()
+
+
+def gen(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+def make(rows, vocab, d, seed, ignored=0.2):
+    g = gen(seed)
+    w = torch.randn((vocab, d), generator=g, device=DEV).mul_(3.0 / math.sqrt(d)).to(BF16)
+    target = torch.randint(0, vocab, (rows,), generator=g, device=DEV)
+    x = torch.randn((rows, d), generator=g, device=DEV).to(BF16) + (2.5 * torch.rand((rows, 1), generator=g, device=DEV)).to(BF16) * w[target]
+    target[torch.rand(rows, generator=g, device=DEV) < ignored] = -100
+    return x, w, target, torch.rand(rows, generator=g, device=DEV) + 0.25
+
+
+def exact(x, w, target, dloss, reduction):
+    """Values and bounds in 64 bits: loss, dx, dw and theirs."""
+    x, w = x.double(), w.double()
+    vocab, d = w.shape
+    on = target != -100
+    x = torch.where(on[:, None], x, 0.0)
+    t = target.clamp(min=0)
+    S = x @ w.t()
+    eS = 2 * (d + 1) * U * (x.abs() @ w.abs().t())
+    l = torch.logsumexp(S, 1)
+    el = eS.max(1).values + 2 * (64 + vocab / 64) * U + 8 * U * (l.abs() + 1)
+    St, eSt = (v.gather(1, t[:, None])[:, 0] for v in (S, eS))
+    each = torch.where(on, l - St, 0.0)
+    e_each = torch.where(on, eSt + el + U * (l - St).abs(), 0.0)
+    n = max(1, int(on.sum()))
+    g = dloss.double() if reduction == "none" else dloss.double()[:1].expand(len(t)) / (n if reduction == "mean" else 1)
+    g = torch.where(on, g, 0.0)[:, None]
+    p = torch.exp(S - l[:, None])
+    eG = g * (p * (eS + el[:, None] + 4 * U * ((S - l[:, None]).abs() + 1)) + 2 * U)
+    G = p.clone()
+    G[torch.arange(len(t), device=DEV), t] -= 1.0
+    G *= g
+    eG += H * (G.abs() + eG)
+
+    def product(a, ea, b):
+        terms = a.abs() @ b.abs()
+        v = a @ b
+        return v, H * v.abs() + (1 + H) * (ea @ b.abs() + 2 * (a.shape[1] + 16) * U * terms) + a.shape[1] * 2.0 ** -126
+
+    if reduction == "none":
+        loss, e_loss = each, e_each
+    else:
+        k = n if reduction == "mean" else 1
+        loss, e_loss = each.sum() / k, e_each.sum() / k + 2 * U * each.sum() / k
+    return (loss, e_loss), product(G, eG, w), product(G.t().contiguous(), eG.t().contiguous(), x)
+
+
+def near(got, want):
+    value, bound = want
+    assert got.shape == value.shape
+    bad = ~((got.double() - value).abs() <= bound + 1e-37)
+    assert not bad.any(), (int(bad.sum()), (got.double() - value).abs().max().item(), bound.max().item())
+
+
+def run(x, w, target, dloss, reduction):
+    from muon_sr_amd import linear_cross_entropy
+    x, w = x.detach().requires_grad_(True), w.detach().requires_grad_(True)
+    loss = linear_cross_entropy(x, w, target, reduction=reduction)
+    assert loss.dtype == torch.float32
+    dx, dw = torch.autograd.grad(loss, (x, w), dloss if reduction == "none" else dloss[0])
+    return loss.detach(), dx, dw
+
+
+def plan(L, rows, vocab, d):
+    out = (ctypes.c_int32 * 7)()
+    check(L, L.msr_head_plan(rows, vocab, d, out))
+    return list(out)
+
+
+SIZES = [(1, 1, 8), (1, 17, 8), (7, 512, 256), (2, 9001, 64), (65, 130, 72), (300, 1000, 1032), (257, 4099, 136), (1025, 70, 2048),
+         (3000, 8192, 64), (2047, 3001, 1024), (16384, 9000, 64), (5000, 777, 264), (129, 20011, 520), (64, 64, 64), (4096, 8200, 2048)]
+
+
+@pytest.mark.parametrize("rows,vocab,d", SIZES)
+def test_against_64_bits(rows, vocab, d):
+    x, w, target, dloss = make(rows, vocab, d, rows + vocab)
+    for reduction in REDUCTIONS:
+        want = exact(x, w, target, dloss, reduction)
+        for got, value in zip(run(x, w, target, dloss, reduction), want):
+            near(got, value)
+
+
+def test_the_sizes_take_every_tile(L):
+    """Tiles of 64, 128 and 256, splits and several pieces are among the sizes above."""
+    plans = [plan(L, *s) for s in SIZES]
+    for i in (0, 1, 2, 4):
+        assert {p[i] for p in plans} == {64, 128, 256}, (i, {p[i] for p in plans})
+    assert any(p[3] > 1 for p in plans) and any(p[5] > 1 for p in plans)
+    assert any(-(-s[1] // p[6]) > 1 for s, p in zip(SIZES, plans))
+
+
+def test_ignored_rows_reach_nothing():
+    """What ignored rows hold, NaN and infinities too, changes no bit of the others' results; their loss and gradient are 0."""
+    x, w, target, dloss = make(700, 1500, 96, 3, ignored=0.4)
+    off = target == -100
+    want = run(x, w, target, dloss, "none")
+    dirty = x.clone()
+    dirty[off] = torch.tensor([math.nan, math.inf, -math.inf], device=DEV).to(BF16).repeat(32)
+    for a, b in zip(run(dirty, w, target, dloss, "none"), want):
+        assert torch.equal(a, b)
+    assert not want[0][off].any() and not want[1][off].any()
+
+
+def test_nothing_to_learn_from():
+    """No rows, or ignored ones only: loss 0, gradients 0."""
+    for rows in (0, 5):
+        x, w, target, dloss = make(rows, 300, 64, 4)
+        target.fill_(-100)
+        for reduction in REDUCTIONS:
+            loss, dx, dw = run(x, w, target, torch.ones(max(rows, 1), device=DEV)[:rows if reduction == "none" else None], reduction)
+            assert loss.shape == ((rows,) if reduction == "none" else ()) and not loss.any() and not dx.any() and not dw.any()
+            assert dx.shape == x.shape and dw.shape == w.shape
+
+
+def test_targets_that_are_no_word():
+    """Their loss is NaN, and so are their row's gradient and the words'; the other rows' losses are as they are."""
+    x, w, target, dloss = make(200, 333, 64, 5, ignored=0.1)
+    want = run(x, w, target, dloss, "none")[0]
+    at = int((target != -100).nonzero()[7])
+    for bad in (333, -1, 1 << 40, -(1 << 33)):
+        wrong = target.clone()
+        wrong[at] = bad
+        loss, dx, dw = run(x, w, wrong, dloss, "none")
+        assert loss[at].isnan() and dx[at].isnan().all() and dw.isnan().all()
+        others = torch.arange(200, device=DEV) != at
+        assert torch.equal(loss[others], want[others]) and not dx[others].isnan().any()
+        assert run(x, w, wrong, dloss, "mean")[0].isnan()
+
+
+def test_other_ignore_index_and_int32():
+    from muon_sr_amd import linear_cross_entropy
+    x, w, target, dloss = make(150, 200, 64, 6, ignored=0.3)
+    want = linear_cross_entropy(x, w, target, reduction="none")
+    zero = torch.where(target == -100, 7, torch.where(target == 7, 8, target))      # word 7 is ignored
+    assert torch.equal(linear_cross_entropy(x, w, zero, ignore_index=7, reduction="none")[target != 7], want[target != 7])
+    assert torch.equal(linear_cross_entropy(x, w, target.int(), reduction="none"), want)
+
+
+def test_extreme_logits():
+    """Logits of +-1e4 and more: the loss is the distance to the maximum, nothing overflows; a row of infinite logits is NaN, alone."""
+    g = gen(7)
+    x = torch.randn((90, 64), generator=g, device=DEV).mul_(300).to(BF16)
+    w = torch.randn((500, 64), generator=g, device=DEV).mul_(30).to(BF16)
+    target = torch.randint(0, 500, (90,), generator=g, device=DEV)
+    dloss = torch.ones(90, device=DEV)
+    for got, want in zip(run(x, w, target, dloss, "none"), exact(x, w, target, dloss, "none")):
+        near(got, want)
+    clean = run(x, w, target, dloss, "none")
+    x[3, 5] = math.inf
+    loss, dx, _ = run(x, w, target, dloss, "none")
+    others = torch.arange(90, device=DEV) != 3
+    assert loss[3].isnan() and torch.equal(loss[others], clean[0][others]) and torch.equal(dx[others], clean[1][others])
+
+
+def test_shapes_strides_and_wanted_gradients():
+    from muon_sr_amd import linear_cross_entropy
+    x, w, target, dloss = make(132, 257, 64, 8)
+    want = run(x, w, target, dloss, "none")
+    wide = torch.zeros((132, 200), dtype=BF16, device=DEV)
+    wide[:, 3:67] = x
+    turned = x.t().contiguous().t()
+    for v in (wide[:, 3:67], turned, x.view(11, 12, 64)):
+        leaf, word = v.detach().requires_grad_(True), w.clone().requires_grad_(True)
+        t = target.view(v.shape[:-1])
+        loss = linear_cross_entropy(leaf, word, t, reduction="none")
+        assert torch.equal(loss.detach().flatten(), want[0]) and loss.shape == t.shape
+        dx, dw = torch.autograd.grad(loss, (leaf, word), dloss.view(t.shape))
+        assert torch.equal(dx.reshape(132, 64), want[1]) and torch.equal(dw, want[2]) and dx.shape == v.shape
+    one = x[5:6].expand(40, 64)
+    assert torch.equal(linear_cross_entropy(one, w, target[:40]), linear_cross_entropy(one.contiguous(), w, target[:40]))
+    assert linear_cross_entropy(x[5], w, target[5]).shape == ()
+    # only one gradient wanted
+    leaf, word = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    assert torch.equal(torch.autograd.grad(linear_cross_entropy(leaf, w, target, reduction="none"), leaf, dloss)[0], want[1])
+    assert torch.equal(torch.autograd.grad(linear_cross_entropy(x, word, target, reduction="none"), word, dloss)[0], want[2])
+    assert not linear_cross_entropy(x, w, target).requires_grad
+
+
+@pytest.mark.parametrize("noise", ["philox8", "triton"])
+@pytest.mark.parametrize("rows,vocab,d", [(70, 333, 72), (3000, 8192, 64), (1, 40, 8), (16384, 9000, 64), (1025, 70, 2048)])
+def test_accumulated_weight_gradient(L, rows, vocab, d, noise):
+    """SRHead's accumulator is, bit for bit, what the stored gradient and msr_sr_accum give, over three micro-batches."""
+    import muon_sr_amd as M
+    from muon_sr_amd import _lib
+    head = M.SRHead(d, vocab, device=DEV)
+    was = M.get_sr_noise()
+    M.set_sr_noise(noise)
+    try:
+        want = None
+        for micro in range(3):
+            x, w, target, dloss = make(rows, vocab, d, micro)
+            with torch.no_grad():
+                head.weight.copy_(w)
+            random.seed(micro)
+            seed = random.getrandbits(32)
+            random.seed(micro)
+            leaf = x.clone().requires_grad_(True)
+            head.loss(leaf, target).backward(dloss[0])
+            _, dx, dw = run(x, w, target, dloss, "mean")
+            first = want is None
+            want = torch.empty_like(dw) if first else want
+            check(L, L.msr_sr_accum(want.data_ptr(), dw.data_ptr(), 0, dw.numel(), seed, int(first), _lib.noise_mode(), None, stream()))
+            assert head.weight.grad is None and torch.equal(head.weight.acc_grad, want) and torch.equal(leaf.grad, dx)
+    finally:
+        M.set_sr_noise(was)
+
+
+def test_refused_accumulators_and_parametrized_weights():
+    import muon_sr_amd as M
+    head = M.SRHead(64, 100, device=DEV)
+    x, _, target, _ = make(20, 100, 64, 9)
+    for bad in (torch.zeros((100, 64), device=DEV), torch.zeros((64, 100), dtype=BF16, device=DEV).t(), None):
+        head.weight.acc_grad = bad
+        with pytest.raises(ValueError, match="acc_grad"):
+            head.loss(x, target).backward()
+    del head.weight.acc_grad
+    torch.nn.utils.parametrizations.weight_norm(head)
+    head.loss(x, target).backward()
+    assert head.parametrizations.weight.original1.grad is not None
+
+
+def test_gradient_is_that_of_differences():
+    """(L(x + h s) - L(x - h s)) / 2h for signs s against <dx, s>, and the same for a word.  The third derivative of log-sum-exp
+    along s is the third central moment of the words' slopes under p, at most R^3 / (6 sqrt 3) for slopes of range
+    R; x and x +- h s are exact in bf16."""
+    from muon_sr_amd import linear_cross_entropy
+    g, h = gen(11), 2.0 ** -5
+    x = (torch.randint(-16, 17, (6, 64), generator=g, device=DEV) / 16).to(BF16)
+    w = (torch.randint(-16, 17, (90, 64), generator=g, device=DEV) / 16).to(BF16)
+    target = torch.randint(0, 90, (6,), generator=g, device=DEV)
+    (loss, e_loss), (dx, e_dx), (dw, e_dw) = exact(x, w, target, torch.ones(6, device=DEV), "none")
+    _, got_dx, got_dw = run(x, w, target, torch.ones(6, device=DEV), "none")
+    f = lambda a, b: linear_cross_entropy(a, b, target, reduction="none").double()  # noqa: E731
+    for k in range(6):
+        s = torch.zeros((6, 64), device=DEV, dtype=BF16)
+        s[:, k::6] = torch.randint(0, 2, s[:, k::6].shape, generator=g, device=DEV).to(BF16) * 2 - 1
+        diff = (f(x + h * s, w) - f(x - h * s, w)) / (2 * h)
+        slopes = s.double() @ w.double().t()
+        R = slopes.max(1).values - slopes.min(1).values
+        tol = h * h / 6 * R ** 3 / (6 * math.sqrt(3)) + e_loss / h + (e_dx * s.abs()).sum(1)
+        assert ((diff - (got_dx.double() * s).sum(1)).abs() <= tol).all()
+        # word k along the same signs: its slope in row n is <x[n], s>, those of the others 0
+        ws = torch.zeros((90, 64), device=DEV, dtype=BF16)
+        ws[k] = s[0]
+        diff = (f(x, w + h * ws) - f(x, w - h * ws)).sum() / (2 * h)
+        R = (x.double() @ s[0].double()).abs()
+        tol = h * h / 6 * (R ** 3).sum() / (6 * math.sqrt(3)) + e_loss.sum() / h + (e_dw[k] * s[0].abs()).sum()
+        assert (diff - (got_dw[k].double() * s[0]).sum()).abs() <= tol
+
+
+def test_same_call_same_bits_and_evaluation():
+    from muon_sr_amd import linear_cross_entropy
+    x, w, target, dloss = make(3000, 8192, 64, 12)
+    a = run(x, w, target, dloss, "mean")
+    for _ in range(3):
+        assert all(torch.equal(p, q) for p, q in zip(a, run(x, w, target, dloss, "mean")))
+    with torch.no_grad():
+        assert torch.equal(linear_cross_entropy(x, w, target), a[0])
+    leaf = x.clone().requires_grad_(True)
+    dx, = torch.autograd.grad(linear_cross_entropy(leaf, w, target), leaf, create_graph=True)
+    with pytest.raises(RuntimeError):
+        dx.float().sum().backward()
