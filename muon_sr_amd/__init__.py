@@ -16,7 +16,7 @@ from .clip import clip_grad_norm_, clip_grads, grad_norm
 from .experts import (SRExperts, TokenOrder, combine_tokens, dispatch_tokens, expert_linear, experts_wgrad_sr_accum,
                       order_tokens)
 from .balance import balance_loss
-from .embedding import SREmbedding, embedding, embedding_grad_sr_accum
+from .embed import SREmbedding, embedding, embedding_grad_sr_accum
 from .head import SRHead, linear_cross_entropy
 from .norm import LayerNorm, layer_norm
 
