@@ -4,15 +4,15 @@
 //     loss = experts / n sum_e f[e] sum_t p[t][e]
 //     dlogits[t][e] = dloss p[t][e] (u[e] - sum_j u[j] p[t][j]),   u[e] = experts / n f[e]
 // Both passes read the logits once; the probabilities are not stored, but the log of each token's sum is.  A token is held by
-// L lanes, V experts each, so that a wave sums its tokens' probabilities in registers; the work-groups' sums (fp32) and counts are
-// added in order by a second kernel.  Logits of -inf have probability 0, and a token that has no others counts with 0
+// L lanes, U cells of 16 bytes each, so that a wave sums the probabilities of 64 / L tokens at a time in registers, the next
+// tokens' logits on their way; the work-groups' sums (fp32) and counts are added in order by a second kernel.  Logits of -inf have probability 0, and a token that has no others counts with 0
 // everywhere.
 #include "rows.hpp"
 #include "../../include/muon_sr_amd.h"
 
 namespace msr {
 
-constexpr int BAL_WGS = 256;
+constexpr int BAL_WGS = 256, BAL_THREADS = 1024;   // at most: one work-group to a CU, whose sums the second kernel adds
 
 struct BalanceArgs {
     const void *logits;
@@ -27,79 +27,114 @@ struct BalanceArgs {
     int32_t experts, k, i64;
 };
 
-template <int L>
-__device__ __forceinline__ float group_max(float x) {
-#pragma unroll
-    for (int w = 1; w < L; w <<= 1) x = fmaxf(x, __shfl_xor(x, w));
+// Sums and maxima over groups of L = 8, 16, 32 or 64 lanes, in every lane of the group
+struct Add {
+    __device__ __forceinline__ float operator()(float a, float b) const { return a + b; }
+};
+struct Max {
+    __device__ __forceinline__ float operator()(float a, float b) const { return fmaxf(a, b); }
+};
+template <int L, typename Op>
+__device__ __forceinline__ float over_group(float x, Op op) {
+    x = op(x, turned<0xB1>(x));                        // quad_perm [1, 0, 3, 2]
+    x = op(x, turned<0x4E>(x));                        // quad_perm [2, 3, 0, 1]
+    x = op(x, turned<0x141>(x));                       // row_half_mirror
+    if constexpr (L >= 16) x = op(x, turned<0x140>(x));   // row_mirror
+    if constexpr (L >= 32) {
+        const auto q = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+        x = op(__uint_as_float(q[0]), __uint_as_float(q[1]));
+    }
+    if constexpr (L >= 64) {
+        const auto h = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+        x = op(__uint_as_float(h[0]), __uint_as_float(h[1]));
+    }
     return x;
-}
-template <int L>
-__device__ __forceinline__ float group_sum(float x) {
-    if constexpr (L == 64) return wave_sum(x);
-#pragma unroll
-    for (int w = 1; w < L; w <<= 1) x += __shfl_xor(x, w);
-    return x;
-}
-template <typename T>
-__device__ __forceinline__ float logit(const T *row, int e) {
-    if constexpr (sizeof(T) == 2) return bf16_to_f32(row[e]);
-    else return row[e];
 }
 
-// expert e is element e / L of lane e % L of its token's L lanes
-template <typename T, int L, int V>
-__global__ __launch_bounds__(256) void balance_kernel(BalanceArgs a) {
-    constexpr int TOK = 256 / L;                      // tokens of a work-group at a time
-    __shared__ float part[4][MSR_EXPERTS_MAX];
+constexpr float LOG2E = 1.4426950408889634f;
+
+// Work-group b's tokens: [b per, (b + 1) per).  blockDim.x: 256 or 1024.
+template <typename T, int L, int U>
+__global__ __launch_bounds__(BAL_THREADS) void balance_kernel(BalanceArgs a, int64_t per) {
+    using C = Cells<T>;
+    constexpr int N = C::N;
+    __shared__ float part[U * N * L][17];   // [experts][waves]
     __shared__ int hist[MSR_EXPERTS_MAX + 1];
-    const int tid = threadIdx.x, sub = tid / L, l = tid % L;
-    for (int e = tid; e <= a.experts; e += 256) hist[e] = 0;
+    const int tid = threadIdx.x, sub = tid / L, l = tid % L, toks = blockDim.x / L, waves = blockDim.x / 64;
+    for (int e = tid; e <= a.experts; e += blockDim.x) hist[e] = 0;
     __syncthreads();
-    float sum[V] = {};
+    const int64_t first = (int64_t)blockIdx.x * per, last = min(first + per, a.tokens);
+    // the counts
     int counted = 0;
-    for (int64_t t0 = (int64_t)blockIdx.x * TOK; t0 < a.tokens; t0 += (int64_t)gridDim.x * TOK) {
-        const int64_t t = t0 + sub;
-        const bool on = t < a.tokens && (!a.mask || a.mask[t]);
-        const T *const row = static_cast<const T *>(a.logits) + t * a.ld;
-        float x[V], m = -INFINITY, s = 0.0f;
+    if (a.mask)
+        for (int64_t t = first + tid; t < last; t += blockDim.x) counted += a.mask[t] != 0;
+    else if (tid == 0 && last > first)
+        counted = (int)(last - first);
+    if (counted) atomicAdd(&hist[a.experts], counted);
+#pragma unroll 4
+    for (int64_t i = first * a.k + tid; i < last * a.k; i += blockDim.x) {
+        const int64_t e = a.i64 ? static_cast<const int64_t *>(a.ids)[i] : static_cast<const int32_t *>(a.ids)[i];
+        if (e >= 0 && e < a.experts && (!a.mask || a.mask[(uint32_t)i / (uint32_t)a.k])) atomicAdd(&hist[e], 1);
+    }
+    // the probabilities
+    float sum[U][N] = {};
+    C next[U];
+    bool next_on = false;
+    auto fetch = [&](int64_t t) __attribute__((always_inline)) {
+        next_on = t < last && (!a.mask || a.mask[t]);
+        if (!next_on) return;
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-            x[v] = on && v * L + l < a.experts ? logit(row, v * L + l) : -INFINITY;
-            m = fmaxf(m, x[v]);
+        for (int u = 0; u < U; ++u) next[u].load(static_cast<const T *>(a.logits) + t * a.ld, (u * L + l) * N, a.experts);
+    };
+    fetch(first + sub);
+    for (int64_t t0 = first; t0 < last; t0 += toks) {
+        const int64_t t = t0 + sub;
+        const bool on = next_on;
+        float x[U][N], m = -INFINITY, s = 0.0f;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            next[u].get(x[u]);
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                if (!on || (u * L + l) * N + e >= a.experts) x[u][e] = -INFINITY;
+                m = fmaxf(m, x[u][e]);
+            }
         }
-        m = group_max<L>(m);
+        fetch(t + toks);
+        m = over_group<L>(m, Max{});
         const float at = m == -INFINITY ? 0.0f : m;
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-            x[v] = __builtin_amdgcn_exp2f((x[v] - at) * 1.4426950408889634f);
-            s += x[v];
-        }
-        s = group_sum<L>(s);
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                x[u][e] = __builtin_amdgcn_exp2f((x[u][e] - at) * LOG2E);
+                s += x[u][e];
+            }
+        s = over_group<L>(s, Add{});
         const float inv = s == 0.0f ? 0.0f : 1.0f / s;
 #pragma unroll
-        for (int v = 0; v < V; ++v) sum[v] = __builtin_fmaf(x[v], inv, sum[v]);
-        if (on && l == 0) {
-            a.lse[t] = s == 0.0f ? INFINITY : at + logf(s);      // exp(logit - lse) is 0 where there is no probability
-            ++counted;
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int e = 0; e < N; ++e) sum[u][e] = __builtin_fmaf(x[u][e], inv, sum[u][e]);
+        if (on && l == 0) a.lse[t] = s == 0.0f ? INFINITY : at + logf(s);      // exp(logit - lse) is 0 where there is no probability
+    }
+    // over a wave's groups of lanes, then over the waves
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            float v = sum[u][e];
+#pragma unroll
+            for (int w = L; w < 64; w <<= 1) v += __shfl_xor(v, w);
+            if ((tid & 63) < L) part[(u * L + l) * N + e][tid >> 6] = v;
         }
-        if (on)
-            for (int j = l; j < a.k; j += L) {
-                const int64_t e = a.i64 ? static_cast<const int64_t *>(a.ids)[t * a.k + j] : static_cast<const int32_t *>(a.ids)[t * a.k + j];
-                if (e >= 0 && e < a.experts) atomicAdd(&hist[e], 1);
-            }
-    }
-    if (counted) atomicAdd(&hist[a.experts], counted);
-    // the sums over a wave's groups of lanes, then over the waves
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-#pragma unroll
-        for (int w = L; w < 64; w <<= 1) sum[v] += __shfl_xor(sum[v], w);
-        if ((tid & 63) < L && v * L + l < a.experts) part[tid >> 6][v * L + l] = sum[v];
-    }
     __syncthreads();
-    for (int e = tid; e <= a.experts; e += 256) {
+    for (int e = tid; e <= a.experts; e += blockDim.x) {
         a.counts[(int64_t)blockIdx.x * (a.experts + 1) + e] = hist[e];
-        if (e < a.experts) a.sums[(int64_t)blockIdx.x * a.experts + e] = ((part[0][e] + part[1][e]) + part[2][e]) + part[3][e];
+        if (e == a.experts) continue;
+        float v = part[e][0];
+        for (int w = 1; w < waves; ++w) v += part[e][w];
+        a.sums[(int64_t)blockIdx.x * a.experts + e] = v;
     }
 }
 
@@ -151,50 +186,80 @@ __global__ __launch_bounds__(1024) void balance_join_kernel(const float *sums, c
     loss[0] = (float)mine;
 }
 
-template <typename T, int L, int V>
+template <typename T, int L, int U>
 __global__ __launch_bounds__(256) void balance_grad_kernel(BalanceArgs a) {
-    constexpr int TOK = 256 / L;
+    using C = Cells<T>;
+    constexpr int N = C::N, TOK = 256 / L;
     const int sub = threadIdx.x / L, l = threadIdx.x % L;
     const float up = a.dloss[0];
-    float u[V];
+    float slope[U][N];
 #pragma unroll
-    for (int v = 0; v < V; ++v) u[v] = v * L + l < a.experts ? a.slope[v * L + l] : 0.0f;
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int e = 0; e < N; ++e) slope[u][e] = (u * L + l) * N + e < a.experts ? a.slope[(u * L + l) * N + e] : 0.0f;
     for (int64_t t = (int64_t)blockIdx.x * TOK + sub; t < a.tokens; t += (int64_t)gridDim.x * TOK) {
         const bool on = !a.mask || a.mask[t];
-        const T *const row = static_cast<const T *>(a.logits) + t * a.ld;
-        const float lse = on ? a.lse[t] : 0.0f;
-        float p[V], dot = 0.0f;
+        float p[U][N] = {}, dot = 0.0f;
+        C v[U];
+        if (on) {
+            const float lse = a.lse[t];
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-            p[v] = on && v * L + l < a.experts ? __builtin_amdgcn_exp2f((logit(row, v * L + l) - lse) * 1.4426950408889634f) : 0.0f;
-            dot = __builtin_fmaf(p[v], u[v], dot);
+            for (int u = 0; u < U; ++u) v[u].load(static_cast<const T *>(a.logits) + t * a.ld, (u * L + l) * N, a.experts);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                v[u].get(p[u]);
+#pragma unroll
+                for (int e = 0; e < N; ++e) {           // (what is beyond the experts is not stored, and its slope is 0)
+                    p[u][e] = (u * L + l) * N + e < a.experts ? __builtin_amdgcn_exp2f((p[u][e] - lse) * LOG2E) : 0.0f;
+                    dot = __builtin_fmaf(p[u][e], slope[u][e], dot);
+                }
+            }
         }
-        dot = group_sum<L>(dot);
+        dot = over_group<L>(dot, Add{});
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-            if (v * L + l >= a.experts) continue;
-            const float d = on ? up * (p[v] * (u[v] - dot)) : 0.0f;
-            T *const to = static_cast<T *>(a.out) + t * a.experts + v * L + l;
-            if constexpr (sizeof(T) == 2) *to = (T)rne_bf16(d);
-            else *to = d;
+        for (int u = 0; u < U; ++u) {
+            float d[N];
+#pragma unroll
+            for (int e = 0; e < N; ++e) d[e] = on ? up * (p[u][e] * (slope[u][e] - dot)) : 0.0f;
+            v[u].set(d);
+            v[u].store(static_cast<T *>(a.out) + t * a.experts, (u * L + l) * N, a.experts);
         }
     }
 }
 
-static int balance_groups(int64_t tokens) { return (int)std::min<int64_t>(std::max<int64_t>((tokens + 15) / 16, 1), BAL_WGS); }
-
-// lanes per token and experts per lane
-template <typename F>
-static void balance_shape(int experts, F &&f) {
+// Cells of a row, lanes per token and cells per lane
+template <typename T, typename F>
+static void balance_lanes(int experts, F &&f) {
     using std::integral_constant;
-    if (experts <= 8) f(integral_constant<int, 8>{}, integral_constant<int, 1>{});
-    else if (experts <= 16) f(integral_constant<int, 16>{}, integral_constant<int, 1>{});
-    else if (experts <= 32) f(integral_constant<int, 32>{}, integral_constant<int, 1>{});
-    else if (experts <= 64) f(integral_constant<int, 64>{}, integral_constant<int, 1>{});
-    else if (experts <= 128) f(integral_constant<int, 64>{}, integral_constant<int, 2>{});
-    else if (experts <= 256) f(integral_constant<int, 64>{}, integral_constant<int, 4>{});
-    else if (experts <= 512) f(integral_constant<int, 64>{}, integral_constant<int, 8>{});
-    else f(integral_constant<int, 64>{}, integral_constant<int, 16>{});
+    const int cells = (experts + Cells<T>::N - 1) / Cells<T>::N;
+    if (cells <= 8) f(integral_constant<int, 8>{}, integral_constant<int, 1>{});
+    else if (cells <= 16) f(integral_constant<int, 16>{}, integral_constant<int, 1>{});
+    else if (cells <= 32) f(integral_constant<int, 32>{}, integral_constant<int, 1>{});
+    else if (cells <= 64) f(integral_constant<int, 64>{}, integral_constant<int, 1>{});
+    else if (cells <= 128) f(integral_constant<int, 64>{}, integral_constant<int, 2>{});
+    else if constexpr (sizeof(T) == 4) f(integral_constant<int, 64>{}, integral_constant<int, 4>{});
+}
+// f(type, lanes, cells per lane)
+template <typename F>
+static void balance_shape(int32_t elem, int experts, F &&f) {
+    if (elem == MSR_BF16) balance_lanes<uint16_t>(experts, [&](auto l, auto u) { f(uint16_t{}, l, u); });
+    else balance_lanes<float>(experts, [&](auto l, auto u) { f(float{}, l, u); });
+}
+
+// Work-groups of 256 threads while they leave CUs idle, 1024 beyond; the tokens of each.
+struct BalancePlan {
+    int groups, threads;
+    int64_t per;
+};
+static BalancePlan balance_plan(int64_t tokens, int32_t experts, int32_t elem) {
+    int lanes = 64;
+    balance_shape(elem, experts, [&](auto, auto l, auto) { lanes = decltype(l)::value; });
+    BalancePlan p{};
+    p.threads = tokens <= (int64_t)BAL_WGS * 256 / lanes ? 256 : BAL_THREADS;
+    const int64_t at_once = p.threads / lanes, rounds = (tokens + at_once * BAL_WGS - 1) / (at_once * BAL_WGS);
+    p.per = std::max<int64_t>(rounds, 1) * at_once;
+    p.groups = (int)std::max<int64_t>((tokens + p.per - 1) / p.per, 1);
+    return p;
 }
 
 static int balance_check(const char *name, int64_t tokens, int32_t experts, int32_t k, int32_t elem) {
@@ -213,10 +278,10 @@ using namespace msr;
 extern "C" {
 
 int msr_balance_workspace_bytes(int64_t tokens, int32_t experts, size_t *bytes) {
-    const int rc = balance_check("msr_balance_workspace_bytes", tokens, experts, 1, MSR_F32);
+    const int rc = balance_check("msr_balance_workspace_bytes", tokens, experts, 1, MSR_F32);   // (as much for either type)
     if (rc) return rc;
     if (!bytes) { set_error("msr_balance_workspace_bytes: a pointer is NULL"); return MSR_ERR_ARG; }
-    *bytes = (size_t)balance_groups(tokens) * (size_t)(2 * experts + 1) * 4;
+    *bytes = (size_t)std::max(balance_plan(tokens, experts, MSR_BF16).groups, balance_plan(tokens, experts, MSR_F32).groups) * (size_t)(2 * experts + 1) * 4;
     return MSR_OK;
 }
 
@@ -232,7 +297,8 @@ int msr_balance_loss(const void *logits, int64_t ld, const void *ids, int32_t id
         set_error("%s: operands must be aligned to their types", name);
         return MSR_ERR_ALIGN;
     }
-    const int groups = balance_groups(tokens);
+    const BalancePlan p = balance_plan(tokens, experts, elem);
+    const int groups = p.groups;
     const size_t need = (size_t)groups * (size_t)(2 * experts + 1) * 4, n = (size_t)tokens;
     if (!workspace || workspace_bytes < need) {
         set_error("%s: workspace of %zu bytes is smaller than the %zu required", name, workspace_bytes, need);
@@ -247,9 +313,8 @@ int msr_balance_loss(const void *logits, int64_t ld, const void *ids, int32_t id
     a.logits = logits; a.ld = ld; a.tokens = tokens; a.ids = ids; a.i64 = ids_i64 != 0; a.mask = mask; a.lse = lse; a.experts = experts; a.k = k;
     a.sums = static_cast<float *>(workspace);
     a.counts = reinterpret_cast<int32_t *>(a.sums + (size_t)groups * (size_t)experts);
-    balance_shape(experts, [&](auto l, auto v) {
-        if (elem == MSR_BF16) hipLaunchKernelGGL((balance_kernel<uint16_t, decltype(l)::value, decltype(v)::value>), dim3(groups), dim3(256), 0, s, a);
-        else hipLaunchKernelGGL((balance_kernel<float, decltype(l)::value, decltype(v)::value>), dim3(groups), dim3(256), 0, s, a);
+    balance_shape(elem, experts, [&](auto t, auto l, auto u) {
+        hipLaunchKernelGGL((balance_kernel<decltype(t), decltype(l)::value, decltype(u)::value>), dim3(groups), dim3(p.threads), 0, s, a, p.per);
     });
     if ((rc = check_launch("balance_kernel"))) return rc;
     hipLaunchKernelGGL(balance_join_kernel, dim3(1), dim3(1024), 0, s, a.sums, a.counts, groups, experts, k, loss, counts, slope);
@@ -274,10 +339,9 @@ int msr_balance_grad(const void *logits, int64_t ld, const uint8_t *mask, const 
     BalanceArgs a{};
     a.logits = logits; a.ld = ld; a.tokens = tokens; a.mask = mask; a.lse = const_cast<float *>(lse); a.slope = slope; a.dloss = dloss;
     a.out = dlogits; a.experts = experts;
-    balance_shape(experts, [&](auto l, auto v) {
+    balance_shape(elem, experts, [&](auto t, auto l, auto u) {
         const dim3 grid(grid_for(tokens, 256 / decltype(l)::value, 256 * 8));
-        if (elem == MSR_BF16) hipLaunchKernelGGL((balance_grad_kernel<uint16_t, decltype(l)::value, decltype(v)::value>), grid, dim3(256), 0, (hipStream_t)stream, a);
-        else hipLaunchKernelGGL((balance_grad_kernel<float, decltype(l)::value, decltype(v)::value>), grid, dim3(256), 0, (hipStream_t)stream, a);
+        hipLaunchKernelGGL((balance_grad_kernel<decltype(t), decltype(l)::value, decltype(u)::value>), grid, dim3(256), 0, (hipStream_t)stream, a);
     });
     return check_launch("balance_grad_kernel");
 }

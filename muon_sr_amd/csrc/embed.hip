@@ -3,18 +3,20 @@
 // An id outside [0, vocab) has no word: its y is 0 and it gives no gradient.  The padding id gives none either.
 //
 // The tokens are sorted by word, earlier tokens first: runs of SORT_RUN tokens by one work-group each (a radix sort in
-// LDS), then merged pairwise.  Waves then take CHUNK sorted tokens each and add up the rows of one word after the other
-// in fp32, so that no sum depends on a race.  A word whose tokens lie in one chunk is finished there; of a word that
+// LDS), then merged, MERGE_WAYS runs at a time.  Waves then take CHUNK sorted tokens each and add up the rows of one word after
+// the other in fp32, so that no sum depends on a race.  A word whose tokens lie in one chunk is finished there; of a word that
 // crosses chunks each leaves a part, which join_rows_kernel adds up in their order.  Rows of dW without a token are
-// written by the same launch, found by a search in the sorted tokens.
+// written by the same launch, found by a search in the sorted tokens.  Up to FEW tokens are not sorted: the wave of a
+// word's first token finds the others itself, one launch instead of three.
 #include "rows.hpp"
 #include "../../include/muon_sr_amd.h"
 
 namespace msr {
 
-constexpr int SORT_THREADS = 1024, SORT_EACH = 16, SORT_RUN = SORT_THREADS * SORT_EACH;
+constexpr int SORT_THREADS = 1024, SORT_EACH = 2, SORT_RUN = SORT_THREADS * SORT_EACH, MERGE_WAYS = 32;
 constexpr int SORT_WAVES = SORT_THREADS / 64, SORT_BITS = 9;    // bits of a pass at most
 constexpr int CHUNK = 32;                                       // sorted tokens of a wave
+constexpr int FEW = 256;                                        // tokens that are not sorted
 
 struct EmbedArgs {
     const void *ids;
@@ -187,21 +189,33 @@ __device__ __forceinline__ int64_t below(const uint64_t *keys, int64_t n, uint64
     return lo;
 }
 
-// Pairs of runs of `run` keys merged: a key's place is its own number in its run plus how many of the other are below it.
+// Runs of `run` keys (a power of two), MERGE_WAYS at a time, merged: a key's place is its own number in its run plus how many of
+// each other are below it, searched for in four runs at once (a search is a chain of loads).
 __global__ __launch_bounds__(256) void merge_kernel(const uint64_t *in, uint64_t *out, int64_t n, int64_t run) {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= n) return;
-    const int64_t pair = i / (2 * run) * (2 * run), mine = i / run * run, other = mine == pair ? min(pair + run, n) : pair;
-    const int64_t len = min(other + run, n) - other;
+    const int64_t first = i / (run * MERGE_WAYS) * (run * MERGE_WAYS), mine = i / run * run, end = min(first + run * MERGE_WAYS, n);
     const uint64_t key = in[i];
-    out[pair + (i - mine) + (len > 0 ? below(in + other, len, key) : 0)] = key;
+    int64_t place = first + (i - mine);
+    for (int64_t r0 = first; r0 < end; r0 += 4 * run) {
+        int64_t lo[4] = {0, 0, 0, 0}, len[4];
+#pragma unroll
+        for (int y = 0; y < 4; ++y) len[y] = r0 + y * run == mine ? 0 : max((int64_t)0, min(run, end - (r0 + y * run)));
+        for (int64_t step = run; step; step >>= 1) {
+#pragma unroll
+            for (int y = 0; y < 4; ++y)
+                if (lo[y] + step <= len[y] && in[r0 + y * run + lo[y] + step - 1] < key) lo[y] += step;
+        }
+        place += (lo[0] + lo[1]) + (lo[2] + lo[3]);
+    }
+    out[place] = key;
 }
 
 // ---------------------------------------------------------------------------
 // sums
 // ---------------------------------------------------------------------------
 
-constexpr int SUM_AHEAD = 4;     // rows whose loads are in flight together
+constexpr int SUM_AHEAD = 4, JOIN_AHEAD = 4;     // rows, and parts, whose loads are in flight together
 
 // What is done with the sum of a word's rows, N columns from c on: stored in T (MODE -1), or added to the bf16 accumulator
 // with SR as round(scale sum) would be by msr_sr_accum.
@@ -235,10 +249,42 @@ __device__ __forceinline__ void finish(const EmbedArgs &a, int v, int64_t c, con
     x.store(row, c, a.d);
 }
 
-// Job j: chunk j / pieces of the sorted tokens and a piece of 64 cells of their rows; behind those, 64 words that
+// Words that a wave looks up and zeroes where no token has them: 64, or 8 where that leaves waves idle (512 words of 256: 18 us
+// and 8).
+constexpr int zero_words(int64_t vocab, int64_t pieces) { return vocab * pieces >= 64 * 4096 ? 64 : 8; }
+
+template <typename T>
+__device__ __forceinline__ void zero_rows(const EmbedArgs &a, int64_t v0, uint64_t none, int64_t c) {
+    Cells<T> zero;
+    zero.v = Bytes16{};
+    for (; none; none &= none - 1)
+        if (c < a.d) zero.store(static_cast<T *>(a.out) + (v0 + __builtin_ctzll(none)) * a.d, c, a.d);
+}
+
+// floats [c, c + N) of a part of d
+template <int N>
+__device__ __forceinline__ void load_part(const float *part, int64_t c, int64_t d, float (&f)[N]) {
+    Cells<float> x[N / 4];
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) x[i].load(part, c + 4 * i, d);
+#pragma unroll
+    for (int e = 0; e < N; ++e) f[e] = __uint_as_float(x[e / 4].v.w[e % 4]);
+}
+template <int N>
+__device__ __forceinline__ void store_part(float *part, int64_t c, int64_t d, const float (&f)[N]) {
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) {
+        Cells<float> x;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x.v.w[e] = __float_as_uint(f[4 * i + e]);
+        x.store(part, c + 4 * i, d);
+    }
+}
+
+// Job j: chunk j / pieces of the sorted tokens and a piece of 64 cells of their rows; behind those, `words` words that
 // are looked up and, where no token has them, zeroed.
 template <typename T, int MODE>
-__global__ __launch_bounds__(256) void sums_kernel(EmbedArgs a, int64_t sum_jobs, int64_t zero_jobs) {
+__global__ __launch_bounds__(256) void sums_kernel(EmbedArgs a, int64_t sum_jobs, int64_t zero_jobs, int words) {
     using C = Cells<T>;
     constexpr int WIDTH = 64 * C::N;
     const int lane = threadIdx.x & 63;
@@ -247,17 +293,13 @@ __global__ __launch_bounds__(256) void sums_kernel(EmbedArgs a, int64_t sum_jobs
     if (j >= sum_jobs) {
         j -= sum_jobs;
         if (j >= zero_jobs) return;
-        const int64_t v0 = j / pieces * 64, c = (j % pieces) * WIDTH + lane * C::N, v = v0 + lane;
-        bool hit = v >= a.vocab;
+        const int64_t v0 = j / pieces * words, v = v0 + lane;
+        bool hit = lane >= words || v >= a.vocab;
         if (!hit) {
             const int64_t at = below(a.sorted, a.n, (uint64_t)v << 32);
             hit = at < a.n && (int64_t)(a.sorted[at] >> 32) == v;
         }
-        uint64_t none = ~__ballot(hit);
-        C zero;
-        zero.v = Bytes16{};
-        for (; none; none &= none - 1)
-            if (c < a.d) zero.store(static_cast<T *>(a.out) + (v0 + __builtin_ctzll(none)) * a.d, c, a.d);
+        zero_rows<T>(a, v0, ~__ballot(hit), (j % pieces) * WIDTH + lane * C::N);
         return;
     }
     const int64_t chunk = j / pieces, p0 = chunk * CHUNK, c = (j % pieces) * WIDTH + lane * C::N;
@@ -290,10 +332,7 @@ __global__ __launch_bounds__(256) void sums_kernel(EmbedArgs a, int64_t sum_jobs
             if (whole && after != v) {
                 finish<T, MODE>(a, v, c, sum);
             } else {
-                float *const part = a.parts + (2 * chunk + (whole ? 1 : 0)) * a.d;
-#pragma unroll
-                for (int e = 0; e < C::N; ++e)
-                    if (c + e < a.d) part[c + e] = sum[e];
+                store_part(a.parts + (2 * chunk + (whole ? 1 : 0)) * a.d, c, a.d, sum);
             }
             whole = true;
 #pragma unroll
@@ -325,16 +364,91 @@ __global__ __launch_bounds__(256) void join_rows_kernel(EmbedArgs a) {
     }
     if (c >= a.d) return;
     float sum[C::N];
-    auto add = [&](int64_t part, bool set) __attribute__((always_inline)) {
+    load_part(a.parts + (2 * chunk + 1) * a.d, c, a.d, sum);
+    for (int64_t k = chunk + 1; k < end; k += JOIN_AHEAD) {
+        float f[JOIN_AHEAD][C::N];
 #pragma unroll
-        for (int e = 0; e < C::N; ++e) {
-            const float f = c + e < a.d ? a.parts[part * a.d + c + e] : 0.0f;
-            sum[e] = set ? f : sum[e] + f;
+        for (int y = 0; y < JOIN_AHEAD; ++y)
+            if (k + y < end) load_part(a.parts + 2 * (k + y) * a.d, c, a.d, f[y]);
+#pragma unroll
+        for (int y = 0; y < JOIN_AHEAD; ++y) {
+            if (k + y >= end) continue;
+#pragma unroll
+            for (int e = 0; e < C::N; ++e) sum[e] += f[y][e];
         }
-    };
-    add(2 * chunk + 1, true);
-#pragma unroll 4
-    for (int64_t k = chunk + 1; k < end; ++k) add(2 * k, false);
+    }
+    finish<T, MODE>(a, v, c, sum);
+}
+
+// At most FEW tokens, not sorted.  Job j: token j / pieces, if it is the first of its word, with the others of that word;
+// behind those, 8 words that are zeroed where no token has them.  Every wave holds all ids, 64 to a register.
+template <typename T, int MODE>
+__global__ __launch_bounds__(256) void few_kernel(EmbedArgs a, int64_t sum_jobs, int64_t zero_jobs) {
+    using C = Cells<T>;
+    constexpr int WIDTH = 64 * C::N, R = FEW / 64;
+    const int lane = threadIdx.x & 63;
+    int64_t j = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t pieces = (a.d + WIDTH - 1) / WIDTH;
+    if (j >= sum_jobs + zero_jobs) return;
+    int word[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        word[r] = -1;
+        if (r * 64 + lane < a.n) word[r] = word_at(a, r * 64 + lane);
+        if (word[r] == a.padding) word[r] = -1;
+    }
+    if (j >= sum_jobs) {
+        j -= sum_jobs;
+        const int v0 = (int)(j / pieces * 8);
+        uint64_t none = 0;
+        for (int i = 0; i < 8 && v0 + i < a.vocab; ++i) {
+            bool hit = false;
+#pragma unroll
+            for (int r = 0; r < R; ++r) hit |= word[r] == v0 + i;
+            none |= (uint64_t)(__ballot(hit) == 0) << i;
+        }
+        zero_rows<T>(a, v0, none, (j % pieces) * WIDTH + lane * C::N);
+        return;
+    }
+    const int i = (int)(j / pieces);
+    const int64_t c = (j % pieces) * WIDTH + lane * C::N;
+    int v = -1;
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+        if (i / 64 == r) v = __builtin_amdgcn_readlane(word[r], i % 64);
+    if (v < 0) return;
+    uint64_t same[R];
+    bool first = true;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        same[r] = __ballot(word[r] == v);
+        if (r < i / 64) first = first && same[r] == 0;
+        if (r == i / 64) first = first && (same[r] & ((1ull << (i % 64)) - 1)) == 0;
+    }
+    if (!first) return;
+    float sum[C::N] = {};
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        uint64_t left = same[r];
+        while (left) {
+            C x[SUM_AHEAD];
+            bool on[SUM_AHEAD];
+#pragma unroll
+            for (int y = 0; y < SUM_AHEAD; ++y) {
+                on[y] = left != 0;
+                if (on[y]) x[y].load(static_cast<const T *>(a.dy) + (int64_t)(r * 64 + __builtin_ctzll(left)) * a.lddy, c, a.d);
+                left &= left - 1;
+            }
+#pragma unroll
+            for (int y = 0; y < SUM_AHEAD; ++y) {
+                if (!on[y]) continue;
+                float f[C::N];
+                x[y].get(f);
+#pragma unroll
+                for (int e = 0; e < C::N; ++e) sum[e] += f[e];
+            }
+        }
+    }
     finish<T, MODE>(a, v, c, sum);
 }
 
@@ -347,7 +461,8 @@ struct EmbedPlan {
 static EmbedPlan embed_plan(int64_t n, int64_t d) {
     EmbedPlan p{};
     p.runs = (int)((n + SORT_RUN - 1) / SORT_RUN);
-    for (int64_t r = 1; r < p.runs; r *= 2) ++p.merges;
+    for (int64_t r = 1; r < p.runs; r *= MERGE_WAYS) ++p.merges;
+    if (n <= FEW) return p;
     p.sorted = ((size_t)n * 8 + 255) & ~(size_t)255;
     p.parts = (size_t)((n + CHUNK - 1) / CHUNK) * 2 * (size_t)d * 4;
     p.bytes = p.sorted * (p.merges ? 2 : 1) + p.parts;
@@ -367,9 +482,16 @@ template <typename T, int MODE>
 static int embed_sums(const EmbedArgs &a, hipStream_t s) {
     constexpr int WIDTH = 64 * Cells<T>::N;
     const int64_t pieces = (a.d + WIDTH - 1) / WIDTH, chunks = (a.n + CHUNK - 1) / CHUNK;
-    const int64_t sums = chunks * pieces, zeros = MODE < 0 || a.zero_init ? ((int64_t)a.vocab + 63) / 64 * pieces : 0;
+    const bool few = a.n <= FEW, zero = MODE < 0 || a.zero_init;
+    const int words = few ? 8 : zero_words(a.vocab, pieces);
+    const int64_t sums = (few ? a.n : chunks) * pieces, zeros = zero ? ((int64_t)a.vocab + words - 1) / words * pieces : 0;
+    const dim3 grid((unsigned)((sums + zeros + 3) / 4));
+    if (few) {
+        if (sums + zeros > 0) hipLaunchKernelGGL((few_kernel<T, MODE>), grid, dim3(256), 0, s, a, sums, zeros);
+        return check_launch("few_kernel");
+    }
     if (sums + zeros > 0) {
-        hipLaunchKernelGGL((sums_kernel<T, MODE>), dim3((unsigned)((sums + zeros + 3) / 4)), dim3(256), 0, s, a, sums, zeros);
+        hipLaunchKernelGGL((sums_kernel<T, MODE>), grid, dim3(256), 0, s, a, sums, zeros, words);
         const int rc = check_launch("sums_kernel");
         if (rc || chunks < 2) return rc;
         hipLaunchKernelGGL((join_rows_kernel<T, MODE>), dim3((unsigned)((sums + 3) / 4)), dim3(256), 0, s, a);
@@ -394,17 +516,17 @@ static int embed_grad(const char *name, const void *ids, int32_t ids_i64, int64_
         return MSR_ERR_ALIGN;
     }
     const EmbedPlan p = embed_plan(n, d);
-    if (n > 0 && d > 0 && (!workspace || workspace_bytes < p.bytes)) {
+    if (p.bytes > 0 && d > 0 && (!workspace || workspace_bytes < p.bytes)) {
         set_error("%s: workspace of %zu bytes is smaller than the %zu required", name, workspace_bytes, p.bytes);
         return MSR_ERR_WORKSPACE;
     }
     const size_t wb = (size_t)vocab * (size_t)d * es;
-    const Range r[5] = {{out, wb}, {workspace, n > 0 ? p.bytes : 0}, {ids, (size_t)n * (ids_i64 ? 8 : 4)}, {dy, rows_bytes(n, lddy, d, es)},
+    const Range r[5] = {{out, wb}, {workspace, p.bytes}, {ids, (size_t)n * (ids_i64 ? 8 : 4)}, {dy, rows_bytes(n, lddy, d, es)},
                         {inject, noise_mode == NOISE_INJECT ? wb : 0}};
     rc = ranges_apart(name, r, 5, 2);
     if (rc || d == 0) return rc;
     const int64_t pieces = (d + 64 * (16 / (int64_t)es) - 1) / (64 * (16 / (int64_t)es));
-    if ((((int64_t)n + CHUNK - 1) / CHUNK + (vocab + 63) / 64) * pieces >= (int64_t(1) << 25)) {
+    if ((((int64_t)n + CHUNK - 1) / CHUNK + FEW + (vocab + 63) / 64 + 4096) * pieces >= (int64_t(1) << 25)) {
         set_error("%s: too many rows for a launch (%lld tokens, %lld words of %lld)", name, (long long)n, (long long)vocab, (long long)d);
         return MSR_ERR_ARG;
     }
@@ -413,7 +535,7 @@ static int embed_grad(const char *name, const void *ids, int32_t ids_i64, int64_
     a.padding = padding; a.out = out; a.zero_init = zero_init != 0;
     a.ns.key = seed_key(seed, 0);
     a.ns.inject = inject;
-    if (n > 0) {
+    if (n > FEW) {
         char *const ws = static_cast<char *>(workspace);
         uint64_t *list[2] = {reinterpret_cast<uint64_t *>(ws), reinterpret_cast<uint64_t *>(ws + p.sorted)};
         a.parts = reinterpret_cast<float *>(ws + p.sorted * (p.merges ? 2 : 1));
@@ -422,7 +544,7 @@ static int embed_grad(const char *name, const void *ids, int32_t ids_i64, int64_
         hipLaunchKernelGGL(sort_kernel, dim3((unsigned)p.runs), dim3(SORT_THREADS), 0, s, a);
         if ((rc = check_launch("sort_kernel"))) return rc;
         int64_t run = SORT_RUN;
-        for (int m = 0; m < p.merges; ++m, run *= 2) {
+        for (int m = 0; m < p.merges; ++m, run *= MERGE_WAYS) {
             hipLaunchKernelGGL(merge_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, list[m & 1], list[~m & 1], n, run);
             if ((rc = check_launch("merge_kernel"))) return rc;
             a.sorted = list[~m & 1];

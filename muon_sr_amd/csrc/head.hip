@@ -79,42 +79,51 @@ struct ListArgs {
     int32_t rows, vocab, i64;
 };
 
-// One work-group numbers the rows that are not ignored, in order.
+// One work-group numbers the rows that are not ignored, in order: LIST_EACH rows per thread at a time, LIST_THREADS apart, so that a
+// wave's accesses are 64 elements on end (4096 rows 9.4 us with eight neighbouring rows per thread, 4.7 so).
 __global__ __launch_bounds__(LIST_THREADS) void list_kernel(ListArgs a) {
-    __shared__ int sums[LIST_THREADS / 64];
+    constexpr int WAVES = LIST_THREADS / 64;
+    static_assert(WAVES * LIST_EACH == 128, "two counts per lane of a wave");
+    __shared__ int at[WAVES * LIST_EACH], total;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     int base = 0;
     for (int64_t n0 = 0; n0 < a.rows; n0 += LIST_THREADS * LIST_EACH) {
-        const int64_t n = n0 + (int64_t)tid * LIST_EACH;
         int64_t t[LIST_EACH];
-        int c = 0;
+        uint64_t kept[LIST_EACH];
 #pragma unroll
         for (int i = 0; i < LIST_EACH; ++i) {
+            const int64_t n = n0 + i * LIST_THREADS + tid;
             t[i] = a.ignore;
-            if (n + i < a.rows) t[i] = a.i64 ? static_cast<const int64_t *>(a.target)[n + i] : static_cast<const int32_t *>(a.target)[n + i];
-            c += t[i] != a.ignore;
-        }
-        const int to = wave_scan(c);
-        if (lane == 63) sums[wave] = to;
-        __syncthreads();
-        int at = base + to - c;
-        for (int w = 0; w < LIST_THREADS / 64; ++w) {
-            at += w < wave ? sums[w] : 0;
-            base += sums[w];
+            if (n < a.rows) t[i] = a.i64 ? static_cast<const int64_t *>(a.target)[n] : static_cast<const int32_t *>(a.target)[n];
         }
 #pragma unroll
         for (int i = 0; i < LIST_EACH; ++i) {
-            if (n + i >= a.rows) break;
+            kept[i] = __ballot(t[i] != a.ignore);
+            if (lane == 0) at[i * WAVES + wave] = __popcll(kept[i]);
+        }
+        __syncthreads();
+        if (wave == 0) {
+            const int c0 = at[2 * lane], c1 = at[2 * lane + 1], to = wave_scan(c0 + c1);
+            at[2 * lane] = to - c0 - c1;
+            at[2 * lane + 1] = to - c1;
+            if (lane == 63) total = to;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < LIST_EACH; ++i) {
+            const int64_t n = n0 + i * LIST_THREADS + tid;
+            if (n >= a.rows) continue;
             const bool on = t[i] != a.ignore;
-            a.pos[n + i] = on ? at : -1;
+            const int place = base + at[i * WAVES + wave] + __popcll(kept[i] & ((1ull << lane) - 1));
+            a.pos[n] = on ? place : -1;
             if (on) {
-                a.kept[1 + at] = (int32_t)(n + i);
-                a.kept[1 + a.rows + at] = t[i] >= 0 && t[i] < a.vocab ? (int32_t)t[i] : HEAD_BAD;
-                ++at;
+                a.kept[1 + place] = (int32_t)n;
+                a.kept[1 + a.rows + place] = t[i] >= 0 && t[i] < a.vocab ? (int32_t)t[i] : HEAD_BAD;
             } else if (a.loss) {
-                a.loss[n + i] = 0.0f;
+                a.loss[n] = 0.0f;
             }
         }
+        base += total;
         __syncthreads();
     }
     if (tid == 0) a.kept[0] = base;
