@@ -37,7 +37,9 @@ struct HeadArgs {
     Noise ns;
 };
 
-__device__ __forceinline__ int kept_rows(const HeadArgs &a) { return __builtin_amdgcn_readfirstlane(min(max(a.kept[0], 0), a.rows)); }
+// (through the constant address space: a scalar load, as every work-group waits for it first)
+typedef const __attribute__((address_space(4))) int32_t *const_i32_t;
+__device__ __forceinline__ int kept_rows(const HeadArgs &a) { return min(max(*(const_i32_t)(uintptr_t)a.kept, 0), a.rows); }
 __device__ __forceinline__ int word_of(const HeadArgs &a, int r) { return a.kept[1 + a.rows + r]; }
 // dloss of packed row r; NaN where its target is no word
 __device__ __forceinline__ float slope_of(const HeadArgs &a, int r, int count) {
@@ -46,18 +48,25 @@ __device__ __forceinline__ float slope_of(const HeadArgs &a, int r, int count) {
     return a.reduction == HEAD_MEAN ? g / (float)count : g;
 }
 
-// Tile v of tiles_m x tiles_n.  Consecutive work-groups go to the 8 XCDs in turn: each XCD takes a contiguous eighth
-// of the tiles, G rows of tiles at a time, column by column, so that its L2 holds what they share.
+// Tile v of tiles_m x tiles_n in each of `splits` shares of K.  Consecutive work-groups go to the 8 XCDs in turn: each XCD takes a
+// contiguous eighth of the shares' tiles, G rows of tiles at a time, column by column, so that its L2 holds what they
+// share.
 template <int G>
-__device__ __forceinline__ bool find_tile(int v, int tiles_m, int tiles_n, int &mt, int &nt) {
-    const int total = tiles_m * tiles_n, per = total / NXCD;
+__device__ __forceinline__ bool find_tile(int v, int tiles_m, int tiles_n, int splits, int &mt, int &nt, int &split) {
+    const int tiles = tiles_m * tiles_n, total = tiles * splits, per = total / NXCD;
     if (v >= total) return false;
     if (v < per * NXCD) v = (v % NXCD) * per + v / NXCD;
+    split = v / tiles;
+    v -= split * tiles;
     const int pg = G * tiles_n, g = v / pg, rows = min(G, tiles_m - G * g), r = v - g * pg;
     mt = G * g + r % rows;
     nt = r / rows;
     return true;
 }
+
+// exp(x - m) as exp2(x log2(e) - m log2(e)): the rounding of m's product is common to a row's terms, and no larger than
+// that of the row's logits
+__device__ __forceinline__ float exp_from(float x, float neg_m2) { return __builtin_amdgcn_exp2f(__builtin_fmaf(x, LOG2E, neg_m2)); }
 
 // (m, s) of the union of two sets, s = sum exp(x - m); an empty set is (-inf, 0)
 __device__ __forceinline__ float2 joined(float2 a, float2 b) {
@@ -153,11 +162,27 @@ __global__ __launch_bounds__(64 * Shape<T>::NW, 2) void logits_kernel(HeadArgs a
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave / SH::WN, wn = wave % SH::WN;
     const int count = kept_rows(a);
-    int mt, nt;
-    if (!find_tile<T == 256 ? 8 : 4>(blockIdx.x, (count + T - 1) / T, a.tiles_n, mt, nt)) return;
+    int mt, nt, split;
+    if (!find_tile<T == 256 ? 8 : 4>(blockIdx.x, (count + T - 1) / T, a.tiles_n, 1, mt, nt, split)) return;
     const int m0 = mt * T, n0 = nt * T;                           // n0: from v0 on
     PR pr;
     pr.init(wave, lane, a.d, a.d);
+    // what the epilogue needs of the lane's rows, loaded ahead of the products
+    int word[FM];
+    float lse[FM], slope[FM];
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+        const int row = m0 + wm * SH::TM + 32 * i + (lane & 31);
+        word[i] = HEAD_BAD;
+        lse[i] = slope[i] = 0.0f;
+        if (row < count) {
+            word[i] = word_of(a, row);
+            if constexpr (GRAD) {
+                lse[i] = a.lse[row];
+                slope[i] = slope_of(a, row, count);
+            }
+        }
+    }
     auto lds_p = [&](auto ST) __attribute__((always_inline)) -> char * { return decltype(ST)::value == 0 ? p_0 : p_1; };
     auto lds_q = [&](auto ST) __attribute__((always_inline)) -> char * { return decltype(ST)::value == 0 ? q_0 : q_1; };
     pr.run(lds_p, lds_q, {a.x + (int64_t)m0 * a.d, a.d, min(T, count - m0), 0, a.d},
@@ -189,16 +214,16 @@ __global__ __launch_bounds__(64 * Shape<T>::NW, 2) void logits_kernel(HeadArgs a
 #pragma unroll
                 for (int x = 0; x < 16; ++x) m = fmaxf(m, pr.acc[i][j][x]);
             m = fmaxf(m, __shfl_xor(m, 32));
-            const float at = m == -INFINITY ? 0.0f : m;
+            const float at = m == -INFINITY ? 0.0f : -m * LOG2E;
             float s = 0.0f;
 #pragma unroll
             for (int j = 0; j < FN; ++j)
 #pragma unroll
-                for (int x = 0; x < 16; ++x) s += __builtin_amdgcn_exp2f((pr.acc[i][j][x] - at) * LOG2E);
+                for (int x = 0; x < 16; ++x) s += exp_from(pr.acc[i][j][x], at);
             s += __shfl_xor(s, 32);
             if (khalf == 0) stat[wn * T + wm * SH::TM + 32 * i + r32] = make_float2(m, s);
             const int row = m1 + 32 * i;
-            const int rel = row < count ? word_of(a, row) - a.v0 - nw : -1;   // this lane's columns: those with bit 2 of rel clear
+            const int rel = word[i] - a.v0 - nw;                  // this lane's columns: those with bit 2 of rel clear
             if (__any(rel >= 0 && rel < TN && !(rel & 4))) {
 #pragma unroll
                 for (int j = 0; j < FN; ++j)
@@ -223,18 +248,12 @@ __global__ __launch_bounds__(64 * Shape<T>::NW, 2) void logits_kernel(HeadArgs a
         const int crow = elane / WC, cchk = elane % WC, nc = n0 + wn * TN + 8 * cchk;
 #pragma unroll
         for (int i = 0; i < FM; ++i) {
-            const int row = m1 + 32 * i;
-            float g = 0.0f, l = 0.0f;
-            int rel = -1;
-            if (row < count) {
-                g = slope_of(a, row, count);
-                l = a.lse[row];
-                rel = word_of(a, row) - a.v0 - nw;
-            }
+            const float g = slope[i], l = -lse[i] * LOG2E;
+            const int rel = word[i] - a.v0 - nw;
 #pragma unroll
             for (int j = 0; j < FN; ++j)
 #pragma unroll
-                for (int x = 0; x < 16; ++x) pr.acc[i][j][x] = g * __builtin_amdgcn_exp2f((pr.acc[i][j][x] - l) * LOG2E);
+                for (int x = 0; x < 16; ++x) pr.acc[i][j][x] = g * exp_from(pr.acc[i][j][x], l);
             if (__any(rel >= 0 && rel < TN && !(rel & 4))) {
 #pragma unroll
                 for (int j = 0; j < FN; ++j)
@@ -327,9 +346,8 @@ __global__ __launch_bounds__(64 * Shape<T>::NW, WPS) void piece_kernel(HeadArgs 
     const int wm = wave / SH::WN, wn = wave % SH::WN;
     const int count = kept_rows(a);
     const int M = KIND == HD_DX ? count : a.vn, K = KIND == HD_DX ? a.vn : count;
-    const int tiles_m = (M + T - 1) / T, split = blockIdx.x % a.splits;
-    int mt, nt;
-    if (!find_tile<4>(blockIdx.x / a.splits, tiles_m, a.tiles_n, mt, nt)) return;
+    int mt, nt, split;
+    if (!find_tile<4>(blockIdx.x, (M + T - 1) / T, a.tiles_n, a.splits, mt, nt, split)) return;
     const int m0 = mt * T, n0 = nt * T;
     // this split's share of K: `slabs` of them from kb on.  The words of a piece are rounded up to 8 in G, whose columns
     // there are 0, not in W.
@@ -457,25 +475,36 @@ __global__ __launch_bounds__(256) void dw_kernel(HeadArgs a) {
 // plans
 // ---------------------------------------------------------------------------
 
-// The estimated time (us) of M x N results over K in tiles of T: p per slab of 64 k of a tile with every CU busy, u for a
-// tile that has its CU to itself, o for its start and end.
+// The estimated time (us) of M x N results over K in tiles of T, `splits` shares of K: p per slab of 64 k of a tile with every CU
+// busy, u for a tile that has its CU to itself, o for its start and end; the last round of tiles counts half if it is not full.
+// Fitted to these times of whole backward passes with one product's tile (and shares of K) changed, us, best and others:
+//   rows, words, width       logits 64  128  256     dx                                dW
+//   4096, 16384, 384                265  237  230    (128, 4) 231 (256, 8) 240         (128, 1) 209 (256, 1) 227 (128, 2) 219
+//   1024, 32000, 1024               271  241  230    (256, 12) 224 (128, 8) 227        (256, 1) 226 (128, 1) 229 (64, 1) 270
+//   300, 50257, 768                 141  132  137    (128, 12) 129 (64, 12) 134        (128, 1) 132 (256, 1) 137
+//   2000, 8000, 4096                478  422  401    (256, 2) 401 (128, 1) 420         (256, 1) 401 (128, 1) 418
+//   16384, 512, 512                  77   76   76    (64, 1) 75 (128, 1) 76            (128, 16) 75 (64, 8) 76 (128, 1) 192
+//   8191, 32000, 2048              3548 3035 2810    (256, 1) 2811 (256, 2) 2845       (256, 1) 2814 (256, 2) 3048
+// and of forward passes (64, 128, 256): 700, 3000, 2048 34 40 58; 64, 128256, 4096 246 214 246; 300, 50257, 768 73 58 58.
 static float tiles_cost(int64_t M, int64_t N, int64_t K, int T, int splits) {
     const int i = T == 256 ? 2 : T == 128 ? 1 : 0;
-    constexpr float P[3] = {0.25f, 0.62f, 1.9f}, U[3] = {0.5f, 0.75f, 1.2f}, O[3] = {2.0f, 4.0f, 8.0f};
-    const float n = (float)((M + T - 1) / T) * (float)((N + T - 1) / T) * (float)splits / 256.0f, ks = ceilf((float)K / 64.0f / (float)splits);
-    return ks * std::max(n * P[i], U[i]) + std::max(n, 1.0f) * O[i];
+    constexpr float P[3] = {0.32f, 0.62f, 1.9f}, U[3] = {0.5f, 1.0f, 1.3f}, O[3] = {2.0f, 4.0f, 8.0f};
+    const float all = (float)((M + T - 1) / T) * (float)((N + T - 1) / T) * (float)splits / 256.0f, n = 0.5f * (all + ceilf(all));
+    return ceilf((float)K / 64.0f / (float)splits) * std::max(n * P[i], U[i]) + std::max(n, 1.0f) * O[i];
 }
 struct Tiling {
     int tile, splits;
 };
-static Tiling tiling(int64_t M, int64_t N, int64_t K, bool split) {
+// slots: 0: K is not split; 1: results go through a slot anyway (dx); 2: they do where K is split, in one more launch (dW)
+static Tiling tiling(int64_t M, int64_t N, int64_t K, int slots) {
     Tiling best{128, 1};
     float least = 1e30f;
     for (const int T : {64, 128, 256})
-        for (int s = 1; s <= (split ? 16 : 1); ++s) {
+        for (int s = 1; s <= (slots ? 16 : 1); ++s) {
             if (s > 1 && K < 256 * s) break;
-            // a slot more is written, read and added to: 8 bytes per result at 4 TB/s
-            const float c = tiles_cost(M, N, K, T, s) + (float)(s - 1) * (float)(M * N) * 8.0f / 4e6f;
+            // a slot is written and read: 8 bytes per result at 4 TB/s
+            const float each = (float)(M * N) * 8.0f / 4e6f;
+            const float c = tiles_cost(M, N, K, T, s) + (s == 1 ? 0.0f : slots == 1 ? (float)(s - 1) * each : (float)s * each + 5.0f);
             if (c < least) {
                 least = c;
                 best = {T, s};
@@ -484,7 +513,9 @@ static Tiling tiling(int64_t M, int64_t N, int64_t K, bool split) {
     return best;
 }
 
-constexpr int64_t PIECE_BYTES = int64_t(128) << 20;   // of G, about
+// Of G, about.  Gradients of 8192 rows, 128256 words of 4096: 20.62 ms in pieces of 128 MiB, 20.58 of 256, 20.32 of 512, 20.28 of
+// 1024; of 8191 rows, 32000 words of 2048: 2.79, 2.81, 2.77, 2.77 ms.
+constexpr int64_t PIECE_BYTES = int64_t(512) << 20;
 constexpr int64_t PIECE_WORDS = 1 << 18;              // at most: a slab's rows of G span less than 2^31 bytes
 struct HeadPlan {
     Tiling fwd, logits, dx, dw;
@@ -495,7 +526,7 @@ static size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 
 static HeadPlan head_plan(int64_t rows, int64_t vocab, int64_t d) {
     HeadPlan p{};
-    p.fwd = tiling(rows, vocab, d, false);
+    p.fwd = tiling(rows, vocab, d, 0);
     const int64_t tn = (vocab + p.fwd.tile - 1) / p.fwd.tile;
     p.fwd_bytes = up256((size_t)tn * (size_t)rows * 8) + 2 * up256((size_t)rows * 4);
     // whole tiles of 256 words, in pieces of one size
@@ -503,9 +534,9 @@ static HeadPlan head_plan(int64_t rows, int64_t vocab, int64_t d) {
     const int64_t pieces = (vocab + most - 1) / most;
     p.piece = std::min<int64_t>(((vocab + pieces - 1) / pieces + 255) / 256 * 256, (vocab + 7) / 8 * 8);
     p.ldg = p.piece;
-    p.logits = tiling(rows, p.piece, d, false);
-    p.dx = tiling(rows, d, p.piece, true);
-    p.dw = tiling(p.piece, d, rows, true);
+    p.logits = tiling(rows, p.piece, d, 0);
+    p.dx = tiling(rows, d, p.piece, 1);
+    p.dw = tiling(p.piece, d, rows, 2);
     p.g_at = 0;
     p.dx_at = up256((size_t)rows * (size_t)p.ldg * 2);
     p.dw_at = p.dx_at + up256((size_t)p.dx.splits * (size_t)rows * (size_t)d * 4);

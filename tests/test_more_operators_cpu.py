@@ -28,8 +28,8 @@ def test_head_sizes(lib):
         assert 0 < piece <= max(8, (vocab + 7) // 8 * 8) and (piece % 256 == 0 or piece >= vocab)
         assert f.value >= 8 * rows * -(-vocab // fwd) + 8 * rows
         assert b.value >= 2 * rows * piece + 4 * dxs * rows * d + (4 * dws * piece * d if dws > 1 else 0)
-        # neither grows with rows x words: a piece of G is 128 MiB, or 256 words of every row
-        assert 2 * rows * piece <= max(128 << 20, 2 * 256 * rows)
+        # neither grows with rows x words: a piece of G is 512 MiB, or 256 words of every row
+        assert 2 * rows * piece <= max(512 << 20, 2 * 256 * rows)
     for rows, vocab, d in ((-1, 5, 8), (1 << 24, 5, 8), (5, 0, 8), (5, 1 << 24, 8), (5, 5, 0), (5, 5, 12), (5, 5, 1 << 17), ((1 << 23), 1 << 23, 8)):
         assert lib.msr_head_workspace_bytes(rows, vocab, d, ctypes.byref(f), ctypes.byref(b)) == ARG
         assert lib.msr_head_plan(rows, vocab, d, plan) == ARG
