@@ -1,16 +1,19 @@
-"""Builds libmuon_sr_amd.so (the gfx950 HIP kernels + C ABI) in-tree.
+"""Builds libmuon_sr_amd.so (the gfx950 HIP kernels + C ABI) and _nodes.so (autograd nodes that call it) in-tree.
 
-The library depends only on the HIP runtime; it is loaded with ctypes.
+The library depends only on the HIP runtime; it is loaded with ctypes.  _nodes.so is host code against torch's C++
+headers, a Python module; it finds the library beside itself.
 """
 from __future__ import annotations
 
 import glob
 import os
 import subprocess
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libmuon_sr_amd.so")
+NODES = os.path.join(HERE, "_nodes.so")
 ARCH = os.environ.get("MSR_OFFLOAD_ARCH", "gfx950")
 
 # IEEE fp32 without contraction (the kernels restate the reference's expression
@@ -53,19 +56,38 @@ def _run(cmd, verbose):
     _finish(cmd, subprocess.run(cmd, capture_output=True, text=True), verbose)
 
 
+def nodes_commands(obj: str, out: str):
+    """Of the autograd nodes: compile, and link (after the library, which they are linked with)."""
+    import torch
+    from torch.utils.cpp_extension import include_paths
+    includes = [*include_paths("cuda"), sysconfig.get_paths()["include"]]
+    compile_ = ["g++", "-O2", "-std=c++17", "-fPIC", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", "-DTORCH_API_INCLUDE_EXTENSION_H",
+                "-DTORCH_EXTENSION_NAME=_nodes", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+                *(f for i in includes for f in ("-isystem", i)), "-c", "-o", obj, os.path.join(CSRC, "nodes.cpp")]
+    link = ["g++", "-shared", "-o", out, obj, f"-L{HERE}", "-lmuon_sr_amd", "-Wl,-rpath,$ORIGIN",
+            f"-L{os.path.join(os.path.dirname(torch.__file__), 'lib')}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_hip"]
+    return compile_, link
+
+
 def build(verbose: bool = False) -> str:
     """Compile every HIP source (each with its own flags, all at once) and link one
-    shared library.  Always recompiles; objects go to muon_sr_amd/_build/."""
+    shared library, then the autograd nodes.  Always recompiles; objects go to muon_sr_amd/_build/."""
     objdir = os.path.join(HERE, "_build")
     os.makedirs(objdir, exist_ok=True)
     objs, jobs = [], []
+
+    def start(cmd):
+        if verbose:
+            print(" ".join(cmd), flush=True)
+        jobs.append((cmd, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.PIPE, text=True)))
+
+    nodes_compile, nodes_link = nodes_commands(os.path.join(objdir, "nodes.cpp.o"), NODES + ".tmp")
+    start(nodes_compile)
     for src in sources():
         obj = os.path.join(objdir, os.path.basename(src) + ".o")
         flags = [f for f in HIPCC_FLAGS if f != "-shared"]
         cmd = [hipcc(), *flags, *EXTRA_FLAGS.get(os.path.basename(src), []), "-c", "-o", obj, src]
-        if verbose:
-            print(" ".join(cmd), flush=True)
-        jobs.append((cmd, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.PIPE, text=True)))
+        start(cmd)
         objs.append(obj)
     for cmd, proc in jobs:
         out, err = proc.communicate()
@@ -73,6 +95,8 @@ def build(verbose: bool = False) -> str:
     tmp = LIB + ".tmp"
     _run([hipcc(), f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", tmp, *objs], verbose)
     os.replace(tmp, LIB)
+    _run(nodes_link, verbose)
+    os.replace(NODES + ".tmp", NODES)
     return LIB
 
 

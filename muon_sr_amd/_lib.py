@@ -157,7 +157,7 @@ SIGNATURES = {
 # MSR_ERR_ARG, _ALIGN and _OVERLAP: a call that returns one of these has launched nothing
 REFUSED = (1001, 1002, 1005)
 
-_lib = None
+_lib = _nodes = None
 _lock = threading.Lock()
 
 
@@ -182,6 +182,20 @@ def lib():
                     fn.argtypes = args
                 _lib = L
     return _lib
+
+
+def nodes():
+    """The autograd nodes (csrc/nodes.cpp), which call the same library (raises if they have not been built)."""
+    global _nodes
+    if _nodes is None:
+        lib()
+        try:
+            from . import _nodes as built
+        except ImportError as e:
+            raise MuonSRLibraryError(f"muon_sr_amd/_nodes.so cannot be loaded ({e}): build it with `python -m muon_sr_amd._build`") from e
+        built.set_error_type(MuonSRLibraryError)
+        _nodes = built
+    return _nodes
 
 
 def check(rc: int, what: str) -> None:

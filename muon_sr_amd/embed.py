@@ -16,27 +16,10 @@ import random
 import torch
 
 from . import _lib
-from .experts import _ELEM, _elem, _once, _one_gpu
+from .experts import _once, _one_gpu
 from .head import _flat_rows
 
 __all__ = ["embedding", "embedding_grad_sr_accum", "SREmbedding"]
-
-
-def _check(what, ids, weight, padding_idx):
-    _one_gpu(what, weight, ids)
-    _elem(weight, f"{what}: weight")
-    if weight.dim() != 2 or not weight.is_contiguous():
-        raise ValueError(f"{what} needs a contiguous weight [vocab, d], got {tuple(weight.shape)}")
-    if ids.dtype not in (torch.int32, torch.int64):
-        raise ValueError(f"{what} needs int32 or int64 ids, got {ids.dtype}")
-    vocab = weight.shape[0]
-    if vocab == 0:
-        raise ValueError(f"{what} needs words, got {tuple(weight.shape)}")
-    if padding_idx is None:
-        return -1
-    if not -vocab <= padding_idx < vocab:
-        raise ValueError(f"{what}: padding_idx {padding_idx} is outside the {vocab} words")
-    return padding_idx % vocab
 
 
 def _grad_args(ids, dy, vocab, d, scale, padding):
@@ -47,14 +30,6 @@ def _grad_args(ids, dy, vocab, d, scale, padding):
     _lib.check(_lib.lib().msr_embedding_workspace_bytes(ids.numel(), vocab, d, ctypes.byref(size)), "msr_embedding_workspace_bytes")
     ws = _lib.workspace(dy, size.value)
     return (ids.data_ptr(), int(ids.dtype == torch.int64), ids.numel(), dy.data_ptr(), ld, vocab, d, scale, padding), (ids, dy), ws, size.value
-
-
-def _grad(weight, ids, dy, scale, padding):
-    vocab, d = weight.shape
-    dw = torch.empty_like(weight, memory_format=torch.contiguous_format)
-    args, keep, ws, size = _grad_args(ids, dy, vocab, d, scale, padding)
-    _lib.call(weight, "msr_embedding_grad", *args, dw.data_ptr(), _ELEM[weight.dtype], _lib.ptr(ws), size)
-    return dw
 
 
 def _accumulate(weight, ids, dy, scale, padding, seed):
@@ -71,37 +46,26 @@ def _accumulate(weight, ids, dy, scale, padding, seed):
         weight.acc_grad = acc
 
 
-class _Embedding(torch.autograd.Function):
+class _Accumulating(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, ids, weight, scale, padding, accumulate):
-        vocab, d = weight.shape
-        ids = ids.contiguous()
-        y = torch.empty((*ids.shape, d), dtype=weight.dtype, device=weight.device)
-        _lib.call(weight, "msr_embedding", ids.data_ptr(), int(ids.dtype == torch.int64), ids.numel(), weight.data_ptr(), vocab, d, scale,
-                  y.data_ptr(), _ELEM[weight.dtype])
-        ctx.save_for_backward(ids, weight)
-        ctx.scale, ctx.padding = scale, padding
-        # the tensor that holds acc_grad: saved-tensor hooks unpack another one.  A weight that is computed (a
-        # parametrization) holds nothing that lasts, and one that is not bf16 has no accumulator: autograd gets the gradient.
-        ctx.owner = weight if accumulate and weight.is_leaf and weight.dtype == torch.bfloat16 else None
-        return y
+    def forward(ctx, ids, weight, scale, padding_idx):
+        ctx.save_for_backward(ids)
+        # the tensor that holds acc_grad: saved-tensor hooks (activation checkpointing, offloading) would unpack another one
+        ctx.owner, ctx.scale, ctx.padding_idx = weight, scale, padding_idx
+        return _lib.nodes().embedding(ids, weight, padding_idx, scale)
 
     @staticmethod
     @_once
     def backward(ctx, dy):
-        ids, weight = ctx.saved_tensors
-        if ctx.owner is None:
-            return None, _grad(weight, ids, dy, ctx.scale, ctx.padding), None, None, None
-        _accumulate(ctx.owner, ids, dy, ctx.scale, ctx.padding, None)
-        return None, None, None, None, None
+        embedding_grad_sr_accum(ctx.owner, *ctx.saved_tensors, dy, ctx.padding_idx, ctx.scale)
+        return None, None, None, None
 
 
 def embedding(ids: torch.Tensor, weight: torch.Tensor, padding_idx: int = None, scale: float = 1.0) -> torch.Tensor:
     """``scale * weight[ids]``, rounded once, as [*ids.shape, d].  ``weight``: bf16 or fp32 [vocab, d]; ``ids``: int32 or int64; one
     outside [0, vocab) has no word: its row is 0 and gives no gradient.  ``padding_idx`` gives none either (its row is
     looked up as any other).  The gradient goes to autograd, whole; ``SREmbedding`` adds it to its accumulator."""
-    padding = _check("embedding", ids, weight, padding_idx)
-    return _Embedding.apply(ids, weight, float(scale), padding, False)
+    return _lib.nodes().embedding(ids, weight, padding_idx, scale)
 
 
 def embedding_grad_sr_accum(weight: torch.Tensor, ids: torch.Tensor, dy: torch.Tensor, padding_idx: int = None,
@@ -110,7 +74,7 @@ def embedding_grad_sr_accum(weight: torch.Tensor, ids: torch.Tensor, dy: torch.T
     other rows are not touched.  ``weight``: bf16 [vocab, d], ``dy``: bf16 [*ids.shape, d].  The buffer is created (as
     zeros) on the first call, and one that is there has to be like it (ValueError); ``seed``: 32 bits, drawn from ``random``
     if not given, as the accumulator's hook draws it."""
-    padding = _check("embedding_grad_sr_accum", ids, weight, padding_idx)
+    padding = _lib.nodes().check_embedding("embedding_grad_sr_accum", ids, weight, padding_idx)
     _one_gpu("embedding_grad_sr_accum", weight, dy)
     if weight.dtype != torch.bfloat16 or dy.dtype != torch.bfloat16:
         raise ValueError(f"embedding_grad_sr_accum needs bf16 tensors, got {weight.dtype} and {dy.dtype}")
@@ -131,8 +95,12 @@ class SREmbedding(torch.nn.Embedding):
         self.scale = float(scale)
 
     def forward(self, ids: torch.Tensor) -> torch.Tensor:
-        padding = _check("SREmbedding", ids, self.weight, self.padding_idx)
-        return _Embedding.apply(ids, self.weight, self.scale, padding, True)
+        weight = self.weight
+        # a weight that is computed (a parametrization) holds nothing that lasts, and one that is not bf16 has no accumulator: autograd
+        # gets the gradient
+        if weight.is_leaf and weight.dtype == torch.bfloat16 and weight.requires_grad and torch.is_grad_enabled():
+            return _Accumulating.apply(ids, weight, self.scale, self.padding_idx)
+        return embedding(ids, weight, self.padding_idx, self.scale)
 
     def extra_repr(self):
         return super().extra_repr() + (f", scale={self.scale}" if self.scale != 1.0 else "")

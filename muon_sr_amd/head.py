@@ -17,29 +17,10 @@ import random
 import torch
 
 from . import _lib
-from .experts import _once, _one_gpu
+from .experts import _once
 from .linear import SRLinear
 
 __all__ = ["linear_cross_entropy", "SRHead"]
-
-_REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
-
-
-def _check(what, x, weight, target, reduction):
-    _one_gpu(what, x, weight, target)
-    if reduction not in _REDUCTIONS:
-        raise ValueError(f"{what}: reduction must be one of {sorted(_REDUCTIONS)}, got {reduction!r}")
-    if weight.dim() != 2 or not weight.is_contiguous():
-        raise ValueError(f"{what} needs a contiguous weight [vocab, d], got {tuple(weight.shape)}")
-    if x.dtype != torch.bfloat16 or weight.dtype != torch.bfloat16:
-        raise ValueError(f"{what} needs bf16 x and weight, got {x.dtype} and {weight.dtype}")
-    if target.dtype not in (torch.int32, torch.int64):
-        raise ValueError(f"{what} needs int32 or int64 targets, got {target.dtype}")
-    d = weight.shape[1]
-    if x.dim() < 1 or x.shape[-1] != d or target.shape != x.shape[:-1]:
-        raise ValueError(f"{what} needs x [..., {d}] and a target for each row, got {tuple(x.shape)} and {tuple(target.shape)}")
-    if d % 8 or d == 0 or weight.shape[0] == 0:
-        raise ValueError(f"{what} needs words, and a width that is a multiple of 8, got {tuple(weight.shape)}")
 
 
 def _flat_rows(t: torch.Tensor, d: int):
@@ -65,9 +46,9 @@ def _sizes(rows, vocab, d):
     return forward.value, backward.value
 
 
-class _HeadLoss(torch.autograd.Function):
+class _Accumulating(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, target, ignore_index, reduction, accumulate):
+    def forward(ctx, x, weight, target, ignore_index, reduction):
         vocab, d = weight.shape
         rows2, ld = _flat_rows(x, d)
         rows, target = rows2.shape[0], target.contiguous()
@@ -82,9 +63,8 @@ class _HeadLoss(torch.autograd.Function):
                   _lib.ptr(ws), size)
         ctx.save_for_backward(packed, weight, kept, lse)
         ctx.shape, ctx.reduction = x.shape, reduction
-        # the tensor that holds acc_grad: saved-tensor hooks (activation checkpointing, offloading) unpack another one.  A
-        # weight that is computed (a parametrization) holds nothing that lasts, so its gradient goes to autograd.
-        ctx.owner = weight if accumulate and weight.is_leaf else None
+        # the tensor that holds acc_grad: saved-tensor hooks (activation checkpointing, offloading) unpack another one
+        ctx.owner = weight
         return loss
 
     @staticmethod
@@ -94,24 +74,19 @@ class _HeadLoss(torch.autograd.Function):
         packed, weight, kept, lse = _packed(packed), _packed(weight), kept.contiguous(), lse.contiguous()
         vocab, d = weight.shape
         rows, dloss, owner = packed.shape[0], dloss.contiguous(), ctx.owner
-        want_dx, want_dw = ctx.needs_input_grad[:2]
-        dx = torch.empty(ctx.shape, dtype=torch.bfloat16, device=packed.device) if want_dx else None
-        out, mode, seed, first = None, -1, 0, False
-        if want_dw and owner is not None:
-            first, mode = not hasattr(owner, "acc_grad"), _lib.noise_mode()
-            if not first:
-                _lib.check_accumulator(owner, "SRHead")
-            seed = random.getrandbits(32)
-            out = torch.empty_like(owner, memory_format=torch.contiguous_format) if first else owner.acc_grad
-        elif want_dw:
-            out = torch.empty_like(weight)
+        first = not hasattr(owner, "acc_grad")
+        if not first:
+            _lib.check_accumulator(owner, "SRHead")
+        seed = random.getrandbits(32)
+        acc = torch.empty_like(owner, memory_format=torch.contiguous_format) if first else owner.acc_grad
+        dx = torch.empty(ctx.shape, dtype=torch.bfloat16, device=packed.device) if ctx.needs_input_grad[0] else None
         _, size = _sizes(rows, vocab, d)
         ws = _lib.workspace(packed, size)
         _lib.call(packed, "msr_head_backward", packed.data_ptr(), weight.data_ptr(), kept.data_ptr(), lse.data_ptr(), dloss.data_ptr(),
-                  rows, vocab, d, ctx.reduction, _lib.ptr(dx), _lib.ptr(out), mode, seed, int(first), None, _lib.ptr(ws), size)
+                  rows, vocab, d, ctx.reduction, _lib.ptr(dx), acc.data_ptr(), _lib.noise_mode(), seed, int(first), None, _lib.ptr(ws), size)
         if first:
-            owner.acc_grad = out
-        return dx, out if owner is None else None, None, None, None, None
+            owner.acc_grad = acc
+        return dx, None, None, None, None
 
 
 def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, ignore_index: int = -100,
@@ -122,8 +97,7 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     ignored (0 where all are: torch's mean is NaN there).  Any other target outside [0, vocab) gives NaN, in the loss
     and the gradients.  The gradients are bf16, of products with fp32 accumulation; the weight gradient
     goes to autograd (``TritonSRAccumulator``'s hook accumulates it as any other)."""
-    _check("linear_cross_entropy", x, weight, target, reduction)
-    return _HeadLoss.apply(x, weight, target, ignore_index, _REDUCTIONS[reduction], False)
+    return _lib.nodes().linear_cross_entropy(x, weight, target, ignore_index, reduction)
 
 
 class SRHead(SRLinear):
@@ -137,5 +111,9 @@ class SRHead(SRLinear):
         super().__init__(in_features, vocab, bias=False, device=device, dtype=dtype)
 
     def loss(self, x: torch.Tensor, target: torch.Tensor, ignore_index: int = -100, reduction: str = "mean") -> torch.Tensor:
-        _check("SRHead", x, self.weight, target, reduction)
-        return _HeadLoss.apply(x, self.weight, target, ignore_index, _REDUCTIONS[reduction], True)
+        weight = self.weight
+        # a weight that is computed (a parametrization) holds nothing that lasts: autograd gets its gradient
+        if not (weight.is_leaf and weight.requires_grad and torch.is_grad_enabled()):
+            return linear_cross_entropy(x, weight, target, ignore_index, reduction)
+        code = _lib.nodes().check_head("SRHead", x, weight, target, reduction)
+        return _Accumulating.apply(x, weight, target, ignore_index, code)
