@@ -18,6 +18,8 @@ constexpr int SORT_WAVES = SORT_THREADS / 64, SORT_BITS = 9;    // bits of a pas
 constexpr int CHUNK = 32;                                       // sorted tokens of a wave
 constexpr int FEW = 256;                                        // tokens that are not sorted
 
+// Rows are written past the caches: a batch's y, and a whole dW, are larger than they (16384 tokens, 128256 words of 4096: lookup
+// 52 us with cached stores, 36 so; gradient 218 and 213).
 struct EmbedArgs {
     const void *ids;
     const void *w;               // [vocab][d]
@@ -70,7 +72,7 @@ __global__ __launch_bounds__(256) void lookup_kernel(EmbedArgs a) {
                 for (int e = 0; e < C::N; ++e) f[e] *= a.scale;
                 x[u].set(f);
             }
-            x[u].store(static_cast<T *>(a.out) + i * a.d, c, a.d);
+            x[u].template store<true>(static_cast<T *>(a.out) + i * a.d, c, a.d);
         }
     }
 }
@@ -190,23 +192,25 @@ __device__ __forceinline__ int64_t below(const uint64_t *keys, int64_t n, uint64
 }
 
 // Runs of `run` keys (a power of two), MERGE_WAYS at a time, merged: a key's place is its own number in its run plus how many of
-// each other are below it, searched for in four runs at once (a search is a chain of loads).
+// each other are below it, searched for in eight runs at once (a search is a chain of loads).
 __global__ __launch_bounds__(256) void merge_kernel(const uint64_t *in, uint64_t *out, int64_t n, int64_t run) {
+    constexpr int AT_ONCE = 8;
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= n) return;
     const int64_t first = i / (run * MERGE_WAYS) * (run * MERGE_WAYS), mine = i / run * run, end = min(first + run * MERGE_WAYS, n);
     const uint64_t key = in[i];
     int64_t place = first + (i - mine);
-    for (int64_t r0 = first; r0 < end; r0 += 4 * run) {
-        int64_t lo[4] = {0, 0, 0, 0}, len[4];
+    for (int64_t r0 = first; r0 < end; r0 += AT_ONCE * run) {
+        int lo[AT_ONCE] = {}, len[AT_ONCE];
 #pragma unroll
-        for (int y = 0; y < 4; ++y) len[y] = r0 + y * run == mine ? 0 : max((int64_t)0, min(run, end - (r0 + y * run)));
-        for (int64_t step = run; step; step >>= 1) {
+        for (int y = 0; y < AT_ONCE; ++y) len[y] = r0 + y * run == mine ? 0 : (int)max((int64_t)0, min(run, end - (r0 + y * run)));
+        for (int step = (int)run; step; step >>= 1) {
 #pragma unroll
-            for (int y = 0; y < 4; ++y)
+            for (int y = 0; y < AT_ONCE; ++y)
                 if (lo[y] + step <= len[y] && in[r0 + y * run + lo[y] + step - 1] < key) lo[y] += step;
         }
-        place += (lo[0] + lo[1]) + (lo[2] + lo[3]);
+#pragma unroll
+        for (int y = 0; y < AT_ONCE; ++y) place += lo[y];
     }
     out[place] = key;
 }
@@ -246,7 +250,7 @@ __device__ __forceinline__ void finish(const EmbedArgs &a, int v, int64_t c, con
             o[q] = pack2(sr_bf16(bf16_lo(old.v.w[q]) + bf16_lo(x.v.w[q]), rn[2 * q]), sr_bf16(bf16_hi(old.v.w[q]) + bf16_hi(x.v.w[q]), rn[2 * q + 1]));
         x.v = Bytes16{{o[0], o[1], o[2], o[3]}};
     }
-    x.store(row, c, a.d);
+    x.template store<true>(row, c, a.d);
 }
 
 // Words that a wave looks up and zeroes where no token has them: 64, or 8 where that leaves waves idle (512 words of 256: 18 us
@@ -258,7 +262,7 @@ __device__ __forceinline__ void zero_rows(const EmbedArgs &a, int64_t v0, uint64
     Cells<T> zero;
     zero.v = Bytes16{};
     for (; none; none &= none - 1)
-        if (c < a.d) zero.store(static_cast<T *>(a.out) + (v0 + __builtin_ctzll(none)) * a.d, c, a.d);
+        if (c < a.d) zero.template store<true>(static_cast<T *>(a.out) + (v0 + __builtin_ctzll(none)) * a.d, c, a.d);
 }
 
 // floats [c, c + N) of a part of d

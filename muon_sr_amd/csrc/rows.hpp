@@ -10,6 +10,10 @@
 namespace msr {
 
 struct __attribute__((packed, aligned(2))) Bytes16 { uint32_t w[4]; };   // 16 bytes at any address of an element type
+typedef uint32_t u32x4_any_t __attribute__((ext_vector_type(4), aligned(2)));
+__device__ __forceinline__ void st_nt16(void *p, const Bytes16 &v) {
+    __builtin_nontemporal_store(u32x4_any_t{v.w[0], v.w[1], v.w[2], v.w[3]}, static_cast<u32x4_any_t *>(p));
+}
 
 // 16 bytes of a row: N elements from column c on, those from d on zero and not stored.  Rows may begin at any element:
 // global accesses of 16 bytes need no more alignment than that.
@@ -32,9 +36,12 @@ struct Cells {
             }
         }
     }
+    // NT: past the caches
+    template <bool NT = false>
     __device__ __forceinline__ void store(T *row, int64_t c, int64_t d) const {
         if (c + N <= d) {
-            *reinterpret_cast<Bytes16 *>(row + c) = v;
+            if constexpr (NT) st_nt16(row + c, v);
+            else *reinterpret_cast<Bytes16 *>(row + c) = v;
         } else {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
