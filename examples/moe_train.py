@@ -1,12 +1,12 @@
 """Trains a small mixture-of-experts language model with this package's operators on one GPU.
 
 A byte of text predicts the next one through an embedding, two mixture-of-experts blocks (a
-router's top 2 of 8 experts for every token) and a head, all bf16.  Each step runs
+router's top 2 of 8 experts for every token) and a head, all bf16.  Each step runs ``SREmbedding``, then per block
 
-    router (torch) -> order_tokens -> dispatch_tokens -> SRExperts -> GELU -> SRExperts -> combine_tokens
+    LayerNorm -> router (torch) -> order_tokens -> dispatch_tokens -> SRExperts -> GELU -> SRExperts -> combine_tokens
 
-forward and backward over a few micro-batches, whose gradients ``TritonSRAccumulator`` and
-``SRExperts`` accumulate with stochastic rounding; ``clip_grad_norm_`` cuts their global norm;
+with the router's ``balance_loss``, and ``SRHead``'s loss, forward and backward over a few micro-batches, whose gradients
+``TritonSRAccumulator``, ``SREmbedding``, ``SRExperts`` and ``SRHead`` accumulate with stochastic rounding; ``clip_grad_norm_`` cuts their global norm;
 ``TritonMuonSRWithAuxAdam`` steps the experts' matrices with Muon and the rest with AdamW.
 
     python examples/moe_train.py [--steps 200] [--micro 4] [--tokens 4096]
@@ -25,8 +25,8 @@ import torch.nn.functional as F
 
 sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 
-from muon_sr_amd import (SRExperts, TritonMuonSRWithAuxAdam, TritonSRAccumulator, clip_grad_norm_,  # noqa: E402
-                         combine_tokens, dispatch_tokens, order_tokens)
+from muon_sr_amd import (LayerNorm, SREmbedding, SRExperts, SRHead, TritonMuonSRWithAuxAdam,  # noqa: E402
+                         TritonSRAccumulator, balance_loss, clip_grad_norm_, combine_tokens, dispatch_tokens, order_tokens)
 
 BF16 = torch.bfloat16
 
@@ -42,35 +42,43 @@ class MoE(nn.Module):
         self.down = SRExperts(experts, hidden, d, device=device)
 
     def forward(self, x):
-        scores = torch.softmax(self.router(x).float(), -1)
+        logits = self.router(x)
+        scores = torch.softmax(logits.float(), -1)
         weights, ids = torch.topk(scores, self.k, dim=-1)
         weights = weights / weights.sum(-1, keepdim=True)
         order = order_tokens(ids, self.experts)
         rows = dispatch_tokens(x, order)
         rows = self.down(F.gelu(self.up(rows, order.offsets)), order.offsets)
-        y = combine_tokens(rows, weights, order)
-        # the usual balance term: experts times the product of their share of the slots and of the scores
-        share = (order.offsets[1:] - order.offsets[:-1]).float() / ids.numel()
-        return y, self.experts * (share * scores.mean(0)).sum()
+        return combine_tokens(rows, weights, order), balance_loss(logits, ids)[0]
 
 
 class Model(nn.Module):
     def __init__(self, d=256, hidden=512, experts=8, k=2, blocks=2, context=4, device="cuda"):
         super().__init__()
         self.context = context
-        self.embed = nn.Embedding(256, d, device=device, dtype=BF16)
+        self.embed = SREmbedding(256, d, device=device)
         self.mix = nn.Linear(context * d, d, bias=False, device=device, dtype=BF16)
-        self.norms = nn.ModuleList(nn.LayerNorm(d, device=device, dtype=BF16) for _ in range(blocks))
+        self.norms = nn.ModuleList(LayerNorm(d, device=device, dtype=BF16) for _ in range(blocks))
         self.moe = nn.ModuleList(MoE(d, hidden, experts, k, device) for _ in range(blocks))
-        self.head = nn.Linear(d, 256, bias=False, device=device, dtype=BF16)
+        self.head = SRHead(d, 256, device=device)
 
-    def forward(self, idx):
-        """idx: [tokens, context] bytes -> logits [tokens, 256] and the balance term."""
+    def features(self, idx):
+        """idx: [tokens, context] bytes -> the head's input [tokens, d] and the balance term."""
         x, balance = self.mix(self.embed(idx).flatten(1)), 0.0
         for norm, moe in zip(self.norms, self.moe):
             y, b = moe(norm(x))
             x, balance = x + y, balance + b
+        return x, balance
+
+    def forward(self, idx):
+        """Logits [tokens, 256] and the balance term."""
+        x, balance = self.features(idx)
         return self.head(x), balance
+
+    def loss(self, idx, target):
+        """The mean cross entropy and the balance term, without the logits in memory."""
+        x, balance = self.features(idx)
+        return self.head.loss(x, target), balance
 
 
 def param_groups(model):
@@ -108,8 +116,7 @@ def train(steps=200, micro=4, tokens=4096, max_norm=0.3, seed=0, report=None):
         for _ in range(micro):
             at = torch.randint(0, data.numel() - c, (tokens,), generator=gen, device="cuda")
             window = data[at[:, None] + torch.arange(c + 1, device="cuda")]
-            logits, balance = model(window[:, :c])
-            loss = F.cross_entropy(logits.float(), window[:, c])
+            loss, balance = model.loss(window[:, :c], window[:, c])
             ((loss + 0.01 * balance) / micro).backward()
             total = total + loss.detach() / micro
         TritonSRAccumulator.reassign_grad_buffer(model)
