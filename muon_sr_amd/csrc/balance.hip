@@ -51,7 +51,7 @@ __device__ __forceinline__ float over_group(float x, Op op) {
     return x;
 }
 
-constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 // Work-group b's tokens: [b per, (b + 1) per).  blockDim.x: 256 or 1024.
 template <typename T, int L, int U>
@@ -71,36 +71,52 @@ __global__ __launch_bounds__(BAL_THREADS) void balance_kernel(BalanceArgs a, int
     else if (tid == 0 && last > first)
         counted = (int)(last - first);
     if (counted) atomicAdd(&hist[a.experts], counted);
-#pragma unroll 4
-    for (int64_t i = first * a.k + tid; i < last * a.k; i += blockDim.x) {
-        const int64_t e = a.i64 ? static_cast<const int64_t *>(a.ids)[i] : static_cast<const int32_t *>(a.ids)[i];
-        if (e >= 0 && e < a.experts && (!a.mask || a.mask[(uint32_t)i / (uint32_t)a.k])) atomicAdd(&hist[e], 1);
+    constexpr int SLOTS = 4;                          // whose loads are in flight together
+    for (int64_t i0 = first * a.k + tid; i0 < last * a.k; i0 += SLOTS * blockDim.x) {
+        int64_t e[SLOTS];
+        bool on[SLOTS];
+#pragma unroll
+        for (int y = 0; y < SLOTS; ++y) {
+            const int64_t i = i0 + y * blockDim.x;
+            on[y] = i < last * a.k;
+            e[y] = -1;
+            if (on[y]) {
+                e[y] = a.i64 ? static_cast<const int64_t *>(a.ids)[i] : static_cast<const int32_t *>(a.ids)[i];
+                if (a.mask) on[y] = a.mask[(uint32_t)i / (uint32_t)a.k];
+            }
+        }
+#pragma unroll
+        for (int y = 0; y < SLOTS; ++y)
+            if (on[y] && e[y] >= 0 && e[y] < a.experts) atomicAdd(&hist[e[y]], 1);
     }
     // the probabilities
     float sum[U][N] = {};
-    C next[U];
-    bool next_on = false;
-    auto fetch = [&](int64_t t) __attribute__((always_inline)) {
-        next_on = t < last && (!a.mask || a.mask[t]);
-        if (!next_on) return;
+    // A tokens ahead, in turn (131071 tokens of 256 experts: 43 us with one, 40 with two, 39 with four)
+    constexpr int A = U == 1 ? 4 : 2;
+    C next[A][U];
+    bool next_on[A] = {};
+    auto fetch = [&](int64_t t, auto I) __attribute__((always_inline)) {
+        constexpr int i = decltype(I)::value;
+        next_on[i] = t < last && (!a.mask || a.mask[t]);
+        if (!next_on[i]) return;
 #pragma unroll
-        for (int u = 0; u < U; ++u) next[u].load(static_cast<const T *>(a.logits) + t * a.ld, (u * L + l) * N, a.experts);
+        for (int u = 0; u < U; ++u) next[i][u].load(static_cast<const T *>(a.logits) + t * a.ld, (u * L + l) * N, a.experts);
     };
-    fetch(first + sub);
-    for (int64_t t0 = first; t0 < last; t0 += toks) {
-        const int64_t t = t0 + sub;
-        const bool on = next_on;
+    auto token = [&](int64_t t, auto I) __attribute__((always_inline)) {
+        constexpr int i = decltype(I)::value;
+        const bool on = next_on[i];
         float x[U][N], m = -INFINITY, s = 0.0f;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            next[u].get(x[u]);
+            next[i][u].get(x[u]);
+            const int held = on ? a.experts - (u * L + l) * N : 0;   // (a select for each: a branch around them was compiled wrongly)
 #pragma unroll
             for (int e = 0; e < N; ++e) {
-                if (!on || (u * L + l) * N + e >= a.experts) x[u][e] = -INFINITY;
+                x[u][e] = e < held ? x[u][e] : -INFINITY;
                 m = fmaxf(m, x[u][e]);
             }
         }
-        fetch(t + toks);
+        fetch(t + A * toks, I);
         m = over_group<L>(m, Max{});
         const float at = m == -INFINITY ? 0.0f : m;
 #pragma unroll
@@ -111,13 +127,27 @@ __global__ __launch_bounds__(BAL_THREADS) void balance_kernel(BalanceArgs a, int
                 s += x[u][e];
             }
         s = over_group<L>(s, Add{});
-        const float inv = s == 0.0f ? 0.0f : 1.0f / s;
+        // (the instructions for 1 / s and log2 s, within an ulp: the arithmetic is what bounds this kernel)
+        const float inv = s == 0.0f ? 0.0f : __builtin_amdgcn_rcpf(s);
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int e = 0; e < N; ++e) sum[u][e] = __builtin_fmaf(x[u][e], inv, sum[u][e]);
-        if (on && l == 0) a.lse[t] = s == 0.0f ? INFINITY : at + logf(s);      // exp(logit - lse) is 0 where there is no probability
-    }
+        if (on && l == 0) a.lse[t] = s == 0.0f ? INFINITY : at + __builtin_amdgcn_logf(s) * LN2;      // exp(logit - lse) is 0 where there is no probability
+    };
+    auto each = [&](auto &&f) __attribute__((always_inline)) {
+        f(std::integral_constant<int, 0>{});
+        f(std::integral_constant<int, 1>{});
+        if constexpr (A > 2) {
+            f(std::integral_constant<int, 2>{});
+            f(std::integral_constant<int, 3>{});
+        }
+    };
+    each([&](auto I) __attribute__((always_inline)) { fetch(first + sub + decltype(I)::value * toks, I); });
+    for (int64_t t0 = first; t0 < last; t0 += A * toks)
+        each([&](auto I) __attribute__((always_inline)) {
+            if (t0 + decltype(I)::value * toks < last) token(t0 + sub + decltype(I)::value * toks, I);
+        });
     // over a wave's groups of lanes, then over the waves
 #pragma unroll
     for (int u = 0; u < U; ++u)
@@ -157,7 +187,7 @@ __global__ __launch_bounds__(1024) void balance_join_kernel(const float *sums, c
         }
     } else if (share < shares) {
         int c = 0;
-#pragma unroll 8
+#pragma unroll 16
         for (int g = share; g < groups; g += shares) c += parts[(int64_t)g * E1 + e];
         atomicAdd(&all[e], c);
     }
@@ -165,7 +195,7 @@ __global__ __launch_bounds__(1024) void balance_join_kernel(const float *sums, c
     const int lanes = max(1, 1024 / experts), x = tid % experts, part = tid / experts;
     float s = 0.0f;
     if (part < lanes) {
-#pragma unroll 8
+#pragma unroll 16
         for (int g = part; g < groups; g += lanes) s += sums[(int64_t)g * experts + x];
     }
     probs[tid] = s;

@@ -86,7 +86,16 @@ struct ListArgs {
     int32_t *kept, *pos;         // pos [rows]: a row's packed number, -1 for an ignored one
     float *loss;                 // [rows], or null: 0 for ignored rows
     int32_t rows, vocab, i64;
+    const uint16_t *x;           // where the same launch packs the rows
+    int64_t ldx;
+    uint16_t *packed;
+    int32_t d;
 };
+
+// packed[r] = x[row of r] by one wave
+__device__ __forceinline__ void pack_row(const uint16_t *from, uint16_t *to, int d) {
+    for (int c = 8 * (int)(threadIdx.x & 63); c < d; c += 512) *reinterpret_cast<Bytes16 *>(to + c) = *reinterpret_cast<const Bytes16 *>(from + c);
+}
 
 // One work-group numbers the rows that are not ignored, in order: LIST_EACH rows per thread at a time, LIST_THREADS apart, so that a
 // wave's accesses are 64 elements on end (4096 rows 9.4 us with eight neighbouring rows per thread, 4.7 so).
@@ -136,177 +145,203 @@ __global__ __launch_bounds__(LIST_THREADS) void list_kernel(ListArgs a) {
         __syncthreads();
     }
     if (tid == 0) a.kept[0] = base;
+    if (!a.packed) return;
+    __syncthreads();                                  // (kept was written by this work-group)
+    for (int r = wave; r < base; r += WAVES) pack_row(a.x + (int64_t)a.kept[1 + r] * a.ldx, a.packed + (int64_t)r * a.d, a.d);
 }
 
-// packed[r] = x[row of r], a wave per row
 __global__ __launch_bounds__(256) void pack_kernel(const uint16_t *x, int64_t ldx, uint16_t *packed, const int32_t *kept, int rows, int d) {
-    const int count = min(max(kept[0], 0), rows), lane = threadIdx.x & 63;
-    for (int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); r < count; r += (int64_t)gridDim.x * 4) {
-        const uint16_t *const from = x + (int64_t)kept[1 + r] * ldx;
-        for (int c = 8 * lane; c < d; c += 512) *reinterpret_cast<Bytes16 *>(packed + r * d + c) = *reinterpret_cast<const Bytes16 *>(from + c);
-    }
+    const int count = min(max(kept[0], 0), rows);
+    for (int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); r < count; r += (int64_t)gridDim.x * 4)
+        pack_row(x + (int64_t)kept[1 + r] * ldx, packed + r * d, d);
 }
 
 // ---------------------------------------------------------------------------
 // logits: their row maxima and sums, or a piece of G
 // ---------------------------------------------------------------------------
 
-template <bool GRAD, int T, int BK, int S_>
+// A work-group takes tiles blockIdx.x, blockIdx.x + gridDim.x, ..: the first slab of its next tile is on its way while the
+// epilogue works in LDS of its own.  T = 256 has one work-group to a CU, whose epilogue nothing else covers (us, forward and a piece of G,
+// with a tile per work-group and so: 4096 rows, 16384 words of 384 60.3 68.2, 58.6 64.9; 7370 rows, 32000 words of 2048 854 940, 844 925).
+// What is left of the epilogue is its own arithmetic: 128 exponentials per lane and tile, some 3 of 15 us at width 384.
+template <bool GRAD, int T, int BK>
 __global__ __launch_bounds__(64 * Shape<T>::NW, 2) void logits_kernel(HeadArgs a) {
     using SH = Shape<T>;
     constexpr int NW = SH::NW, FM = SH::FM, FN = SH::FN, TN = SH::TN;
-    using PR = Product<T, BK, S_, false, false>;
+    using PR = Product<T, BK, 2, false, false>;
     constexpr int PB = PR::SP::BYTES;
-    static_assert(S_ == 2, "two stages");
+    constexpr int WROW = TN * 2;                                  // bytes of a staged row of G
     __shared__ __attribute__((aligned(1024))) char p_0[PB], p_1[PB], q_0[PB], q_1[PB];
+    __shared__ __attribute__((aligned(16))) char own[GRAD ? NW * 32 * WROW : SH::WN * T * 8];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave / SH::WN, wn = wave % SH::WN;
-    const int count = kept_rows(a);
-    int mt, nt, split;
-    if (!find_tile<T == 256 ? 8 : 4>(blockIdx.x, (count + T - 1) / T, a.tiles_n, 1, mt, nt, split)) return;
-    const int m0 = mt * T, n0 = nt * T;                           // n0: from v0 on
+    const int count = kept_rows(a), tiles_m = (count + T - 1) / T, slabs = (a.d + BK - 1) / BK;
     PR pr;
-    pr.init(wave, lane, a.d, a.d);
-    // what the epilogue needs of the lane's rows, loaded ahead of the products
-    int word[FM];
-    float lse[FM], slope[FM];
-#pragma unroll
-    for (int i = 0; i < FM; ++i) {
-        const int row = m0 + wm * SH::TM + 32 * i + (lane & 31);
-        word[i] = HEAD_BAD;
-        lse[i] = slope[i] = 0.0f;
-        if (row < count) {
-            word[i] = word_of(a, row);
-            if constexpr (GRAD) {
-                lse[i] = a.lse[row];
-                slope[i] = slope_of(a, row, count);
-            }
-        }
-    }
     auto lds_p = [&](auto ST) __attribute__((always_inline)) -> char * { return decltype(ST)::value == 0 ? p_0 : p_1; };
     auto lds_q = [&](auto ST) __attribute__((always_inline)) -> char * { return decltype(ST)::value == 0 ? q_0 : q_1; };
-    pr.run(lds_p, lds_q, {a.x + (int64_t)m0 * a.d, a.d, min(T, count - m0), 0, a.d},
-           {a.w + (int64_t)(a.v0 + n0) * a.d, a.d, min(T, a.vn - n0), 0, a.d}, 0, (a.d + BK - 1) / BK);
-    wait_vm<0>();                                                 // no load writes LDS any more
-    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    auto side_p = [&](int mt) __attribute__((always_inline)) {
+        return typename PR::Side{a.x + (int64_t)mt * T * a.d, a.d, min(T, count - mt * T), 0, a.d};
+    };
+    auto side_q = [&](int nt) __attribute__((always_inline)) {    // nt: from v0 on
+        return typename PR::Side{a.w + (int64_t)(a.v0 + nt * T) * a.d, a.d, min(T, a.vn - nt * T), 0, a.d};
+    };
+    int mt, nt, split;
+    int v = blockIdx.x;
+    if (!find_tile<T == 256 ? 8 : 4>(v, tiles_m, a.tiles_n, 1, mt, nt, split)) return;
+    pr.init(wave, lane, a.d, a.d);
+    pr.ahead(lds_p, lds_q, side_p(mt), side_q(nt), 0, slabs);
+    for (;;) {
+        const int m0 = mt * T, n0 = nt * T;
+        // what the epilogue needs of the lane's rows, loaded ahead of the products
+        int word[FM];
+        float lse[FM], slope[FM];
+#pragma unroll
+        for (int i = 0; i < FM; ++i) {
+            const int row = m0 + wm * SH::TM + 32 * i + (lane & 31);
+            word[i] = HEAD_BAD;
+            lse[i] = slope[i] = 0.0f;
+            if (row < count) {
+                word[i] = word_of(a, row);
+                if constexpr (GRAD) {
+                    lse[i] = a.lse[row];
+                    slope[i] = slope_of(a, row, count);
+                }
+            }
+        }
+        pr.template run<true>(lds_p, lds_q, side_p(mt), side_q(nt), 0, slabs);
+        wait_vm<0>();                                             // no load writes the stages any more
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        v += gridDim.x;
+        const bool more = find_tile<T == 256 ? 8 : 4>(v, tiles_m, a.tiles_n, 1, mt, nt, split);
+        if (more) pr.ahead(lds_p, lds_q, side_p(mt), side_q(nt), 0, slabs);
 
-    // lane l: row l % 32 of each 32-row block i, columns 32 j + 8 r + 4 (l / 32) + q
-    int etid = tid;
-    asm volatile("" : "+v"(etid));                                // (addresses formed here, not kept through the loop)
-    const int elane = etid & 63, r32 = elane & 31, khalf = elane >> 5;
-    const int nw = n0 + wn * TN + 4 * khalf, m1 = m0 + wm * SH::TM + r32;
-    if (n0 + T > a.vn) {                                          // words that are not there
+        // lane l: row l % 32 of each 32-row block i, columns 32 j + 8 r + 4 (l / 32) + q
+        int etid = tid;
+        asm volatile("" : "+v"(etid));                            // (addresses formed here, not kept through the loop)
+        const int elane = etid & 63, r32 = elane & 31, khalf = elane >> 5;
+        const int nw = n0 + wn * TN + 4 * khalf, m1 = m0 + wm * SH::TM + r32;
+        if (n0 + T > a.vn) {                                      // words that are not there
 #pragma unroll
-        for (int i = 0; i < FM; ++i)
-#pragma unroll
-            for (int j = 0; j < FN; ++j)
-#pragma unroll
-                for (int x = 0; x < 16; ++x)
-                    if (nw + 32 * j + 8 * (x >> 2) + (x & 3) >= a.vn) pr.acc[i][j][x] = -INFINITY;
-    }
-    if constexpr (!GRAD) {
-        float2 *const stat = reinterpret_cast<float2 *>(p_0);     // [WN][T]
-#pragma unroll
-        for (int i = 0; i < FM; ++i) {
-            float m = -INFINITY;
-#pragma unroll
-            for (int j = 0; j < FN; ++j)
-#pragma unroll
-                for (int x = 0; x < 16; ++x) m = fmaxf(m, pr.acc[i][j][x]);
-            m = fmaxf(m, __shfl_xor(m, 32));
-            const float at = m == -INFINITY ? 0.0f : -m * LOG2E;
-            float s = 0.0f;
-#pragma unroll
-            for (int j = 0; j < FN; ++j)
-#pragma unroll
-                for (int x = 0; x < 16; ++x) s += exp_from(pr.acc[i][j][x], at);
-            s += __shfl_xor(s, 32);
-            if (khalf == 0) stat[wn * T + wm * SH::TM + 32 * i + r32] = make_float2(m, s);
-            const int row = m1 + 32 * i;
-            const int rel = word[i] - a.v0 - nw;                  // this lane's columns: those with bit 2 of rel clear
-            if (__any(rel >= 0 && rel < TN && !(rel & 4))) {
+            for (int i = 0; i < FM; ++i)
 #pragma unroll
                 for (int j = 0; j < FN; ++j)
 #pragma unroll
                     for (int x = 0; x < 16; ++x)
-                        if (rel == 32 * j + 8 * (x >> 2) + (x & 3)) a.picked[row] = pr.acc[i][j][x];
-            }
+                        if (nw + 32 * j + 8 * (x >> 2) + (x & 3) >= a.vn) pr.acc[i][j][x] = -INFINITY;
         }
-        __syncthreads();
-        for (int m = tid; m < T && m0 + m < count; m += 64 * NW) {
-            float2 v = stat[m];
+        if constexpr (!GRAD) {
+            float2 *const stat = reinterpret_cast<float2 *>(own);   // [WN][T]
 #pragma unroll
-            for (int k = 1; k < SH::WN; ++k) v = joined(v, stat[k * T + m]);
-            a.part[(int64_t)nt * a.rows + m0 + m] = v;
-        }
-    } else {
-        constexpr int EP = TN + 8, WC = TN / 8, RPP = 64 / WC, NP = 32 / RPP;   // staging pitch; chunks per row, rows per access
-        constexpr int PER = PB / (32 * EP * 2);                                 // waves that stage in one variable
-        static_assert(PER > 0 && NW <= 4 * PER, "the staging fits");
-        const int sv = wave / PER;
-        char *const wst = (sv == 0 ? p_0 : sv == 1 ? q_0 : sv == 2 ? p_1 : q_1) + (wave % PER) * (32 * EP * 2);
-        const int crow = elane / WC, cchk = elane % WC, nc = n0 + wn * TN + 8 * cchk;
-#pragma unroll
-        for (int i = 0; i < FM; ++i) {
-            const float g = slope[i], l = -lse[i] * LOG2E;
-            const int rel = word[i] - a.v0 - nw;
-#pragma unroll
-            for (int j = 0; j < FN; ++j)
-#pragma unroll
-                for (int x = 0; x < 16; ++x) pr.acc[i][j][x] = g * exp_from(pr.acc[i][j][x], l);
-            if (__any(rel >= 0 && rel < TN && !(rel & 4))) {
+            for (int i = 0; i < FM; ++i) {
+                float m = -INFINITY;
 #pragma unroll
                 for (int j = 0; j < FN; ++j)
 #pragma unroll
-                    for (int x = 0; x < 16; ++x)
-                        if (rel == 32 * j + 8 * (x >> 2) + (x & 3)) pr.acc[i][j][x] -= g;
+                    for (int x = 0; x < 16; ++x) m = fmaxf(m, pr.acc[i][j][x]);
+                m = fmaxf(m, __shfl_xor(m, 32));
+                const float at = m == -INFINITY ? 0.0f : -m * LOG2E;
+                float s = 0.0f;
+#pragma unroll
+                for (int j = 0; j < FN; ++j)
+#pragma unroll
+                    for (int x = 0; x < 16; ++x) s += exp_from(pr.acc[i][j][x], at);
+                s += __shfl_xor(s, 32);
+                if (khalf == 0) stat[wn * T + wm * SH::TM + 32 * i + r32] = make_float2(m, s);
+                const int row = m1 + 32 * i;
+                const int rel = word[i] - a.v0 - nw;              // this lane's columns: those with bit 2 of rel clear
+                if (__any(rel >= 0 && rel < TN && !(rel & 4))) {
+#pragma unroll
+                    for (int j = 0; j < FN; ++j)
+#pragma unroll
+                        for (int x = 0; x < 16; ++x)
+                            if (rel == 32 * j + 8 * (x >> 2) + (x & 3)) a.picked[row] = pr.acc[i][j][x];
+                }
             }
+            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");   // (the next tile's loads stay on their way)
+            for (int m = tid; m < T && m0 + m < count; m += 64 * NW) {
+                float2 all = stat[m];
 #pragma unroll
-            for (int j = 0; j < FN; ++j)
+                for (int k = 1; k < SH::WN; ++k) all = joined(all, stat[k * T + m]);
+                a.part[(int64_t)(n0 / T) * a.rows + m0 + m] = all;
+            }
+        } else {
+            // Each wave stages its sub-tile, one 32-row block at a time (LDS accesses of one wave execute in order): 16-byte
+            // chunk c of row r at c ^ (r & (chunks - 1)), so that the rows of a write fall in different banks
+            constexpr int WC = TN / 8, RPP = 64 / WC, NP = 32 / RPP;   // chunks per row, rows per access, accesses per block
+            char *const wst = own + wave * (32 * WROW);
+            const int crow = elane / WC, cchk = elane % WC, nc = n0 + wn * TN + 8 * cchk;
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    *reinterpret_cast<uint2 *>(wst + r32 * (EP * 2) + (j * 32 + 8 * r + 4 * khalf) * 2) =
-                        make_uint2(rne_bf16x2(pr.acc[i][j][4 * r], pr.acc[i][j][4 * r + 1]),
-                                   rne_bf16x2(pr.acc[i][j][4 * r + 2], pr.acc[i][j][4 * r + 3]));
+            for (int i = 0; i < FM; ++i) {
+                const float g = slope[i], l = -lse[i] * LOG2E;
+                const int rel = word[i] - a.v0 - nw;
 #pragma unroll
-            for (int y = 0; y < NP; ++y) {
-                const int m = m0 + wm * SH::TM + 32 * i + crow + RPP * y;
-                const u32x4_t v = *reinterpret_cast<const u32x4_t *>(wst + (crow + RPP * y) * (EP * 2) + 16 * cchk);
-                if (m < count && nc < a.vn) *reinterpret_cast<u32x4_t *>(a.g + (int64_t)m * a.ldg + nc) = v;
+                for (int j = 0; j < FN; ++j)
+#pragma unroll
+                    for (int x = 0; x < 16; ++x) pr.acc[i][j][x] = g * exp_from(pr.acc[i][j][x], l);
+                if (__any(rel >= 0 && rel < TN && !(rel & 4))) {
+#pragma unroll
+                    for (int j = 0; j < FN; ++j)
+#pragma unroll
+                        for (int x = 0; x < 16; ++x)
+                            if (rel == 32 * j + 8 * (x >> 2) + (x & 3)) pr.acc[i][j][x] -= g;
+                }
+#pragma unroll
+                for (int j = 0; j < FN; ++j)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        *reinterpret_cast<uint2 *>(wst + r32 * WROW + (((4 * j + r) ^ (r32 & (WC - 1))) * 16 + khalf * 8)) =
+                            make_uint2(rne_bf16x2(pr.acc[i][j][4 * r], pr.acc[i][j][4 * r + 1]),
+                                       rne_bf16x2(pr.acc[i][j][4 * r + 2], pr.acc[i][j][4 * r + 3]));
+#pragma unroll
+                for (int y = 0; y < NP; ++y) {
+                    const int rr = crow + RPP * y, m = m0 + wm * SH::TM + 32 * i + rr;
+                    const u32x4_t c = *reinterpret_cast<const u32x4_t *>(wst + rr * WROW + ((cchk ^ (rr & (WC - 1))) * 16));
+                    if (m < count && nc < a.vn) *reinterpret_cast<u32x4_t *>(a.g + (int64_t)m * a.ldg + nc) = c;
+                }
             }
         }
+        if (!more) return;
+        pr.clear();
     }
 }
 
-// l[n] and the loss of a row from its tiles' parts: 16 rows per work-group, 16 threads each
-__global__ __launch_bounds__(256) void join_kernel(HeadArgs a, float *loss) {
-    __shared__ float2 part[16][17];
-    const int r = threadIdx.x & 15, g = threadIdx.x >> 4, count = kept_rows(a);
-    const int n = (int)blockIdx.x * 16 + r;
+// l[n] and the losses of 16 rows from their tiles' parts, 16 threads each
+__device__ __forceinline__ void join_rows(const HeadArgs &a, float *loss, int n0, int count, float2 (&part)[16][17]) {
+    const int r = threadIdx.x & 15, g = threadIdx.x >> 4, n = n0 + r;
     float2 v = make_float2(-INFINITY, 0.0f);
     if (n < count)
         for (int t = g; t < a.tiles_n; t += 16) v = joined(v, a.part[(int64_t)t * a.rows + n]);
     part[g][r] = v;
     __syncthreads();
-    if (g > 0 || n >= count) return;
-    for (int k = 1; k < 16; ++k) v = joined(v, part[k][r]);
-    const float l = v.x + logf(v.y);
-    a.lse[n] = l;
-    loss[a.reduction == HEAD_NONE ? a.kept[1 + n] : n] = word_of(a, n) == HEAD_BAD ? __builtin_nanf("") : l - a.picked[n];
+    if (g == 0 && n < count) {
+        for (int k = 1; k < 16; ++k) v = joined(v, part[k][r]);
+        const float l = v.x + logf(v.y);
+        a.lse[n] = l;
+        loss[a.reduction == HEAD_NONE ? a.kept[1 + n] : n] = word_of(a, n) == HEAD_BAD ? __builtin_nanf("") : l - a.picked[n];
+    }
+    __syncthreads();
 }
-
-// The sum or the mean (0 of no rows) of the rows' losses: one work-group, in 64 bits
-__global__ __launch_bounds__(1024) void total_kernel(const float *loss, const int32_t *kept, int rows, int mean, float *out) {
+// The sum or the mean (0 of no rows) of the rows' losses, in 64 bits, by one work-group
+__device__ __forceinline__ void total_loss(const float *loss, int count, bool mean, float *out) {
     __shared__ double sums[16];
-    const int count = min(max(kept[0], 0), rows);
     double s = 0.0;
-    for (int n = threadIdx.x; n < count; n += 1024) s += loss[n];
+    for (int n = threadIdx.x; n < count; n += blockDim.x) s += loss[n];
     for (int w = 32; w; w >>= 1) s += __shfl_xor(s, w);
     if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = s;
     __syncthreads();
     if (threadIdx.x) return;
-    for (int w = 1; w < 16; ++w) s += sums[w];
+    for (int w = 1; w < (int)blockDim.x / 64; ++w) s += sums[w];
     out[0] = (float)(mean ? s / max(count, 1) : s);
+}
+// total: the one work-group of a small call adds the losses up too
+__global__ __launch_bounds__(256) void join_kernel(HeadArgs a, float *loss, float *total) {
+    __shared__ float2 part[16][17];
+    const int count = kept_rows(a);
+    for (int n0 = (int)blockIdx.x * 16; n0 < count; n0 += (int)gridDim.x * 16) join_rows(a, loss, n0, count, part);
+    if (total) total_loss(loss, count, a.reduction == HEAD_MEAN, total);
+}
+__global__ __launch_bounds__(1024) void total_kernel(const float *loss, const int32_t *kept, int rows, int mean, float *out) {
+    total_loss(loss, min(max(kept[0], 0), rows), mean, out);
 }
 
 // ---------------------------------------------------------------------------
@@ -517,6 +552,10 @@ static Tiling tiling(int64_t M, int64_t N, int64_t K, int slots) {
 // 1024; of 8191 rows, 32000 words of 2048: 2.79, 2.81, 2.77, 2.77 ms.
 constexpr int64_t PIECE_BYTES = int64_t(512) << 20;
 constexpr int64_t PIECE_WORDS = 1 << 18;              // at most: a slab's rows of G span less than 2^31 bytes
+// A call of at most so many rows packs them where it lists them, and adds up its losses, of at most so many parts, where it
+// joins them: a launch less each (7 rows, 512 words of 256: 78 us a pass with the launches, 71 so).
+constexpr int64_t FEW_ROWS = 32, FEW_PARTS = 1 << 12;
+
 struct HeadPlan {
     Tiling fwd, logits, dx, dw;
     int64_t piece, ldg;                                // words of a piece
@@ -552,11 +591,13 @@ static int head_grids(const char *name, const HeadPlan &p, int64_t rows, int64_t
     return MSR_ERR_ARG;
 }
 
+constexpr int64_t HEAD_WGS = 256;                     // work-groups of 256-wide tiles: one per CU
 template <bool GRAD>
 static int logits_launch(const HeadArgs &a, int T, int64_t tiles, hipStream_t s) {
-    if (T == 256) hipLaunchKernelGGL((logits_kernel<GRAD, 256, 64, 2>), dim3((unsigned)tiles), dim3(512), 0, s, a);
-    else if (T == 128) hipLaunchKernelGGL((logits_kernel<GRAD, 128, 64, 2>), dim3((unsigned)tiles), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((logits_kernel<GRAD, 64, 64, 2>), dim3((unsigned)tiles), dim3(256), 0, s, a);
+    const unsigned grid = (unsigned)(T == 256 ? std::min<int64_t>(tiles, HEAD_WGS) : tiles);
+    if (T == 256) hipLaunchKernelGGL((logits_kernel<GRAD, 256, 64>), dim3(grid), dim3(512), 0, s, a);
+    else if (T == 128) hipLaunchKernelGGL((logits_kernel<GRAD, 128, 64>), dim3(grid), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((logits_kernel<GRAD, 64, 64>), dim3(grid), dim3(256), 0, s, a);
     return check_launch("logits_kernel");
 }
 
@@ -658,17 +699,23 @@ int msr_head_forward(const uint16_t *x, int64_t ldx, const uint16_t *w, const vo
     float *const losses = reduction == HEAD_NONE ? loss : reinterpret_cast<float *>(after + up256(n * 4));
     a.rows = (int)rows; a.vocab = (int)vocab; a.d = (int)d; a.reduction = reduction;
     a.v0 = 0; a.vn = (int)vocab; a.tiles_n = (int)tn;
-    const ListArgs l{target, ignore_index, kept, kept + 1 + 2 * rows, reduction == HEAD_NONE ? loss : nullptr, (int)rows, (int)vocab, target_i64 != 0};
+    ListArgs l{target, ignore_index, kept, kept + 1 + 2 * rows, reduction == HEAD_NONE ? loss : nullptr, (int)rows, (int)vocab, target_i64 != 0};
+    const bool few = rows <= FEW_ROWS, alone = few && reduction != HEAD_NONE && rows * tn <= FEW_PARTS;
+    if (few) {
+        l.x = x; l.ldx = ldx; l.packed = packed; l.d = (int)d;
+    }
     hipLaunchKernelGGL(list_kernel, dim3(1), dim3(LIST_THREADS), 0, s, l);
     if ((rc = check_launch("list_kernel"))) return rc;
     if (rows > 0) {
-        hipLaunchKernelGGL(pack_kernel, dim3(grid_for(rows, 4, 256 * 8)), dim3(256), 0, s, x, ldx, packed, kept, (int)rows, (int)d);
-        if ((rc = check_launch("pack_kernel"))) return rc;
+        if (!few) {
+            hipLaunchKernelGGL(pack_kernel, dim3(grid_for(rows, 4, 256 * 8)), dim3(256), 0, s, x, ldx, packed, kept, (int)rows, (int)d);
+            if ((rc = check_launch("pack_kernel"))) return rc;
+        }
         if ((rc = logits_launch<false>(a, T, tiles, s))) return rc;
-        hipLaunchKernelGGL(join_kernel, dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, s, a, losses);
+        hipLaunchKernelGGL(join_kernel, dim3(alone ? 1 : (unsigned)((rows + 15) / 16)), dim3(256), 0, s, a, losses, alone ? loss : nullptr);
         if ((rc = check_launch("join_kernel"))) return rc;
     }
-    if (reduction != HEAD_NONE) {
+    if (reduction != HEAD_NONE && !(alone && rows > 0)) {
         hipLaunchKernelGGL(total_kernel, dim3(1), dim3(1024), 0, s, losses, kept, (int)rows, reduction == HEAD_MEAN, loss);
         rc = check_launch("total_kernel");
     }

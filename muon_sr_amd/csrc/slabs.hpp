@@ -118,12 +118,7 @@ struct Product {
         sq.init(wave, lane, ldq);
         rp.init(lane, wave / SH::WN * SH::TM);
         rq.init(lane, wave % SH::WN * SH::TN);
-#pragma unroll
-        for (int i = 0; i < FM; ++i)
-#pragma unroll
-            for (int j = 0; j < FN; ++j)
-#pragma unroll
-                for (int x = 0; x < 16; ++x) acc[i][j][x] = 0.0f;
+        clear();
     }
 
     // One operand's tile: its address at k = 0, row stride, valid rows (row-major: at most T) or valid columns
@@ -136,8 +131,9 @@ struct Product {
 
     // acc += the products over `slabs` slabs from k = kb on.  lds_p, lds_q: the LDS of a stage (an
     // integral_constant); one variable per stage and operand, so that the compiler knows that fragment reads of one
-    // stage do not alias the loads into the others.
-    template <class LP, class LQ>
+    // stage do not alias the loads into the others.  AHEAD: the first slabs are on their way (by ahead, with the same
+    // arguments, after a barrier behind the last use of the stages).
+    template <bool AHEAD = false, class LP, class LQ>
     __device__ __forceinline__ void run(LP lds_p, LQ lds_q, const Side &p, const Side &q, int kb, int slabs) {
         auto load = [&](auto ST, int k0) __attribute__((always_inline)) {
             sp.load(lds_p(ST), wave, p.base, p.ld, p.rows, p.width, kb + k0, p.kend);
@@ -182,9 +178,11 @@ struct Product {
         const int r = slabs % S;
         auto begin = [&](auto ST) __attribute__((always_inline)) {
             constexpr int st = decltype(ST)::value;
-            load(std::integral_constant<int, st>{}, 0);
-            if constexpr (S > 2) load(std::integral_constant<int, (st + 1) % S>{}, BK);
-            if constexpr (S > 3) load(std::integral_constant<int, (st + 2) % S>{}, 2 * BK);
+            if constexpr (!AHEAD) {
+                load(std::integral_constant<int, st>{}, 0);
+                if constexpr (S > 2) load(std::integral_constant<int, (st + 1) % S>{}, BK);
+                if constexpr (S > 3) load(std::integral_constant<int, (st + 2) % S>{}, 2 * BK);
+            }
             wait_vm<(S - 2) * LPS>();
             asm volatile("s_barrier" ::: "memory");
             read(ST, 0, 0);
@@ -214,6 +212,26 @@ struct Product {
             if constexpr (S > 2) slab(I2{}, k0 + 2 * BK);
             if constexpr (S > 3) slab(I3{}, k0 + 3 * BK);
         }
+    }
+
+    // The first slab of a product of two stages, into the stage that run takes it from.
+    template <class LP, class LQ>
+    __device__ __forceinline__ void ahead(LP lds_p, LQ lds_q, const Side &p, const Side &q, int kb, int slabs) {
+        static_assert(S == 2, "one slab ahead");
+        auto load = [&](auto ST) __attribute__((always_inline)) {
+            sp.load(lds_p(ST), wave, p.base, p.ld, p.rows, p.width, kb, p.kend);
+            sq.load(lds_q(ST), wave, q.base, q.ld, q.rows, q.width, kb, q.kend);
+        };
+        if (slabs % S) load(std::integral_constant<int, 1>{});
+        else load(std::integral_constant<int, 0>{});
+    }
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+            for (int j = 0; j < FN; ++j)
+#pragma unroll
+                for (int x = 0; x < 16; ++x) acc[i][j][x] = 0.0f;
     }
 };
 

@@ -1,7 +1,7 @@
 """The router's balance loss against its definition in 64 bits.
 
 Bounds, with u = 2^-24.  exp of an argument a costs 4 u (|a| + 1) (the difference, its product with log2 e, that constant, the
-function); the sum of E of them is off by E u more, so a probability is off by ep = p (4 u (|x - max| + 1) + 2 (E + 8) u), and from the
+function); the sum of E of them is off by E u more, and its reciprocal within 2 u, so a probability is off by ep = p (4 u (|x - max| + 1) + 2 (E + 8) u), and from the
 stored log-sum-exp l by u (|l| + 1) p more.  The mean over n tokens adds (n + 8) u, the loss's stored value u.
 dlogits = up p (u_e - sum_j u_j p_j): up (ep |.| + p (sum u_j ep_j + (E + 4) u sum u_j p_j)) + 4 u |value|, and the
 stored value's rounding."""
