@@ -519,7 +519,7 @@ int msr_head_backward(const uint16_t *packed, const uint16_t *w, const int32_t *
  *   msr_embedding_grad_sr_accum   acc[v] <- SR(acc[v] + f32(bf16(dw[v]))) with the arithmetic and noise of
  *                                 msr_sr_accum on [vocab][d]; words without a token are not touched (with
  *                                 zero_init they are set to 0)
- * Sums in fp32, tokens in order (in parts of up to 32).  Ids outside [0, vocab) and the id
+ * Sums in fp32, in an order that depends on the ids alone.  Ids outside [0, vocab) and the id
  * `padding` (negative: none) give no gradient.  ids: int32, or int64 with ids_i64; W, y, dy, dw: elem
  * (MSR_BF16 or MSR_F32), contiguous but for dy's row stride lddy; aligned to their
  * types.  Fewer than 2^28 tokens and 2^27 words.  workspace:

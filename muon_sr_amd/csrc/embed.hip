@@ -3,7 +3,7 @@
 // An id outside [0, vocab) has no word: its y is 0 and it gives no gradient.  The padding id gives none either.
 //
 // The tokens are sorted by word, earlier tokens first: runs of SORT_RUN tokens by one work-group each (a radix sort in
-// LDS), then merged, MERGE_WAYS runs at a time.  Waves then take CHUNK sorted tokens each and add up the rows of one word after
+// LDS), then merged, MERGE_WAYS runs at a time.  Waves then take 16 or 32 sorted tokens each and add up the rows of one word after
 // the other in fp32, so that no sum depends on a race.  A word whose tokens lie in one chunk is finished there; of a word that
 // crosses chunks each leaves a part, which join_rows_kernel adds up in their order.  Rows of dW without a token are
 // written by the same launch, found by a search in the sorted tokens.  Up to FEW tokens are not sorted: the wave of a
@@ -13,9 +13,14 @@
 
 namespace msr {
 
-constexpr int SORT_THREADS = 1024, SORT_EACH = 2, SORT_RUN = SORT_THREADS * SORT_EACH, MERGE_WAYS = 32;
+constexpr int SORT_THREADS = 1024, SORT_EACH = 2, SORT_RUN = SORT_THREADS * SORT_EACH;
+constexpr int SORT_LOG = 11, MERGE_LOG = 5, MERGE_WAYS = 1 << MERGE_LOG;
+static_assert(SORT_RUN == 1 << SORT_LOG, "runs are searched by halves");
 constexpr int SORT_WAVES = SORT_THREADS / 64, SORT_BITS = 9;    // bits of a pass at most
-constexpr int CHUNK = 32;                                       // sorted tokens of a wave
+// Sorted tokens of a wave: 32 where as many rows as tokens, or more, are zeroed meanwhile, else 16, which shortens each wave's chain of
+// rows (us of sums and join: 16384 tokens, 128256 words of 4096, all of dW written, 216 with 32 and 235 with 16; accumulated into 32000
+// words of 2048, 42 and 37).
+constexpr int CHUNK_MIN = 16, CHUNK_MAX = 32;
 constexpr int FEW = 256;                                        // tokens that are not sorted
 
 // Rows are written past the caches: a batch's y, and a whole dW, are larger than they (16384 tokens, 128256 words of 4096: lookup
@@ -29,7 +34,7 @@ struct EmbedArgs {
     uint64_t *sorted;            // word << 32 | token; a token without a word has word = vocab
     float *parts;                // [chunks][2][d]: what a chunk adds to the word it shares with the one before, and begins for the one after
     int64_t n, d, padding;
-    int32_t vocab, i64, zero_init, bits;
+    int32_t vocab, i64, zero_init, bits, chunk;
     float scale;
     Noise ns;
 };
@@ -192,19 +197,39 @@ __device__ __forceinline__ int64_t below(const uint64_t *keys, int64_t n, uint64
 }
 
 // Runs of `run` keys (a power of two), MERGE_WAYS at a time, merged: a key's place is its own number in its run plus how many of
-// each other are below it, searched for in eight runs at once (a search is a chain of loads).
-__global__ __launch_bounds__(256) void merge_kernel(const uint64_t *in, uint64_t *out, int64_t n, int64_t run) {
+// each other are below it.  A search in memory is a chain of loads, so every work-group holds each stride-th key of its group of
+// runs in LDS, searches there first and in memory among the last `stride` only, in eight runs at once (16384 tokens: 17 us with
+// the whole search in memory, 12.5 so).
+constexpr int MERGE_HELD = 8192;
+__global__ __launch_bounds__(256) void merge_kernel(const uint64_t *in, uint64_t *out, int64_t n, int log_run) {
     constexpr int AT_ONCE = 8;
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    __shared__ uint64_t held[MERGE_HELD];
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, run = (int64_t)1 << log_run;
+    const int log_group = log_run + MERGE_LOG;
+    const int64_t first = ((int64_t)blockIdx.x * 256) >> log_group << log_group, end = min(first + ((int64_t)1 << log_group), n);
+    int log_stride = 3;
+    while ((end - first) >> log_stride > MERGE_HELD) ++log_stride;
+    const int log_per = log_run - log_stride, keys = (int)((end - first) >> log_stride), all = (int)((end - first + run - 1) >> log_run) << log_per;
+    for (int k = threadIdx.x; k < min(all, MERGE_HELD); k += 256) held[k] = k < keys ? in[first + ((int64_t)(k + 1) << log_stride) - 1] : ~0ull;
+    __syncthreads();
     if (i >= n) return;
-    const int64_t first = i / (run * MERGE_WAYS) * (run * MERGE_WAYS), mine = i / run * run, end = min(first + run * MERGE_WAYS, n);
+    const int64_t mine = i >> log_run << log_run;
     const uint64_t key = in[i];
     int64_t place = first + (i - mine);
     for (int64_t r0 = first; r0 < end; r0 += AT_ONCE * run) {
-        int lo[AT_ONCE] = {}, len[AT_ONCE];
+        int64_t lo[AT_ONCE], len[AT_ONCE];
+        int k[AT_ONCE] = {};
+        const int base = (int)((r0 - first) >> log_run) << log_per;
 #pragma unroll
-        for (int y = 0; y < AT_ONCE; ++y) len[y] = r0 + y * run == mine ? 0 : (int)max((int64_t)0, min(run, end - (r0 + y * run)));
-        for (int step = (int)run; step; step >>= 1) {
+        for (int y = 0; y < AT_ONCE; ++y) len[y] = r0 + y * run == mine ? 0 : max((int64_t)0, min(run, end - (r0 + y * run)));
+        for (int step = 1 << log_per; step; step >>= 1) {
+#pragma unroll
+            for (int y = 0; y < AT_ONCE; ++y)
+                if (k[y] + step <= (int)(len[y] >> log_stride) && held[base + (y << log_per) + k[y] + step - 1] < key) k[y] += step;
+        }
+#pragma unroll
+        for (int y = 0; y < AT_ONCE; ++y) lo[y] = (int64_t)k[y] << log_stride;
+        for (int64_t step = (int64_t)1 << (log_stride - 1); step; step >>= 1) {
 #pragma unroll
             for (int y = 0; y < AT_ONCE; ++y)
                 if (lo[y] + step <= len[y] && in[r0 + y * run + lo[y] + step - 1] < key) lo[y] += step;
@@ -219,7 +244,7 @@ __global__ __launch_bounds__(256) void merge_kernel(const uint64_t *in, uint64_t
 // sums
 // ---------------------------------------------------------------------------
 
-constexpr int SUM_AHEAD = 4, JOIN_AHEAD = 4;     // rows, and parts, whose loads are in flight together
+constexpr int SUM_AHEAD = 4, JOIN_AHEAD = 8;     // rows, and parts, whose loads are in flight together
 
 // What is done with the sum of a word's rows, N columns from c on: stored in T (MODE -1), or added to the bf16 accumulator
 // with SR as round(scale sum) would be by msr_sr_accum.
@@ -306,8 +331,8 @@ __global__ __launch_bounds__(256) void sums_kernel(EmbedArgs a, int64_t sum_jobs
         zero_rows<T>(a, v0, ~__ballot(hit), (j % pieces) * WIDTH + lane * C::N);
         return;
     }
-    const int64_t chunk = j / pieces, p0 = chunk * CHUNK, c = (j % pieces) * WIDTH + lane * C::N;
-    const int count = (int)min((int64_t)CHUNK, a.n - p0);
+    const int64_t chunk = j / pieces, p0 = chunk * a.chunk, c = (j % pieces) * WIDTH + lane * C::N;
+    const int count = (int)min((int64_t)a.chunk, a.n - p0);
     // lane l: token l of the chunk; the words before and after it
     const uint64_t key = lane < count ? a.sorted[p0 + lane] : ~0ull;
     const int word = (int)(key >> 32), token = (int)(uint32_t)key;
@@ -353,16 +378,16 @@ __global__ __launch_bounds__(256) void join_rows_kernel(EmbedArgs a) {
     const int lane = threadIdx.x & 63;
     const int64_t j = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t pieces = (a.d + WIDTH - 1) / WIDTH, chunk = j / pieces, c = (j % pieces) * WIDTH + lane * C::N;
-    const int64_t chunks = (a.n + CHUNK - 1) / CHUNK;
+    const int64_t chunks = (a.n + a.chunk - 1) / a.chunk;
     if (chunk + 1 >= chunks) return;
     auto at = [&](int64_t p) __attribute__((always_inline)) { return (int)(a.sorted[p] >> 32); };
-    const int v = __builtin_amdgcn_readfirstlane(at((chunk + 1) * CHUNK));
-    if (v >= a.vocab || at((chunk + 1) * CHUNK - 1) != v) return;                    // no word crosses
-    if (chunk > 0 && at(chunk * CHUNK) == v && at(chunk * CHUNK - 1) == v) return;   // it began before
+    const int v = __builtin_amdgcn_readfirstlane(at((chunk + 1) * a.chunk));
+    if (v >= a.vocab || at((chunk + 1) * a.chunk - 1) != v) return;                    // no word crosses
+    if (chunk > 0 && at(chunk * a.chunk) == v && at(chunk * a.chunk - 1) == v) return;   // it began before
     int64_t end = chunk + 1;                                                         // chunks that begin with the word
     for (;;) {
         const int64_t k = end + lane;
-        const uint64_t same = __ballot(k < chunks && at(k * CHUNK) == v);
+        const uint64_t same = __ballot(k < chunks && at(k * a.chunk) == v);
         end += same == ~0ull ? 64 : __builtin_ctzll(~same);
         if (same != ~0ull) break;
     }
@@ -468,7 +493,7 @@ static EmbedPlan embed_plan(int64_t n, int64_t d) {
     for (int64_t r = 1; r < p.runs; r *= MERGE_WAYS) ++p.merges;
     if (n <= FEW) return p;
     p.sorted = ((size_t)n * 8 + 255) & ~(size_t)255;
-    p.parts = (size_t)((n + CHUNK - 1) / CHUNK) * 2 * (size_t)d * 4;
+    p.parts = (size_t)((n + CHUNK_MIN - 1) / CHUNK_MIN) * 2 * (size_t)d * 4;
     p.bytes = p.sorted * (p.merges ? 2 : 1) + p.parts;
     return p;
 }
@@ -483,10 +508,12 @@ static int embed_check(const char *name, int64_t n, int64_t vocab, int64_t d, in
 }
 
 template <typename T, int MODE>
-static int embed_sums(const EmbedArgs &a, hipStream_t s) {
+static int embed_sums(EmbedArgs a, hipStream_t s) {
     constexpr int WIDTH = 64 * Cells<T>::N;
-    const int64_t pieces = (a.d + WIDTH - 1) / WIDTH, chunks = (a.n + CHUNK - 1) / CHUNK;
+    const int64_t pieces = (a.d + WIDTH - 1) / WIDTH;
     const bool few = a.n <= FEW, zero = MODE < 0 || a.zero_init;
+    a.chunk = zero && a.vocab >= a.n ? CHUNK_MAX : CHUNK_MIN;
+    const int64_t chunks = (a.n + a.chunk - 1) / a.chunk;
     const int words = few ? 8 : zero_words(a.vocab, pieces);
     const int64_t sums = (few ? a.n : chunks) * pieces, zeros = zero ? ((int64_t)a.vocab + words - 1) / words * pieces : 0;
     const dim3 grid((unsigned)((sums + zeros + 3) / 4));
@@ -530,7 +557,7 @@ static int embed_grad(const char *name, const void *ids, int32_t ids_i64, int64_
     rc = ranges_apart(name, r, 5, 2);
     if (rc || d == 0) return rc;
     const int64_t pieces = (d + 64 * (16 / (int64_t)es) - 1) / (64 * (16 / (int64_t)es));
-    if ((((int64_t)n + CHUNK - 1) / CHUNK + FEW + (vocab + 63) / 64 + 4096) * pieces >= (int64_t(1) << 25)) {
+    if ((((int64_t)n + CHUNK_MIN - 1) / CHUNK_MIN + FEW + (vocab + 63) / 64 + 4096) * pieces >= (int64_t(1) << 25)) {
         set_error("%s: too many rows for a launch (%lld tokens, %lld words of %lld)", name, (long long)n, (long long)vocab, (long long)d);
         return MSR_ERR_ARG;
     }
@@ -547,9 +574,8 @@ static int embed_grad(const char *name, const void *ids, int32_t ids_i64, int64_
         while ((int64_t(1) << a.bits) <= vocab) ++a.bits;               // words 0 to vocab
         hipLaunchKernelGGL(sort_kernel, dim3((unsigned)p.runs), dim3(SORT_THREADS), 0, s, a);
         if ((rc = check_launch("sort_kernel"))) return rc;
-        int64_t run = SORT_RUN;
-        for (int m = 0; m < p.merges; ++m, run *= MERGE_WAYS) {
-            hipLaunchKernelGGL(merge_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, list[m & 1], list[~m & 1], n, run);
+        for (int m = 0; m < p.merges; ++m) {
+            hipLaunchKernelGGL(merge_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, list[m & 1], list[~m & 1], n, SORT_LOG + m * MERGE_LOG);
             if ((rc = check_launch("merge_kernel"))) return rc;
             a.sorted = list[~m & 1];
         }

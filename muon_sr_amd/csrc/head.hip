@@ -49,17 +49,18 @@ __device__ __forceinline__ float slope_of(const HeadArgs &a, int r, int count) {
 }
 
 // Tile v of tiles_m x tiles_n in each of `splits` shares of K.  Consecutive work-groups go to the 8 XCDs in turn: each XCD takes a
-// contiguous eighth of the shares' tiles, G rows of tiles at a time, column by column, so that its L2 holds what they
-// share.
-template <int G>
+// contiguous eighth of the shares' tiles, WALK rows of tiles at a time, column by column, so that its L2 holds what they
+// share (8192 rows, 128256 words of 4096, walks of 4, 8, 16, 32 rows: logits 6.70, 6.73, 7.08, 7.95 ms, dx 6.88 with 2 and 4, 6.87, 6.93,
+// 7.20).
+constexpr int WALK = 4;
 __device__ __forceinline__ bool find_tile(int v, int tiles_m, int tiles_n, int splits, int &mt, int &nt, int &split) {
     const int tiles = tiles_m * tiles_n, total = tiles * splits, per = total / NXCD;
     if (v >= total) return false;
     if (v < per * NXCD) v = (v % NXCD) * per + v / NXCD;
     split = v / tiles;
     v -= split * tiles;
-    const int pg = G * tiles_n, g = v / pg, rows = min(G, tiles_m - G * g), r = v - g * pg;
-    mt = G * g + r % rows;
+    const int pg = WALK * tiles_n, g = v / pg, rows = min(WALK, tiles_m - WALK * g), r = v - g * pg;
+    mt = WALK * g + r % rows;
     nt = r / rows;
     return true;
 }
@@ -187,7 +188,7 @@ __global__ __launch_bounds__(64 * Shape<T>::NW, 2) void logits_kernel(HeadArgs a
     };
     int mt, nt, split;
     int v = blockIdx.x;
-    if (!find_tile<T == 256 ? 8 : 4>(v, tiles_m, a.tiles_n, 1, mt, nt, split)) return;
+    if (!find_tile(v, tiles_m, a.tiles_n, 1, mt, nt, split)) return;
     pr.init(wave, lane, a.d, a.d);
     pr.ahead(lds_p, lds_q, side_p(mt), side_q(nt), 0, slabs);
     for (;;) {
@@ -212,7 +213,7 @@ __global__ __launch_bounds__(64 * Shape<T>::NW, 2) void logits_kernel(HeadArgs a
         wait_vm<0>();                                             // no load writes the stages any more
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
         v += gridDim.x;
-        const bool more = find_tile<T == 256 ? 8 : 4>(v, tiles_m, a.tiles_n, 1, mt, nt, split);
+        const bool more = find_tile(v, tiles_m, a.tiles_n, 1, mt, nt, split);
         if (more) pr.ahead(lds_p, lds_q, side_p(mt), side_q(nt), 0, slabs);
 
         // lane l: row l % 32 of each 32-row block i, columns 32 j + 8 r + 4 (l / 32) + q
@@ -382,7 +383,7 @@ __global__ __launch_bounds__(64 * Shape<T>::NW, WPS) void piece_kernel(HeadArgs 
     const int count = kept_rows(a);
     const int M = KIND == HD_DX ? count : a.vn, K = KIND == HD_DX ? a.vn : count;
     int mt, nt, split;
-    if (!find_tile<4>(blockIdx.x, (M + T - 1) / T, a.tiles_n, a.splits, mt, nt, split)) return;
+    if (!find_tile(blockIdx.x, (M + T - 1) / T, a.tiles_n, a.splits, mt, nt, split)) return;
     const int m0 = mt * T, n0 = nt * T;
     // this split's share of K: `slabs` of them from kb on.  The words of a piece are rounded up to 8 in G, whose columns
     // there are 0, not in W.
