@@ -213,3 +213,32 @@ def test_same_call_same_bits():
     a = run(ids, w, dy)
     for _ in range(3):
         assert all(torch.equal(p, q) for p, q in zip(a, run(ids, w, dy)))
+
+
+def test_weights_beyond_32_bit_offsets(L):
+    """270000 words of 8008: 2.16e9 elements, with tokens on the last ones; the accumulator's noise has offsets past 2^31."""
+    import muon_sr_amd as M
+    from muon_sr_amd import _lib
+    vocab, d = 270000, 8008
+    g = gen(8)
+    w = torch.nn.Parameter(torch.randn((vocab, d), generator=g, device=DEV, dtype=BF16))
+    for n in (50, 600):
+        ids = torch.cat([torch.randint(vocab - 30, vocab, (n // 2,), generator=g, device=DEV), torch.randint(0, vocab, (n // 2,), generator=g, device=DEV)])
+        dy = torch.randn((n, d), generator=g, device=DEV).to(BF16)
+        y = M.embedding(ids, w)
+        assert torch.equal(y, w[ids])
+        dw, = torch.autograd.grad(y, w, dy)
+        first = vocab - 30
+        late = ids >= first
+        value, bound, count = want_grad(torch.where(late, ids - first, -1), dy, 30, 1.0)
+        assert ((dw[first:].double() - value).abs() <= UNIT[BF16] * value.abs() + bound).all()
+        assert int((dw != 0).any(1).sum()) == len(ids.unique())
+        w.acc_grad = torch.full_like(w, 0.5)
+        M.embedding_grad_sr_accum(w, ids, dy, seed=77)
+        noise = torch.empty(30 * d, dtype=torch.int16, device=DEV)
+        check(L, L.msr_noise_fill(noise.data_ptr(), noise.numel(), first * d, 77, 0, _lib.noise_mode(), stream()))
+        want = torch.full((30, d), 0.5, dtype=BF16, device=DEV)
+        check(L, L.msr_sr_accum(want.data_ptr(), dw[first:].contiguous().data_ptr(), 0, want.numel(), 0, 0, _lib.NOISE_INJECT, noise.data_ptr(), stream()))
+        assert torch.equal(w.acc_grad[first:], torch.where((count > 0)[:, None], want, 0.5))
+        assert torch.equal((w.acc_grad != 0.5).any(1).nonzero().flatten(), ids.unique())
+        del w.acc_grad, dw

@@ -294,3 +294,53 @@ def test_same_call_same_bits_and_evaluation():
     dx, = torch.autograd.grad(linear_cross_entropy(leaf, w, target), leaf, create_graph=True)
     with pytest.raises(RuntimeError):
         dx.float().sum().backward()
+
+
+def test_weights_beyond_32_bit_offsets(L):
+    """270000 words of 8008: 2.16e9 elements.  The loss, dx, the gradient's last rows and the accumulated ones, whose noise has offsets past
+    2^31."""
+    import muon_sr_amd as M
+    from muon_sr_amd import _lib
+    vocab, d, rows = 270000, 8008, 5
+    g = gen(13)
+    w = torch.randn((vocab, d), generator=g, device=DEV, dtype=BF16).mul_(0.03)
+    x = torch.randn((rows, d), generator=g, device=DEV).to(BF16)
+    target = torch.tensor([vocab - 1, 3, -100, vocab - 2, 200000], device=DEV)
+    dloss = torch.rand(rows, generator=g, device=DEV) + 0.25
+    loss, dx, dw = run(x, w, target, dloss, "none")
+    S = torch.cat([x.double() @ part.double().t() for part in w.split(30000)], 1)
+    eS = 2 * (d + 1) * U * torch.cat([x.double().abs() @ part.double().abs().t() for part in w.split(30000)], 1)
+    lse = torch.logsumexp(S, 1)
+    el = eS.max(1).values + 2 * (64 + vocab / 64) * U + 8 * U * (lse.abs() + 1) + 2 * U * S.abs().max(1).values
+    on = (target != -100).nonzero().flatten()
+    near(loss[on], (lse[on] - S[on, target[on]], eS[on, target[on]] + el[on] + U * lse[on].abs()))
+    p = torch.exp(S - lse[:, None])
+    eG = p * (eS + el[:, None] + 4 * U * ((S - lse[:, None]).abs() + 1) + 2 * U * lse[:, None].abs()) + 2 * U
+    G = p.clone()
+    G[on, target[on]] -= 1.0
+    G, eG = ((torch.where(target != -100, dloss, 0.0).double())[:, None] * v for v in (G, eG))
+    eG = eG + H * (G.abs() + eG)
+    for rows_ in (slice(vocab - 300, vocab), slice(199990, 200010), slice(0, 8)):
+        value, terms = G[:, rows_].t() @ x.double(), (eG + 2 * 32 * U * G.abs())[:, rows_].t() @ x.double().abs()
+        near(dw[rows_], (value, H * value.abs() + (1 + H) * terms + 1e-30))
+    value = torch.zeros((rows, d), dtype=torch.float64, device=DEV)
+    terms = torch.zeros_like(value)
+    for a in range(0, vocab, 30000):
+        part = w[a:a + 30000].double()
+        value += G[:, a:a + 30000] @ part
+        terms += (eG[:, a:a + 30000] + 2 * (vocab + 16) * U * G[:, a:a + 30000].abs()) @ part.abs()
+    near(dx, (value, H * value.abs() + (1 + H) * terms + 1e-30))
+    del S, eS, p, G, eG, part
+    head = M.SRHead(d, vocab, device="meta")
+    head.weight = torch.nn.Parameter(w)
+    head.weight.acc_grad = torch.full_like(w, 0.01)
+    random.seed(3)
+    seed = random.getrandbits(32)
+    random.seed(3)
+    head.loss(x, target, reduction="none").backward(dloss)
+    first = vocab - 40
+    noise = torch.empty(40 * d, dtype=torch.int16, device=DEV)
+    check(L, L.msr_noise_fill(noise.data_ptr(), noise.numel(), first * d, seed, 0, _lib.noise_mode(), stream()))
+    want = torch.full((40, d), 0.01, dtype=BF16, device=DEV)
+    check(L, L.msr_sr_accum(want.data_ptr(), dw[first:].contiguous().data_ptr(), 0, want.numel(), 0, 0, _lib.NOISE_INJECT, noise.data_ptr(), stream()))
+    assert torch.equal(head.weight.acc_grad[first:], want)
