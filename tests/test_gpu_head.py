@@ -210,6 +210,17 @@ def test_shapes_strides_and_wanted_gradients():
     assert not linear_cross_entropy(x, w, target).requires_grad
 
 
+@pytest.mark.parametrize("rows,vocab,d", [(7, 512, 256), (2047, 3001, 1024), (300, 1000, 1032), (4096, 8200, 384), (257, 4099, 136), (4096, 8200, 2048)])
+def test_one_gradient_is_that_of_both(rows, vocab, d):
+    """Each gradient has the same bits when it is wanted alone."""
+    from muon_sr_amd import linear_cross_entropy
+    x, w, target, dloss = make(rows, vocab, d, 14)
+    _, dx, dw = run(x, w, target, dloss, "none")
+    leaf, word = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    assert torch.equal(torch.autograd.grad(linear_cross_entropy(leaf, w, target, reduction="none"), leaf, dloss)[0], dx)
+    assert torch.equal(torch.autograd.grad(linear_cross_entropy(x, word, target, reduction="none"), word, dloss)[0], dw)
+
+
 @pytest.mark.parametrize("noise", ["philox8", "triton"])
 @pytest.mark.parametrize("rows,vocab,d", [(70, 333, 72), (3000, 8192, 64), (1, 40, 8), (16384, 17001, 64), (1025, 70, 2048)])
 def test_accumulated_weight_gradient(L, rows, vocab, d, noise):
