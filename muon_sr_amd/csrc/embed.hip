@@ -21,7 +21,10 @@ constexpr int SORT_WAVES = SORT_THREADS / 64, SORT_BITS = 9;    // bits of a pas
 // rows (us of sums and join: 16384 tokens, 128256 words of 4096, all of dW written, 216 with 32 and 235 with 16; accumulated into 32000
 // words of 2048, 42 and 37).
 constexpr int CHUNK_MIN = 16, CHUNK_MAX = 32;
-constexpr int FEW = 256;                                        // tokens that are not sorted
+// Tokens that are not sorted, at most.  us of accumulating 500 tokens, sorted and not: of 2000 words of 512 20 and 9; of 4096, half of them
+// padding, 23 and 31; all of one word, which one wave adds up, FEW_AHEAD rows in flight, 18 and 55.  1000 tokens of one word would take
+// 110 us of a pass (sorted 50).
+constexpr int FEW = 512, FEW_AHEAD = 16;
 
 // Rows are written past the caches: a batch's y, and a whole dW, are larger than they (16384 tokens, 128256 words of 4096: lookup
 // 52 us with cached stores, 36 so; gradient 218 and 213).
@@ -456,20 +459,22 @@ __global__ __launch_bounds__(256) void few_kernel(EmbedArgs a, int64_t sum_jobs,
     }
     if (!first) return;
     float sum[C::N] = {};
+#pragma unroll 1
+    for (int r = i / 64; r < R; ++r) {
+        uint64_t left = 0;
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-        uint64_t left = same[r];
+        for (int q = 0; q < R; ++q) left = q == r ? same[q] : left;
         while (left) {
-            C x[SUM_AHEAD];
-            bool on[SUM_AHEAD];
+            C x[FEW_AHEAD];
+            bool on[FEW_AHEAD];
 #pragma unroll
-            for (int y = 0; y < SUM_AHEAD; ++y) {
+            for (int y = 0; y < FEW_AHEAD; ++y) {
                 on[y] = left != 0;
                 if (on[y]) x[y].load(static_cast<const T *>(a.dy) + (int64_t)(r * 64 + __builtin_ctzll(left)) * a.lddy, c, a.d);
                 left &= left - 1;
             }
 #pragma unroll
-            for (int y = 0; y < SUM_AHEAD; ++y) {
+            for (int y = 0; y < FEW_AHEAD; ++y) {
                 if (!on[y]) continue;
                 float f[C::N];
                 x[y].get(f);

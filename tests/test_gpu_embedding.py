@@ -83,7 +83,7 @@ def test_against_64_bits(n, vocab, d, dtype):
 
 def test_words_that_span_many_chunks():
     """One word for all tokens; a few; and runs whose borders fall on those of the 16- and 32-token chunks and one beside (more than
-    256 tokens, which are sorted; as many words as tokens for chunks of 32)."""
+    512 tokens, which are sorted; as many words as tokens for chunks of 32)."""
     g = gen(2)
     for n in (31, 32, 33, 64, 65, 4096, 20000, 50001):
         dy = torch.randn((n, 72), generator=g, device=DEV).to(BF16)
@@ -91,11 +91,11 @@ def test_words_that_span_many_chunks():
         compare(torch.full((n,), 4, device=DEV), w, dy)
         compare((torch.arange(n, device=DEV) * 3 // n) * 5, w, dy)
     for lengths in ([32, 32, 64, 31, 1, 33], [1, 31, 32, 96, 2], [63, 65, 64, 5], [16, 16, 16, 16, 128], [15, 1, 17, 15, 16, 48]):
-        for more in (0, 256, 272):
+        for more in (0, 512, 528):
             lengths_ = lengths + [more]
             ids = torch.repeat_interleave(torch.arange(len(lengths_), device=DEV), torch.tensor(lengths_, device=DEV))
             ids = ids[torch.randperm(len(ids), generator=g, device=DEV)]
-            for vocab in (9, 600):
+            for vocab in (9, 900):
                 compare(ids, torch.randn((vocab, 72), generator=g, device=DEV).to(BF16), torch.randn((len(ids), 72), generator=g, device=DEV).to(BF16))
 
 
@@ -222,7 +222,7 @@ def test_weights_beyond_32_bit_offsets(L):
     vocab, d = 270000, 8008
     g = gen(8)
     w = torch.nn.Parameter(torch.randn((vocab, d), generator=g, device=DEV, dtype=BF16))
-    for n in (50, 600):
+    for n in (50, 1200):
         ids = torch.cat([torch.randint(vocab - 30, vocab, (n // 2,), generator=g, device=DEV), torch.randint(0, vocab, (n // 2,), generator=g, device=DEV)])
         dy = torch.randn((n, d), generator=g, device=DEV).to(BF16)
         y = M.embedding(ids, w)

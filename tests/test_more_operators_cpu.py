@@ -73,14 +73,14 @@ def test_embedding(lib):
     assert look(ids=A + 4) == ALIGN and look(w=B + 1) == ALIGN and look(y=C + 2, elem=1) == ALIGN
     assert look(y=A) == OVERLAP and look(y=B + 32) == OVERLAP
     size = ctypes.c_size_t()
-    assert lib.msr_embedding_workspace_bytes(1000, 50, 16, ctypes.byref(size)) == 0 and size.value >= 8000 + 32 * 2 * 64
+    assert lib.msr_embedding_workspace_bytes(2000, 50, 16, ctypes.byref(size)) == 0 and size.value >= 16000 + 32 * 2 * 64
     assert lib.msr_embedding_workspace_bytes(100, 50, 16, ctypes.byref(size)) == 0 and size.value == 0
     assert lib.msr_embedding_workspace_bytes(100, 50, 16, None) == ARG and lib.msr_embedding_workspace_bytes(-1, 50, 16, ctypes.byref(size)) == ARG
 
-    def grad(ids=A, i64=1, n=1000, dy=B, ld=16, vocab=50, d=16, dw=C, elem=0, ws=W, size=BIG):
+    def grad(ids=A, i64=1, n=2000, dy=B, ld=16, vocab=50, d=16, dw=C, elem=0, ws=W, size=BIG):
         return lib.msr_embedding_grad(ids, i64, n, dy, ld, vocab, d, 1.0, -1, dw, elem, ws, size, None)
 
-    def accum(ids=A, n=1000, dy=B, ld=16, vocab=50, d=16, acc=C, mode=1, inject=None, ws=W, size=BIG):
+    def accum(ids=A, n=2000, dy=B, ld=16, vocab=50, d=16, acc=C, mode=1, inject=None, ws=W, size=BIG):
         return lib.msr_embedding_grad_sr_accum(ids, 1, n, dy, ld, vocab, d, 1.0, -1, acc, 7, 0, mode, inject, ws, size, None)
     assert grad(d=0, ld=0) == 0
     for bad in (dict(ids=None), dict(dy=None), dict(dw=None), dict(ld=15), dict(n=1 << 28), dict(vocab=1 << 27), dict(elem=3)):
