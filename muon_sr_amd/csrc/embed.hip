@@ -562,7 +562,9 @@ static int embed_grad(const char *name, const void *ids, int32_t ids_i64, int64_
     rc = ranges_apart(name, r, 5, 2);
     if (rc || d == 0) return rc;
     const int64_t pieces = (d + 64 * (16 / (int64_t)es) - 1) / (64 * (16 / (int64_t)es));
-    if ((((int64_t)n + CHUNK_MIN - 1) / CHUNK_MIN + FEW + (vocab + 63) / 64 + 4096) * pieces >= (int64_t(1) << 25)) {
+    const int64_t words = n <= FEW ? 8 : zero_words(vocab, pieces);
+    const int64_t waves = ((n <= FEW ? n : (n + CHUNK_MIN - 1) / CHUNK_MIN) + (vocab + words - 1) / words) * pieces;   // at most
+    if (waves >= (int64_t(1) << 26) - 4) {          // 64 threads each: fewer than 2^32 in a launch
         set_error("%s: too many rows for a launch (%lld tokens, %lld words of %lld)", name, (long long)n, (long long)vocab, (long long)d);
         return MSR_ERR_ARG;
     }

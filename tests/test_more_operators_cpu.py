@@ -89,6 +89,7 @@ def test_embedding(lib):
     assert grad(ws=None) == WORKSPACE and grad(size=64) == WORKSPACE
     assert grad(dw=A) == OVERLAP and grad(dw=B + 64) == OVERLAP and grad(ws=B) == OVERLAP and grad(ws=C) == OVERLAP
     assert grad(vocab=(1 << 27) - 1, d=1 << 14, ld=1 << 14, dw=1 << 50) == ARG and b"launch" in lib.msr_last_error()
+    assert grad(n=500, vocab=(1 << 27) - 1, d=1 << 12, ld=1 << 12, dw=1 << 50) == ARG and b"launch" in lib.msr_last_error()
     for bad in (dict(mode=-1), dict(mode=3), dict(mode=2)):
         assert accum(**bad) == ARG, bad
     assert accum(mode=2, inject=C + 64) == OVERLAP
