@@ -3,7 +3,10 @@
 //     G[n][v] = g[n] (exp(S[n][v] - l[n]) - [v = t[n]]),   dx = G W,   dW = G^T x
 // with g[n] the gradient of loss[n].  S is never in memory: the forward pass keeps the maximum and the sum of each row of each
 // tile, the backward pass forms S again, piece by piece of the vocabulary, and stores the piece's G as the bf16 operand of
-// the two products that follow.  8 rows vocab d flop with gradients where 6 are the least; the logits kept in fp32 would be 4.2 GB
+// the two products that follow, as G / c: c is the significand of the first row's g (every row's, but for the reduction "none"), by
+// which the products' sums are multiplied in fp32.  The target's element of an unlikely word is -g, a factor of its whole row:
+// rounded with g, every such row would be off by the same share, up to 2^-8 (8192 rows, 128256 words of 4096, gradients against 64 bits:
+// 0.0021 or, at an unlucky g, 0.0030, and 0.0018 so at any; 0.0017 is the rounding of the results).  8 rows vocab d flop with gradients where 6 are the least; the logits kept in fp32 would be 4.2 GB
 // for 8192 rows of 128256 words.
 //
 // Rows that are ignored take part in nothing: list_kernel numbers the others, pack_kernel lays them out one after the
@@ -27,7 +30,7 @@ struct HeadArgs {
     float2 *part;                // [tiles of words][rows]: a tile's maximum and sum
     float *picked;               // [rows]: S[n][t[n]]
     const float *dloss;          // [rows] in the given order, or one
-    uint16_t *g;                 // [rows][ldg]: a piece of G
+    uint16_t *g;                 // [rows][ldg]: a piece of G / c
     float *slots;                // fp32 sums [splits][M][N]
     uint16_t *out;               // dW or the accumulator
     int64_t ldg;
@@ -41,11 +44,20 @@ struct HeadArgs {
 typedef const __attribute__((address_space(4))) int32_t *const_i32_t;
 __device__ __forceinline__ int kept_rows(const HeadArgs &a) { return min(max(*(const_i32_t)(uintptr_t)a.kept, 0), a.rows); }
 __device__ __forceinline__ int word_of(const HeadArgs &a, int r) { return a.kept[1 + a.rows + r]; }
-// dloss of packed row r; NaN where its target is no word
-__device__ __forceinline__ float slope_of(const HeadArgs &a, int r, int count) {
+// g of packed row r
+__device__ __forceinline__ float dloss_of(const HeadArgs &a, int r, int count) {
     const float g = a.dloss[a.reduction == HEAD_NONE ? a.kept[1 + r] : 0];
-    if (word_of(a, r) == HEAD_BAD) return __builtin_nanf("");
     return a.reduction == HEAD_MEAN ? g / (float)count : g;
+}
+// c, in [1, 2); 1 where the first row's g has no significand
+__device__ __forceinline__ float unit_of(const HeadArgs &a, int count) {
+    if (count == 0) return 1.0f;
+    const float m = 2.0f * fabsf(__builtin_amdgcn_frexp_mantf(dloss_of(a, 0, count)));
+    return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(m >= 1.0f && m < 2.0f ? m : 1.0f)));
+}
+// g / c of packed row r; NaN where its target is no word
+__device__ __forceinline__ float slope_of(const HeadArgs &a, int r, int count, float unit) {
+    return word_of(a, r) == HEAD_BAD ? __builtin_nanf("") : dloss_of(a, r, count) / unit;
 }
 
 // Tile v of tiles_m x tiles_n in each of `splits` shares of K.  Consecutive work-groups go to the 8 XCDs in turn: each XCD takes a
@@ -177,6 +189,7 @@ __global__ __launch_bounds__(64 * Shape<T>::NW, 2) void logits_kernel(HeadArgs a
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave / SH::WN, wn = wave % SH::WN;
     const int count = kept_rows(a), tiles_m = (count + T - 1) / T, slabs = (a.d + BK - 1) / BK;
+    const float unit = GRAD ? unit_of(a, count) : 1.0f;
     PR pr;
     auto lds_p = [&](auto ST) __attribute__((always_inline)) -> char * { return decltype(ST)::value == 0 ? p_0 : p_1; };
     auto lds_q = [&](auto ST) __attribute__((always_inline)) -> char * { return decltype(ST)::value == 0 ? q_0 : q_1; };
@@ -205,7 +218,7 @@ __global__ __launch_bounds__(64 * Shape<T>::NW, 2) void logits_kernel(HeadArgs a
                 word[i] = word_of(a, row);
                 if constexpr (GRAD) {
                     lse[i] = a.lse[row];
-                    slope[i] = slope_of(a, row, count);
+                    slope[i] = slope_of(a, row, count, unit);
                 }
             }
         }
@@ -381,6 +394,7 @@ __global__ __launch_bounds__(64 * Shape<T>::NW, WPS) void piece_kernel(HeadArgs 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave / SH::WN, wn = wave % SH::WN;
     const int count = kept_rows(a);
+    const float unit = OUT == OUT_SLOTS ? 1.0f : unit_of(a, count);
     const int M = KIND == HD_DX ? count : a.vn, K = KIND == HD_DX ? a.vn : count;
     int mt, nt, split;
     if (!find_tile(blockIdx.x, (M + T - 1) / T, a.tiles_n, a.splits, mt, nt, split)) return;
@@ -445,8 +459,8 @@ __global__ __launch_bounds__(64 * Shape<T>::NW, WPS) void piece_kernel(HeadArgs 
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
                     *reinterpret_cast<uint2 *>(wst + r32 * (EP * 2) + (j * 32 + 8 * r + 4 * khalf) * 2) =
-                        make_uint2(rne_bf16x2(pr.acc[i][j][4 * r], pr.acc[i][j][4 * r + 1]),
-                                   rne_bf16x2(pr.acc[i][j][4 * r + 2], pr.acc[i][j][4 * r + 3]));
+                        make_uint2(rne_bf16x2(unit * pr.acc[i][j][4 * r], unit * pr.acc[i][j][4 * r + 1]),
+                                   rne_bf16x2(unit * pr.acc[i][j][4 * r + 2], unit * pr.acc[i][j][4 * r + 3]));
 #pragma unroll
             for (int y = 0; y < NP; ++y) {
                 const int m = m0 + wm * SH::TM + 32 * i + crow + RPP * y;
@@ -470,20 +484,25 @@ __global__ __launch_bounds__(64 * Shape<T>::NW, WPS) void piece_kernel(HeadArgs 
     }
 }
 
-// The sum of a row's slots, rounded: dx of every row (0 for an ignored one), 8 elements per thread
-__global__ __launch_bounds__(256) void dx_kernel(const float *slots, int splits, const int32_t *pos, uint16_t *dx, int rows, int d) {
+// The sum of a row's slots times c, rounded: dx of every row (0 for an ignored one), 8 elements per thread
+__global__ __launch_bounds__(256) void dx_kernel(HeadArgs a, uint16_t *dx) {
+    const int rows = a.rows, d = a.d;
+    const int32_t *const pos = a.kept + 1 + 2 * (int64_t)rows;
     const int64_t chunks = (int64_t)rows * (d / 8);
+    const float unit = unit_of(a, kept_rows(a));
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < chunks; i += (int64_t)gridDim.x * 256) {
         const int64_t n = i / (d / 8);
         const int c = (int)(i % (d / 8)) * 8, p = pos[n];
         float f[8] = {};
         if (p >= 0)
-            for (int s = 0; s < splits; ++s) {
+            for (int s = 0; s < a.splits; ++s) {
                 float h[8];
-                load_f32x8<true>(slots, ((int64_t)s * rows + p) * d + c, 8, h);
+                load_f32x8<true>(a.slots, ((int64_t)s * rows + p) * d + c, 8, h);
 #pragma unroll
                 for (int x = 0; x < 8; ++x) f[x] += h[x];
             }
+#pragma unroll
+        for (int x = 0; x < 8; ++x) f[x] *= unit;
         st_nt4(dx + n * d + c, u32x4_t{rne_bf16x2(f[0], f[1]), rne_bf16x2(f[2], f[3]), rne_bf16x2(f[4], f[5]), rne_bf16x2(f[6], f[7])});
     }
 }
@@ -492,6 +511,7 @@ __global__ __launch_bounds__(256) void dx_kernel(const float *slots, int splits,
 template <int OUT>
 __global__ __launch_bounds__(256) void dw_kernel(HeadArgs a) {
     const int64_t n = (int64_t)a.vn * a.d;
+    const float unit = unit_of(a, kept_rows(a));
     for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8; i < n; i += (int64_t)gridDim.x * 2048) {
         float f[8] = {};
         for (int s = 0; s < a.splits; ++s) {
@@ -500,6 +520,8 @@ __global__ __launch_bounds__(256) void dw_kernel(HeadArgs a) {
 #pragma unroll
             for (int x = 0; x < 8; ++x) f[x] += h[x];
         }
+#pragma unroll
+        for (int x = 0; x < 8; ++x) f[x] *= unit;
         const uint32_t gw[4] = {rne_bf16x2(f[0], f[1]), rne_bf16x2(f[2], f[3]), rne_bf16x2(f[4], f[5]), rne_bf16x2(f[6], f[7])};
         const int64_t o0 = (int64_t)a.v0 * a.d + i;
         if constexpr (OUT == OUT_STORE) st_nt4(a.out + o0, u32x4_t{gw[0], gw[1], gw[2], gw[3]});
@@ -781,8 +803,9 @@ int msr_head_backward(const uint16_t *packed, const uint16_t *w, const int32_t *
         if (rc) return rc;
     }
     if (dx && rows > 0) {
-        hipLaunchKernelGGL(dx_kernel, dim3(grid_for(rows * (d / 8), 256, 256 * 8)), dim3(256), 0, s, dxs, p.dx.splits, kept + 1 + 2 * rows, dx,
-                           (int)rows, (int)d);
+        a.slots = dxs;
+        a.splits = p.dx.splits;
+        hipLaunchKernelGGL(dx_kernel, dim3(grid_for(rows * (d / 8), 256, 256 * 8)), dim3(256), 0, s, a, dx);
         rc = check_launch("dx_kernel");
     }
     return rc;

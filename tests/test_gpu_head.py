@@ -5,8 +5,9 @@ most eS = 2 (d + 1) u sum|x w| (the factor 2: any order of the sums, and what hi
 a = x - m costs 4 u (|a| + 1) + 2 u |m|: the difference, its product with log2 e, that constant, m's own product and the function.  The sum behind l has at most depth =
 64 + vocab / 64 additions one after the other (32 in a lane, the waves', and a share of the tiles), so l is off by at most
 el = max eS + 2 depth u + 8 u (|l| + 1) + 2 u max|S|, and the loss by eS + el + u |loss|.
-G = g (p - [target]) is off by eG = g (p (eS + el + 4 u (|S - l| + 1) + 2 u |l|) + 2 u), then h |G| by its rounding; a product over
-K terms adds 2 (K + 16) u sum|terms| and the stored value's rounding h |value|.  Values below the smallest normal
+G = g (p - [target]) is off by eG = g (p (eS + el + 4 u (|S - l| + 1) + 2 u |l|) + 2 u), then h |G| by its rounding (a rounding is
+off by less than h / (1 + h), which leaves room for the division by c); a product over
+K terms adds 2 (K + 16) u sum|terms| (c's product among them) and the stored value's rounding h |value|.  Values below the smallest normal
 number may vanish: 2^-126 per term."""
 import ctypes
 import math
@@ -291,6 +292,42 @@ def test_gradient_is_that_of_differences():
         R = (x.double() @ s[0].double()).abs()
         tol = h * h / 6 * (R ** 3).sum() / (6 * math.sqrt(3)) + e_loss.sum() / h + (e_dw[k] * s[0].abs()).sum()
         assert (diff - (got_dw[k].double() * s[0]).sum()).abs() <= tol
+
+
+@pytest.mark.parametrize("reduction", ["sum", "none"])
+def test_the_upstream_gradient_is_not_rounded_with_the_targets(reduction):
+    """4096 words that are nearly equally likely: an element of G is g p but for the target's, -g (1 - p), which carries the row.  With
+    g = 1 + 2^-8, halfway between two bf16 numbers, it would be off by 2^-8 in every row alike, and so would the gradients be along
+    themselves; 1 - p rounds to 1, off by p, which is 2^-12 of the rows on average, and what else is rounded, G's small elements and the
+    results, is off to either side: by some 2^-8 / sqrt(elements) along them, less than 2^-16 here.  Twice the former is allowed."""
+    g = gen(15)
+    x = (torch.randn((512, 256), generator=g, device=DEV) / 64).to(BF16)
+    w = torch.randn((4096, 256), generator=g, device=DEV).to(BF16)
+    target = torch.randint(0, 4096, (512,), generator=g, device=DEV)
+    dloss = torch.full((512,), 1 + 2.0 ** -8, device=DEV)
+    _, (dx, _), (dw, _) = exact(x, w, target, dloss, reduction)
+    for got, want in zip(run(x, w, target, dloss, reduction)[1:], (dx, dw)):
+        along = (got.double() * want).sum() / want.square().sum() - 1
+        assert along.abs() <= 2.0 ** -11, along.item()
+
+
+@pytest.mark.parametrize("first", [0.0, -0.0, math.inf, math.nan, 1e-42, 3.4e38, -1.7])
+def test_any_first_gradient(first):
+    """The first row's upstream gradient, whatever it is, takes part in the others' rows with its significand alone."""
+    x, w, target, dloss = make(200, 333, 64, 16, ignored=0.1)
+    at = int((target != -100).nonzero()[0])
+    dloss[at] = first
+    _, got_dx, got_dw = run(x, w, target, dloss, "none")
+    others = torch.arange(200, device=DEV) != at
+    clean = dloss.clone()
+    clean[at] = 0.0
+    _, want_dx, want_dw = exact(x, w, target, clean, "none")
+    near(got_dx[others], tuple(v[others] for v in want_dx))
+    if first == 0.0:
+        near(got_dw, want_dw)
+        assert not got_dx[at].any()
+    elif not math.isfinite(first):
+        assert not got_dx[at].isfinite().all()
 
 
 def test_same_call_same_bits_and_evaluation():
