@@ -373,43 +373,72 @@ __global__ __launch_bounds__(256) void sums_kernel(EmbedArgs a, int64_t sum_jobs
     }
 }
 
-// Words that cross chunks, by the wave of the chunk that they begin in.
+// Words that cross chunks: a work-group takes a piece of 64 cells of the words that begin in four chunks, one to a wave.  A word of many
+// chunks (one of the four at most), whose parts are a chain of loads, is shared by the work-group: every fourth part to a wave, the
+// waves' sums added in order (60000 tokens of 1000 words of 512, of which one has a tenth: 52 us by one wave, 20 so; 13399 tokens of
+// 970 words of 20: 32 and 13).
 template <typename T, int MODE>
 __global__ __launch_bounds__(256) void join_rows_kernel(EmbedArgs a) {
     using C = Cells<T>;
-    constexpr int WIDTH = 64 * C::N;
-    const int lane = threadIdx.x & 63;
-    const int64_t j = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t pieces = (a.d + WIDTH - 1) / WIDTH, chunk = j / pieces, c = (j % pieces) * WIDTH + lane * C::N;
-    const int64_t chunks = (a.n + a.chunk - 1) / a.chunk;
-    if (chunk + 1 >= chunks) return;
-    auto at = [&](int64_t p) __attribute__((always_inline)) { return (int)(a.sorted[p] >> 32); };
-    const int v = __builtin_amdgcn_readfirstlane(at((chunk + 1) * a.chunk));
-    if (v >= a.vocab || at((chunk + 1) * a.chunk - 1) != v) return;                    // no word crosses
-    if (chunk > 0 && at(chunk * a.chunk) == v && at(chunk * a.chunk - 1) == v) return;   // it began before
-    int64_t end = chunk + 1;                                                         // chunks that begin with the word
-    for (;;) {
-        const int64_t k = end + lane;
-        const uint64_t same = __ballot(k < chunks && at(k * a.chunk) == v);
-        end += same == ~0ull ? 64 : __builtin_ctzll(~same);
-        if (same != ~0ull) break;
-    }
-    if (c >= a.d) return;
-    float sum[C::N];
-    load_part(a.parts + (2 * chunk + 1) * a.d, c, a.d, sum);
-    for (int64_t k = chunk + 1; k < end; k += JOIN_AHEAD) {
-        float f[JOIN_AHEAD][C::N];
-#pragma unroll
-        for (int y = 0; y < JOIN_AHEAD; ++y)
-            if (k + y < end) load_part(a.parts + 2 * (k + y) * a.d, c, a.d, f[y]);
-#pragma unroll
-        for (int y = 0; y < JOIN_AHEAD; ++y) {
-            if (k + y >= end) continue;
-#pragma unroll
-            for (int e = 0; e < C::N; ++e) sum[e] += f[y][e];
+    constexpr int N = C::N, WIDTH = 64 * N;
+    __shared__ int64_t many[4];                        // parts of a shared word; 0 where the wave's word is none
+    __shared__ float sums[4][64][N + 1];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t chunks = (a.n + a.chunk - 1) / a.chunk, groups = (chunks + 3) / 4, first = blockIdx.x % groups * 4;
+    const int64_t c = blockIdx.x / groups * WIDTH + lane * N;
+    auto at = [&](int64_t p) __attribute__((always_inline)) { return __builtin_amdgcn_readfirstlane((int)(a.sorted[p] >> 32)); };
+    // the chunks from `chunk` on that hold the word that crosses its end, if that begins in it
+    auto parts_of = [&](int64_t chunk) __attribute__((always_inline)) -> int64_t {
+        if (chunk + 1 >= chunks) return 0;
+        const int v = at((chunk + 1) * a.chunk);
+        if (v >= a.vocab || at((chunk + 1) * a.chunk - 1) != v) return 0;                    // no word crosses
+        if (chunk > 0 && at(chunk * a.chunk) == v && at(chunk * a.chunk - 1) == v) return 0;   // it began before
+        int64_t end = chunk + 1;                       // chunks that begin with the word
+        for (;;) {
+            const int64_t k = end + lane;
+            const uint64_t same = __ballot(k < chunks && (int)(a.sorted[k * a.chunk] >> 32) == v);
+            end += same == ~0ull ? 64 : __builtin_ctzll(~same);
+            if (same != ~0ull) return end - chunk;
         }
+    };
+    // parts from, from + step, .. of n, JOIN_AHEAD loads in flight
+    auto add = [&](int64_t chunk, int64_t from, int64_t step, int64_t n, float (&sum)[N]) __attribute__((always_inline)) {
+        for (int64_t k = from; k < n && c < a.d; k += JOIN_AHEAD * step) {
+            float f[JOIN_AHEAD][N];
+#pragma unroll
+            for (int y = 0; y < JOIN_AHEAD; ++y) {
+                const int64_t i = min(k + y * step, n - 1);
+                load_part(a.parts + (2 * (chunk + i) + (i == 0 ? 1 : 0)) * a.d, c, a.d, f[y]);
+            }
+#pragma unroll
+            for (int y = 0; y < JOIN_AHEAD; ++y)
+#pragma unroll
+                for (int e = 0; e < N; ++e) sum[e] = k + y * step < n ? sum[e] + f[y][e] : sum[e];
+        }
+    };
+    const int64_t chunk = first + wave, n = parts_of(chunk);
+    if (n > 0 && n <= JOIN_AHEAD) {
+        float sum[N] = {};
+        add(chunk, 0, 1, n, sum);
+        if (c < a.d) finish<T, MODE>(a, at((chunk + 1) * a.chunk), c, sum);
     }
-    finish<T, MODE>(a, v, c, sum);
+    if (lane == 0) many[wave] = n > JOIN_AHEAD ? n : 0;
+    __syncthreads();
+    for (int q = 0; q < 4; ++q) {
+        const int64_t nq = many[q];
+        if (nq == 0) continue;
+        float sum[N] = {};
+        add(first + q, wave, 4, nq, sum);
+#pragma unroll
+        for (int e = 0; e < N; ++e) sums[wave][lane][e] = sum[e];
+        __syncthreads();
+        if (wave == q && c < a.d) {
+#pragma unroll
+            for (int e = 0; e < N; ++e) sum[e] = ((sums[0][lane][e] + sums[1][lane][e]) + sums[2][lane][e]) + sums[3][lane][e];
+            finish<T, MODE>(a, at((chunk + 1) * a.chunk), c, sum);
+        }
+        __syncthreads();
+    }
 }
 
 // At most FEW tokens, not sorted.  Job j: token j / pieces, if it is the first of its word, with the others of that word;
@@ -530,7 +559,7 @@ static int embed_sums(EmbedArgs a, hipStream_t s) {
         hipLaunchKernelGGL((sums_kernel<T, MODE>), grid, dim3(256), 0, s, a, sums, zeros, words);
         const int rc = check_launch("sums_kernel");
         if (rc || chunks < 2) return rc;
-        hipLaunchKernelGGL((join_rows_kernel<T, MODE>), dim3((unsigned)((sums + 3) / 4)), dim3(256), 0, s, a);
+        hipLaunchKernelGGL((join_rows_kernel<T, MODE>), dim3((unsigned)((chunks + 3) / 4 * pieces)), dim3(256), 0, s, a);
     }
     return check_launch("join_rows_kernel");
 }

@@ -70,7 +70,7 @@ def compare(ids, w, dy, scale=1.0, padding=None):
 
 @pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "fp32"])
 @pytest.mark.parametrize("n,vocab,d", [(1, 1, 1), (1, 5, 8), (61, 512, 256), (33, 7, 3), (64, 64, 384), (1000, 3, 129), (1025, 5000, 520),
-                                       (5000, 130000, 16), (16384, 1000, 40), (16385, 512, 24), (40001, 70000, 9), (70000, 300, 8)])
+                                       (5000, 130000, 16), (16384, 1000, 40), (16385, 512, 24), (40001, 70000, 9), (70000, 300, 8), (3001, 4, 1100)])
 def test_against_64_bits(n, vocab, d, dtype):
     compare(*make(n, vocab, d, dtype, n + vocab))
     ids, w, dy = make(n, vocab, d, dtype, n + vocab + 1, low=-1)           # some without a word
@@ -142,7 +142,7 @@ def test_strides_and_padding_from_the_end():
 
 
 @pytest.mark.parametrize("noise", ["philox8", "triton"])
-@pytest.mark.parametrize("n,vocab,d", [(61, 512, 256), (700, 90, 13), (20000, 333, 72), (1, 4, 8), (5000, 130000, 16)])
+@pytest.mark.parametrize("n,vocab,d", [(61, 512, 256), (700, 90, 13), (20000, 333, 72), (1, 4, 8), (5000, 130000, 16), (3001, 4, 1100)])
 def test_accumulated(L, n, vocab, d, noise):
     """Bit for bit the stored gradient and msr_sr_accum, for the words that tokens hit; the others are untouched."""
     import muon_sr_amd as M
