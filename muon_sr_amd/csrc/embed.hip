@@ -5,8 +5,8 @@
 // The tokens are sorted by word, earlier tokens first: runs of SORT_RUN tokens by one work-group each (a radix sort in
 // LDS), then merged, MERGE_WAYS runs at a time.  Waves then take 16 or 32 sorted tokens each and add up the rows of one word after
 // the other in fp32, so that no sum depends on a race.  A word whose tokens lie in one chunk is finished there; of a word that
-// crosses chunks each leaves a part, which join_rows_kernel adds up in their order.  Rows of dW without a token are
-// written by the same launch, found by a search in the sorted tokens.  Up to FEW tokens are not sorted: the wave of a
+// crosses chunks each leaves a part, which join_rows_kernel adds up, in an order that the ids alone give.  Rows of dW without a token
+// are written by the launch of the sums, found by a search in the sorted tokens.  Up to FEW tokens are not sorted: the wave of a
 // word's first token finds the others itself, one launch instead of three.
 #include "rows.hpp"
 #include "../../include/muon_sr_amd.h"

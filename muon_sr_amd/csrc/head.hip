@@ -30,11 +30,12 @@ struct HeadArgs {
     float2 *part;                // [tiles of words][rows]: a tile's maximum and sum
     float *picked;               // [rows]: S[n][t[n]]
     const float *dloss;          // [rows] in the given order, or one
-    uint16_t *g;                 // [rows][ldg]: a piece of G / c
+    uint16_t *g;                 // [rows][ldg]: a piece of G / c; [2][rows][ldg] with lo
     float *slots;                // fp32 sums [splits][M][N]
     uint16_t *out;               // dW or the accumulator
     int64_t ldg;
     int32_t rows, vocab, d, reduction;
+    int32_t lo;                  // rows, where G / c is kept as the sum of two bf16 numbers, else 0
     int32_t v0, vn;              // the piece: words v0 to v0 + vn - 1
     int32_t tiles_n, splits, first, zero_init;   // first: the slots hold nothing yet
     Noise ns;
@@ -299,18 +300,29 @@ __global__ __launch_bounds__(64 * Shape<T>::NW, 2) void logits_kernel(HeadArgs a
                         for (int x = 0; x < 16; ++x)
                             if (rel == 32 * j + 8 * (x >> 2) + (x & 3)) pr.acc[i][j][x] -= g;
                 }
+                auto put = [&](int part) __attribute__((always_inline)) {
 #pragma unroll
-                for (int j = 0; j < FN; ++j)
+                    for (int j = 0; j < FN; ++j)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        *reinterpret_cast<uint2 *>(wst + r32 * WROW + (((4 * j + r) ^ (r32 & (WC - 1))) * 16 + khalf * 8)) =
-                            make_uint2(rne_bf16x2(pr.acc[i][j][4 * r], pr.acc[i][j][4 * r + 1]),
-                                       rne_bf16x2(pr.acc[i][j][4 * r + 2], pr.acc[i][j][4 * r + 3]));
+                        for (int r = 0; r < 4; ++r)
+                            *reinterpret_cast<uint2 *>(wst + r32 * WROW + (((4 * j + r) ^ (r32 & (WC - 1))) * 16 + khalf * 8)) =
+                                make_uint2(rne_bf16x2(pr.acc[i][j][4 * r], pr.acc[i][j][4 * r + 1]),
+                                           rne_bf16x2(pr.acc[i][j][4 * r + 2], pr.acc[i][j][4 * r + 3]));
 #pragma unroll
-                for (int y = 0; y < NP; ++y) {
-                    const int rr = crow + RPP * y, m = m0 + wm * SH::TM + 32 * i + rr;
-                    const u32x4_t c = *reinterpret_cast<const u32x4_t *>(wst + rr * WROW + ((cchk ^ (rr & (WC - 1))) * 16));
-                    if (m < count && nc < a.vn) *reinterpret_cast<u32x4_t *>(a.g + (int64_t)m * a.ldg + nc) = c;
+                    for (int y = 0; y < NP; ++y) {
+                        const int rr = crow + RPP * y, m = m0 + wm * SH::TM + 32 * i + rr;
+                        const u32x4_t c = *reinterpret_cast<const u32x4_t *>(wst + rr * WROW + ((cchk ^ (rr & (WC - 1))) * 16));
+                        if (m < count && nc < a.vn) *reinterpret_cast<u32x4_t *>(a.g + (int64_t)(part * a.lo + m) * a.ldg + nc) = c;
+                    }
+                };
+                put(0);
+                if constexpr (T < 256) {
+                    if (!a.lo) continue;
+#pragma unroll
+                    for (int j = 0; j < FN; ++j)
+#pragma unroll
+                        for (int x = 0; x < 16; ++x) pr.acc[i][j][x] -= bf16_to_f32((uint16_t)rne_bf16(pr.acc[i][j][x]));
+                    put(1);
                 }
             }
         }
@@ -395,7 +407,7 @@ __global__ __launch_bounds__(64 * Shape<T>::NW, WPS) void piece_kernel(HeadArgs 
     const int wm = wave / SH::WN, wn = wave % SH::WN;
     const int count = kept_rows(a);
     const float unit = OUT == OUT_SLOTS ? 1.0f : unit_of(a, count);
-    const int M = KIND == HD_DX ? count : a.vn, K = KIND == HD_DX ? a.vn : count;
+    const int M = KIND == HD_DX ? a.lo + count : a.vn, K = KIND == HD_DX ? a.vn : count;
     int mt, nt, split;
     if (!find_tile(blockIdx.x, (M + T - 1) / T, a.tiles_n, a.splits, mt, nt, split)) return;
     const int m0 = mt * T, n0 = nt * T;
@@ -419,6 +431,13 @@ __global__ __launch_bounds__(64 * Shape<T>::NW, WPS) void piece_kernel(HeadArgs 
                    {a.w + (int64_t)a.v0 * a.d + n0, a.d, 0, a.d - n0, kend}, kb, slabs);
         else
             pr.run(lds_p, lds_q, {a.g + m0, a.ldg, 0, vn8 - m0, kend}, {a.x + n0, a.d, 0, a.d - n0, kend}, kb, slabs);
+        if constexpr (KIND == HD_DW && T < 256) {
+            if (a.lo) {
+                wait_vm<0>();
+                asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+                pr.run(lds_p, lds_q, {a.g + (int64_t)a.lo * a.ldg + m0, a.ldg, 0, vn8 - m0, kend}, {a.x + n0, a.d, 0, a.d - n0, kend}, kb, slabs);
+            }
+        }
     }
     wait_vm<0>();
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
@@ -426,7 +445,7 @@ __global__ __launch_bounds__(64 * Shape<T>::NW, WPS) void piece_kernel(HeadArgs 
     asm volatile("" : "+v"(etid));
     const int elane = etid & 63, r32 = elane & 31, khalf = elane >> 5;
     if constexpr (OUT == OUT_SLOTS) {
-        const int64_t rows = KIND == HD_DX ? a.rows : a.vn;
+        const int64_t rows = KIND == HD_DX ? a.lo + a.rows : a.vn;
 #pragma unroll
         for (int i = 0; i < FM; ++i) {
             const int m = m0 + wm * SH::TM + 32 * i + r32;
@@ -497,7 +516,11 @@ __global__ __launch_bounds__(256) void dx_kernel(HeadArgs a, uint16_t *dx) {
         if (p >= 0)
             for (int s = 0; s < a.splits; ++s) {
                 float h[8];
-                load_f32x8<true>(a.slots, ((int64_t)s * rows + p) * d + c, 8, h);
+                load_f32x8<true>(a.slots, ((int64_t)s * (a.lo + rows) + p) * d + c, 8, h);
+#pragma unroll
+                for (int x = 0; x < 8; ++x) f[x] += h[x];
+                if (!a.lo) continue;
+                load_f32x8<true>(a.slots, ((int64_t)s * (a.lo + rows) + a.lo + p) * d + c, 8, h);
 #pragma unroll
                 for (int x = 0; x < 8; ++x) f[x] += h[x];
             }
@@ -554,10 +577,11 @@ struct Tiling {
     int tile, splits;
 };
 // slots: 0: K is not split; 1: results go through a slot anyway (dx); 2: they do where K is split, in one more launch (dW)
-static Tiling tiling(int64_t M, int64_t N, int64_t K, int slots) {
+static Tiling tiling(int64_t M, int64_t N, int64_t K, int slots, int most = 256) {
     Tiling best{128, 1};
     float least = 1e30f;
     for (const int T : {64, 128, 256})
+        if (T <= most)
         for (int s = 1; s <= (slots ? 16 : 1); ++s) {
             if (s > 1 && K < 256 * s) break;
             // a slot is written and read: 8 bytes per result at 4 TB/s
@@ -578,15 +602,22 @@ constexpr int64_t PIECE_WORDS = 1 << 18;              // at most: a slab's rows 
 // A call of at most so many rows packs them where it lists them, and adds up its losses, of at most so many parts, where it
 // joins them: a launch less each (7 rows, 512 words of 256: 78 us a pass with the launches, 71 so).
 constexpr int64_t FEW_ROWS = 32, FEW_PARTS = 1 << 12;
+// Of so few rows the roundings of G's largest elements do not average out over a gradient's sums, and the products' tiles have rows to
+// spare: there G / c is the sum of two bf16 numbers, in tiles of up to 128.  Each row has its own g for the reduction "none", which c
+// does not take out, so there more rows count as few.  Largest of 12 errors against 64 bits, where the rounding of the results is 0.0017:
+// with one number 33 rows, 512 words of 256 0.0022 (0.0027 "none"), 128 rows, 896 words of 144 0.0021 (0.0025); with two 0.0017.
+// us of backward passes: 7 rows, 512 words of 256 15.3 with one and 16.9 with two, 128256 of 4096 584 and 636, 64 rows of the latter
+// 664 and 790.
+constexpr int64_t LO_ROWS = 32, LO_ROWS_NONE = 128;
 
 struct HeadPlan {
     Tiling fwd, logits, dx, dw;
-    int64_t piece, ldg;                                // words of a piece
+    int64_t piece, ldg, lo;                            // words of a piece
     size_t fwd_bytes, bwd_bytes, g_at, dx_at, dw_at;
 };
 static size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 
-static HeadPlan head_plan(int64_t rows, int64_t vocab, int64_t d) {
+static HeadPlan head_plan(int64_t rows, int64_t vocab, int64_t d, int32_t reduction) {
     HeadPlan p{};
     p.fwd = tiling(rows, vocab, d, 0);
     const int64_t tn = (vocab + p.fwd.tile - 1) / p.fwd.tile;
@@ -596,19 +627,21 @@ static HeadPlan head_plan(int64_t rows, int64_t vocab, int64_t d) {
     const int64_t pieces = (vocab + most - 1) / most;
     p.piece = std::min<int64_t>(((vocab + pieces - 1) / pieces + 255) / 256 * 256, (vocab + 7) / 8 * 8);
     p.ldg = p.piece;
-    p.logits = tiling(rows, p.piece, d, 0);
-    p.dx = tiling(rows, d, p.piece, 1);
-    p.dw = tiling(p.piece, d, rows, 2);
+    p.lo = rows <= (reduction == HEAD_NONE ? LO_ROWS_NONE : LO_ROWS) ? rows : 0;
+    const int most_tile = p.lo ? 128 : 256;
+    p.logits = tiling(rows, p.piece, d, 0, most_tile);
+    p.dx = tiling(p.lo + rows, d, p.piece, 1, most_tile);
+    p.dw = tiling(p.piece, d, rows, 2, most_tile);
     p.g_at = 0;
-    p.dx_at = up256((size_t)rows * (size_t)p.ldg * 2);
-    p.dw_at = p.dx_at + up256((size_t)p.dx.splits * (size_t)rows * (size_t)d * 4);
+    p.dx_at = up256((size_t)(p.lo + rows) * (size_t)p.ldg * 2);
+    p.dw_at = p.dx_at + up256((size_t)p.dx.splits * (size_t)(p.lo + rows) * (size_t)d * 4);
     p.bwd_bytes = p.dw_at + (p.dw.splits > 1 ? up256((size_t)p.dw.splits * (size_t)p.piece * (size_t)d * 4) : 0);
     return p;
 }
 
 static int64_t tiles_of(int64_t M, int64_t N, const Tiling &t) { return (M + t.tile - 1) / t.tile * ((N + t.tile - 1) / t.tile) * t.splits; }
 static int head_grids(const char *name, const HeadPlan &p, int64_t rows, int64_t vocab, int64_t d) {
-    const int64_t most = std::max({tiles_of(rows, vocab, p.fwd), tiles_of(rows, p.piece, p.logits), tiles_of(rows, d, p.dx), tiles_of(p.piece, d, p.dw)});
+    const int64_t most = std::max({tiles_of(rows, vocab, p.fwd), tiles_of(rows, p.piece, p.logits), tiles_of(p.lo + rows, d, p.dx), tiles_of(p.piece, d, p.dw)});
     if (most < (1 << 22)) return MSR_OK;       // 512 threads each: fewer than 2^31 in a launch
     set_error("%s: too many tiles for a launch (%lld)", name, (long long)most);
     return MSR_ERR_ARG;
@@ -626,7 +659,7 @@ static int logits_launch(const HeadArgs &a, int T, int64_t tiles, hipStream_t s)
 
 template <int KIND, int OUT>
 static int piece_launch(HeadArgs a, const Tiling &t, hipStream_t s) {
-    const int64_t M = KIND == HD_DX ? a.rows : a.vn;
+    const int64_t M = KIND == HD_DX ? a.lo + a.rows : a.vn;
     a.tiles_n = (a.d + t.tile - 1) / t.tile;
     a.splits = t.splits;
     const unsigned grid = (unsigned)((M + t.tile - 1) / t.tile * a.tiles_n * t.splits);
@@ -667,9 +700,9 @@ int msr_head_workspace_bytes(int64_t rows, int64_t vocab, int64_t d, size_t *for
     const int rc = head_check("msr_head_workspace_bytes", rows, vocab, d);
     if (rc) return rc;
     if (!forward || !backward) { set_error("msr_head_workspace_bytes: a pointer is NULL"); return MSR_ERR_ARG; }
-    const HeadPlan p = head_plan(rows, vocab, d);
+    const HeadPlan p = head_plan(rows, vocab, d, HEAD_MEAN);
     *forward = p.fwd_bytes;
-    *backward = p.bwd_bytes;
+    *backward = std::max(p.bwd_bytes, head_plan(rows, vocab, d, HEAD_NONE).bwd_bytes);
     return MSR_OK;
 }
 
@@ -677,7 +710,7 @@ int msr_head_plan(int64_t rows, int64_t vocab, int64_t d, int32_t *plan) {
     const int rc = head_check("msr_head_plan", rows, vocab, d);
     if (rc) return rc;
     if (!plan) { set_error("msr_head_plan: a pointer is NULL"); return MSR_ERR_ARG; }
-    const HeadPlan p = head_plan(rows, vocab, d);
+    const HeadPlan p = head_plan(rows, vocab, d, HEAD_MEAN);
     const int32_t out[7] = {p.fwd.tile, p.logits.tile, p.dx.tile, p.dx.splits, p.dw.tile, p.dw.splits, (int32_t)p.piece};
     for (int i = 0; i < 7; ++i) plan[i] = out[i];
     return MSR_OK;
@@ -699,7 +732,7 @@ int msr_head_forward(const uint16_t *x, int64_t ldx, const uint16_t *w, const vo
         set_error("%s: w, packed and the workspace must be 16-byte aligned, the others to their types", name);
         return MSR_ERR_ALIGN;
     }
-    const HeadPlan p = head_plan(rows, vocab, d);
+    const HeadPlan p = head_plan(rows, vocab, d, reduction);
     if ((rc = head_grids(name, p, rows, vocab, d))) return rc;
     if (rows > 0 && (!workspace || workspace_bytes < p.fwd_bytes)) {
         set_error("%s: workspace of %zu bytes is smaller than the %zu required", name, workspace_bytes, p.fwd_bytes);
@@ -762,7 +795,7 @@ int msr_head_backward(const uint16_t *packed, const uint16_t *w, const int32_t *
         set_error("%s: operands and the workspace must be 16-byte aligned, kept, lse and dloss to their types", name);
         return MSR_ERR_ALIGN;
     }
-    const HeadPlan p = head_plan(rows, vocab, d);
+    const HeadPlan p = head_plan(rows, vocab, d, reduction);
     if ((rc = head_grids(name, p, rows, vocab, d))) return rc;
     if (rows > 0 && (!workspace || workspace_bytes < p.bwd_bytes)) {
         set_error("%s: workspace of %zu bytes is smaller than the %zu required", name, workspace_bytes, p.bwd_bytes);
@@ -778,7 +811,7 @@ int msr_head_backward(const uint16_t *packed, const uint16_t *w, const int32_t *
     HeadArgs a{};
     char *const ws = static_cast<char *>(workspace);
     a.x = packed; a.w = w; a.kept = kept; a.lse = const_cast<float *>(lse); a.dloss = dloss;
-    a.g = reinterpret_cast<uint16_t *>(ws); a.ldg = p.ldg; a.out = dw;
+    a.g = reinterpret_cast<uint16_t *>(ws); a.ldg = p.ldg; a.lo = (int)p.lo; a.out = dw;
     a.rows = (int)rows; a.vocab = (int)vocab; a.d = (int)d; a.reduction = reduction; a.zero_init = zero_init != 0;
     a.ns.key = seed_key(seed, 0);
     a.ns.inject = inject;

@@ -6,7 +6,8 @@ a = x - m costs 4 u (|a| + 1) + 2 u |m|: the difference, its product with log2 e
 64 + vocab / 64 additions one after the other (32 in a lane, the waves', and a share of the tiles), so l is off by at most
 el = max eS + 2 depth u + 8 u (|l| + 1) + 2 u max|S|, and the loss by eS + el + u |loss|.
 G = g (p - [target]) is off by eG = g (p (eS + el + 4 u (|S - l| + 1) + 2 u |l|) + 2 u), then h |G| by its rounding (a rounding is
-off by less than h / (1 + h), which leaves room for the division by c); a product over
+off by less than h / (1 + h), which leaves room for the division by c), or h^2 |G| of up to 32 rows (128 where each has its own g), whose G is kept
+as two numbers; a product over
 K terms adds 2 (K + 16) u sum|terms| (c's product among them) and the stored value's rounding h |value|.  Values below the smallest normal
 number may vanish: 2^-126 per term."""
 import ctypes
@@ -65,7 +66,7 @@ def exact(x, w, target, dloss, reduction):
     G = p.clone()
     G[torch.arange(len(t), device=DEV), t] -= 1.0
     G *= g
-    eG += H * (G.abs() + eG)
+    eG += (H if len(t) > (128 if reduction == "none" else 32) else H * H) * (G.abs() + eG)
 
     def product(a, ea, b):
         terms = a.abs() @ b.abs()
@@ -103,7 +104,7 @@ def plan(L, rows, vocab, d):
 
 
 SIZES = [(1, 1, 8), (1, 17, 8), (7, 512, 256), (2, 9001, 64), (65, 130, 72), (300, 1000, 1032), (257, 4099, 136), (1025, 70, 2048),
-         (3000, 8192, 64), (2047, 3001, 1024), (16384, 17001, 64), (5000, 777, 264), (129, 20011, 520), (64, 64, 64), (4096, 8200, 2048)]
+         (3000, 8192, 64), (2047, 3001, 1024), (16384, 17001, 64), (5000, 777, 264), (129, 20011, 520), (64, 64, 64), (32, 3001, 1032), (31, 70000, 72), (128, 900, 136), (100, 30011, 520), (4096, 8200, 2048)]
 
 
 @pytest.mark.parametrize("rows,vocab,d", SIZES)
@@ -367,7 +368,7 @@ def test_weights_beyond_32_bit_offsets(L):
     G = p.clone()
     G[on, target[on]] -= 1.0
     G, eG = ((torch.where(target != -100, dloss, 0.0).double())[:, None] * v for v in (G, eG))
-    eG = eG + H * (G.abs() + eG)
+    eG = eG + H * H * (G.abs() + eG)
     for rows_ in (slice(vocab - 300, vocab), slice(199990, 200010), slice(0, 8)):
         value, terms = G[:, rows_].t() @ x.double(), (eG + 2 * 32 * U * G.abs())[:, rows_].t() @ x.double().abs()
         near(dw[rows_], (value, H * value.abs() + (1 + H) * terms + 1e-30))
