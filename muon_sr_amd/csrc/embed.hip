@@ -201,46 +201,55 @@ __device__ __forceinline__ int64_t below(const uint64_t *keys, int64_t n, uint64
 
 // Runs of `run` keys (a power of two), MERGE_WAYS at a time, merged: a key's place is its own number in its run plus how many of
 // each other are below it.  A search in memory is a chain of loads, so every work-group holds each stride-th key of its group of
-// runs in LDS, searches there first and in memory among the last `stride` only, in eight runs at once (16384 tokens: 17 us with
-// the whole search in memory, 12.5 so).
-constexpr int MERGE_HELD = 8192;
-__global__ __launch_bounds__(256) void merge_kernel(const uint64_t *in, uint64_t *out, int64_t n, int log_run) {
-    constexpr int AT_ONCE = 8;
+// runs in LDS, searches there first and in memory among the last `stride` only, in four runs at once; the searches are chains all the same,
+// so four threads share those of a key (us with the whole search in memory by one thread, with the LDS, and so: 16384 tokens 17, 12, 7;
+// 60000 tokens 45 with the LDS, 16 so).
+constexpr int MERGE_HELD = 8192, MERGE_KEYS = 256, MERGE_SHARES = 4;
+__global__ __launch_bounds__(MERGE_KEYS * MERGE_SHARES) void merge_kernel(const uint64_t *in, uint64_t *out, int64_t n, int log_run) {
+    constexpr int AT_ONCE = 4, THREADS = MERGE_KEYS * MERGE_SHARES;
     __shared__ uint64_t held[MERGE_HELD];
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, run = (int64_t)1 << log_run;
+    __shared__ int64_t below[MERGE_SHARES][MERGE_KEYS];
+    const int share = threadIdx.x / MERGE_KEYS, own = threadIdx.x % MERGE_KEYS;
+    const int64_t i = (int64_t)blockIdx.x * MERGE_KEYS + own, run = (int64_t)1 << log_run;
     const int log_group = log_run + MERGE_LOG;
-    const int64_t first = ((int64_t)blockIdx.x * 256) >> log_group << log_group, end = min(first + ((int64_t)1 << log_group), n);
+    const int64_t first = ((int64_t)blockIdx.x * MERGE_KEYS) >> log_group << log_group, end = min(first + ((int64_t)1 << log_group), n);
+    const uint64_t key = i < n ? in[i] : 0;
     int log_stride = 3;
     while ((end - first) >> log_stride > MERGE_HELD) ++log_stride;
     const int log_per = log_run - log_stride, keys = (int)((end - first) >> log_stride), all = (int)((end - first + run - 1) >> log_run) << log_per;
-    for (int k = threadIdx.x; k < min(all, MERGE_HELD); k += 256) held[k] = k < keys ? in[first + ((int64_t)(k + 1) << log_stride) - 1] : ~0ull;
+    for (int k = threadIdx.x; k < min(all, MERGE_HELD); k += THREADS) held[k] = k < keys ? in[first + ((int64_t)(k + 1) << log_stride) - 1] : ~0ull;
     __syncthreads();
-    if (i >= n) return;
     const int64_t mine = i >> log_run << log_run;
-    const uint64_t key = in[i];
-    int64_t place = first + (i - mine);
-    for (int64_t r0 = first; r0 < end; r0 += AT_ONCE * run) {
+    int64_t place = 0;
+    for (int64_t r0 = first + share * run; r0 < end; r0 += AT_ONCE * MERGE_SHARES * run) {
         int64_t lo[AT_ONCE], len[AT_ONCE];
         int k[AT_ONCE] = {};
         const int base = (int)((r0 - first) >> log_run) << log_per;
 #pragma unroll
-        for (int y = 0; y < AT_ONCE; ++y) len[y] = r0 + y * run == mine ? 0 : max((int64_t)0, min(run, end - (r0 + y * run)));
+        for (int y = 0; y < AT_ONCE; ++y) {
+            const int64_t r = r0 + y * MERGE_SHARES * run;
+            len[y] = r == mine || i >= n ? 0 : max((int64_t)0, min(run, end - r));
+        }
         for (int step = 1 << log_per; step; step >>= 1) {
 #pragma unroll
             for (int y = 0; y < AT_ONCE; ++y)
-                if (k[y] + step <= (int)(len[y] >> log_stride) && held[base + (y << log_per) + k[y] + step - 1] < key) k[y] += step;
+                if (k[y] + step <= (int)(len[y] >> log_stride) && held[base + (y * MERGE_SHARES << log_per) + k[y] + step - 1] < key) k[y] += step;
         }
 #pragma unroll
         for (int y = 0; y < AT_ONCE; ++y) lo[y] = (int64_t)k[y] << log_stride;
         for (int64_t step = (int64_t)1 << (log_stride - 1); step; step >>= 1) {
 #pragma unroll
             for (int y = 0; y < AT_ONCE; ++y)
-                if (lo[y] + step <= len[y] && in[r0 + y * run + lo[y] + step - 1] < key) lo[y] += step;
+                if (lo[y] + step <= len[y] && in[r0 + y * MERGE_SHARES * run + lo[y] + step - 1] < key) lo[y] += step;
         }
 #pragma unroll
         for (int y = 0; y < AT_ONCE; ++y) place += lo[y];
     }
-    out[place] = key;
+    below[share][own] = place;
+    __syncthreads();
+    if (share || i >= n) return;
+    for (int s = 1; s < MERGE_SHARES; ++s) place += below[s][own];
+    out[first + (i - mine) + place] = key;
 }
 
 // ---------------------------------------------------------------------------
@@ -611,7 +620,7 @@ static int embed_grad(const char *name, const void *ids, int32_t ids_i64, int64_
         hipLaunchKernelGGL(sort_kernel, dim3((unsigned)p.runs), dim3(SORT_THREADS), 0, s, a);
         if ((rc = check_launch("sort_kernel"))) return rc;
         for (int m = 0; m < p.merges; ++m) {
-            hipLaunchKernelGGL(merge_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, list[m & 1], list[~m & 1], n, SORT_LOG + m * MERGE_LOG);
+            hipLaunchKernelGGL(merge_kernel, dim3((unsigned)((n + MERGE_KEYS - 1) / MERGE_KEYS)), dim3(MERGE_KEYS * MERGE_SHARES), 0, s, list[m & 1], list[~m & 1], n, SORT_LOG + m * MERGE_LOG);
             if ((rc = check_launch("merge_kernel"))) return rc;
             a.sorted = list[~m & 1];
         }
