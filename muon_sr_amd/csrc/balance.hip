@@ -27,30 +27,6 @@ struct BalanceArgs {
     int32_t experts, k, i64;
 };
 
-// Sums and maxima over groups of L = 8, 16, 32 or 64 lanes, in every lane of the group
-struct Add {
-    __device__ __forceinline__ float operator()(float a, float b) const { return a + b; }
-};
-struct Max {
-    __device__ __forceinline__ float operator()(float a, float b) const { return fmaxf(a, b); }
-};
-template <int L, typename Op>
-__device__ __forceinline__ float over_group(float x, Op op) {
-    x = op(x, turned<0xB1>(x));                        // quad_perm [1, 0, 3, 2]
-    x = op(x, turned<0x4E>(x));                        // quad_perm [2, 3, 0, 1]
-    x = op(x, turned<0x141>(x));                       // row_half_mirror
-    if constexpr (L >= 16) x = op(x, turned<0x140>(x));   // row_mirror
-    if constexpr (L >= 32) {
-        const auto q = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-        x = op(__uint_as_float(q[0]), __uint_as_float(q[1]));
-    }
-    if constexpr (L >= 64) {
-        const auto h = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-        x = op(__uint_as_float(h[0]), __uint_as_float(h[1]));
-    }
-    return x;
-}
-
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 // Work-group b's tokens: [b per, (b + 1) per).  blockDim.x: 256 or 1024.

@@ -1,8 +1,8 @@
 // Layer norm over the last dimension, rows x [rows][d]:
 //     mu = mean(x), r = 1 / sqrt(mean((x - mu)^2) + eps), h = (x - mu) r,   y = h w + b
 //     q = dy w,   dx = r (q - mean(q) - h mean(q h)),   dw = sum_n dy h,   db = sum_n dy
-// HBM bounds both passes (x and y; x, dy and dx).  A row is held in the registers of one wave or of the four of a
-// work-group, read once: a mean first, then the sums of what is left of it and of its squares, so that a mean far from zero costs no
+// HBM bounds both passes (x and y; x, dy and dx).  A row is held in the registers of L lanes, 8 to 64 of a wave or a whole work-group of
+// 256 or 1024, read once: a mean first, then the sums of what is left of it and of its squares, so that a mean far from zero costs no
 // digits: with z = x - (that mean), mean += mean(z) and the variance is mean(z^2) - mean(z)^2.  The
 // backward pass adds dw and db up in registers over the rows that a work-group takes, in order; the
 // work-groups' sums, in fp32, are added by a second kernel, in order.
@@ -33,31 +33,38 @@ __device__ __forceinline__ void vector_cells(const void *p, int w32, int64_t c, 
     }
 }
 
-// Sums over the lanes that hold a row: a wave (W = 1), or the work-group's four.
-template <int W>
+// Sums over the L lanes that hold a row.
+template <int L>
 struct RowSum {
-    float2 (*lds)[4];            // [2][4], used in turn
+    static constexpr int WAVES = L > 64 ? L / 64 : 1;
+    float2 (*lds)[WAVES];        // [2][WAVES], used in turn
     int turn = 0;
     __device__ __forceinline__ float2 of(float x, float y) {
+        if constexpr (L < 64) return make_float2(over_group<L>(x, Add{}), over_group<L>(y, Add{}));
         float2 v = wave_sum2(x, y);
-        if constexpr (W > 1) {
+        if constexpr (L > 64) {
             float2 *const at = lds[turn];
             turn ^= 1;
             if ((threadIdx.x & 63) == 0) at[threadIdx.x >> 6] = v;
             __syncthreads();
-            v = make_float2(((at[0].x + at[1].x) + at[2].x) + at[3].x, ((at[0].y + at[1].y) + at[2].y) + at[3].y);
+            v = at[0];
+#pragma unroll
+            for (int w = 1; w < WAVES; ++w) v = make_float2(v.x + at[w].x, v.y + at[w].y);
         }
         return v;
     }
 };
+constexpr int norm_threads(int L) { return L > 256 ? L : 256; }
 
-// U cells per lane; W waves per row.
-template <typename T, int U, int W>
-__global__ __launch_bounds__(256) void norm_kernel(NormArgs a) {
+// U cells per lane, L lanes per row: few lanes to a short row, so that a wave holds up to eight (us, forward and gradient, a wave to a
+// row and so: 131072 rows of 64 46 92, 12 16; of 128 47 94, 23 24), 1024 to a long one (rows read as often as they are needed, and so: 8000
+// rows of 16384 501 1312, 122 223; 3000 fp32 rows of 16000 144 449, 83 167).
+template <typename T, int U, int L>
+__global__ __launch_bounds__(norm_threads(L)) void norm_kernel(NormArgs a) {
     using C = Cells<T>;
-    constexpr int N = C::N, L = 64 * W;
-    __shared__ float2 lds[2][4];
-    RowSum<W> sums{lds};
+    constexpr int N = C::N, ROWS = norm_threads(L) / L;
+    __shared__ float2 lds[2][RowSum<L>::WAVES];
+    RowSum<L> sums{lds};
     const int lane = threadIdx.x % L, sub = threadIdx.x / L;
     const float d = (float)a.d;
     float w[U][N], b[U][N];
@@ -66,15 +73,16 @@ __global__ __launch_bounds__(256) void norm_kernel(NormArgs a) {
         vector_cells<N>(a.w, a.w32, (int64_t)(u * L + lane) * N, a.d, 1.0f, w[u]);
         vector_cells<N>(a.b, a.w32, (int64_t)(u * L + lane) * N, a.d, 0.0f, b[u]);
     }
-    const int64_t step = (int64_t)gridDim.x * (4 / W);
-    int64_t n = (int64_t)blockIdx.x * (4 / W) + sub;
+    const int64_t step = (int64_t)gridDim.x * ROWS;
     C next[U];
     auto fetch = [&](int64_t r) __attribute__((always_inline)) {
         if (r >= a.rows) return;
 #pragma unroll
         for (int u = 0; u < U; ++u) next[u].load(static_cast<const T *>(a.x) + r * a.ldx, (int64_t)(u * L + lane) * N, a.d);
     };
-    for (fetch(n); n < a.rows; n += step) {
+    int64_t n = (int64_t)blockIdx.x * ROWS + sub;
+    fetch(n);
+    for (; n - (L < 64 ? sub : 0) < a.rows; n += step) {   // (the same for every lane of a wave: lanes without a row go along)
         float x[U][N];
 #pragma unroll
         for (int u = 0; u < U; ++u) next[u].get(x[u]);
@@ -95,6 +103,7 @@ __global__ __launch_bounds__(256) void norm_kernel(NormArgs a) {
                 q = __builtin_fmaf(x[u][e], x[u][e], q);
             }
         const float2 left = sums.of(z, q);
+        if (L < 64 && n >= a.rows) continue;
         const float c = left.x / d, r = 1.0f / sqrtf(fmaxf(left.y / d - c * c, 0.0f) + a.eps);
         mean += c;
         if (lane == 0) {
@@ -113,12 +122,15 @@ __global__ __launch_bounds__(256) void norm_kernel(NormArgs a) {
     }
 }
 
-template <typename T, int U, int W>
-__global__ __launch_bounds__(256) void norm_grad_kernel(NormArgs a) {
+template <typename T, int U, int L>
+__global__ __launch_bounds__(norm_threads(L)) void norm_grad_kernel(NormArgs a) {
     using C = Cells<T>;
-    constexpr int N = C::N, L = 64 * W;
-    __shared__ float2 lds[2][4];
-    RowSum<W> sums{lds};
+    constexpr int N = C::N, ROWS = norm_threads(L) / L;
+    // the next row on its way meanwhile: not where its registers, of 128 that a thread of 1024 has, cost more (us with it and without:
+    // 3000 fp32 rows of 16000 236 and 167, bf16 8000 of 16384 223 and 234, fp32 4000 of 8192 69 and 71)
+    constexpr bool AHEAD = L <= 256 || sizeof(T) == 2 || U * N <= 8;
+    __shared__ float2 lds[2][RowSum<L>::WAVES];
+    RowSum<L> sums{lds};
     const int lane = threadIdx.x % L, sub = threadIdx.x / L;
     const float inv = 1.0f / (float)a.d;
     float w[U][N], dw[U][N], db[U][N];
@@ -128,11 +140,15 @@ __global__ __launch_bounds__(256) void norm_grad_kernel(NormArgs a) {
 #pragma unroll
         for (int e = 0; e < N; ++e) dw[u][e] = db[u][e] = 0.0f;
     }
-    const int64_t step = (int64_t)gridDim.x * (4 / W);
-    int64_t n = (int64_t)blockIdx.x * (4 / W) + sub;
+    const int64_t step = (int64_t)gridDim.x * ROWS;
     C vx[U], vy[U];
     float next_mean = 0.0f, next_r = 0.0f;
     auto fetch = [&](int64_t i) __attribute__((always_inline)) {
+        if constexpr (L < 64) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) vx[u].v = vy[u].v = Bytes16{};
+            next_mean = next_r = 0.0f;
+        }
         if (i >= a.rows) return;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -142,7 +158,10 @@ __global__ __launch_bounds__(256) void norm_grad_kernel(NormArgs a) {
         next_mean = a.mean[i];
         next_r = a.rstd[i];
     };
-    for (fetch(n); n < a.rows; n += step) {
+    int64_t n = (int64_t)blockIdx.x * ROWS + sub;
+    if (AHEAD) fetch(n);
+    for (; n - (L < 64 ? sub : 0) < a.rows; n += step) {
+        if (!AHEAD) fetch(n);
         const float mean = next_mean, r = next_r;
         float h[U][N], q[U][N], sq = 0.0f, sqh = 0.0f;
 #pragma unroll
@@ -150,7 +169,7 @@ __global__ __launch_bounds__(256) void norm_grad_kernel(NormArgs a) {
             vx[u].get(h[u]);
             vy[u].get(q[u]);
 #pragma unroll
-            for (int e = 0; e < N; ++e) {       // (beyond the row dy is 0, and so is what it is multiplied into)
+            for (int e = 0; e < N; ++e) {       // (beyond the row, and without one, dy is 0, and so is what it is multiplied into)
                 h[u][e] = (h[u][e] - mean) * r;
                 dw[u][e] = __builtin_fmaf(q[u][e], h[u][e], dw[u][e]);
                 db[u][e] += q[u][e];
@@ -159,10 +178,10 @@ __global__ __launch_bounds__(256) void norm_grad_kernel(NormArgs a) {
                 sqh = __builtin_fmaf(q[u][e], h[u][e], sqh);
             }
         }
-        fetch(n + step);
+        if (AHEAD) fetch(n + step);
         const float2 m = sums.of(sq, sqh);
         const float mq = m.x * inv, mh = m.y * inv;
-        if (a.y) {
+        if (a.y && (L >= 64 || n < a.rows)) {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 float f[N];
@@ -176,7 +195,7 @@ __global__ __launch_bounds__(256) void norm_grad_kernel(NormArgs a) {
     }
     if (!a.parts) return;
     float *const to = a.parts + (int64_t)blockIdx.x * 2 * a.d;
-    if constexpr (W > 1) {
+    if constexpr (ROWS == 1) {
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -187,8 +206,8 @@ __global__ __launch_bounds__(256) void norm_grad_kernel(NormArgs a) {
                 to[a.d + c] = db[u][e];
             }
     } else {
-        // the four waves' sums, a cell at a time
-        __shared__ float both[4][2][64 * N];
+        // the rows' sums, a cell of each lane at a time
+        __shared__ float both[ROWS][2][L * N];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             __syncthreads();
@@ -198,10 +217,13 @@ __global__ __launch_bounds__(256) void norm_grad_kernel(NormArgs a) {
                 both[sub][1][lane * N + e] = db[u][e];
             }
             __syncthreads();
-            for (int i = threadIdx.x; i < 2 * 64 * N; i += 256) {
-                const int k = i / (64 * N), c = i % (64 * N);
+            for (int i = threadIdx.x; i < 2 * L * N; i += 256) {
+                const int k = i / (L * N), c = i % (L * N);
                 if ((int64_t)u * L * N + c >= a.d) continue;
-                to[k * a.d + (int64_t)u * L * N + c] = ((both[0][k][c] + both[1][k][c]) + both[2][k][c]) + both[3][k][c];
+                float s = both[0][k][c];
+#pragma unroll
+                for (int g = 1; g < ROWS; ++g) s += both[g][k][c];
+                to[k * a.d + (int64_t)u * L * N + c] = s;
             }
         }
     }
@@ -213,7 +235,7 @@ __global__ __launch_bounds__(256) void norm_long_kernel(NormArgs a) {
     using C = Cells<T>;
     constexpr int N = C::N;
     __shared__ float2 lds[2][4];
-    RowSum<4> sums{lds};
+    RowSum<256> sums{lds};
     const float d = (float)a.d;
     for (int64_t n = blockIdx.x; n < a.rows; n += gridDim.x) {
         const T *const row = static_cast<const T *>(a.x) + n * a.ldx;
@@ -263,7 +285,7 @@ __global__ __launch_bounds__(256) void norm_long_grad_kernel(NormArgs a) {
     using C = Cells<T>;
     constexpr int N = C::N;
     __shared__ float2 lds[2][4];
-    RowSum<4> sums{lds};
+    RowSum<256> sums{lds};
     const float inv = 1.0f / (float)a.d;
     float *const to = a.parts ? a.parts + (int64_t)blockIdx.x * 2 * a.d : nullptr;
     bool first = true;
@@ -334,20 +356,40 @@ __global__ __launch_bounds__(256) void norm_join_kernel(const float *parts, int 
     if (db) put(db, s.y);
 }
 
-// Cells per lane and waves per row; 0 cells: the row does not fit in registers.
-struct NormPlan {
-    int u, w, groups;            // groups: work-groups of the backward pass
-};
-static NormPlan norm_plan(int64_t rows, int64_t d, int32_t elem) {
-    NormPlan p{};
-    const int64_t cells = (d + (elem == MSR_BF16 ? 7 : 3)) / (elem == MSR_BF16 ? 8 : 4);
-    p.w = cells <= 64 * 2 ? 1 : 4;
-    const int64_t per = (cells + 64 * p.w - 1) / (64 * p.w);
-    p.u = per <= 1 ? 1 : per <= 2 ? 2 : per <= 4 ? 4 : 0;
-    if (p.u == 0) p.w = 4;
-    const int64_t at_once = 4 / p.w;
-    p.groups = (int)std::min<int64_t>(std::max<int64_t>((rows + at_once - 1) / at_once, 1), 512);
-    return p;
+// f(cells per lane, lanes per row) of a row of d elements; false, and f is not called, for one that does not fit in registers.
+template <typename T, typename F>
+static bool norm_shape(int64_t d, F &&f) {
+    auto is = [&](auto u, auto l) {
+        if (d > (int64_t)decltype(u)::value * decltype(l)::value * Cells<T>::N) return false;
+        f(u, l);
+        return true;
+    };
+    using std::integral_constant;
+    using U1 = integral_constant<int, 1>;
+    using U2 = integral_constant<int, 2>;
+    using U4 = integral_constant<int, 4>;
+    if (is(U1{}, integral_constant<int, 8>{}) || is(U1{}, integral_constant<int, 16>{}) || is(U1{}, integral_constant<int, 32>{}) ||
+        is(U1{}, integral_constant<int, 64>{}) || is(U2{}, integral_constant<int, 64>{}) || is(U1{}, integral_constant<int, 256>{}) ||
+        is(U2{}, integral_constant<int, 256>{}) || is(U4{}, integral_constant<int, 256>{}) || is(U2{}, integral_constant<int, 1024>{}))
+        return true;
+    if constexpr (sizeof(T) == 4) return is(U4{}, integral_constant<int, 1024>{});
+    return false;
+}
+// Work-groups of the backward pass, each of which leaves sums of dw and db: two of 256 threads per CU, four where their registers allow
+// it and each has rows enough for its sums to be few (us with two and four: 100000 rows of 384 79 and 55, 4096 of them 12 and 18;
+// 100000 of 600, in more registers, 95 and 103), or one of 1024.
+static int norm_groups(int64_t rows, int64_t d, int32_t elem) {
+    int64_t at_once = 1, most = 512;
+    const int n = elem == MSR_BF16 ? 8 : 4;
+    auto of = [&](auto u, auto l) {
+        constexpr int L = decltype(l)::value;
+        at_once = norm_threads(L) / L;
+        if (L > 256) most = 256;
+        if (L >= 32 && L <= 64 && decltype(u)::value * n <= 8 && rows >= 8 * 1024 * at_once) most = 1024;
+    };
+    if (elem == MSR_BF16) norm_shape<uint16_t>(d, of);
+    else norm_shape<float>(d, of);
+    return (int)std::min<int64_t>(std::max<int64_t>((rows + at_once - 1) / at_once, 1), most);
 }
 
 static int norm_check(const char *name, int64_t rows, int64_t d, int32_t elem, int32_t welem) {
@@ -360,25 +402,20 @@ static int norm_check(const char *name, int64_t rows, int64_t d, int32_t elem, i
 }
 
 template <typename T>
-static void norm_launch(const NormArgs &a, const NormPlan &p, hipStream_t s) {
-    const dim3 grid(grid_for(a.rows, 4 / p.w, 256 * 8));
-    auto go = [&](auto u, auto w) { hipLaunchKernelGGL((norm_kernel<T, decltype(u)::value, decltype(w)::value>), grid, dim3(256), 0, s, a); };
-    using I1 = std::integral_constant<int, 1>;
-    using I2 = std::integral_constant<int, 2>;
-    using I4 = std::integral_constant<int, 4>;
-    if (p.u == 0) hipLaunchKernelGGL(norm_long_kernel<T>, dim3(grid_for(a.rows, 1, 256 * 8)), dim3(256), 0, s, a);
-    else if (p.w == 1) p.u == 1 ? go(I1{}, I1{}) : go(I2{}, I1{});
-    else p.u == 1 ? go(I1{}, I4{}) : p.u == 2 ? go(I2{}, I4{}) : go(I4{}, I4{});
+static void norm_launch(const NormArgs &a, hipStream_t s) {
+    const bool held = norm_shape<T>(a.d, [&](auto u, auto l) {
+        constexpr int L = decltype(l)::value, TH = norm_threads(L);
+        hipLaunchKernelGGL((norm_kernel<T, decltype(u)::value, L>), dim3(grid_for(a.rows, TH / L, 256 * 2048 / TH)), dim3(TH), 0, s, a);
+    });
+    if (!held) hipLaunchKernelGGL(norm_long_kernel<T>, dim3(grid_for(a.rows, 1, 256 * 8)), dim3(256), 0, s, a);
 }
 template <typename T>
-static void norm_grad_launch(const NormArgs &a, const NormPlan &p, hipStream_t s) {
-    auto go = [&](auto u, auto w) { hipLaunchKernelGGL((norm_grad_kernel<T, decltype(u)::value, decltype(w)::value>), dim3(p.groups), dim3(256), 0, s, a); };
-    using I1 = std::integral_constant<int, 1>;
-    using I2 = std::integral_constant<int, 2>;
-    using I4 = std::integral_constant<int, 4>;
-    if (p.u == 0) hipLaunchKernelGGL(norm_long_grad_kernel<T>, dim3(p.groups), dim3(256), 0, s, a);
-    else if (p.w == 1) p.u == 1 ? go(I1{}, I1{}) : go(I2{}, I1{});
-    else p.u == 1 ? go(I1{}, I4{}) : p.u == 2 ? go(I2{}, I4{}) : go(I4{}, I4{});
+static void norm_grad_launch(const NormArgs &a, int groups, hipStream_t s) {
+    const bool held = norm_shape<T>(a.d, [&](auto u, auto l) {
+        constexpr int L = decltype(l)::value;
+        hipLaunchKernelGGL((norm_grad_kernel<T, decltype(u)::value, L>), dim3(groups), dim3(norm_threads(L)), 0, s, a);
+    });
+    if (!held) hipLaunchKernelGGL(norm_long_grad_kernel<T>, dim3(groups), dim3(256), 0, s, a);
 }
 
 }  // namespace msr
@@ -404,9 +441,8 @@ int msr_layer_norm(const void *x, int64_t ldx, const void *w, const void *b, flo
     if (rc) return rc;
     NormArgs a{};
     a.x = x; a.ldx = ldx; a.w = w; a.b = b; a.eps = eps; a.rows = rows; a.d = d; a.y = y; a.mean = mean; a.rstd = rstd; a.w32 = welem == MSR_F32;
-    const NormPlan p = norm_plan(rows, d, elem);
-    if (elem == MSR_BF16) norm_launch<uint16_t>(a, p, (hipStream_t)stream);
-    else norm_launch<float>(a, p, (hipStream_t)stream);
+    if (elem == MSR_BF16) norm_launch<uint16_t>(a, (hipStream_t)stream);
+    else norm_launch<float>(a, (hipStream_t)stream);
     return check_launch("norm_kernel");
 }
 
@@ -414,7 +450,7 @@ int msr_layer_norm_workspace_bytes(int64_t rows, int64_t d, int32_t elem, size_t
     const int rc = norm_check("msr_layer_norm_workspace_bytes", rows, d, elem, MSR_F32);
     if (rc) return rc;
     if (!bytes) { set_error("msr_layer_norm_workspace_bytes: a pointer is NULL"); return MSR_ERR_ARG; }
-    *bytes = (size_t)norm_plan(rows, d, elem).groups * 2 * (size_t)d * 4;
+    *bytes = (size_t)norm_groups(rows, d, elem) * 2 * (size_t)d * 4;
     return MSR_OK;
 }
 
@@ -431,8 +467,8 @@ int msr_layer_norm_grad(const void *dy, int64_t lddy, const void *x, int64_t ldx
         set_error("%s: operands must be aligned to their types", name);
         return MSR_ERR_ALIGN;
     }
-    const NormPlan p = norm_plan(rows, d, elem);
-    const size_t need = (size_t)p.groups * 2 * (size_t)d * 4, n = (size_t)rows;
+    const int all = norm_groups(rows, d, elem);
+    const size_t need = (size_t)all * 2 * (size_t)d * 4, n = (size_t)rows;
     if ((dw || db) && (!workspace || workspace_bytes < need)) {
         set_error("%s: workspace of %zu bytes is smaller than the %zu required", name, workspace_bytes, need);
         return MSR_ERR_WORKSPACE;
@@ -447,13 +483,13 @@ int msr_layer_norm_grad(const void *dy, int64_t lddy, const void *x, int64_t ldx
     a.mean = const_cast<float *>(mean); a.rstd = const_cast<float *>(rstd);
     a.parts = dw || db ? static_cast<float *>(workspace) : nullptr;
     if (rows > 0) {
-        if (elem == MSR_BF16) norm_grad_launch<uint16_t>(a, p, s);
-        else norm_grad_launch<float>(a, p, s);
+        if (elem == MSR_BF16) norm_grad_launch<uint16_t>(a, all, s);
+        else norm_grad_launch<float>(a, all, s);
         if ((rc = check_launch("norm_grad_kernel"))) return rc;
     }
     if (!a.parts) return MSR_OK;
     const dim3 grid((unsigned)((d + 31) / 32));
-    const int groups = rows > 0 ? p.groups : 0;
+    const int groups = rows > 0 ? all : 0;
     if (welem == MSR_BF16) hipLaunchKernelGGL(norm_join_kernel<uint16_t>, grid, dim3(256), 0, s, a.parts, groups, d, static_cast<uint16_t *>(dw), static_cast<uint16_t *>(db));
     else hipLaunchKernelGGL(norm_join_kernel<float>, grid, dim3(256), 0, s, a.parts, groups, d, static_cast<float *>(dw), static_cast<float *>(db));
     return check_launch("norm_join_kernel");

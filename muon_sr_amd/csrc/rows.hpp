@@ -99,6 +99,30 @@ __device__ __forceinline__ float2 wave_sum2(float x, float y) {
                        __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(v), 32)));
 }
 
+// Sums and maxima over groups of L = 8, 16, 32 or 64 lanes, in every lane of the group
+struct Add {
+    __device__ __forceinline__ float operator()(float a, float b) const { return a + b; }
+};
+struct Max {
+    __device__ __forceinline__ float operator()(float a, float b) const { return fmaxf(a, b); }
+};
+template <int L, typename Op>
+__device__ __forceinline__ float over_group(float x, Op op) {
+    x = op(x, turned<0xB1>(x));                        // quad_perm [1, 0, 3, 2]
+    x = op(x, turned<0x4E>(x));                        // quad_perm [2, 3, 0, 1]
+    x = op(x, turned<0x141>(x));                       // row_half_mirror
+    if constexpr (L >= 16) x = op(x, turned<0x140>(x));   // row_mirror
+    if constexpr (L >= 32) {
+        const auto q = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+        x = op(__uint_as_float(q[0]), __uint_as_float(q[1]));
+    }
+    if constexpr (L >= 64) {
+        const auto h = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+        x = op(__uint_as_float(h[0]), __uint_as_float(h[1]));
+    }
+    return x;
+}
+
 // A call's memory ranges, the first `outs` of them written: those overlap none of the others and not one another.
 struct Range {
     const void *p;

@@ -77,7 +77,8 @@ def near(got, want):
 
 @pytest.mark.parametrize("dtype,wdtype", [(BF16, BF16), (BF16, F32), (F32, F32), (F32, BF16)], ids=["bf16", "bf16-fp32", "fp32", "fp32-bf16"])
 @pytest.mark.parametrize("rows,d", [(1, 1), (1, 8), (5, 3), (7, 384), (33, 512), (300, 1000), (67, 1024), (2, 1025), (129, 2048), (17, 2049),
-                                    (65, 4096), (3, 5001), (12, 8192), (4, 8193), (5, 16384), (3, 20000), (700, 17), (5000, 64), (3001, 1400)])
+                                    (65, 4096), (3, 5001), (12, 8192), (4, 8193), (5, 16384), (3, 20000), (700, 17), (5000, 64), (3001, 1400), (33001, 384),
+                                    (1001, 128), (515, 256), (300, 12000), (260, 16383), (70, 16385), (65541, 200)])
 def test_against_64_bits(rows, d, dtype, wdtype):
     x, w, b, dy = make(rows, d, dtype, wdtype, rows + d)
     for got, want in zip(run(x, w, b, dy), exact(x, w, b, dy)):
