@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import random
 import threading
 
 import torch
@@ -193,7 +194,7 @@ def nodes():
             from . import _nodes as built
         except ImportError as e:
             raise MuonSRLibraryError(f"muon_sr_amd/_nodes.so cannot be loaded ({e}): build it with `python -m muon_sr_amd._build`") from e
-        built.set_error_type(MuonSRLibraryError)
+        built.set_python(MuonSRLibraryError, accumulator)
         _nodes = built
     return _nodes
 
@@ -283,3 +284,13 @@ def check_accumulator(weight: torch.Tensor, what: str) -> None:
     if not isinstance(acc, torch.Tensor) or acc.dtype != torch.bfloat16 or acc.shape != weight.shape or \
             acc.device != weight.device or not acc.is_contiguous():
         raise ValueError(f"{what} needs an acc_grad that is contiguous bf16 of its weight's shape and device")
+
+
+def accumulator(weight: torch.Tensor, what: str, seed: int = None):
+    """What a gradient of ``weight`` is accumulated into and with: the buffer, a seed (drawn if not given), whether the weight has none yet (the
+    buffer is new, and the caller gives it to the weight after its kernel's call), the noise mode."""
+    first = not hasattr(weight, "acc_grad")
+    if not first:
+        check_accumulator(weight, what)
+    acc = torch.empty_like(weight, memory_format=torch.contiguous_format) if first else weight.acc_grad
+    return acc, random.getrandbits(32) if seed is None else seed, first, noise_mode()

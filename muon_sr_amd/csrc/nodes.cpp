@@ -2,7 +2,7 @@
 //
 // A backward pass runs on a thread of torch's own, and what it costs beyond the kernels is that thread's start and the host
 // code that both threads come back to with cold caches: with the nodes in Python, layer_norm of 4096 x 384 and its gradients
-// took 117 us a pass of which the kernels are 21, and 66 so.  The operators' arguments are checked here, their kernels are called through the C
+// took 117 us a pass of which the kernels are 21, and 66 so; SRHead's loss of 128 rows, 6656 words of 1000 143 and 85.  The operators' arguments are checked here, their kernels are called through the C
 // ABI of libmuon_sr_amd.so on the tensors' device and its current stream, their scratch memory comes from torch's allocator.
 #include <torch/extension.h>
 
@@ -20,6 +20,7 @@ using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
 PyObject *library_error = nullptr;   // _lib.MuonSRLibraryError
+PyObject *accumulator = nullptr;     // _lib.accumulator
 
 void check(int rc, const char *name) {
     if (!rc) return;
@@ -38,6 +39,37 @@ void call(const Tensor &t, const char *name, F fn, Args... args) {
     const c10::DeviceGuard guard(t.device());
     check(fn(args..., (msr_stream_t)c10::hip::getCurrentHIPStream(t.device().index()).stream()), name);
 }
+
+// A weight's accumulator, as a backward pass finds it, and what it is accumulated with.
+struct Accumulator {
+    Tensor acc;
+    uint32_t seed;
+    int32_t noise_mode;
+    bool first;                          // the weight has none yet: acc's elements are undefined
+    // (the weight as Python has it: the accumulator is its attribute)
+    Accumulator(const Tensor &owner, const char *what) {
+        pybind11::gil_scoped_acquire gil;
+        PyObject *const r = PyObject_CallFunction(accumulator, "Ns", THPVariable_Wrap(owner), what);
+        if (!r) fail();
+        const auto t = pybind11::reinterpret_steal<pybind11::tuple>(r);
+        acc = THPVariable_Unpack(pybind11::object(t[0]).ptr());
+        seed = t[1].cast<uint32_t>();
+        first = t[2].cast<bool>();
+        noise_mode = t[3].cast<int32_t>();
+    }
+    // after the call that wrote it
+    void keep(const Tensor &owner) const {
+        if (!first) return;
+        pybind11::gil_scoped_acquire gil;
+        const auto to = pybind11::reinterpret_steal<pybind11::object>(THPVariable_Wrap(owner)), value = pybind11::reinterpret_steal<pybind11::object>(THPVariable_Wrap(acc));
+        if (PyObject_SetAttrString(to.ptr(), "acc_grad", value.ptr())) fail();
+    }
+    [[noreturn]] static void fail() {    // with Python's error
+        python_error e;
+        e.persist();
+        throw e;
+    }
+};
 
 const void *in(const Tensor &t) { return t.defined() ? t.const_data_ptr() : nullptr; }
 void *out(const Tensor &t) { return t.defined() ? t.mutable_data_ptr() : nullptr; }
@@ -149,8 +181,9 @@ Tensor layer_norm(const Tensor &x, const std::optional<Tensor> &weight, const st
 
 // ---------------------------------------------------------------------------
 
+// accumulate: the gradient goes to w.acc_grad
 struct Embedding : torch::autograd::Function<Embedding> {
-    static Tensor forward(AutogradContext *ctx, const Tensor &ids_, const Tensor &w, double scale, int64_t padding) {
+    static Tensor forward(AutogradContext *ctx, const Tensor &ids_, const Tensor &w, double scale, int64_t padding, bool accumulate) {
         const Tensor ids = ids_.contiguous();
         const int64_t vocab = w.size(0), d = w.size(1);
         auto shape = ids.sizes().vec();
@@ -161,19 +194,31 @@ struct Embedding : torch::autograd::Function<Embedding> {
         ctx->saved_data["scale"] = scale;
         ctx->saved_data["padding"] = padding;
         ctx->saved_data["vocab"] = vocab;
+        // the tensor that holds acc_grad: saved-tensor hooks (activation checkpointing, offloading) unpack another one
+        if (accumulate) ctx->saved_data["owner"] = w;
         return y;
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads) {
         const Tensor ids = ctx->get_saved_variables()[0].contiguous(), &dy = grads[0];
         const int64_t vocab = ctx->saved_data["vocab"].toInt(), d = dy.size(-1), n = ids.numel();
         const Rows r = flat_rows(dy, d);
-        const Tensor dw = empty({vocab, d}, dy, dy.scalar_type());
+        const auto owner = ctx->saved_data.find("owner");
         size_t bytes = 0;
         check(msr_embedding_workspace_bytes(n, vocab, d, &bytes), "msr_embedding_workspace_bytes");
-        const Tensor ws = workspace(bytes, dy);
+        if (owner != ctx->saved_data.end()) {
+            const Tensor w = owner->second.toTensor();
+            const Accumulator to(w, "SREmbedding");
+            const Tensor ws = workspace(bytes, dy);
+            call(dy, "msr_embedding_grad_sr_accum", msr_embedding_grad_sr_accum, in(ids), (int32_t)(ids.scalar_type() == at::kLong), n,
+                 static_cast<const uint16_t *>(in(r.t)), r.ld, vocab, d, (float)ctx->saved_data["scale"].toDouble(), ctx->saved_data["padding"].toInt(),
+                 at_<uint16_t>(to.acc), to.seed, (int32_t)to.first, to.noise_mode, (const uint16_t *)nullptr, out(ws), bytes);
+            to.keep(w);
+            return {Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+        }
+        const Tensor dw = empty({vocab, d}, dy, dy.scalar_type()), ws = workspace(bytes, dy);
         call(dy, "msr_embedding_grad", msr_embedding_grad, in(ids), (int32_t)(ids.scalar_type() == at::kLong), n, in(r.t), r.ld, vocab, d,
              (float)ctx->saved_data["scale"].toDouble(), ctx->saved_data["padding"].toInt(), out(dw), elem(dw), out(ws), bytes);
-        return once({Tensor(), dw, Tensor(), Tensor()});
+        return once({Tensor(), dw, Tensor(), Tensor(), Tensor()});
     }
 };
 
@@ -189,15 +234,17 @@ int64_t check_embedding(const char *what, const Tensor &ids, const Tensor &w, st
     TORCH_CHECK_VALUE(*padding >= -vocab && *padding < vocab, what, ": padding_idx ", *padding, " is outside the ", vocab, " words");
     return *padding < 0 ? *padding + vocab : *padding;
 }
-Tensor embedding(const Tensor &ids, const Tensor &w, std::optional<int64_t> padding, double scale) {
+// accumulate: w is a bf16 leaf that wants a gradient
+Tensor embedding(const Tensor &ids, const Tensor &w, std::optional<int64_t> padding, double scale, bool accumulate) {
     const int64_t pad = check_embedding("embedding", ids, w, padding);
-    return Embedding::apply(ids, w, scale, pad);
+    return Embedding::apply(ids, w, scale, pad, accumulate);
 }
 
 // ---------------------------------------------------------------------------
 
+// accumulate: the weight's gradient goes to w.acc_grad
 struct HeadLoss : torch::autograd::Function<HeadLoss> {
-    static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &w, const Tensor &target_, int64_t ignore, int64_t reduction) {
+    static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &w, const Tensor &target_, int64_t ignore, int64_t reduction, bool accumulate) {
         const int64_t vocab = w.size(0), d = w.size(1);
         const Rows r = flat_rows(x, d);
         const Tensor target = target_.contiguous(), packed = empty({r.n, d}, x, at::kBFloat16), kept = empty({3 * r.n + 1}, x, at::kInt),
@@ -211,6 +258,7 @@ struct HeadLoss : torch::autograd::Function<HeadLoss> {
         ctx->save_for_backward({packed, w, kept, lse});
         ctx->saved_data["shape"] = x.sizes().vec();
         ctx->saved_data["reduction"] = reduction;
+        if (accumulate) ctx->saved_data["owner"] = w;   // (as in Embedding)
         return loss;
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads) {
@@ -218,15 +266,25 @@ struct HeadLoss : torch::autograd::Function<HeadLoss> {
         const Tensor packed = packed_rows(saved[0]), w = packed_rows(saved[1]), kept = saved[2].contiguous(), lse = saved[3].contiguous(),
                      dloss = grads[0].contiguous();
         const int64_t n = packed.size(0), vocab = w.size(0), d = w.size(1), reduction = ctx->saved_data["reduction"].toInt();
-        const Tensor dx = ctx->needs_input_grad(0) ? empty(ctx->saved_data["shape"].toIntVector(), packed, at::kBFloat16) : Tensor(),
-                     dw = ctx->needs_input_grad(1) ? empty({vocab, d}, w, at::kBFloat16) : Tensor();
+        const Tensor dx = ctx->needs_input_grad(0) ? empty(ctx->saved_data["shape"].toIntVector(), packed, at::kBFloat16) : Tensor();
+        const auto owner = ctx->saved_data.find("owner");
         size_t forward_bytes = 0, bytes = 0;
         check(msr_head_workspace_bytes(n, vocab, d, &forward_bytes, &bytes), "msr_head_workspace_bytes");
-        const Tensor ws = workspace(bytes, packed);
+        if (owner != ctx->saved_data.end()) {
+            const Tensor weight = owner->second.toTensor();
+            const Accumulator to(weight, "SRHead");
+            const Tensor ws = workspace(bytes, packed);
+            call(packed, "msr_head_backward", msr_head_backward, static_cast<const uint16_t *>(in(packed)), static_cast<const uint16_t *>(in(w)),
+                 static_cast<const int32_t *>(in(kept)), static_cast<const float *>(in(lse)), static_cast<const float *>(in(dloss)), n, vocab, d,
+                 (int32_t)reduction, at_<uint16_t>(dx), at_<uint16_t>(to.acc), to.noise_mode, to.seed, (int32_t)to.first, (const uint16_t *)nullptr, out(ws), bytes);
+            to.keep(weight);
+            return once({dx, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()});
+        }
+        const Tensor dw = ctx->needs_input_grad(1) ? empty({vocab, d}, w, at::kBFloat16) : Tensor(), ws = workspace(bytes, packed);
         call(packed, "msr_head_backward", msr_head_backward, static_cast<const uint16_t *>(in(packed)), static_cast<const uint16_t *>(in(w)),
              static_cast<const int32_t *>(in(kept)), static_cast<const float *>(in(lse)), static_cast<const float *>(in(dloss)), n, vocab, d,
              (int32_t)reduction, at_<uint16_t>(dx), at_<uint16_t>(dw), -1, 0u, 0, (const uint16_t *)nullptr, out(ws), bytes);
-        return once({dx, dw, Tensor(), Tensor(), Tensor()});
+        return once({dx, dw, Tensor(), Tensor(), Tensor(), Tensor()});
     }
 };
 
@@ -243,9 +301,10 @@ int64_t check_head(const char *what, const Tensor &x, const Tensor &w, const Ten
     TORCH_CHECK_VALUE(d % 8 == 0 && d > 0 && w.size(0) > 0, what, " needs words, and a width that is a multiple of 8, got ", w.sizes());
     return code;
 }
-Tensor linear_cross_entropy(const Tensor &x, const Tensor &w, const Tensor &target, int64_t ignore, const std::string &reduction) {
-    const int64_t code = check_head("linear_cross_entropy", x, w, target, reduction);
-    return HeadLoss::apply(x, w, target, ignore, code);
+// accumulate: w is a leaf that wants a gradient
+Tensor linear_cross_entropy(const Tensor &x, const Tensor &w, const Tensor &target, int64_t ignore, const std::string &reduction, bool accumulate) {
+    const int64_t code = check_head(accumulate ? "SRHead" : "linear_cross_entropy", x, w, target, reduction);
+    return HeadLoss::apply(x, w, target, ignore, code, accumulate);
 }
 
 // ---------------------------------------------------------------------------
@@ -295,11 +354,13 @@ std::tuple<Tensor, Tensor> balance_loss(const Tensor &logits, const Tensor &ids,
 }  // namespace
 
 PYBIND11_MODULE(_nodes, m) {
-    m.def("set_error_type", [](pybind11::object type) { library_error = type.release().ptr(); });
+    m.def("set_python", [](pybind11::object error_type, pybind11::object accumulator_) {
+        library_error = error_type.release().ptr();
+        accumulator = accumulator_.release().ptr();
+    });
     m.def("layer_norm", torch::wrap_pybind_function(layer_norm));
     m.def("check_embedding", torch::wrap_pybind_function([](const std::string &what, const Tensor &ids, const Tensor &w, std::optional<int64_t> padding) { return check_embedding(what.c_str(), ids, w, padding); }));
     m.def("embedding", torch::wrap_pybind_function(embedding));
-    m.def("check_head", torch::wrap_pybind_function([](const std::string &what, const Tensor &x, const Tensor &w, const Tensor &target, const std::string &reduction) { return check_head(what.c_str(), x, w, target, reduction); }));
     m.def("linear_cross_entropy", torch::wrap_pybind_function(linear_cross_entropy));
     m.def("balance_loss", torch::wrap_pybind_function(balance_loss));
 }

@@ -11,61 +11,20 @@ same bits.  The reference's training loops call torch's embedding.
 from __future__ import annotations
 
 import ctypes
-import random
 
 import torch
 
 from . import _lib
-from .experts import _once, _one_gpu
-from .head import _flat_rows
+from .experts import _one_gpu
 
 __all__ = ["embedding", "embedding_grad_sr_accum", "SREmbedding"]
-
-
-def _grad_args(ids, dy, vocab, d, scale, padding):
-    """The entry points' first arguments, the tensors that they point to, and the workspace."""
-    ids = ids.contiguous()
-    dy, ld = _flat_rows(dy, d)
-    size = ctypes.c_size_t()
-    _lib.check(_lib.lib().msr_embedding_workspace_bytes(ids.numel(), vocab, d, ctypes.byref(size)), "msr_embedding_workspace_bytes")
-    ws = _lib.workspace(dy, size.value)
-    return (ids.data_ptr(), int(ids.dtype == torch.int64), ids.numel(), dy.data_ptr(), ld, vocab, d, scale, padding), (ids, dy), ws, size.value
-
-
-def _accumulate(weight, ids, dy, scale, padding, seed):
-    vocab, d = weight.shape
-    first = not hasattr(weight, "acc_grad")
-    if not first:
-        _lib.check_accumulator(weight, "embedding_grad_sr_accum")
-    if seed is None:
-        seed = random.getrandbits(32)
-    acc = torch.empty_like(weight, memory_format=torch.contiguous_format) if first else weight.acc_grad
-    args, keep, ws, size = _grad_args(ids, dy, vocab, d, scale, padding)
-    _lib.call(weight, "msr_embedding_grad_sr_accum", *args, acc.data_ptr(), seed, int(first), _lib.noise_mode(), None, _lib.ptr(ws), size)
-    if first:
-        weight.acc_grad = acc
-
-
-class _Accumulating(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, ids, weight, scale, padding_idx):
-        ctx.save_for_backward(ids)
-        # the tensor that holds acc_grad: saved-tensor hooks (activation checkpointing, offloading) would unpack another one
-        ctx.owner, ctx.scale, ctx.padding_idx = weight, scale, padding_idx
-        return _lib.nodes().embedding(ids, weight, padding_idx, scale)
-
-    @staticmethod
-    @_once
-    def backward(ctx, dy):
-        embedding_grad_sr_accum(ctx.owner, *ctx.saved_tensors, dy, ctx.padding_idx, ctx.scale)
-        return None, None, None, None
 
 
 def embedding(ids: torch.Tensor, weight: torch.Tensor, padding_idx: int = None, scale: float = 1.0) -> torch.Tensor:
     """``scale * weight[ids]``, rounded once, as [*ids.shape, d].  ``weight``: bf16 or fp32 [vocab, d]; ``ids``: int32 or int64; one
     outside [0, vocab) has no word: its row is 0 and gives no gradient.  ``padding_idx`` gives none either (its row is
     looked up as any other).  The gradient goes to autograd, whole; ``SREmbedding`` adds it to its accumulator."""
-    return _lib.nodes().embedding(ids, weight, padding_idx, scale)
+    return _lib.nodes().embedding(ids, weight, padding_idx, scale, False)
 
 
 def embedding_grad_sr_accum(weight: torch.Tensor, ids: torch.Tensor, dy: torch.Tensor, padding_idx: int = None,
@@ -80,7 +39,18 @@ def embedding_grad_sr_accum(weight: torch.Tensor, ids: torch.Tensor, dy: torch.T
         raise ValueError(f"embedding_grad_sr_accum needs bf16 tensors, got {weight.dtype} and {dy.dtype}")
     if dy.shape != (*ids.shape, weight.shape[1]):
         raise ValueError(f"embedding_grad_sr_accum needs dy of shape {(*ids.shape, weight.shape[1])}, got {tuple(dy.shape)}")
-    _accumulate(weight, ids, dy, float(scale), padding, seed)
+    vocab, d = weight.shape
+    acc, drawn, first, noise = _lib.accumulator(weight, "embedding_grad_sr_accum", seed)
+    ids, dy = ids.contiguous(), dy.reshape(ids.numel(), d)
+    if len(dy) <= 1 or (d > 1 and dy.stride(1) != 1) or dy.stride(0) < d:
+        dy = dy.contiguous()
+    size = ctypes.c_size_t()
+    _lib.check(_lib.lib().msr_embedding_workspace_bytes(len(dy), vocab, d, ctypes.byref(size)), "msr_embedding_workspace_bytes")
+    ws = _lib.workspace(dy, size.value)
+    _lib.call(weight, "msr_embedding_grad_sr_accum", ids.data_ptr(), int(ids.dtype == torch.int64), len(dy), dy.data_ptr(),
+              max(d, dy.stride(0)), vocab, d, float(scale), padding, acc.data_ptr(), drawn, int(first), noise, None, _lib.ptr(ws), size.value)
+    if first:
+        weight.acc_grad = acc
 
 
 class SREmbedding(torch.nn.Embedding):
@@ -98,9 +68,8 @@ class SREmbedding(torch.nn.Embedding):
         weight = self.weight
         # a weight that is computed (a parametrization) holds nothing that lasts, and one that is not bf16 has no accumulator: autograd
         # gets the gradient
-        if weight.is_leaf and weight.dtype == torch.bfloat16 and weight.requires_grad and torch.is_grad_enabled():
-            return _Accumulating.apply(ids, weight, self.scale, self.padding_idx)
-        return embedding(ids, weight, self.padding_idx, self.scale)
+        accumulate = weight.is_leaf and weight.dtype == torch.bfloat16 and weight.requires_grad and torch.is_grad_enabled()
+        return _lib.nodes().embedding(ids, weight, self.padding_idx, self.scale, accumulate)
 
     def extra_repr(self):
         return super().extra_repr() + (f", scale={self.scale}" if self.scale != 1.0 else "")
