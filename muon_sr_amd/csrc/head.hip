@@ -3,11 +3,13 @@
 //     G[n][v] = g[n] (exp(S[n][v] - l[n]) - [v = t[n]]),   dx = G W,   dW = G^T x
 // with g[n] the gradient of loss[n].  S is never in memory: the forward pass keeps the maximum and the sum of each row of each
 // tile, the backward pass forms S again, piece by piece of the vocabulary, and stores the piece's G as the bf16 operand of
-// the two products that follow, as G / c: c is the significand of the first row's g (every row's, but for the reduction "none"), by
-// which the products' sums are multiplied in fp32.  The target's element of an unlikely word is -g, a factor of its whole row:
-// rounded with g, every such row would be off by the same share, up to 2^-8 (8192 rows, 128256 words of 4096, gradients against 64 bits:
-// 0.0021 or, at an unlucky g, 0.0030, and 0.0018 so at any; 0.0017 is the rounding of the results).  8 rows vocab d flop with gradients where 6 are the least; the logits kept in fp32 would be 4.2 GB
+// the two products that follow.  8 rows vocab d flop with gradients where 6 are the least; the logits kept in fp32 would be 4.2 GB
 // for 8192 rows of 128256 words.
+//
+// What is stored is G / c: c is the significand of the first row's g (every row's, but for the reduction "none"), by which the products'
+// sums are multiplied in fp32.  The target's element of an unlikely word is -g, a factor of its whole row: rounded with g, every such
+// row would be off by the same share, up to 2^-8 (8192 rows, 128256 words of 4096, gradients against 64 bits: 0.0021 or, at an unlucky
+// g, 0.0030, and 0.0018 so at any; 0.0017 is the rounding of the results).
 //
 // Rows that are ignored take part in nothing: list_kernel numbers the others, pack_kernel lays them out one after the
 // other (kept for the backward pass in x's place), and every kernel after it works on *count rows.  What an ignored row holds,

@@ -2,8 +2,9 @@
 //
 // A backward pass runs on a thread of torch's own, and what it costs beyond the kernels is that thread's start and the host
 // code that both threads come back to with cold caches: with the nodes in Python, layer_norm of 4096 x 384 and its gradients
-// took 117 us a pass of which the kernels are 21, and 66 so; SRHead's loss of 128 rows, 6656 words of 1000 143 and 85.  The operators' arguments are checked here, their kernels are called through the C
-// ABI of libmuon_sr_amd.so on the tensors' device and its current stream, their scratch memory comes from torch's allocator.
+// took 117 us a pass of which the kernels are 21, and 66 so; SRHead's loss of 128 rows, 6656 words of 1000 143 and 85.  The
+// operators' arguments are checked here, their kernels are called through the C ABI of libmuon_sr_amd.so on the tensors' device and
+// its current stream, their scratch memory comes from torch's allocator.
 #include <torch/extension.h>
 
 #include <c10/core/DeviceGuard.h>
