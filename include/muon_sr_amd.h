@@ -486,7 +486,9 @@ int msr_experts_wgrad_sr_accum(uint16_t *acc, const uint16_t *x, int64_t ldx, co
  * other target outside [0, vocab) makes its loss NaN, and with it the gradients.
  * reduction: MSR_LOSS_NONE (loss [rows]), _SUM or _MEAN over the rows that are not
  * ignored (loss [1]; 0 where there are none).  Products are of bf16 operands with
- * fp32 accumulation (G rounded to bf16), dx and dW rounded once.
+ * fp32 accumulation, dx and dW rounded once.  G is rounded to bf16, without the significand of
+ * the first row's dloss; of up to 32 rows (128 with MSR_LOSS_NONE) it is kept as two bf16 numbers.
+ * Logits of a magnitude below 2^127.
  *
  * msr_head_forward also writes what the backward pass reads: packed (bf16
  * [rows][d], 16-byte aligned: the rows that are not ignored, one after the other), kept
@@ -519,7 +521,7 @@ int msr_head_backward(const uint16_t *packed, const uint16_t *w, const int32_t *
  *   msr_embedding_grad_sr_accum   acc[v] <- SR(acc[v] + f32(bf16(dw[v]))) with the arithmetic and noise of
  *                                 msr_sr_accum on [vocab][d]; words without a token are not touched (with
  *                                 zero_init they are set to 0)
- * Sums in fp32, in an order that depends on the ids alone.  Ids outside [0, vocab) and the id
+ * Sums in fp32, in an order that depends on the ids and sizes alone, the same for both.  Ids outside [0, vocab) and the id
  * `padding` (negative: none) give no gradient.  ids: int32, or int64 with ids_i64; W, y, dy, dw: elem
  * (MSR_BF16 or MSR_F32), contiguous but for dy's row stride lddy; aligned to their
  * types.  Fewer than 2^28 tokens and 2^27 words.  workspace:

@@ -17,9 +17,10 @@ constexpr int SORT_THREADS = 1024, SORT_EACH = 2, SORT_RUN = SORT_THREADS * SORT
 constexpr int SORT_LOG = 11, MERGE_LOG = 5, MERGE_WAYS = 1 << MERGE_LOG;
 static_assert(SORT_RUN == 1 << SORT_LOG, "runs are searched by halves");
 constexpr int SORT_WAVES = SORT_THREADS / 64, SORT_BITS = 9;    // bits of a pass at most
-// Sorted tokens of a wave: 32 where as many rows as tokens, or more, are zeroed meanwhile, else 16, which shortens each wave's chain of
-// rows (us of sums and join: 16384 tokens, 128256 words of 4096, all of dW written, 216 with 32 and 235 with 16; accumulated into 32000
-// words of 2048, 42 and 37).
+// Sorted tokens of a wave: 32 where the words are many, whose zeroing is most of a whole dW's work, else 16, which shortens each wave's
+// chain of rows (us of sums and join with 32 and with 16: 16384 tokens, 128256 words of 4096, all of dW written, 216 and 235; 32000 words
+// of 2048, written 38 and 45, accumulated 40 and 34).  The same for a stored gradient and an accumulated one: their sums have the same
+// bits.
 constexpr int CHUNK_MIN = 16, CHUNK_MAX = 32;
 // Tokens that are not sorted, at most.  us of accumulating 500 tokens, sorted and not: of 2000 words of 512 20 and 9; of 4096, half of them
 // padding, 23 and 31; all of one word, which one wave adds up, FEW_AHEAD rows in flight, 18 and 55.  1000 tokens of one word would take
@@ -555,7 +556,7 @@ static int embed_sums(EmbedArgs a, hipStream_t s) {
     constexpr int WIDTH = 64 * Cells<T>::N;
     const int64_t pieces = (a.d + WIDTH - 1) / WIDTH;
     const bool few = a.n <= FEW, zero = MODE < 0 || a.zero_init;
-    a.chunk = zero && a.vocab >= a.n ? CHUNK_MAX : CHUNK_MIN;
+    a.chunk = a.vocab >= 4 * a.n ? CHUNK_MAX : CHUNK_MIN;
     const int64_t chunks = (a.n + a.chunk - 1) / a.chunk;
     const int words = few ? 8 : zero_words(a.vocab, pieces);
     const int64_t sums = (few ? a.n : chunks) * pieces, zeros = zero ? ((int64_t)a.vocab + words - 1) / words * pieces : 0;

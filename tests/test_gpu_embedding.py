@@ -173,6 +173,30 @@ def test_accumulated(L, n, vocab, d, noise):
         M.set_sr_noise(was)
 
 
+@pytest.mark.parametrize("n,vocab,d", [(3000, 3500, 512), (3000, 20000, 512), (5000, 700, 520)])
+def test_accumulated_sums_have_the_order_of_the_stored_ones(L, n, vocab, d):
+    """A word whose partial sums are thousands of times as large as their end, so that another order would give other bits: accumulating into a
+    buffer that is there gives what the stored gradient and msr_sr_accum give."""
+    from muon_sr_amd import _lib, embedding_grad_sr_accum
+    g = gen(9)
+    ids = torch.randint(0, vocab, (n,), generator=g, device=DEV)
+    ids[torch.rand(n, generator=g, device=DEV) < 0.5] = 3
+    dy = torch.randn((n, d), generator=g, device=DEV).to(BF16)
+    same = (ids == 3).nonzero().flatten()
+    m = len(same) // 3
+    dy[same[:m]] *= 4096
+    dy[same[m:2 * m]] = -dy[same[:m]]
+    w = torch.nn.Parameter(torch.zeros((vocab, d), dtype=BF16, device=DEV))
+    dw = run(ids, w, dy)[1]
+    want = torch.randn((vocab, d), generator=g, device=DEV).to(BF16)
+    w.acc_grad = want.clone()
+    embedding_grad_sr_accum(w, ids, dy, seed=5)
+    check(L, L.msr_sr_accum(want.data_ptr(), dw.data_ptr(), 0, dw.numel(), 5, 0, _lib.noise_mode(), None, stream()))
+    hit = torch.zeros(vocab, dtype=torch.bool, device=DEV)
+    hit[ids] = True
+    assert torch.equal(w.acc_grad[hit], want[hit])
+
+
 def test_refusals_and_other_weights():
     import muon_sr_amd as M
     ids, w, dy = make(30, 40, 16, BF16, 5)
