@@ -58,7 +58,7 @@ constexpr int norm_threads(int L) { return L > 256 ? L : 256; }
 
 // U cells per lane, L lanes per row: few lanes to a short row, so that a wave holds up to eight (us, forward and gradient, a wave to a
 // row and so: 131072 rows of 64 46 92, 12 16; of 128 47 94, 23 24), 1024 to a long one (rows read as often as they are needed, and so: 8000
-// rows of 16384 501 1312, 122 223; 3000 fp32 rows of 16000 144 449, 83 167).
+// rows of 16384 501 1312, 122 207; 3000 fp32 rows of 16000 144 449, 84 125).
 template <typename T, int U, int L>
 __global__ __launch_bounds__(norm_threads(L)) void norm_kernel(NormArgs a) {
     using C = Cells<T>;
@@ -127,7 +127,7 @@ __global__ __launch_bounds__(norm_threads(L)) void norm_grad_kernel(NormArgs a) 
     using C = Cells<T>;
     constexpr int N = C::N, ROWS = norm_threads(L) / L;
     // the next row on its way meanwhile: not where its registers, of 128 that a thread of 1024 has, cost more (us with it and without:
-    // 3000 fp32 rows of 16000 236 and 167, bf16 8000 of 16384 223 and 234, fp32 4000 of 8192 69 and 71)
+    // 3000 fp32 rows of 16000 236 and 156, bf16 8000 of 16384 223 and 234, fp32 4000 of 8192 69 and 71)
     constexpr bool AHEAD = L <= 256 || sizeof(T) == 2 || U * N <= 8;
     __shared__ float2 lds[2][RowSum<L>::WAVES];
     RowSum<L> sums{lds};
@@ -375,9 +375,9 @@ static bool norm_shape(int64_t d, F &&f) {
     if constexpr (sizeof(T) == 4) return is(U4{}, integral_constant<int, 1024>{});
     return false;
 }
-// Work-groups of the backward pass, each of which leaves sums of dw and db: two of 256 threads per CU, four where their registers allow
-// it and each has rows enough for its sums to be few (us with two and four: 100000 rows of 384 79 and 55, 4096 of them 12 and 18;
-// 100000 of 600, in more registers, 95 and 103), or one of 1024.
+// Work-groups of the backward pass, each of which leaves sums of dw and db: two of 256 threads per CU, or one of 1024.  Four, where their
+// registers allow it, for rows that leave lanes without a cell, if each has rows enough for its sums to be few (us with two and four:
+// 100000 rows of 448 70 and 54, of 512 53 and 60; 32768 of 1400 90 and 66, of 2048 77 and 82; 4096 of 384 12 and 18).
 static int norm_groups(int64_t rows, int64_t d, int32_t elem) {
     int64_t at_once = 1, most = 512;
     const int n = elem == MSR_BF16 ? 8 : 4;
@@ -385,7 +385,7 @@ static int norm_groups(int64_t rows, int64_t d, int32_t elem) {
         constexpr int L = decltype(l)::value;
         at_once = norm_threads(L) / L;
         if (L > 256) most = 256;
-        if (L >= 32 && L <= 64 && decltype(u)::value * n <= 8 && rows >= 8 * 1024 * at_once) most = 1024;
+        if (L >= 32 && L <= 256 && decltype(u)::value * n <= 8 && d < L * decltype(u)::value * n && rows >= 8 * 1024 * at_once) most = 1024;
     };
     if (elem == MSR_BF16) norm_shape<uint16_t>(d, of);
     else norm_shape<float>(d, of);

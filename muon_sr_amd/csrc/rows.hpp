@@ -24,6 +24,8 @@ struct Cells {
     __device__ __forceinline__ void load(const T *row, int64_t c, int64_t d) {
         if (c + N <= d) {
             v = *reinterpret_cast<const Bytes16 *>(row + c);
+        } else if (c >= d) {             // (of a row of whole cells no lane goes through its elements)
+            v = Bytes16{};
         } else {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -42,7 +44,7 @@ struct Cells {
         if (c + N <= d) {
             if constexpr (NT) st_nt16(row + c, v);
             else *reinterpret_cast<Bytes16 *>(row + c) = v;
-        } else {
+        } else if (c < d) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 if constexpr (sizeof(T) == 2) {
