@@ -493,7 +493,8 @@ int msr_experts_wgrad_sr_accum(uint16_t *acc, const uint16_t *x, int64_t ldx, co
  * msr_head_forward also writes what the backward pass reads: packed (bf16
  * [rows][d], 16-byte aligned: the rows that are not ignored, one after the other), kept
  * (int32 [3 * rows + 1]: their number, their places in x, their targets, and every
- * row's place in packed, or -1) and lse (fp32 [rows], packed order).
+ * row's place in packed, or -1) and sums (fp32 [rows][2], packed order, 8-byte aligned:
+ * M and s with l = M ln 2 + log s).
  * msr_head_backward: dloss fp32 [rows] with MSR_LOSS_NONE, else [1].  dx [rows][d]
  * or dw [vocab][d] may be NULL (not wanted).  noise_mode -1 stores dw; a noise mode
  * accumulates dw <- SR(dw + f32(bf16(dW))) with the arithmetic and noise of
@@ -508,8 +509,8 @@ int msr_experts_wgrad_sr_accum(uint16_t *acc, const uint16_t *x, int64_t ldx, co
 int msr_head_workspace_bytes(int64_t rows, int64_t vocab, int64_t d, size_t *forward, size_t *backward);
 int msr_head_forward(const uint16_t *x, int64_t ldx, const uint16_t *w, const void *target, int32_t target_i64,
                      int64_t ignore_index, int64_t rows, int64_t vocab, int64_t d, int32_t reduction, uint16_t *packed,
-                     int32_t *kept, float *lse, float *loss, void *workspace, size_t workspace_bytes, msr_stream_t stream);
-int msr_head_backward(const uint16_t *packed, const uint16_t *w, const int32_t *kept, const float *lse, const float *dloss,
+                     int32_t *kept, float *sums, float *loss, void *workspace, size_t workspace_bytes, msr_stream_t stream);
+int msr_head_backward(const uint16_t *packed, const uint16_t *w, const int32_t *kept, const float *sums, const float *dloss,
                       int64_t rows, int64_t vocab, int64_t d, int32_t reduction, uint16_t *dx, uint16_t *dw,
                       int32_t noise_mode, uint32_t seed, int32_t zero_init, const uint16_t *inject, void *workspace,
                       size_t workspace_bytes, msr_stream_t stream);

@@ -22,14 +22,14 @@ namespace msr {
 
 constexpr int HEAD_NONE = 0, HEAD_SUM = 1, HEAD_MEAN = 2;
 constexpr int HEAD_BAD = -1;                 // a row whose target is no word
-constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 struct HeadArgs {
     const uint16_t *x;           // [rows][d], packed: the rows that are not ignored
     const uint16_t *w;           // [vocab][d]
     const int32_t *kept;         // count, then rows numbers of rows, then their words
-    float *lse;                  // [rows], in the packed order
-    float2 *part;                // [tiles of words][rows]: a tile's maximum and sum
+    float2 *sums;                // [rows], in the packed order: M and s of the row
+    float2 *part;                // [tiles of words][rows]: of a tile
     float *picked;               // [rows]: S[n][t[n]]
     const float *dloss;          // [rows] in the given order, or one
     uint16_t *g;                 // [rows][ldg]: a piece of G / c; [2][rows][ldg] with lo
@@ -80,14 +80,15 @@ __device__ __forceinline__ bool find_tile(int v, int tiles_m, int tiles_n, int s
     return true;
 }
 
-// exp(x - m) as exp2(x log2(e) - m log2(e)): the rounding of m's product is common to a row's terms, and no larger than
-// that of the row's logits
-__device__ __forceinline__ float exp_from(float x, float neg_m2) { return __builtin_amdgcn_exp2f(__builtin_fmaf(x, LOG2E, neg_m2)); }
+// A set of logits is held as M, a number near the largest times log2(e), and s = sum exp2(x log2(e) - M): one multiply-add per
+// exponential, and M is exact, whatever it was rounded from.  l = M ln 2 + log s is never formed: an l of 40 is rounded by 2^-19, and with it
+// the gradient of a row whose word is nearly sure, and its loss.
+__device__ __forceinline__ float exp_from(float x, float M) { return __builtin_amdgcn_exp2f(__builtin_fmaf(x, LOG2E, -M)); }
 
-// (m, s) of the union of two sets, s = sum exp(x - m); an empty set is (-inf, 0)
+// (M, s) of the union of two sets; an empty set is (-inf, 0)
 __device__ __forceinline__ float2 joined(float2 a, float2 b) {
     const float m = fmaxf(a.x, b.x), at = m == -INFINITY ? 0.0f : m;
-    return make_float2(m, a.y * __builtin_amdgcn_exp2f((a.x - at) * LOG2E) + b.y * __builtin_amdgcn_exp2f((b.x - at) * LOG2E));
+    return make_float2(m, a.y * __builtin_amdgcn_exp2f(a.x - at) + b.y * __builtin_amdgcn_exp2f(b.x - at));
 }
 
 // ---------------------------------------------------------------------------
@@ -211,17 +212,19 @@ __global__ __launch_bounds__(64 * Shape<T>::NW, 2) void logits_kernel(HeadArgs a
         const int m0 = mt * T, n0 = nt * T;
         // what the epilogue needs of the lane's rows, loaded ahead of the products
         int word[FM];
-        float lse[FM], slope[FM];
+        float M[FM], slope[FM], share[FM];                    // share: slope / s
 #pragma unroll
         for (int i = 0; i < FM; ++i) {
             const int row = m0 + wm * SH::TM + 32 * i + (lane & 31);
             word[i] = HEAD_BAD;
-            lse[i] = slope[i] = 0.0f;
+            M[i] = slope[i] = share[i] = 0.0f;
             if (row < count) {
                 word[i] = word_of(a, row);
                 if constexpr (GRAD) {
-                    lse[i] = a.lse[row];
+                    const float2 sums = a.sums[row];
+                    M[i] = sums.x;
                     slope[i] = slope_of(a, row, count, unit);
+                    share[i] = slope[i] / sums.y;
                 }
             }
         }
@@ -256,7 +259,8 @@ __global__ __launch_bounds__(64 * Shape<T>::NW, 2) void logits_kernel(HeadArgs a
 #pragma unroll
                     for (int x = 0; x < 16; ++x) m = fmaxf(m, pr.acc[i][j][x]);
                 m = fmaxf(m, __shfl_xor(m, 32));
-                const float at = m == -INFINITY ? 0.0f : -m * LOG2E;
+                m = m == -INFINITY ? m : m * LOG2E;
+                const float at = m == -INFINITY ? 0.0f : m;
                 float s = 0.0f;
 #pragma unroll
                 for (int j = 0; j < FN; ++j)
@@ -289,12 +293,12 @@ __global__ __launch_bounds__(64 * Shape<T>::NW, 2) void logits_kernel(HeadArgs a
             const int crow = elane / WC, cchk = elane % WC, nc = n0 + wn * TN + 8 * cchk;
 #pragma unroll
             for (int i = 0; i < FM; ++i) {
-                const float g = slope[i], l = -lse[i] * LOG2E;
+                const float g = slope[i];
                 const int rel = word[i] - a.v0 - nw;
 #pragma unroll
                 for (int j = 0; j < FN; ++j)
 #pragma unroll
-                    for (int x = 0; x < 16; ++x) pr.acc[i][j][x] = g * exp_from(pr.acc[i][j][x], l);
+                    for (int x = 0; x < 16; ++x) pr.acc[i][j][x] = share[i] * exp_from(pr.acc[i][j][x], M[i]);
                 if (__any(rel >= 0 && rel < TN && !(rel & 4))) {
 #pragma unroll
                     for (int j = 0; j < FN; ++j)
@@ -333,7 +337,7 @@ __global__ __launch_bounds__(64 * Shape<T>::NW, 2) void logits_kernel(HeadArgs a
     }
 }
 
-// l[n] and the losses of 16 rows from their tiles' parts, 16 threads each
+// The sums and losses of 16 rows from their tiles' parts, 16 threads each
 __device__ __forceinline__ void join_rows(const HeadArgs &a, float *loss, int n0, int count, float2 (&part)[16][17]) {
     const int r = threadIdx.x & 15, g = threadIdx.x >> 4, n = n0 + r;
     float2 v = make_float2(-INFINITY, 0.0f);
@@ -343,9 +347,9 @@ __device__ __forceinline__ void join_rows(const HeadArgs &a, float *loss, int n0
     __syncthreads();
     if (g == 0 && n < count) {
         for (int k = 1; k < 16; ++k) v = joined(v, part[k][r]);
-        const float l = v.x + logf(v.y);
-        a.lse[n] = l;
-        loss[a.reduction == HEAD_NONE ? a.kept[1 + n] : n] = word_of(a, n) == HEAD_BAD ? __builtin_nanf("") : l - a.picked[n];
+        a.sums[n] = v;
+        const float l = logf(v.y) + LN2 * __builtin_fmaf(a.picked[n], -LOG2E, v.x);
+        loss[a.reduction == HEAD_NONE ? a.kept[1 + n] : n] = word_of(a, n) == HEAD_BAD ? __builtin_nanf("") : l;
     }
     __syncthreads();
 }
@@ -719,19 +723,19 @@ int msr_head_plan(int64_t rows, int64_t vocab, int64_t d, int32_t *plan) {
 }
 
 int msr_head_forward(const uint16_t *x, int64_t ldx, const uint16_t *w, const void *target, int32_t target_i64, int64_t ignore_index,
-                     int64_t rows, int64_t vocab, int64_t d, int32_t reduction, uint16_t *packed, int32_t *kept, float *lse,
+                     int64_t rows, int64_t vocab, int64_t d, int32_t reduction, uint16_t *packed, int32_t *kept, float *sums,
                      float *loss, void *workspace, size_t workspace_bytes, msr_stream_t stream) {
     const char *const name = "msr_head_forward";
     int rc = head_check(name, rows, vocab, d);
     if (rc) return rc;
-    if (reduction < HEAD_NONE || reduction > HEAD_MEAN || !w || !kept || (rows > 0 && (!x || !target || !packed || !lse)) ||
+    if (reduction < HEAD_NONE || reduction > HEAD_MEAN || !w || !kept || (rows > 0 && (!x || !target || !packed || !sums)) ||
         ((rows > 0 || reduction != HEAD_NONE) && !loss) || ldx < d) {
         set_error("%s: bad arguments", name);
         return MSR_ERR_ARG;
     }
     if (!aligned(x, 2) || !aligned(w, 16) || !aligned(packed, 16) || !aligned(target, target_i64 ? 8 : 4) || !aligned(kept, 4) ||
-        !aligned(lse, 4) || !aligned(loss, 4) || !aligned(workspace, 16)) {
-        set_error("%s: w, packed and the workspace must be 16-byte aligned, the others to their types", name);
+        !aligned(sums, 8) || !aligned(loss, 4) || !aligned(workspace, 16)) {
+        set_error("%s: w, packed and the workspace must be 16-byte aligned, sums 8-byte aligned, the others to their types", name);
         return MSR_ERR_ALIGN;
     }
     const HeadPlan p = head_plan(rows, vocab, d, reduction);
@@ -741,7 +745,7 @@ int msr_head_forward(const uint16_t *x, int64_t ldx, const uint16_t *w, const vo
         return MSR_ERR_WORKSPACE;
     }
     const size_t n = (size_t)rows;
-    const Range r[8] = {{packed, 2 * n * (size_t)d}, {kept, 4 * (3 * n + 1)}, {lse, 4 * n}, {loss, reduction == HEAD_NONE ? 4 * n : 4},
+    const Range r[8] = {{packed, 2 * n * (size_t)d}, {kept, 4 * (3 * n + 1)}, {sums, 8 * n}, {loss, reduction == HEAD_NONE ? 4 * n : 4},
                         {workspace, rows ? p.fwd_bytes : 0}, {x, rows ? 2 * ((n - 1) * (size_t)ldx + (size_t)d) : 0},
                         {w, 2 * (size_t)vocab * (size_t)d}, {target, n * (target_i64 ? 8 : 4)}};
     rc = ranges_apart(name, r, 8, 5);
@@ -750,7 +754,7 @@ int msr_head_forward(const uint16_t *x, int64_t ldx, const uint16_t *w, const vo
     const int64_t tn = (vocab + T - 1) / T, tiles = (rows + T - 1) / T * tn;
     hipStream_t s = (hipStream_t)stream;
     HeadArgs a{};
-    a.x = packed; a.w = w; a.kept = kept; a.lse = lse;
+    a.x = packed; a.w = w; a.kept = kept; a.sums = reinterpret_cast<float2 *>(sums);
     a.part = static_cast<float2 *>(workspace);
     char *const after = static_cast<char *>(workspace) + up256((size_t)tn * n * 8);
     a.picked = reinterpret_cast<float *>(after);
@@ -780,21 +784,21 @@ int msr_head_forward(const uint16_t *x, int64_t ldx, const uint16_t *w, const vo
     return rc;
 }
 
-int msr_head_backward(const uint16_t *packed, const uint16_t *w, const int32_t *kept, const float *lse, const float *dloss,
+int msr_head_backward(const uint16_t *packed, const uint16_t *w, const int32_t *kept, const float *sums, const float *dloss,
                       int64_t rows, int64_t vocab, int64_t d, int32_t reduction, uint16_t *dx, uint16_t *dw, int32_t noise_mode,
                       uint32_t seed, int32_t zero_init, const uint16_t *inject, void *workspace, size_t workspace_bytes,
                       msr_stream_t stream) {
     const char *const name = "msr_head_backward";
     int rc = head_check(name, rows, vocab, d);
     if (rc) return rc;
-    if (reduction < HEAD_NONE || reduction > HEAD_MEAN || !w || !kept || (rows > 0 && (!packed || !lse || !dloss)) || noise_mode < -1 ||
+    if (reduction < HEAD_NONE || reduction > HEAD_MEAN || !w || !kept || (rows > 0 && (!packed || !sums || !dloss)) || noise_mode < -1 ||
         noise_mode > 2 || (noise_mode == NOISE_INJECT && !inject)) {
         set_error("%s: bad arguments", name);
         return MSR_ERR_ARG;
     }
-    if (!aligned(w, 16) || !aligned(packed, 16) || !aligned(dx, 16) || !aligned(dw, 16) || !aligned(kept, 4) || !aligned(lse, 4) ||
+    if (!aligned(w, 16) || !aligned(packed, 16) || !aligned(dx, 16) || !aligned(dw, 16) || !aligned(kept, 4) || !aligned(sums, 8) ||
         !aligned(dloss, 4) || !aligned(inject, 2) || !aligned(workspace, 16)) {
-        set_error("%s: operands and the workspace must be 16-byte aligned, kept, lse and dloss to their types", name);
+        set_error("%s: operands and the workspace must be 16-byte aligned, sums 8-byte aligned, kept and dloss to their types", name);
         return MSR_ERR_ALIGN;
     }
     const HeadPlan p = head_plan(rows, vocab, d, reduction);
@@ -805,14 +809,14 @@ int msr_head_backward(const uint16_t *packed, const uint16_t *w, const int32_t *
     }
     const size_t n = (size_t)rows, wb = 2 * (size_t)vocab * (size_t)d;
     const Range r[9] = {{dx, 2 * n * (size_t)d}, {dw, wb}, {workspace, rows ? p.bwd_bytes : 0}, {packed, 2 * n * (size_t)d}, {w, wb},
-                        {kept, 4 * (3 * n + 1)}, {lse, 4 * n}, {dloss, reduction == HEAD_NONE ? 4 * n : 4},
+                        {kept, 4 * (3 * n + 1)}, {sums, 8 * n}, {dloss, reduction == HEAD_NONE ? 4 * n : 4},
                         {inject, noise_mode == NOISE_INJECT ? wb : 0}};
     rc = ranges_apart(name, r, 9, 3);
     if (rc) return rc;
     hipStream_t s = (hipStream_t)stream;
     HeadArgs a{};
     char *const ws = static_cast<char *>(workspace);
-    a.x = packed; a.w = w; a.kept = kept; a.lse = const_cast<float *>(lse); a.dloss = dloss;
+    a.x = packed; a.w = w; a.kept = kept; a.sums = reinterpret_cast<float2 *>(const_cast<float *>(sums)); a.dloss = dloss;
     a.g = reinterpret_cast<uint16_t *>(ws); a.ldg = p.ldg; a.lo = (int)p.lo; a.out = dw;
     a.rows = (int)rows; a.vocab = (int)vocab; a.d = (int)d; a.reduction = reduction; a.zero_init = zero_init != 0;
     a.ns.key = seed_key(seed, 0);

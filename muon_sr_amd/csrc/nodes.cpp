@@ -249,14 +249,14 @@ struct HeadLoss : torch::autograd::Function<HeadLoss> {
         const int64_t vocab = w.size(0), d = w.size(1);
         const Rows r = flat_rows(x, d);
         const Tensor target = target_.contiguous(), packed = empty({r.n, d}, x, at::kBFloat16), kept = empty({3 * r.n + 1}, x, at::kInt),
-                     lse = empty({r.n}, x, at::kFloat), loss = empty(reduction == MSR_LOSS_NONE ? target.sizes() : at::IntArrayRef(), x, at::kFloat);
+                     sums = empty({r.n, 2}, x, at::kFloat), loss = empty(reduction == MSR_LOSS_NONE ? target.sizes() : at::IntArrayRef(), x, at::kFloat);
         size_t bytes = 0, backward_bytes = 0;
         check(msr_head_workspace_bytes(r.n, vocab, d, &bytes, &backward_bytes), "msr_head_workspace_bytes");
         const Tensor ws = workspace(bytes, x);
         call(x, "msr_head_forward", msr_head_forward, static_cast<const uint16_t *>(in(r.t)), r.ld, static_cast<const uint16_t *>(in(w)), in(target),
              (int32_t)(target.scalar_type() == at::kLong), ignore, r.n, vocab, d, (int32_t)reduction, at_<uint16_t>(packed), at_<int32_t>(kept),
-             at_<float>(lse), at_<float>(loss), out(ws), bytes);
-        ctx->save_for_backward({packed, w, kept, lse});
+             at_<float>(sums), at_<float>(loss), out(ws), bytes);
+        ctx->save_for_backward({packed, w, kept, sums});
         ctx->saved_data["shape"] = x.sizes().vec();
         ctx->saved_data["reduction"] = reduction;
         if (accumulate) ctx->saved_data["owner"] = w;   // (as in Embedding)
@@ -264,7 +264,7 @@ struct HeadLoss : torch::autograd::Function<HeadLoss> {
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads) {
         const variable_list saved = ctx->get_saved_variables();   // saved-tensor hooks may have changed their strides
-        const Tensor packed = packed_rows(saved[0]), w = packed_rows(saved[1]), kept = saved[2].contiguous(), lse = saved[3].contiguous(),
+        const Tensor packed = packed_rows(saved[0]), w = packed_rows(saved[1]), kept = saved[2].contiguous(), sums = saved[3].contiguous(),
                      dloss = grads[0].contiguous();
         const int64_t n = packed.size(0), vocab = w.size(0), d = w.size(1), reduction = ctx->saved_data["reduction"].toInt();
         const Tensor dx = ctx->needs_input_grad(0) ? empty(ctx->saved_data["shape"].toIntVector(), packed, at::kBFloat16) : Tensor();
@@ -276,14 +276,14 @@ struct HeadLoss : torch::autograd::Function<HeadLoss> {
             const Accumulator to(weight, "SRHead");
             const Tensor ws = workspace(bytes, packed);
             call(packed, "msr_head_backward", msr_head_backward, static_cast<const uint16_t *>(in(packed)), static_cast<const uint16_t *>(in(w)),
-                 static_cast<const int32_t *>(in(kept)), static_cast<const float *>(in(lse)), static_cast<const float *>(in(dloss)), n, vocab, d,
+                 static_cast<const int32_t *>(in(kept)), static_cast<const float *>(in(sums)), static_cast<const float *>(in(dloss)), n, vocab, d,
                  (int32_t)reduction, at_<uint16_t>(dx), at_<uint16_t>(to.acc), to.noise_mode, to.seed, (int32_t)to.first, (const uint16_t *)nullptr, out(ws), bytes);
             to.keep(weight);
             return once({dx, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()});
         }
         const Tensor dw = ctx->needs_input_grad(1) ? empty({vocab, d}, w, at::kBFloat16) : Tensor(), ws = workspace(bytes, packed);
         call(packed, "msr_head_backward", msr_head_backward, static_cast<const uint16_t *>(in(packed)), static_cast<const uint16_t *>(in(w)),
-             static_cast<const int32_t *>(in(kept)), static_cast<const float *>(in(lse)), static_cast<const float *>(in(dloss)), n, vocab, d,
+             static_cast<const int32_t *>(in(kept)), static_cast<const float *>(in(sums)), static_cast<const float *>(in(dloss)), n, vocab, d,
              (int32_t)reduction, at_<uint16_t>(dx), at_<uint16_t>(dw), -1, 0u, 0, (const uint16_t *)nullptr, out(ws), bytes);
         return once({dx, dw, Tensor(), Tensor(), Tensor(), Tensor()});
     }

@@ -2,7 +2,7 @@
 
 Bounds, with u = 2^-24 (an fp32 rounding) and h = 2^-8 (a bf16 one).  A logit S formed in fp32 from d products is off by at
 most eS = 2 (d + 1) u sum|x w| (the factor 2: any order of the sums, and what higher terms add).  exp of an argument
-a = x - m costs 4 u (|a| + 1) + 2 u |m|: the difference, its product with log2 e, that constant, m's own product and the function.  The sum behind l has at most depth =
+a = x - m costs 4 u (|a| + 1) + 2 u |m| at most: its product with log2 e, that constant, the difference and the function.  The sum behind l has at most depth =
 64 + vocab / 64 additions one after the other (32 in a lane, the waves', and a share of the tiles), so l is off by at most
 el = max eS + 2 depth u + 8 u (|l| + 1) + 2 u max|S|, and the loss by eS + el + u |loss|.
 G = g (p - [target]) is off by eG = g (p (eS + el + 4 u (|S - l| + 1) + 2 u |l|) + 2 u), then h |G| by its rounding (a rounding is
@@ -310,6 +310,27 @@ def test_the_upstream_gradient_is_not_rounded_with_the_targets(reduction):
     for got, want in zip(run(x, w, target, dloss, reduction)[1:], (dx, dw)):
         along = (got.double() * want).sum() / want.square().sum() - 1
         assert along.abs() <= 2.0 ** -11, along.item()
+
+
+@pytest.mark.parametrize("size", [30.0, 60.0, 1000.0])
+def test_rows_whose_word_is_nearly_sure(size):
+    """Logits (exact in fp32) of `size` and more for the target and 20 less for the 63 others: 1 - p is 1.3e-7, 2 u.  In fp32 a row's l has an ulp
+    of 32 u and more, but its largest term, the same in both passes, is an exponential of what M leaves of it, off by 2 u by the function; the
+    sum by 2 u and the others by what they are; the quotient and its product with that term by 2 u.  8 u bounds the loss and G."""
+    k = torch.arange(8, device=DEV)
+    x = torch.zeros((8, 8), dtype=BF16, device=DEV)
+    x[:, 0] = (size + k / 8 if size < 32 else size + k * size / 128 if size < 64 else 1000 + 4 * k).to(BF16)
+    x[:, 1] = -20
+    w = torch.zeros((64, 8), dtype=BF16, device=DEV)
+    w[:, 0] = 1
+    w[1:, 1] = 1
+    target = torch.zeros(8, dtype=torch.int64, device=DEV)
+    loss, dx, _ = run(x, w, target, torch.ones(8, device=DEV), "none")
+    others = 63 * math.exp(-20)
+    assert ((loss.double() - math.log1p(others)).abs() <= 8 * U).all(), loss
+    assert (dx[:, 0].abs() <= 8 * U).all(), dx[:, 0]                       # the sum of a row of G is 0
+    p = others / (1 + others)
+    assert ((dx[:, 1].double() - p).abs() <= 2 * H * p).all(), dx[:, 1]
 
 
 @pytest.mark.parametrize("first", [0.0, -0.0, math.inf, math.nan, 1e-42, 3.4e38, -1.7])

@@ -37,27 +37,27 @@ def test_head_sizes(lib):
 
 
 def test_head_forward(lib):
-    def call(x=A, ldx=64, w=B, target=C, i64=1, rows=100, vocab=500, d=64, red=2, packed=D, kept=E, lse=F, loss=G, ws=W, n=BIG):
-        return lib.msr_head_forward(x, ldx, w, target, i64, -100, rows, vocab, d, red, packed, kept, lse, loss, ws, n, None)
-    for bad in (dict(x=None), dict(w=None), dict(target=None), dict(packed=None), dict(kept=None), dict(lse=None), dict(loss=None), dict(ldx=63),
+    def call(x=A, ldx=64, w=B, target=C, i64=1, rows=100, vocab=500, d=64, red=2, packed=D, kept=E, sums=F, loss=G, ws=W, n=BIG):
+        return lib.msr_head_forward(x, ldx, w, target, i64, -100, rows, vocab, d, red, packed, kept, sums, loss, ws, n, None)
+    for bad in (dict(x=None), dict(w=None), dict(target=None), dict(packed=None), dict(kept=None), dict(sums=None), dict(loss=None), dict(ldx=63),
                 dict(red=3), dict(red=-1), dict(rows=-1), dict(vocab=0), dict(d=60)):
         assert call(**bad) == ARG, bad
-    for bad in (dict(x=A + 1), dict(w=B + 8), dict(packed=D + 8), dict(target=C + 4), dict(target=C + 2, i64=0), dict(kept=E + 2), dict(lse=F + 2),
+    for bad in (dict(x=A + 1), dict(w=B + 8), dict(packed=D + 8), dict(target=C + 4), dict(target=C + 2, i64=0), dict(kept=E + 2), dict(sums=F + 4),
                 dict(loss=G + 1), dict(ws=W + 8)):
         assert call(**bad) == ALIGN, bad
     assert call(ws=None) == WORKSPACE and call(n=100) == WORKSPACE and b"workspace" in lib.msr_last_error()
-    for bad in (dict(packed=A + 64), dict(kept=C), dict(lse=E + 1200), dict(loss=B + 64), dict(ws=A), dict(ws=D + 16), dict(loss=F + 4), dict(packed=B)):
+    for bad in (dict(packed=A + 64), dict(kept=C), dict(sums=E + 1200), dict(loss=B + 64), dict(ws=A), dict(ws=D + 16), dict(loss=F + 4), dict(packed=B)):
         assert call(**bad) == OVERLAP, bad
     assert call(rows=(1 << 24) - 1, vocab=1 << 16, d=64) == ARG and b"tiles" in lib.msr_last_error()
 
 
 def test_head_backward(lib):
-    def call(packed=A, w=B, kept=C, lse=D, dloss=E, rows=100, vocab=500, d=64, red=2, dx=F, dw=G, mode=-1, seed=0, zero=0, inject=None, ws=W, n=BIG):
-        return lib.msr_head_backward(packed, w, kept, lse, dloss, rows, vocab, d, red, dx, dw, mode, seed, zero, inject, ws, n, None)
-    for bad in (dict(packed=None), dict(w=None), dict(kept=None), dict(lse=None), dict(dloss=None), dict(red=5), dict(mode=3), dict(mode=-2),
+    def call(packed=A, w=B, kept=C, sums=D, dloss=E, rows=100, vocab=500, d=64, red=2, dx=F, dw=G, mode=-1, seed=0, zero=0, inject=None, ws=W, n=BIG):
+        return lib.msr_head_backward(packed, w, kept, sums, dloss, rows, vocab, d, red, dx, dw, mode, seed, zero, inject, ws, n, None)
+    for bad in (dict(packed=None), dict(w=None), dict(kept=None), dict(sums=None), dict(dloss=None), dict(red=5), dict(mode=3), dict(mode=-2),
                 dict(mode=2), dict(d=65)):
         assert call(**bad) == ARG, bad
-    for bad in (dict(packed=A + 8), dict(w=B + 2), dict(dx=F + 8), dict(dw=G + 4), dict(kept=C + 1), dict(lse=D + 2), dict(dloss=E + 2), dict(ws=W + 4)):
+    for bad in (dict(packed=A + 8), dict(w=B + 2), dict(dx=F + 8), dict(dw=G + 4), dict(kept=C + 1), dict(sums=D + 4), dict(dloss=E + 2), dict(ws=W + 4)):
         assert call(**bad) == ALIGN, bad
     assert call(n=1000) == WORKSPACE
     for bad in (dict(dx=A), dict(dw=B), dict(dx=G + 64), dict(ws=G), dict(dw=C - 64), dict(dx=E), dict(dw=A + 64), dict(mode=2, inject=G + 64)):
