@@ -621,7 +621,8 @@ static int embed_grad(const char *name, const void *ids, int32_t ids_i64, int64_
         hipLaunchKernelGGL(sort_kernel, dim3((unsigned)p.runs), dim3(SORT_THREADS), 0, s, a);
         if ((rc = check_launch("sort_kernel"))) return rc;
         for (int m = 0; m < p.merges; ++m) {
-            hipLaunchKernelGGL(merge_kernel, dim3((unsigned)((n + MERGE_KEYS - 1) / MERGE_KEYS)), dim3(MERGE_KEYS * MERGE_SHARES), 0, s, list[m & 1], list[~m & 1], n, SORT_LOG + m * MERGE_LOG);
+            hipLaunchKernelGGL(merge_kernel, dim3((unsigned)((n + MERGE_KEYS - 1) / MERGE_KEYS)), dim3(MERGE_KEYS * MERGE_SHARES), 0, s,
+                               list[m & 1], list[~m & 1], n, SORT_LOG + m * MERGE_LOG);
             if ((rc = check_launch("merge_kernel"))) return rc;
             a.sorted = list[~m & 1];
         }

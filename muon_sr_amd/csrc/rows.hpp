@@ -84,14 +84,7 @@ __device__ __forceinline__ float row16_sum(float v) {
     v += turned<0x124>(v);
     return v + turned<0x128>(v);
 }
-// The sums over the wave, in every lane
-__device__ __forceinline__ float wave_sum(float x) {
-    const auto h = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    float v = __uint_as_float(h[0]) + __uint_as_float(h[1]);
-    const auto q = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return row16_sum(__uint_as_float(q[0]) + __uint_as_float(q[1]));
-}
-// of two values: one exchange more than of one
+// The sums of two values over the wave, in every lane
 __device__ __forceinline__ float2 wave_sum2(float x, float y) {
     const auto h = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(y), false, false);
     float v = __uint_as_float(h[0]) + __uint_as_float(h[1]);            // lanes 0 to 31: x, the others: y
