@@ -545,8 +545,9 @@ int msr_embedding_grad_sr_accum(const void *ids, int32_t ids_i64, int64_t n, con
  *   mean = mean(x), rstd = 1 / sqrt(mean((x - mean)^2) + eps), h = (x - mean) rstd, y = h w + b
  *   q = dy w, dx = rstd (q - mean(q) - h mean(q h)), dw = sum_n dy h, db = sum_n dy
  * x, y, dy, dx: elem, x and dy with row strides ldx and lddy; w (NULL: 1), b (NULL: 0), dw, db:
- * welem.  Statistics and sums in fp32, one rounding.  mean and rstd (fp32 [rows]) are
- * written by the forward pass and read by the other.  dx, dw, db may be NULL (not
+ * welem.  Statistics and sums in fp32, one rounding.  mean (fp32 [2][rows]: two numbers whose sum is
+ * a row's mean, so that rows far from zero keep their digits) and rstd (fp32 [rows]) are written by the
+ * forward pass and read by the other.  dx, dw, db may be NULL (not
  * wanted).  Aligned to their types.  workspace: msr_layer_norm_workspace_bytes (dw or
  * db wanted).  dw and db are sums in an order that depends on the sizes alone.
  * ------------------------------------------------------------------------- */

@@ -137,11 +137,11 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
         const int64_t d = x.size(-1);
         const Rows r = flat_rows(x, d);
         const Tensor weight = contiguous(w), bias = contiguous(b), y = at::empty(x.sizes(), x.options().requires_grad(false)),
-                     stats = empty({2, r.n}, x, at::kFloat);
+                     stats = empty({3, r.n}, x, at::kFloat);   // mean's two numbers, rstd
         const Tensor &vector = weight.defined() ? weight : bias;
         const int32_t welem = vector.defined() ? elem(vector) : MSR_F32;
         float *const mean = at_<float>(stats);
-        call(x, "msr_layer_norm", msr_layer_norm, in(r.t), r.ld, in(weight), in(bias), (float)eps, r.n, d, out(y), mean, mean + r.n, elem(x), welem);
+        call(x, "msr_layer_norm", msr_layer_norm, in(r.t), r.ld, in(weight), in(bias), (float)eps, r.n, d, out(y), mean, mean + 2 * r.n, elem(x), welem);
         ctx->save_for_backward({x, w, stats});
         ctx->saved_data["welem"] = (int64_t)welem;
         ctx->saved_data["weight"] = w.defined();
@@ -163,7 +163,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
         if (dw.defined() || db.defined()) check(msr_layer_norm_workspace_bytes(rx.n, d, elem(x), &bytes), "msr_layer_norm_workspace_bytes");
         const Tensor ws = workspace(bytes, x);
         const float *const mean = static_cast<const float *>(in(stats));
-        call(x, "msr_layer_norm_grad", msr_layer_norm_grad, in(ry.t), ry.ld, in(rx.t), rx.ld, in(w), mean, mean + rx.n, rx.n, d, out(dx), out(dw),
+        call(x, "msr_layer_norm_grad", msr_layer_norm_grad, in(ry.t), ry.ld, in(rx.t), rx.ld, in(w), mean, mean + 2 * rx.n, rx.n, d, out(dx), out(dw),
              out(db), elem(x), welem, out(ws), bytes);
         return once({dx, dw, db, Tensor()});
     }

@@ -2,10 +2,12 @@
 //     mu = mean(x), r = 1 / sqrt(mean((x - mu)^2) + eps), h = (x - mu) r,   y = h w + b
 //     q = dy w,   dx = r (q - mean(q) - h mean(q h)),   dw = sum_n dy h,   db = sum_n dy
 // HBM bounds both passes (x and y; x, dy and dx).  A row is held in the registers of L lanes, 8 to 64 of a wave or a whole work-group of
-// 256 or 1024, read once: a mean first, then the sums of what is left of it and of its squares, so that a mean far from zero costs no
-// digits: with z = x - (that mean), mean += mean(z) and the variance is mean(z^2) - mean(z)^2.  The
-// backward pass adds dw and db up in registers over the rows that a work-group takes, in order; the
-// work-groups' sums, in fp32, are added by a second kernel, in order.
+// 256 or 1024, read once: a mean m first, then the sums of what is left of it and of its squares, so that a mean far from zero costs no
+// digits: with z = x - m and c = mean(z), h = (z - c) r and the variance is mean(z^2) - c^2.  m and c are kept as two numbers for the
+// backward pass too: their sum, rounded at the size of the mean, puts every h of a row off by up to half of its ulp times r (fp32 rows of
+// 768 around 1000 of deviation 1e-2, against 64 bits: dx off by 9e-5 and dw by 1.9e-3, and by 1e-7 each so).  The backward pass adds dw
+// and db up in registers over the rows that a work-group takes, in order; the work-groups' sums, in fp32, are added by a second kernel, in
+// order.
 #include "rows.hpp"
 #include "../../include/muon_sr_amd.h"
 
@@ -17,7 +19,7 @@ struct NormArgs {
     const void *x, *dy, *w, *b;
     int64_t ldx, lddy, rows, d;
     void *y;                     // y, or dx
-    float *mean, *rstd;          // [rows]
+    float *mean, *rstd;          // [2][rows]: m, c; [rows]
     float *parts;                // [work-groups][2][d]: sums of dy h and of dy
     float eps;
     int32_t w32;                 // w and b are fp32
@@ -105,9 +107,9 @@ __global__ __launch_bounds__(norm_threads(L)) void norm_kernel(NormArgs a) {
         const float2 left = sums.of(z, q);
         if (L < 64 && n >= a.rows) continue;
         const float c = left.x / d, r = 1.0f / sqrtf(fmaxf(left.y / d - c * c, 0.0f) + a.eps);
-        mean += c;
         if (lane == 0) {
             a.mean[n] = mean;
+            a.mean[a.rows + n] = c;
             a.rstd[n] = r;
         }
 #pragma unroll
@@ -142,12 +144,12 @@ __global__ __launch_bounds__(norm_threads(L)) void norm_grad_kernel(NormArgs a) 
     }
     const int64_t step = (int64_t)gridDim.x * ROWS;
     C vx[U], vy[U];
-    float next_mean = 0.0f, next_r = 0.0f;
+    float next_mean = 0.0f, next_c = 0.0f, next_r = 0.0f;
     auto fetch = [&](int64_t i) __attribute__((always_inline)) {
         if constexpr (L < 64) {
 #pragma unroll
             for (int u = 0; u < U; ++u) vx[u].v = vy[u].v = Bytes16{};
-            next_mean = next_r = 0.0f;
+            next_mean = next_c = next_r = 0.0f;
         }
         if (i >= a.rows) return;
 #pragma unroll
@@ -156,13 +158,14 @@ __global__ __launch_bounds__(norm_threads(L)) void norm_grad_kernel(NormArgs a) 
             vy[u].load(static_cast<const T *>(a.dy) + i * a.lddy, (int64_t)(u * L + lane) * N, a.d);
         }
         next_mean = a.mean[i];
+        next_c = a.mean[a.rows + i];
         next_r = a.rstd[i];
     };
     int64_t n = (int64_t)blockIdx.x * ROWS + sub;
     if (AHEAD) fetch(n);
     for (; n - (L < 64 ? sub : 0) < a.rows; n += step) {
         if (!AHEAD) fetch(n);
-        const float mean = next_mean, r = next_r;
+        const float mean = next_mean, c = next_c, r = next_r;
         float h[U][N], q[U][N], sq = 0.0f, sqh = 0.0f;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -170,7 +173,7 @@ __global__ __launch_bounds__(norm_threads(L)) void norm_grad_kernel(NormArgs a) 
             vy[u].get(q[u]);
 #pragma unroll
             for (int e = 0; e < N; ++e) {       // (beyond the row, and without one, dy is 0, and so is what it is multiplied into)
-                h[u][e] = (h[u][e] - mean) * r;
+                h[u][e] = ((h[u][e] - mean) - c) * r;
                 dw[u][e] = __builtin_fmaf(q[u][e], h[u][e], dw[u][e]);
                 db[u][e] += q[u][e];
                 q[u][e] *= w[u][e];
@@ -261,7 +264,8 @@ __global__ __launch_bounds__(256) void norm_long_kernel(NormArgs a) {
             r = 1.0f / sqrtf(fmaxf(sum.y / d - left * left, 0.0f) + a.eps);
         }
         if (threadIdx.x == 0) {
-            a.mean[n] = mean + left;
+            a.mean[n] = mean;
+            a.mean[a.rows + n] = left;
             a.rstd[n] = r;
         }
         for (int64_t c = (int64_t)threadIdx.x * N; c < a.d; c += 256 * N) {
@@ -290,7 +294,7 @@ __global__ __launch_bounds__(256) void norm_long_grad_kernel(NormArgs a) {
     float *const to = a.parts ? a.parts + (int64_t)blockIdx.x * 2 * a.d : nullptr;
     bool first = true;
     for (int64_t n = blockIdx.x; n < a.rows; n += gridDim.x) {
-        const float mean = a.mean[n], r = a.rstd[n];
+        const float mean = a.mean[n], left = a.mean[a.rows + n], r = a.rstd[n];
         float2 m = make_float2(0.0f, 0.0f);
         for (int pass = 0; pass < 2; ++pass) {
             float sq = 0.0f, sqh = 0.0f;
@@ -304,7 +308,7 @@ __global__ __launch_bounds__(256) void norm_long_grad_kernel(NormArgs a) {
                 vector_cells<N>(a.w, a.w32, c, a.d, 1.0f, w);
 #pragma unroll
                 for (int e = 0; e < N; ++e) {
-                    h[e] = (h[e] - mean) * r;
+                    h[e] = ((h[e] - mean) - left) * r;
                     if (!pass && to && c + e < a.d) {
                         to[c + e] = __builtin_fmaf(q[e], h[e], first ? 0.0f : to[c + e]);
                         to[a.d + c + e] = q[e] + (first ? 0.0f : to[a.d + c + e]);
@@ -436,7 +440,7 @@ int msr_layer_norm(const void *x, int64_t ldx, const void *w, const void *b, flo
         return MSR_ERR_ALIGN;
     }
     const size_t n = (size_t)rows;
-    const Range r[6] = {{y, n * (size_t)d * es}, {mean, 4 * n}, {rstd, 4 * n}, {x, rows_bytes(rows, ldx, d, es)}, {w, (size_t)d * ws}, {b, (size_t)d * ws}};
+    const Range r[6] = {{y, n * (size_t)d * es}, {mean, 8 * n}, {rstd, 4 * n}, {x, rows_bytes(rows, ldx, d, es)}, {w, (size_t)d * ws}, {b, (size_t)d * ws}};
     rc = ranges_apart(name, r, 6, 3);
     if (rc) return rc;
     NormArgs a{};
@@ -474,7 +478,7 @@ int msr_layer_norm_grad(const void *dy, int64_t lddy, const void *x, int64_t ldx
         return MSR_ERR_WORKSPACE;
     }
     const Range r[9] = {{dx, n * (size_t)d * es}, {dw, (size_t)d * ws}, {db, (size_t)d * ws}, {workspace, dw || db ? need : 0},
-                        {dy, rows_bytes(rows, lddy, d, es)}, {x, rows_bytes(rows, ldx, d, es)}, {w, (size_t)d * ws}, {mean, 4 * n}, {rstd, 4 * n}};
+                        {dy, rows_bytes(rows, lddy, d, es)}, {x, rows_bytes(rows, ldx, d, es)}, {w, (size_t)d * ws}, {mean, 8 * n}, {rstd, 4 * n}};
     rc = ranges_apart(name, r, 9, 4);
     if (rc) return rc;
     hipStream_t s = (hipStream_t)stream;

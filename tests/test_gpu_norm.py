@@ -204,3 +204,46 @@ def test_same_call_same_bits():
     a = run(x, w, b, dy)
     for _ in range(3):
         assert all(torch.equal(p, q) for p, q in zip(a, run(x, w, b, dy)))
+
+
+def exact_far(x, w, b, dy, eps, depth):
+    """As `exact`, for rows whose mean is far from zero and held as two numbers, m and c.  A sum has at most `depth` additions one after the
+    other (and a division), so m is off by em = depth u mean|x|.  z = x - m is exact (x and m are within a factor of 2 of one another) and at most
+    Z = |x - mean| + em; c = mean(z) is off by ec = depth u mean Z, z - c by ec + u (Z + em + ec).  mean(z^2) - c^2 is off by
+    (depth + 4) u mean Z^2 + 2 (em + ec) (ec + u em), the variance's relative error twice that of rstd, which adds 4 u."""
+    n, d = x.shape
+    x, w, b, dy = (t.double() for t in (x, w, b, dy))
+    mean = x.mean(1, keepdim=True)
+    assert (x.amax(1) < 2 * x.amin(1)).all()
+    em = depth * U * x.abs().mean(1, keepdim=True)
+    Z = (x - mean).abs() + em
+    ec = depth * U * Z.mean(1, keepdim=True)
+    var = (x - mean).square().mean(1, keepdim=True) + eps
+    r = var.rsqrt()
+    er = ((depth + 4) * U * Z.square().mean(1, keepdim=True) + 2 * (em + ec) * (ec + U * em)) / var + 4 * U
+    h = (x - mean) * r
+    eh = r * (ec + U * (Z + em + ec)) + h.abs() * (er + 2 * U)
+    y = (h * w + b, w.abs() * eh + 2 * U * ((h * w).abs() + b.abs()))
+    q = dy * w
+    m1, m2 = q.mean(1, keepdim=True), (q * h).mean(1, keepdim=True)
+    e1 = (depth + 1) * U * q.abs().mean(1, keepdim=True)
+    e2 = (depth + 2) * U * (q * h).abs().mean(1, keepdim=True) + (q.abs() * eh).mean(1, keepdim=True)
+    dx = r * (q - m1 - h * m2)
+    ex = r * (e1 + h.abs() * e2 + eh * (m2.abs() + e2) + 4 * U * (q.abs() + m1.abs() + (h * m2).abs())) + (er + 2 * U) * dx.abs()
+    dw = ((dy * h).sum(0), (n + 8) * U * (dy * h).abs().sum(0) + (dy.abs() * eh).sum(0))
+    db = (dy.sum(0), (n + 8) * U * dy.abs().sum(0))
+    return y, (dx, ex), dw, db
+
+
+@pytest.mark.parametrize("d", [40, 200, 768, 4096, 8000, 20000])
+def test_gradients_of_rows_far_from_zero(d):
+    """fp32 rows around 1000 with deviations of 1e-2, in every way that a row is held: their h, and with it the gradients, keep the digits that
+    y keeps.  A mean rounded to one number would be off by 2^-15, and h by 3e-3 with it.  One lane adds up at most 32 elements (of a long row d / 256,
+    4 at a time), a wave 6 times two, and 16 waves their sums; the bounds are below 3e-4 of the values' size, so such a mean does not pass."""
+    g = gen(30 + d)
+    x = 1000 + 1e-2 * torch.randn((40, d), generator=g, device=DEV)
+    _, w, b, dy = make(40, d, F32, F32, 31)
+    depth = (32 if d <= 16384 else d // 256 + 4) + 6 + 16
+    for got, want in zip(run(x, w, b, dy, 1e-6), exact_far(x, w, b, dy, 1e-6, depth)):
+        near(got, want)
+        assert torch.linalg.norm(want[1]) <= 3e-4 * torch.linalg.norm(want[0])
