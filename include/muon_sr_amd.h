@@ -566,15 +566,15 @@ int msr_layer_norm_grad(const void *dy, int64_t lddy, const void *x, int64_t ldx
  *   dlogits[t][e] = dloss p[t][e] (u[e] - sum_j u[j] p[t][j]), u[e] = experts / n f[e]; 0 for the other tokens
  * ids outside [0, experts) are dropped slots.  Logits of -inf have probability 0 (a token without any
  * other: 0 everywhere).  logits: elem, row stride ld; ids: int32, or int64 with ids_i64,
- * contiguous [tokens][k]; counts int32 [experts]; lse (fp32 [tokens]) and slope (u, fp32
- * [experts]) are written for the gradient.  tokens * k < 2^30, experts <= MSR_EXPERTS_MAX.
+ * contiguous [tokens][k]; counts int32 [experts]; stats (fp32 [2][tokens]: a token's largest logit m and
+ * 1 / sum exp(logit - m)) and slope (u, fp32 [experts]) are written for the gradient.  tokens * k < 2^30, experts <= MSR_EXPERTS_MAX.
  * workspace: msr_balance_workspace_bytes.
  * ------------------------------------------------------------------------- */
 int msr_balance_workspace_bytes(int64_t tokens, int32_t experts, size_t *bytes);
 int msr_balance_loss(const void *logits, int64_t ld, const void *ids, int32_t ids_i64, const uint8_t *mask, int64_t tokens,
-                     int32_t experts, int32_t k, float *loss, int32_t *counts, float *lse, float *slope, int32_t elem,
+                     int32_t experts, int32_t k, float *loss, int32_t *counts, float *stats, float *slope, int32_t elem,
                      void *workspace, size_t workspace_bytes, msr_stream_t stream);
-int msr_balance_grad(const void *logits, int64_t ld, const uint8_t *mask, const float *lse, const float *slope,
+int msr_balance_grad(const void *logits, int64_t ld, const uint8_t *mask, const float *stats, const float *slope,
                      const float *dloss, int64_t tokens, int32_t experts, void *dlogits, int32_t elem, msr_stream_t stream);
 
 /* ---------------------------------------------------------------------------

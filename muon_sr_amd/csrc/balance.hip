@@ -3,7 +3,10 @@
 //     p[t] = softmax(logits[t]),   c[e] = slots of these tokens with expert e,   f[e] = c[e] / (n k)
 //     loss = experts / n sum_e f[e] sum_t p[t][e]
 //     dlogits[t][e] = dloss p[t][e] (u[e] - sum_j u[j] p[t][j]),   u[e] = experts / n f[e]
-// Both passes read the logits once; the probabilities are not stored, but the log of each token's sum is.  A token is held by
+// Both passes read the logits once; the probabilities are not stored, but each token's largest logit m and 1 / s, s = sum exp(logit - m), are:
+// both passes form p = exp(logit - m) / s by the same instructions.  (m + log s in one number is rounded at the size of the logits, and all p of a
+// token are off by a common factor, which u[e] - sum_j u[j] p[j] multiplies where the load is nearly even: 64 experts, u spread by 1 %,
+// logits of deviation 1 around 1000, dlogits off by 2e-3, and by 5e-6 so wherever they are.)  A token is held by
 // L lanes, U cells of 16 bytes each, so that a wave sums the probabilities of 64 / L tokens at a time in registers, the next
 // tokens' logits on their way; the work-groups' sums (fp32) and counts are added in order by a second kernel.  Logits of -inf have probability 0, and a token that has no others counts with 0
 // everywhere.
@@ -19,7 +22,7 @@ struct BalanceArgs {
     int64_t ld, tokens;
     const void *ids;
     const uint8_t *mask;         // [tokens], or null: every token counts
-    float *lse;                  // [tokens]
+    float *stats;                // [2][tokens]: m (0 of a token without probabilities), 1 / s (0 of it)
     float *sums;                 // [work-groups][experts]
     int32_t *counts;             // [work-groups][experts + 1]: slots, and the tokens that count
     const float *dloss, *slope;  // one; u [experts]
@@ -27,7 +30,7 @@ struct BalanceArgs {
     int32_t experts, k, i64;
 };
 
-constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr float LOG2E = 1.4426950408889634f;
 
 // Work-group b's tokens: [b per, (b + 1) per).  blockDim.x: 256 or 1024.
 template <typename T, int L, int U>
@@ -103,13 +106,16 @@ __global__ __launch_bounds__(BAL_THREADS) void balance_kernel(BalanceArgs a, int
                 s += x[u][e];
             }
         s = over_group<L>(s, Add{});
-        // (the instructions for 1 / s and log2 s, within an ulp: the arithmetic is what bounds this kernel)
-        const float inv = s == 0.0f ? 0.0f : __builtin_amdgcn_rcpf(s);
+        // (the instruction for 1 / s is within an ulp, one step of Newton's rounds it)
+        const float near = __builtin_amdgcn_rcpf(s), inv = s == 0.0f ? 0.0f : __builtin_fmaf(__builtin_fmaf(-s, near, 1.0f), near, near);
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int e = 0; e < N; ++e) sum[u][e] = __builtin_fmaf(x[u][e], inv, sum[u][e]);
-        if (on && l == 0) a.lse[t] = s == 0.0f ? INFINITY : at + __builtin_amdgcn_logf(s) * LN2;      // exp(logit - lse) is 0 where there is no probability
+        if (on && l == 0) {
+            a.stats[t] = at;
+            a.stats[a.tokens + t] = inv;
+        }
     };
     auto each = [&](auto &&f) __attribute__((always_inline)) {
         f(std::integral_constant<int, 0>{});
@@ -208,7 +214,7 @@ __global__ __launch_bounds__(256) void balance_grad_kernel(BalanceArgs a) {
         float p[U][N] = {}, dot = 0.0f;
         C v[U];
         if (on) {
-            const float lse = a.lse[t];
+            const float at = a.stats[t], inv = a.stats[a.tokens + t];
 #pragma unroll
             for (int u = 0; u < U; ++u) v[u].load(static_cast<const T *>(a.logits) + t * a.ld, (u * L + l) * N, a.experts);
 #pragma unroll
@@ -216,7 +222,7 @@ __global__ __launch_bounds__(256) void balance_grad_kernel(BalanceArgs a) {
                 v[u].get(p[u]);
 #pragma unroll
                 for (int e = 0; e < N; ++e) {           // (what is beyond the experts is not stored, and its slope is 0)
-                    p[u][e] = (u * L + l) * N + e < a.experts ? __builtin_amdgcn_exp2f((p[u][e] - lse) * LOG2E) : 0.0f;
+                    p[u][e] = (u * L + l) * N + e < a.experts ? __builtin_amdgcn_exp2f((p[u][e] - at) * LOG2E) * inv : 0.0f;
                     dot = __builtin_fmaf(p[u][e], slope[u][e], dot);
                 }
             }
@@ -292,14 +298,14 @@ int msr_balance_workspace_bytes(int64_t tokens, int32_t experts, size_t *bytes) 
 }
 
 int msr_balance_loss(const void *logits, int64_t ld, const void *ids, int32_t ids_i64, const uint8_t *mask, int64_t tokens, int32_t experts,
-                     int32_t k, float *loss, int32_t *counts, float *lse, float *slope, int32_t elem, void *workspace, size_t workspace_bytes,
+                     int32_t k, float *loss, int32_t *counts, float *stats, float *slope, int32_t elem, void *workspace, size_t workspace_bytes,
                      msr_stream_t stream) {
     const char *const name = "msr_balance_loss";
     int rc = balance_check(name, tokens, experts, k, elem);
     if (rc) return rc;
-    if (!loss || !counts || !slope || (tokens > 0 && (!logits || !ids || !lse)) || ld < experts) { set_error("%s: bad arguments", name); return MSR_ERR_ARG; }
+    if (!loss || !counts || !slope || (tokens > 0 && (!logits || !ids || !stats)) || ld < experts) { set_error("%s: bad arguments", name); return MSR_ERR_ARG; }
     const size_t es = elem_bytes(elem), is = ids_i64 ? 8 : 4;
-    if (!aligned(logits, es) || !aligned(ids, is) || !aligned(loss, 4) || !aligned(counts, 4) || !aligned(lse, 4) || !aligned(slope, 4) || !aligned(workspace, 4)) {
+    if (!aligned(logits, es) || !aligned(ids, is) || !aligned(loss, 4) || !aligned(counts, 4) || !aligned(stats, 4) || !aligned(slope, 4) || !aligned(workspace, 4)) {
         set_error("%s: operands must be aligned to their types", name);
         return MSR_ERR_ALIGN;
     }
@@ -310,13 +316,13 @@ int msr_balance_loss(const void *logits, int64_t ld, const void *ids, int32_t id
         set_error("%s: workspace of %zu bytes is smaller than the %zu required", name, workspace_bytes, need);
         return MSR_ERR_WORKSPACE;
     }
-    const Range r[8] = {{loss, 4}, {counts, 4 * (size_t)experts}, {lse, 4 * n}, {slope, 4 * (size_t)experts}, {workspace, need},
+    const Range r[8] = {{loss, 4}, {counts, 4 * (size_t)experts}, {stats, 8 * n}, {slope, 4 * (size_t)experts}, {workspace, need},
                         {logits, rows_bytes(tokens, ld, experts, es)}, {ids, n * (size_t)k * is}, {mask, n}};
     rc = ranges_apart(name, r, 8, 5);
     if (rc) return rc;
     hipStream_t s = (hipStream_t)stream;
     BalanceArgs a{};
-    a.logits = logits; a.ld = ld; a.tokens = tokens; a.ids = ids; a.i64 = ids_i64 != 0; a.mask = mask; a.lse = lse; a.experts = experts; a.k = k;
+    a.logits = logits; a.ld = ld; a.tokens = tokens; a.ids = ids; a.i64 = ids_i64 != 0; a.mask = mask; a.stats = stats; a.experts = experts; a.k = k;
     a.sums = static_cast<float *>(workspace);
     a.counts = reinterpret_cast<int32_t *>(a.sums + (size_t)groups * (size_t)experts);
     balance_shape(elem, experts, [&](auto t, auto l, auto u) {
@@ -327,23 +333,23 @@ int msr_balance_loss(const void *logits, int64_t ld, const void *ids, int32_t id
     return check_launch("balance_join_kernel");
 }
 
-int msr_balance_grad(const void *logits, int64_t ld, const uint8_t *mask, const float *lse, const float *slope, const float *dloss,
+int msr_balance_grad(const void *logits, int64_t ld, const uint8_t *mask, const float *stats, const float *slope, const float *dloss,
                      int64_t tokens, int32_t experts, void *dlogits, int32_t elem, msr_stream_t stream) {
     const char *const name = "msr_balance_grad";
     int rc = balance_check(name, tokens, experts, 1, elem);
     if (rc || tokens == 0) return rc;
-    if (!logits || !lse || !slope || !dloss || !dlogits || ld < experts) { set_error("%s: bad arguments", name); return MSR_ERR_ARG; }
+    if (!logits || !stats || !slope || !dloss || !dlogits || ld < experts) { set_error("%s: bad arguments", name); return MSR_ERR_ARG; }
     const size_t es = elem_bytes(elem), n = (size_t)tokens;
-    if (!aligned(logits, es) || !aligned(dlogits, es) || !aligned(lse, 4) || !aligned(slope, 4) || !aligned(dloss, 4)) {
+    if (!aligned(logits, es) || !aligned(dlogits, es) || !aligned(stats, 4) || !aligned(slope, 4) || !aligned(dloss, 4)) {
         set_error("%s: operands must be aligned to their types", name);
         return MSR_ERR_ALIGN;
     }
-    const Range r[6] = {{dlogits, n * (size_t)experts * es}, {logits, rows_bytes(tokens, ld, experts, es)}, {mask, n}, {lse, 4 * n},
+    const Range r[6] = {{dlogits, n * (size_t)experts * es}, {logits, rows_bytes(tokens, ld, experts, es)}, {mask, n}, {stats, 8 * n},
                         {slope, 4 * (size_t)experts}, {dloss, 4}};
     rc = ranges_apart(name, r, 6, 1);
     if (rc) return rc;
     BalanceArgs a{};
-    a.logits = logits; a.ld = ld; a.tokens = tokens; a.mask = mask; a.lse = const_cast<float *>(lse); a.slope = slope; a.dloss = dloss;
+    a.logits = logits; a.ld = ld; a.tokens = tokens; a.mask = mask; a.stats = const_cast<float *>(stats); a.slope = slope; a.dloss = dloss;
     a.out = dlogits; a.experts = experts;
     balance_shape(elem, experts, [&](auto t, auto l, auto u) {
         const dim3 grid(grid_for(tokens, 256 / decltype(l)::value, 256 * 8));

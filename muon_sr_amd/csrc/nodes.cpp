@@ -315,13 +315,13 @@ struct Balance : torch::autograd::Function<Balance> {
         const int64_t tokens = logits.size(0), experts = logits.size(1);
         const Rows r = flat_rows(logits, experts);
         const Tensor ids = ids_.contiguous(), mask = contiguous(mask_.value_or(Tensor())), loss = empty({}, logits, at::kFloat), counts = empty({experts}, logits, at::kInt),
-                     kept = empty({tokens + experts}, logits, at::kFloat);   // log-sum-exps, then slopes
+                     kept = empty({2 * tokens + experts}, logits, at::kFloat);   // the tokens' statistics, then slopes
         size_t bytes = 0;
         check(msr_balance_workspace_bytes(tokens, (int32_t)experts, &bytes), "msr_balance_workspace_bytes");
         const Tensor ws = workspace(bytes, logits);
         call(logits, "msr_balance_loss", msr_balance_loss, in(r.t), r.ld, in(ids), (int32_t)(ids.scalar_type() == at::kLong),
              static_cast<const uint8_t *>(in(mask)), tokens, (int32_t)experts, (int32_t)ids.size(1), at_<float>(loss), at_<int32_t>(counts),
-             at_<float>(kept), at_<float>(kept) + tokens, elem(logits), out(ws), bytes);
+             at_<float>(kept), at_<float>(kept) + 2 * tokens, elem(logits), out(ws), bytes);
         ctx->save_for_backward({logits, mask, kept});
         ctx->mark_non_differentiable({counts});
         return {loss, counts};
@@ -332,8 +332,8 @@ struct Balance : torch::autograd::Function<Balance> {
         const int64_t tokens = logits.size(0), experts = logits.size(1);
         const Rows r = flat_rows(logits, experts);
         const Tensor d = empty({tokens, experts}, logits, logits.scalar_type());
-        const float *const lse = static_cast<const float *>(in(kept));
-        call(logits, "msr_balance_grad", msr_balance_grad, in(r.t), r.ld, static_cast<const uint8_t *>(in(mask)), lse, lse + tokens,
+        const float *const stats = static_cast<const float *>(in(kept));
+        call(logits, "msr_balance_grad", msr_balance_grad, in(r.t), r.ld, static_cast<const uint8_t *>(in(mask)), stats, stats + 2 * tokens,
              static_cast<const float *>(in(dloss)), tokens, (int32_t)experts, out(d), elem(logits));
         return once({d, Tensor(), Tensor()});
     }

@@ -167,3 +167,26 @@ def test_same_call_same_bits():
     a = run(*case)
     for _ in range(3):
         assert all(torch.equal(p, q) for p, q in zip(a, run(*case)))
+
+
+@pytest.mark.parametrize("tokens,experts", [(8192, 64), (2050, 257), (513, 1000)])
+@pytest.mark.parametrize("offset", [0.0, 1000.0, -10000.0])
+def test_logits_far_from_zero_and_an_even_load(tokens, experts, offset):
+    """Every expert has nearly the same load, so that u[e] - sum_j u[j] p[j] is small beside u: an error that all p of a token have in common
+    remains in dlogits as that error times u p.  p is formed from a maximum and a sum, whatever size the logits have: exp costs 4 u (|x - max| + 1), the
+    sum has at most 16 additions in a lane and 6 of a wave's after one another, its reciprocal and the product with it 3 u.  The log of the sum
+    added to the maximum would be off by up to u |offset|."""
+    g = gen(40 + tokens)
+    logits = offset + torch.randn((tokens, experts), generator=g, device=DEV)
+    ids = (torch.arange(2 * tokens, device=DEV) % experts).view(tokens, 2)
+    ids[:tokens // 100, 0] = 3
+    up = torch.tensor(0.73, device=DEV)
+    _, counts, d = run(logits, ids, None, up)
+    x = logits.double()
+    p = torch.softmax(x, 1)
+    ep = p * (4 * U * ((x.amax(1, keepdim=True) - x) + 1) + (16 + 6 + 4) * U)
+    slope = counts.double() * experts / (2 * tokens * tokens)
+    dot, edot = (p * slope).sum(1, keepdim=True), ((ep + 26 * U * p) * slope).sum(1, keepdim=True)
+    want = up.double() * p * (slope - dot)
+    bound = up.double() * (ep * (slope - dot).abs() + p * (edot + 4 * U * slope)) + 4 * U * want.abs()
+    assert ((d.double() - want).abs() <= bound).all()
