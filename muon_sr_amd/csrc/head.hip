@@ -32,12 +32,12 @@ struct HeadArgs {
     float2 *part;                // [tiles of words][rows]: of a tile
     float *picked;               // [rows]: S[n][t[n]]
     const float *dloss;          // [rows] in the given order, or one
-    uint16_t *g;                 // [rows][ldg]: a piece of G / c; [2][rows][ldg] with lo
-    float *slots;                // fp32 sums [splits][M][N]
+    uint16_t *g;                 // [g_rows][ldg]: a piece of G / c, of few rows two numbers (low_of)
+    float *slots;                // fp32 sums [splits][g_rows][d] of dx, [splits][words of the piece][d] of dW
     uint16_t *out;               // dW or the accumulator
     int64_t ldg;
     int32_t rows, vocab, d, reduction;
-    int32_t lo;                  // rows, where G / c is kept as the sum of two bf16 numbers, else 0
+    int32_t few, g_rows;         // rows that count, at most, for G / c to be the sum of two bf16 numbers; room for either
     int32_t v0, vn;              // the piece: words v0 to v0 + vn - 1
     int32_t tiles_n, splits, first, zero_init;   // first: the slots hold nothing yet
     Noise ns;
@@ -47,6 +47,8 @@ struct HeadArgs {
 typedef const __attribute__((address_space(4))) int32_t *const_i32_t;
 __device__ __forceinline__ int kept_rows(const HeadArgs &a) { return min(max(*(const_i32_t)(uintptr_t)a.kept, 0), a.rows); }
 __device__ __forceinline__ int word_of(const HeadArgs &a, int r) { return a.kept[1 + a.rows + r]; }
+// The row of G where the second numbers of its rows begin; 0 where it has none
+__device__ __forceinline__ int low_of(const HeadArgs &a, int count) { return count <= a.few ? count : 0; }
 // g of packed row r
 __device__ __forceinline__ float dloss_of(const HeadArgs &a, int r, int count) {
     const float g = a.dloss[a.reduction == HEAD_NONE ? a.kept[1 + r] : 0];
@@ -192,7 +194,7 @@ __global__ __launch_bounds__(64 * Shape<T>::NW, 2) void logits_kernel(HeadArgs a
     __shared__ __attribute__((aligned(16))) char own[GRAD ? NW * 32 * WROW : SH::WN * T * 8];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave / SH::WN, wn = wave % SH::WN;
-    const int count = kept_rows(a), tiles_m = (count + T - 1) / T, slabs = (a.d + BK - 1) / BK;
+    const int count = kept_rows(a), tiles_m = (count + T - 1) / T, slabs = (a.d + BK - 1) / BK, low = low_of(a, count);
     const float unit = GRAD ? unit_of(a, count) : 1.0f;
     PR pr;
     auto lds_p = [&](auto ST) __attribute__((always_inline)) -> char * { return decltype(ST)::value == 0 ? p_0 : p_1; };
@@ -306,7 +308,7 @@ __global__ __launch_bounds__(64 * Shape<T>::NW, 2) void logits_kernel(HeadArgs a
                         for (int x = 0; x < 16; ++x)
                             if (rel == 32 * j + 8 * (x >> 2) + (x & 3)) pr.acc[i][j][x] -= g;
                 }
-                auto put = [&](int part) __attribute__((always_inline)) {
+                auto put = [&](int first) __attribute__((always_inline)) {
 #pragma unroll
                     for (int j = 0; j < FN; ++j)
 #pragma unroll
@@ -318,18 +320,16 @@ __global__ __launch_bounds__(64 * Shape<T>::NW, 2) void logits_kernel(HeadArgs a
                     for (int y = 0; y < NP; ++y) {
                         const int rr = crow + RPP * y, m = m0 + wm * SH::TM + 32 * i + rr;
                         const u32x4_t c = *reinterpret_cast<const u32x4_t *>(wst + rr * WROW + ((cchk ^ (rr & (WC - 1))) * 16));
-                        if (m < count && nc < a.vn) *reinterpret_cast<u32x4_t *>(a.g + (int64_t)(part * a.lo + m) * a.ldg + nc) = c;
+                        if (m < count && nc < a.vn) *reinterpret_cast<u32x4_t *>(a.g + (int64_t)(first + m) * a.ldg + nc) = c;
                     }
                 };
                 put(0);
-                if constexpr (T < 256) {
-                    if (!a.lo) continue;
+                if (!low) continue;
 #pragma unroll
-                    for (int j = 0; j < FN; ++j)
+                for (int j = 0; j < FN; ++j)
 #pragma unroll
-                        for (int x = 0; x < 16; ++x) pr.acc[i][j][x] -= bf16_to_f32((uint16_t)rne_bf16(pr.acc[i][j][x]));
-                    put(1);
-                }
+                    for (int x = 0; x < 16; ++x) pr.acc[i][j][x] -= bf16_to_f32((uint16_t)rne_bf16(pr.acc[i][j][x]));
+                put(low);
             }
         }
         if (!more) return;
@@ -413,7 +413,7 @@ __global__ __launch_bounds__(64 * Shape<T>::NW, WPS) void piece_kernel(HeadArgs 
     const int wm = wave / SH::WN, wn = wave % SH::WN;
     const int count = kept_rows(a);
     const float unit = OUT == OUT_SLOTS ? 1.0f : unit_of(a, count);
-    const int M = KIND == HD_DX ? a.lo + count : a.vn, K = KIND == HD_DX ? a.vn : count;
+    const int low = low_of(a, count), M = KIND == HD_DX ? low + count : a.vn, K = KIND == HD_DX ? a.vn : count;
     int mt, nt, split;
     if (!find_tile(blockIdx.x, (M + T - 1) / T, a.tiles_n, a.splits, mt, nt, split)) return;
     const int m0 = mt * T, n0 = nt * T;
@@ -436,14 +436,12 @@ __global__ __launch_bounds__(64 * Shape<T>::NW, WPS) void piece_kernel(HeadArgs 
             pr.run(lds_p, lds_q, {a.g + (int64_t)m0 * a.ldg, a.ldg, min(T, M - m0), 0, min(vn8, kb + slabs * BK)},
                    {a.w + (int64_t)a.v0 * a.d + n0, a.d, 0, a.d - n0, kend}, kb, slabs);
         else
-            pr.run(lds_p, lds_q, {a.g + m0, a.ldg, 0, vn8 - m0, kend}, {a.x + n0, a.d, 0, a.d - n0, kend}, kb, slabs);
-        if constexpr (KIND == HD_DW && T < 256) {
-            if (a.lo) {
+            for (int first = 0;; first = low) {
+                pr.run(lds_p, lds_q, {a.g + (int64_t)first * a.ldg + m0, a.ldg, 0, vn8 - m0, kend}, {a.x + n0, a.d, 0, a.d - n0, kend}, kb, slabs);
+                if (first == low) break;
                 wait_vm<0>();
                 asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-                pr.run(lds_p, lds_q, {a.g + (int64_t)a.lo * a.ldg + m0, a.ldg, 0, vn8 - m0, kend}, {a.x + n0, a.d, 0, a.d - n0, kend}, kb, slabs);
             }
-        }
     }
     wait_vm<0>();
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
@@ -451,7 +449,7 @@ __global__ __launch_bounds__(64 * Shape<T>::NW, WPS) void piece_kernel(HeadArgs 
     asm volatile("" : "+v"(etid));
     const int elane = etid & 63, r32 = elane & 31, khalf = elane >> 5;
     if constexpr (OUT == OUT_SLOTS) {
-        const int64_t rows = KIND == HD_DX ? a.lo + a.rows : a.vn;
+        const int64_t rows = KIND == HD_DX ? a.g_rows : a.vn;
 #pragma unroll
         for (int i = 0; i < FM; ++i) {
             const int m = m0 + wm * SH::TM + 32 * i + r32;
@@ -514,7 +512,8 @@ __global__ __launch_bounds__(256) void dx_kernel(HeadArgs a, uint16_t *dx) {
     const int rows = a.rows, d = a.d;
     const int32_t *const pos = a.kept + 1 + 2 * (int64_t)rows;
     const int64_t chunks = (int64_t)rows * (d / 8);
-    const float unit = unit_of(a, kept_rows(a));
+    const int count = kept_rows(a), low = low_of(a, count);
+    const float unit = unit_of(a, count);
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < chunks; i += (int64_t)gridDim.x * 256) {
         const int64_t n = i / (d / 8);
         const int c = (int)(i % (d / 8)) * 8, p = pos[n];
@@ -522,11 +521,11 @@ __global__ __launch_bounds__(256) void dx_kernel(HeadArgs a, uint16_t *dx) {
         if (p >= 0)
             for (int s = 0; s < a.splits; ++s) {
                 float h[8];
-                load_f32x8<true>(a.slots, ((int64_t)s * (a.lo + rows) + p) * d + c, 8, h);
+                load_f32x8<true>(a.slots, ((int64_t)s * a.g_rows + p) * d + c, 8, h);
 #pragma unroll
                 for (int x = 0; x < 8; ++x) f[x] += h[x];
-                if (!a.lo) continue;
-                load_f32x8<true>(a.slots, ((int64_t)s * (a.lo + rows) + a.lo + p) * d + c, 8, h);
+                if (!low) continue;
+                load_f32x8<true>(a.slots, ((int64_t)s * a.g_rows + low + p) * d + c, 8, h);
 #pragma unroll
                 for (int x = 0; x < 8; ++x) f[x] += h[x];
             }
@@ -609,7 +608,8 @@ constexpr int64_t PIECE_WORDS = 1 << 18;              // at most: a slab's rows 
 // joins them: a launch less each (7 rows, 512 words of 256: 78 us a pass with the launches, 71 so).
 constexpr int64_t FEW_ROWS = 32, FEW_PARTS = 1 << 12;
 // Of so few rows the roundings of G's largest elements do not average out over a gradient's sums, and the products' tiles have rows to
-// spare: there G / c is the sum of two bf16 numbers, in tiles of up to 128.  Each row has its own g for the reduction "none", which c
+// spare: there G / c is the sum of two bf16 numbers.  The rows that count decide, so the kernels do: a padded batch of thousands of
+// rows has its second numbers behind the first ones in the same space.  Each row has its own g for the reduction "none", which c
 // does not take out, so there more rows count as few.  Largest of 12 errors against 64 bits, where the rounding of the results is 0.0017:
 // with one number 33 rows, 512 words of 256 0.0022 (0.0027 "none"), 128 rows, 896 words of 144 0.0021 (0.0025); with two 0.0017.
 // us of backward passes: 7 rows, 512 words of 256 15.3 with one and 16.9 with two, 128256 of 4096 584 and 636, 64 rows of the latter
@@ -618,7 +618,7 @@ constexpr int64_t LO_ROWS = 32, LO_ROWS_NONE = 128;
 
 struct HeadPlan {
     Tiling fwd, logits, dx, dw;
-    int64_t piece, ldg, lo;                            // words of a piece
+    int64_t piece, ldg, few, g_rows;                   // words of a piece
     size_t fwd_bytes, bwd_bytes, g_at, dx_at, dw_at;
 };
 static size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
@@ -633,21 +633,23 @@ static HeadPlan head_plan(int64_t rows, int64_t vocab, int64_t d, int32_t reduct
     const int64_t pieces = (vocab + most - 1) / most;
     p.piece = std::min<int64_t>(((vocab + pieces - 1) / pieces + 255) / 256 * 256, (vocab + 7) / 8 * 8);
     p.ldg = p.piece;
-    p.lo = rows <= (reduction == HEAD_NONE ? LO_ROWS_NONE : LO_ROWS) ? rows : 0;
-    const int most_tile = p.lo ? 128 : 256;
+    p.few = std::min<int64_t>(rows, reduction == HEAD_NONE ? LO_ROWS_NONE : LO_ROWS);
+    p.g_rows = std::max(rows, 2 * p.few);
+    const int64_t products = p.few == rows ? 2 * rows : rows;   // rows of G, if all count
+    const int most_tile = p.few == rows ? 128 : 256;
     p.logits = tiling(rows, p.piece, d, 0, most_tile);
-    p.dx = tiling(p.lo + rows, d, p.piece, 1, most_tile);
+    p.dx = tiling(products, d, p.piece, 1, most_tile);
     p.dw = tiling(p.piece, d, rows, 2, most_tile);
     p.g_at = 0;
-    p.dx_at = up256((size_t)(p.lo + rows) * (size_t)p.ldg * 2);
-    p.dw_at = p.dx_at + up256((size_t)p.dx.splits * (size_t)(p.lo + rows) * (size_t)d * 4);
+    p.dx_at = up256((size_t)p.g_rows * (size_t)p.ldg * 2);
+    p.dw_at = p.dx_at + up256((size_t)p.dx.splits * (size_t)p.g_rows * (size_t)d * 4);
     p.bwd_bytes = p.dw_at + (p.dw.splits > 1 ? up256((size_t)p.dw.splits * (size_t)p.piece * (size_t)d * 4) : 0);
     return p;
 }
 
 static int64_t tiles_of(int64_t M, int64_t N, const Tiling &t) { return (M + t.tile - 1) / t.tile * ((N + t.tile - 1) / t.tile) * t.splits; }
 static int head_grids(const char *name, const HeadPlan &p, int64_t rows, int64_t vocab, int64_t d) {
-    const int64_t most = std::max({tiles_of(rows, vocab, p.fwd), tiles_of(rows, p.piece, p.logits), tiles_of(p.lo + rows, d, p.dx), tiles_of(p.piece, d, p.dw)});
+    const int64_t most = std::max({tiles_of(rows, vocab, p.fwd), tiles_of(rows, p.piece, p.logits), tiles_of(p.g_rows, d, p.dx), tiles_of(p.piece, d, p.dw)});
     if (most < (1 << 22)) return MSR_OK;       // 512 threads each: fewer than 2^31 in a launch
     set_error("%s: too many tiles for a launch (%lld)", name, (long long)most);
     return MSR_ERR_ARG;
@@ -665,7 +667,7 @@ static int logits_launch(const HeadArgs &a, int T, int64_t tiles, hipStream_t s)
 
 template <int KIND, int OUT>
 static int piece_launch(HeadArgs a, const Tiling &t, hipStream_t s) {
-    const int64_t M = KIND == HD_DX ? a.lo + a.rows : a.vn;
+    const int64_t M = KIND == HD_DX ? a.g_rows : a.vn;
     a.tiles_n = (a.d + t.tile - 1) / t.tile;
     a.splits = t.splits;
     const unsigned grid = (unsigned)((M + t.tile - 1) / t.tile * a.tiles_n * t.splits);
@@ -817,7 +819,7 @@ int msr_head_backward(const uint16_t *packed, const uint16_t *w, const int32_t *
     HeadArgs a{};
     char *const ws = static_cast<char *>(workspace);
     a.x = packed; a.w = w; a.kept = kept; a.sums = reinterpret_cast<float2 *>(const_cast<float *>(sums)); a.dloss = dloss;
-    a.g = reinterpret_cast<uint16_t *>(ws); a.ldg = p.ldg; a.lo = (int)p.lo; a.out = dw;
+    a.g = reinterpret_cast<uint16_t *>(ws); a.ldg = p.ldg; a.few = (int)p.few; a.g_rows = (int)p.g_rows; a.out = dw;
     a.rows = (int)rows; a.vocab = (int)vocab; a.d = (int)d; a.reduction = reduction; a.zero_init = zero_init != 0;
     a.ns.key = seed_key(seed, 0);
     a.ns.inject = inject;

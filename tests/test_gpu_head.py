@@ -414,3 +414,47 @@ def test_weights_beyond_32_bit_offsets(L):
     want = torch.full((40, d), 0.01, dtype=BF16, device=DEV)
     check(L, L.msr_sr_accum(want.data_ptr(), dw[first:].contiguous().data_ptr(), 0, want.numel(), 0, 0, _lib.NOISE_INJECT, noise.data_ptr(), stream()))
     assert torch.equal(head.weight.acc_grad[first:], want)
+
+
+@pytest.mark.parametrize("rows,vocab,d", [(100, 512, 256), (260, 40001, 72), (2047, 3001, 1024), (4096, 8200, 384), (4096, 8200, 2048), (16384, 17001, 64)])
+@pytest.mark.parametrize("kept", [1, 5, 14, 32, 100, 128])
+def test_few_rows_of_a_padded_batch(rows, vocab, d, kept):
+    """The rows that count decide whether G is kept as two numbers (up to 32, 128 where each has its own g), in tiles of every size: their results
+    are as near as those of a call of these rows alone.  The other rows' gradients are 0."""
+    kept = min(kept, rows - 1)
+    x, w, target, dloss = make(rows, vocab, d, rows + kept, ignored=0.0)
+    on = torch.sort(torch.randperm(rows, generator=gen(kept), device=DEV)[:kept]).values
+    off = torch.ones(rows, dtype=torch.bool, device=DEV)
+    off[on] = False
+    target[off] = -100
+    for reduction in ("mean", "none"):
+        if kept > 32 and reduction == "mean":
+            continue
+        some = dloss[on] if reduction == "none" else dloss
+        want = exact(x[on], w, target[on], some, reduction)
+        loss, dx, dw = run(x, w, target, dloss, reduction)
+        near(loss[on] if reduction == "none" else loss, want[0])
+        near(dx[on], want[1])
+        near(dw, want[2])
+        assert not dx[off].any()
+
+
+def test_accumulated_gradient_of_few_rows_of_a_padded_batch(L):
+    """As the stored one and msr_sr_accum, where G's second numbers are in use in tiles of 256 and of 128."""
+    import muon_sr_amd as M
+    from muon_sr_amd import _lib
+    for rows, vocab, d in ((4096, 8200, 2048), (4096, 8200, 384)):
+        x, w, target, dloss = make(rows, vocab, d, 21)
+        target[9:] = -100
+        head = M.SRHead(d, vocab, device=DEV)
+        with torch.no_grad():
+            head.weight.copy_(w)
+        acc = torch.randn((vocab, d), generator=gen(22), device=DEV).to(BF16)
+        head.weight.acc_grad = acc.clone()
+        random.seed(3)
+        seed = random.getrandbits(32)
+        random.seed(3)
+        head.loss(x, target).backward(dloss[0])
+        dw = run(x, w, target, dloss, "mean")[2]
+        check(L, L.msr_sr_accum(acc.data_ptr(), dw.data_ptr(), 0, dw.numel(), seed, 0, _lib.noise_mode(), None, stream()))
+        assert torch.equal(head.weight.acc_grad, acc)
