@@ -11,6 +11,8 @@ nor a gradient.  The reference's training loops call torch's cross entropy on a 
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from . import _lib
@@ -35,13 +37,24 @@ class SRHead(SRLinear):
     ``linear_cross_entropy`` whose weight gradient is accumulated into ``weight.acc_grad`` with stochastic rounding
     inside the product (for training with ``TritonSRAccumulator``).  The accumulator is the
     parameter's under activation checkpointing and other saved-tensor hooks too; a parametrized weight's
-    gradient goes to autograd."""
+    gradient goes to autograd.
+
+    ``loss`` is a call of the module: its forward hooks and pre-hooks run, with ``loss``'s arguments and its result (those of a
+    subclass with a ``forward`` of its own, which takes ``x`` alone, do not)."""
 
     def __init__(self, in_features: int, vocab: int, device=None, dtype=torch.bfloat16):
         super().__init__(in_features, vocab, bias=False, device=device, dtype=dtype)
 
-    def loss(self, x: torch.Tensor, target: torch.Tensor, ignore_index: int = -100, reduction: str = "mean") -> torch.Tensor:
+    def forward(self, x: torch.Tensor, *loss):
+        """Logits; with the other arguments of ``loss``, the loss."""
+        if not loss:
+            return super().forward(x)
         weight = self.weight
         # a weight that is computed (a parametrization) holds nothing that lasts: autograd gets its gradient
         accumulate = weight.is_leaf and weight.requires_grad and torch.is_grad_enabled()
-        return _lib.nodes().linear_cross_entropy(x, weight, target, ignore_index, reduction, accumulate)
+        return _lib.nodes().linear_cross_entropy(x, weight, *loss, accumulate)
+
+    def loss(self, x: torch.Tensor, target: torch.Tensor, ignore_index: int = -100, reduction: str = "mean") -> torch.Tensor:
+        # (a hook may compute the weight, as torch.nn.utils.weight_norm's does)
+        call = self if getattr(type(self), "forward", None) is SRHead.forward else functools.partial(SRHead.forward, self)
+        return call(x, target, ignore_index, reduction)

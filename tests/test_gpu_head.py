@@ -458,3 +458,32 @@ def test_accumulated_gradient_of_few_rows_of_a_padded_batch(L):
         dw = run(x, w, target, dloss, "mean")[2]
         check(L, L.msr_sr_accum(acc.data_ptr(), dw.data_ptr(), 0, dw.numel(), seed, 0, _lib.noise_mode(), None, stream()))
         assert torch.equal(head.weight.acc_grad, acc)
+
+
+def test_hooks_see_the_loss():
+    """Forward hooks and pre-hooks of the module run around its loss; a weight that torch.nn.utils' weight_norm or spectral_norm computes
+    in a pre-hook is that of the parameters as they are, and its gradient goes to them."""
+    import muon_sr_amd as M
+    x, _, target, _ = make(50, 100, 64, 23)
+    plain = M.SRHead(64, 100, device=DEV)
+    seen = []
+    plain.register_forward_pre_hook(lambda m, args: (2 * args[0], *args[1:]))
+    plain.register_forward_hook(lambda m, args, out: seen.append(out))
+    loss = plain.loss(x, target)
+    assert torch.equal(loss, M.linear_cross_entropy(2 * x, plain.weight, target)) and seen[0] is loss
+    for norm, leaf in ((torch.nn.utils.weight_norm, "weight_g"), (torch.nn.utils.spectral_norm, "weight_orig")):
+        head = norm(M.SRHead(64, 100, device=DEV))
+        head.eval()                                        # (spectral_norm's estimate stays)
+        head.loss(x, target)
+        with torch.no_grad():
+            getattr(head, leaf).mul_(3)
+        loss = head.loss(x, target)
+        if norm is torch.nn.utils.weight_norm:
+            v = head.weight_v.detach()
+            weight = torch._weight_norm(v, head.weight_g.detach(), 0)
+        else:
+            weight = head.weight_orig.detach()
+            weight = weight / torch.dot(head.weight_u, torch.mv(weight, head.weight_v))
+        assert torch.equal(loss, M.linear_cross_entropy(x, weight, target))
+        loss.backward()
+        assert getattr(head, leaf).grad is not None and not hasattr(head.weight, "acc_grad")

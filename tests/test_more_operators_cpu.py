@@ -150,3 +150,31 @@ def test_python_needs_a_gpu():
     # the modules' states are torch's
     assert set(head.state_dict()) == {"weight"} and set(table.state_dict()) == {"weight"} and set(norm.state_dict()) == {"weight", "bias"}
     assert head.weight.shape == (9, 16) and head.weight.dtype == table.weight.dtype == torch.bfloat16 and not table.weight[2].any()
+
+
+def test_hooks_of_the_head_see_its_loss():
+    """A loss is a call of the module: its pre-hooks run before the arguments are checked (here: that they are on a GPU), with the loss's
+    arguments; torch.nn.utils.weight_norm's computes the weight.  A subclass whose forward takes x alone keeps its loss."""
+    import muon_sr_amd as M
+    x, ids = torch.zeros((4, 16), dtype=torch.bfloat16), torch.zeros(4, dtype=torch.int64)
+    head, seen = M.SRHead(16, 9), []
+    torch.nn.utils.weight_norm(head)
+    head.register_forward_pre_hook(lambda module, args: seen.append(args))
+    with torch.no_grad():
+        head.weight_g.mul_(2)
+    before = head.weight.clone()
+    with pytest.raises(ValueError, match="GPU"):
+        head.loss(x, ids, reduction="sum")
+    (args,) = seen
+    assert args[0] is x and args[1] is ids and args[2:] == (-100, "sum")
+    assert torch.equal(head.weight, 2 * before)
+
+    class Last(M.SRHead):
+        def forward(self, x):
+            return super().forward(x[-1:])
+    last = Last(16, 9)
+    assert last(x).shape == (1, 9)
+    with pytest.raises(ValueError, match="GPU"):
+        last.loss(x, ids)
+    with pytest.raises(TypeError):
+        head.loss(x, None)
