@@ -64,6 +64,16 @@ class SREmbedding(torch.nn.Embedding):
         super().__init__(num_embeddings, embedding_dim, padding_idx=padding_idx, device=device, dtype=dtype)
         self.scale = float(scale)
 
+    @classmethod
+    def from_pretrained(cls, embeddings: torch.Tensor, freeze: bool = True, padding_idx: int = None, *, scale: float = 1.0):
+        """The module whose weight is ``embeddings`` [vocab, d] (not a copy), frozen unless ``freeze`` is False; ``nn.Embedding``'s other options
+        are not taken."""
+        if embeddings.dim() != 2:
+            raise ValueError(f"SREmbedding.from_pretrained needs embeddings [vocab, d], got {tuple(embeddings.shape)}")
+        module = cls(*embeddings.shape, padding_idx=padding_idx, scale=scale, device="meta", dtype=embeddings.dtype)
+        module.weight = torch.nn.Parameter(embeddings, requires_grad=not freeze)
+        return module
+
     def forward(self, ids: torch.Tensor) -> torch.Tensor:
         weight = self.weight
         # a weight that is computed (a parametrization) holds nothing that lasts, and one that is not bf16 has no accumulator: autograd

@@ -266,3 +266,17 @@ def test_weights_beyond_32_bit_offsets(L):
         assert torch.equal(w.acc_grad[first:], torch.where((count > 0)[:, None], want, 0.5))
         assert torch.equal((w.acc_grad != 0.5).any(1).nonzero().flatten(), ids.unique())
         del w.acc_grad, dw
+
+
+def test_from_pretrained():
+    """The module of given embeddings looks them up, and accumulates where it is not frozen."""
+    import muon_sr_amd as M
+    ids, w, dy = make(700, 90, 24, BF16, 10)
+    assert torch.equal(M.SREmbedding.from_pretrained(w, scale=2.0)(ids), run(ids, w, dy, 2.0)[0])
+    layer = M.SREmbedding.from_pretrained(w, freeze=False, padding_idx=3)
+    random.seed(1)
+    layer(ids).backward(dy)
+    want = torch.nn.Parameter(w)
+    random.seed(1)
+    M.embedding_grad_sr_accum(want, ids, dy, padding_idx=3)
+    assert layer.weight.grad is None and torch.equal(layer.weight.acc_grad, want.acc_grad)

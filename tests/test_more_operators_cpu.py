@@ -178,3 +178,22 @@ def test_hooks_of_the_head_see_its_loss():
         last.loss(x, ids)
     with pytest.raises(TypeError):
         head.loss(x, None)
+
+
+def test_embedding_from_pretrained():
+    """As nn.Embedding's: the weight is the given tensor, frozen unless asked; options that are not taken are refused."""
+    import muon_sr_amd as M
+    for dtype in (torch.bfloat16, torch.float32):
+        table = torch.randn((9, 16)).to(dtype)
+        m = M.SREmbedding.from_pretrained(table)
+        theirs = torch.nn.Embedding.from_pretrained(table)
+        assert isinstance(m, M.SREmbedding) and m.weight.data_ptr() == table.data_ptr() and not m.weight.requires_grad
+        assert (m.num_embeddings, m.embedding_dim, m.padding_idx) == (theirs.num_embeddings, theirs.embedding_dim, theirs.padding_idx)
+        m = M.SREmbedding.from_pretrained(table, False, -1, scale=4.0)
+        assert m.weight.requires_grad and m.weight.is_leaf and m.padding_idx == 8 and m.scale == 4.0
+        assert torch.equal(m.weight, table) and m.state_dict().keys() == theirs.state_dict().keys()
+    with pytest.raises(ValueError, match="vocab"):
+        M.SREmbedding.from_pretrained(table[0])
+    for bad in (dict(max_norm=1.0), dict(sparse=True)):
+        with pytest.raises(TypeError):
+            M.SREmbedding.from_pretrained(table, **bad)
