@@ -1,7 +1,7 @@
 """Builds libmuon_sr_amd.so (the gfx950 HIP kernels + C ABI) and _nodes.so (autograd nodes that call it) in-tree.
 
 The library depends only on the HIP runtime; it is loaded with ctypes.  _nodes.so is host code against torch's C++
-headers, a Python module; it finds the library beside itself.
+headers, a Python module; it finds the library beside itself.  The library is built whether or not they can be.
 """
 from __future__ import annotations
 
@@ -45,7 +45,7 @@ _NOISE = "is not a recognized feature for this target"  # hipcc host pass; harml
 def _finish(cmd, res, verbose):
     err = "\n".join(line for line in res.stderr.splitlines() if _NOISE not in line)
     if res.returncode != 0:
-        raise RuntimeError(f"hipcc failed ({res.returncode}): {' '.join(cmd)}\n{err}")
+        raise RuntimeError(f"{os.path.basename(cmd[0])} failed ({res.returncode}): {' '.join(cmd)}\n{err}")
     if verbose and err.strip():
         print(err)
 
@@ -71,7 +71,8 @@ def nodes_commands(obj: str, out: str):
 
 def build(verbose: bool = False) -> str:
     """Compile every HIP source (each with its own flags, all at once) and link one
-    shared library, then the autograd nodes.  Always recompiles; objects go to muon_sr_amd/_build/."""
+    shared library, then the autograd nodes.  Always recompiles; objects go to muon_sr_amd/_build/.  Where the nodes cannot be built (no g++, no
+    headers of Python or torch) the library is there all the same when the error is raised."""
     objdir = os.path.join(HERE, "_build")
     os.makedirs(objdir, exist_ok=True)
     objs, jobs = [], []
@@ -79,23 +80,39 @@ def build(verbose: bool = False) -> str:
     def start(cmd):
         if verbose:
             print(" ".join(cmd), flush=True)
-        jobs.append((cmd, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.PIPE, text=True)))
+        return cmd, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.PIPE, text=True)
 
-    nodes_compile, nodes_link = nodes_commands(os.path.join(objdir, "nodes.cpp.o"), NODES + ".tmp")
-    start(nodes_compile)
+    def end(cmd, proc):
+        out, err = proc.communicate()
+        _finish(cmd, subprocess.CompletedProcess(cmd, proc.returncode, out, err), verbose)
+
+    nodes = failed = None
+    try:
+        nodes_compile, nodes_link = nodes_commands(os.path.join(objdir, "nodes.cpp.o"), NODES + ".tmp")
+        nodes = start(nodes_compile)
+    except (ImportError, OSError) as e:
+        failed = e
     for src in sources():
         obj = os.path.join(objdir, os.path.basename(src) + ".o")
         flags = [f for f in HIPCC_FLAGS if f != "-shared"]
-        cmd = [hipcc(), *flags, *EXTRA_FLAGS.get(os.path.basename(src), []), "-c", "-o", obj, src]
-        start(cmd)
+        jobs.append(start([hipcc(), *flags, *EXTRA_FLAGS.get(os.path.basename(src), []), "-c", "-o", obj, src]))
         objs.append(obj)
-    for cmd, proc in jobs:
-        out, err = proc.communicate()
-        _finish(cmd, subprocess.CompletedProcess(cmd, proc.returncode, out, err), verbose)
+    for job in jobs:
+        end(*job)
     tmp = LIB + ".tmp"
     _run([hipcc(), f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", tmp, *objs], verbose)
+    # (nodes of an earlier build know that build's library)
+    if os.path.exists(NODES):
+        os.remove(NODES)
     os.replace(tmp, LIB)
-    _run(nodes_link, verbose)
+    try:
+        if failed is not None:
+            raise failed
+        end(*nodes)
+        _run(nodes_link, verbose)
+    except (ImportError, OSError, RuntimeError) as e:
+        raise RuntimeError(f"{LIB} is built, but not the autograd nodes of layer_norm, embedding, linear_cross_entropy and balance_loss, "
+                           f"which need g++ and the headers of Python and torch: {e}") from e
     os.replace(NODES + ".tmp", NODES)
     return LIB
 
