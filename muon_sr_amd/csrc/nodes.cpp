@@ -111,8 +111,8 @@ Rows flat_rows(const Tensor &t, int64_t d) {
     return r;
 }
 Tensor contiguous(const Tensor &t) { return t.defined() ? t.contiguous() : t; }
-// contiguous and 16-byte aligned
-Tensor packed_rows(const Tensor &t) {
+// contiguous and 16-byte aligned, as saved tensors were made and their hooks may not give them back
+Tensor aligned(const Tensor &t) {
     const Tensor c = t.contiguous();
     return (uintptr_t)c.const_data_ptr() % 16 ? c.clone() : c;
 }
@@ -264,7 +264,7 @@ struct HeadLoss : torch::autograd::Function<HeadLoss> {
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads) {
         const variable_list saved = ctx->get_saved_variables();   // saved-tensor hooks may have changed their strides
-        const Tensor packed = packed_rows(saved[0]), w = packed_rows(saved[1]), kept = saved[2].contiguous(), sums = saved[3].contiguous(),
+        const Tensor packed = aligned(saved[0]), w = aligned(saved[1]), kept = saved[2].contiguous(), sums = aligned(saved[3]),
                      dloss = grads[0].contiguous();
         const int64_t n = packed.size(0), vocab = w.size(0), d = w.size(1), reduction = ctx->saved_data["reduction"].toInt();
         const Tensor dx = ctx->needs_input_grad(0) ? empty(ctx->saved_data["shape"].toIntVector(), packed, at::kBFloat16) : Tensor();

@@ -291,3 +291,19 @@ def test_example_uses_them():
     # the logits that torch gives are rounded to bf16, 2^-8 of up to their largest
     want = torch.nn.functional.cross_entropy(logits.double(), window[:, 4])
     assert abs(loss.item() - want.item()) <= 2 * H * logits.abs().max().item() + 1e-5
+
+
+def shifted(f, *args):
+    """Tensors come back one element behind the start of their memory, as those of a buffer that they share."""
+    def behind(t):
+        flat = torch.empty(t.numel() + 1, dtype=t.dtype, device=t.device)
+        flat[1:] = t.flatten()
+        return flat[1:].view(t.shape)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.clone(), behind):
+        return f(*args)
+
+
+def test_saved_tensors_of_a_shared_buffer():
+    """Such hooks change no bit, and refuse nothing, with the accumulators and without."""
+    test_saved_tensors(shifted)
+    test_accumulators_under_saved_tensor_hooks(shifted)
