@@ -487,7 +487,7 @@ int msr_experts_wgrad_sr_accum(uint16_t *acc, const uint16_t *x, int64_t ldx, co
  * reduction: MSR_LOSS_NONE (loss [rows]), _SUM or _MEAN over the rows that are not
  * ignored (loss [1]; 0 where there are none).  Products are of bf16 operands with
  * fp32 accumulation, dx and dW rounded once.  G is rounded to bf16, without the significand of
- * the first row's dloss; of up to 32 rows that are not ignored (128 with MSR_LOSS_NONE) it is kept as two
+ * the first row's dloss, and but for the targets' elements in dx; of up to 32 rows that are not ignored (128 with MSR_LOSS_NONE) it is kept as two
  * bf16 numbers.
  * Logits of a magnitude below 2^127.
  *

@@ -6,10 +6,13 @@
 // the two products that follow.  8 rows vocab d flop with gradients where 6 are the least; the logits kept in fp32 would be 4.2 GB
 // for 8192 rows of 128256 words.
 //
-// What is stored is G / c: c is the significand of the first row's g (every row's, but for the reduction "none"), by which the products'
-// sums are multiplied in fp32.  The target's element of an unlikely word is -g, a factor of its whole row: rounded with g, every such
-// row would be off by the same share, up to 2^-8 (8192 rows, 128256 words of 4096, gradients against 64 bits: 0.0021 or, at an unlucky
-// g, 0.0030, and 0.0018 so at any; 0.0017 is the rounding of the results).
+// What is stored is G / c, rounded to bf16: c is the significand of the first row's g (every row's, but for the reduction "none"), by which
+// the products' sums are multiplied in fp32.  The target's element of an unlikely word is -g, a factor of its whole row: rounded with g, every
+// such row would be off by the same share, up to 2^-8.  In dx, which has one such element to a row, what its rounding leaves is added
+// exactly (rest W[t], by dx_kernel).  In dW it stays.  Gradients against 64 bits, dx and dW, where the rounding of the results is 0.0017: 8192 rows,
+// 128256 words of 4096 0.0017 and 0.0019 (0.0019 and 0.0019 without the rest); 8192 rows, 32000 words of 2048 of the reduction "none",
+// where c takes out the first row's significand alone, 0.0017 and 0.0022 (0.0022 both).  G as the sum of two bf16 numbers gives 0.0017
+// throughout and takes 1.7 times as long (backward passes of these 21.2 and 35.8, 2.78 and 4.68 ms), so only few rows have it (LO_ROWS).
 //
 // Rows that are ignored take part in nothing: list_kernel numbers the others, pack_kernel lays them out one after the
 // other (kept for the backward pass in x's place), and every kernel after it works on *count rows.  What an ignored row holds,
@@ -33,6 +36,7 @@ struct HeadArgs {
     float *picked;               // [rows]: S[n][t[n]]
     const float *dloss;          // [rows] in the given order, or one
     uint16_t *g;                 // [g_rows][ldg]: a piece of G / c, of few rows two numbers (low_of)
+    float *rest;                 // [rows]: what rounding leaves of the target's element of G / c
     float *slots;                // fp32 sums [splits][g_rows][d] of dx, [splits][words of the piece][d] of dW
     uint16_t *out;               // dW or the accumulator
     int64_t ldg;
@@ -301,12 +305,17 @@ __global__ __launch_bounds__(64 * Shape<T>::NW, 2) void logits_kernel(HeadArgs a
                 for (int j = 0; j < FN; ++j)
 #pragma unroll
                     for (int x = 0; x < 16; ++x) pr.acc[i][j][x] = share[i] * exp_from(pr.acc[i][j][x], M[i]);
-                if (__any(rel >= 0 && rel < TN && !(rel & 4))) {
+                const bool mine = rel >= 0 && rel < TN && !(rel & 4);
+                if (__any(mine)) {
+                    float rest = 0.0f;
 #pragma unroll
                     for (int j = 0; j < FN; ++j)
 #pragma unroll
                         for (int x = 0; x < 16; ++x)
-                            if (rel == 32 * j + 8 * (x >> 2) + (x & 3)) pr.acc[i][j][x] -= g;
+                            if (rel == 32 * j + 8 * (x >> 2) + (x & 3)) rest = pr.acc[i][j][x] -= g;
+                    rest -= bf16_to_f32((uint16_t)rne_bf16(rest));
+                    if (low) rest -= bf16_to_f32((uint16_t)rne_bf16(rest));
+                    if (mine) a.rest[m1 + 32 * i] = rest;
                 }
                 auto put = [&](int first) __attribute__((always_inline)) {
 #pragma unroll
@@ -507,7 +516,8 @@ __global__ __launch_bounds__(64 * Shape<T>::NW, WPS) void piece_kernel(HeadArgs 
     }
 }
 
-// The sum of a row's slots times c, rounded: dx of every row (0 for an ignored one), 8 elements per thread
+// The sum of a row's slots and of what the target's element of G / c left, times W[target], times c, rounded: dx of every row (0 for an
+// ignored one), 8 elements per thread
 __global__ __launch_bounds__(256) void dx_kernel(HeadArgs a, uint16_t *dx) {
     const int rows = a.rows, d = a.d;
     const int32_t *const pos = a.kept + 1 + 2 * (int64_t)rows;
@@ -518,7 +528,15 @@ __global__ __launch_bounds__(256) void dx_kernel(HeadArgs a, uint16_t *dx) {
         const int64_t n = i / (d / 8);
         const int c = (int)(i % (d / 8)) * 8, p = pos[n];
         float f[8] = {};
-        if (p >= 0)
+        if (p >= 0) {
+            const int word = word_of(a, p);
+            if (word != HEAD_BAD) {
+                const float rest = a.rest[p];
+                float h[8];
+                unpack8(reinterpret_cast<const Bytes16 *>(a.w + (int64_t)word * d + c)->w, h);
+#pragma unroll
+                for (int x = 0; x < 8; ++x) f[x] = rest * h[x];
+            }
             for (int s = 0; s < a.splits; ++s) {
                 float h[8];
                 load_f32x8<true>(a.slots, ((int64_t)s * a.g_rows + p) * d + c, 8, h);
@@ -529,6 +547,7 @@ __global__ __launch_bounds__(256) void dx_kernel(HeadArgs a, uint16_t *dx) {
 #pragma unroll
                 for (int x = 0; x < 8; ++x) f[x] += h[x];
             }
+        }
 #pragma unroll
         for (int x = 0; x < 8; ++x) f[x] *= unit;
         st_nt4(dx + n * d + c, u32x4_t{rne_bf16x2(f[0], f[1]), rne_bf16x2(f[2], f[3]), rne_bf16x2(f[4], f[5]), rne_bf16x2(f[6], f[7])});
@@ -610,7 +629,7 @@ constexpr int64_t FEW_ROWS = 32, FEW_PARTS = 1 << 12;
 // Of so few rows the roundings of G's largest elements do not average out over a gradient's sums, and the products' tiles have rows to
 // spare: there G / c is the sum of two bf16 numbers.  The rows that count decide, so the kernels do: a padded batch of thousands of
 // rows has its second numbers behind the first ones in the same space.  Each row has its own g for the reduction "none", which c
-// does not take out, so there more rows count as few.  Largest of 12 errors against 64 bits, where the rounding of the results is 0.0017:
+// does not take out, so there more rows count as few.  Largest of 12 errors of dW against 64 bits, where the rounding of the results is 0.0017:
 // with one number 33 rows, 512 words of 256 0.0022 (0.0027 "none"), 128 rows, 896 words of 144 0.0021 (0.0025); with two 0.0017.
 // us of backward passes: 7 rows, 512 words of 256 15.3 with one and 16.9 with two, 128256 of 4096 584 and 636, 64 rows of the latter
 // 664 and 790.
@@ -619,7 +638,7 @@ constexpr int64_t LO_ROWS = 32, LO_ROWS_NONE = 128;
 struct HeadPlan {
     Tiling fwd, logits, dx, dw;
     int64_t piece, ldg, few, g_rows;                   // words of a piece
-    size_t fwd_bytes, bwd_bytes, g_at, dx_at, dw_at;
+    size_t fwd_bytes, bwd_bytes, g_at, rest_at, dx_at, dw_at;
 };
 static size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 
@@ -641,7 +660,8 @@ static HeadPlan head_plan(int64_t rows, int64_t vocab, int64_t d, int32_t reduct
     p.dx = tiling(products, d, p.piece, 1, most_tile);
     p.dw = tiling(p.piece, d, rows, 2, most_tile);
     p.g_at = 0;
-    p.dx_at = up256((size_t)p.g_rows * (size_t)p.ldg * 2);
+    p.rest_at = up256((size_t)p.g_rows * (size_t)p.ldg * 2);
+    p.dx_at = p.rest_at + up256((size_t)rows * 4);
     p.dw_at = p.dx_at + up256((size_t)p.dx.splits * (size_t)p.g_rows * (size_t)d * 4);
     p.bwd_bytes = p.dw_at + (p.dw.splits > 1 ? up256((size_t)p.dw.splits * (size_t)p.piece * (size_t)d * 4) : 0);
     return p;
@@ -823,6 +843,7 @@ int msr_head_backward(const uint16_t *packed, const uint16_t *w, const int32_t *
     a.rows = (int)rows; a.vocab = (int)vocab; a.d = (int)d; a.reduction = reduction; a.zero_init = zero_init != 0;
     a.ns.key = seed_key(seed, 0);
     a.ns.inject = inject;
+    a.rest = reinterpret_cast<float *>(ws + p.rest_at);
     float *const dxs = reinterpret_cast<float *>(ws + p.dx_at), *const dws = reinterpret_cast<float *>(ws + p.dw_at);
     const int T = p.logits.tile;
     for (int64_t v0 = 0; v0 < vocab && (dx || dw); v0 += p.piece) {
