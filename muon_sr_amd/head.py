@@ -5,9 +5,9 @@
 ``SRHead`` is ``SRLinear`` for the head (its call gives logits) with a ``loss`` whose weight
 gradient is accumulated into ``weight.acc_grad`` with stochastic rounding inside the product, with the arithmetic, seeds and
 noise of ``TritonSRAccumulator``'s hook (muon_sr/triton_adamw.py:206-229, 252-265).  Logits exist
-a tile at a time: the forward pass keeps each row's log-sum-exp, the backward pass forms them again, a piece of
-the vocabulary at a time.  Rows of ``ignore_index`` cost nothing, and what they hold (NaN too) reaches neither the loss
-nor a gradient.  The reference's training loops call torch's cross entropy on a linear layer.
+a tile at a time: the forward pass keeps a number near each row's largest logit and the sum of its exponentials from there, the backward
+pass forms the logits again, a piece of the vocabulary at a time.  Rows of ``ignore_index`` cost nothing, and what they hold (NaN too) reaches neither the
+loss nor a gradient.  The reference's training loops call torch's cross entropy on a linear layer.
 """
 from __future__ import annotations
 
@@ -27,8 +27,8 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     [..., d], ``weight``: bf16 [vocab, d], d a multiple of 8; ``target``: int32 or int64 [...].  ``reduction``
     ``"none"`` gives a loss per row, 0 for ignored ones, ``"sum"`` and ``"mean"`` sum them, over the rows that are not
     ignored (0 where all are: torch's mean is NaN there).  Any other target outside [0, vocab) gives NaN, in the loss
-    and the gradients.  The gradients are bf16, of products with fp32 accumulation; the weight gradient
-    goes to autograd (``TritonSRAccumulator``'s hook accumulates it as any other)."""
+    and the gradients.  The gradients are bf16, of products with fp32 accumulation whose operand, the logits' gradient, is bf16 too, as
+    in a training loop in bf16; the weight gradient goes to autograd (``TritonSRAccumulator``'s hook accumulates it as any other)."""
     return _lib.nodes().linear_cross_entropy(x, weight, target, ignore_index, reduction, False)
 
 
