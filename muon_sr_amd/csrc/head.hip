@@ -346,16 +346,30 @@ __global__ __launch_bounds__(64 * Shape<T>::NW, 2) void logits_kernel(HeadArgs a
     }
 }
 
+// The tiles' sets are joined with s in 64 bits: beside a tile that holds a row's nearly sure word, s near 1, each of the others may be
+// less than half an ulp, and hundreds of them more than what is left of the row's loss.
+struct Joined {
+    float m;
+    double s;
+};
+__device__ __forceinline__ Joined joined(Joined a, float m2, double s2) {
+    const float m = fmaxf(a.m, m2), at = m == -INFINITY ? 0.0f : m;
+    return {m, a.s * (double)__builtin_amdgcn_exp2f(a.m - at) + s2 * (double)__builtin_amdgcn_exp2f(m2 - at)};
+}
 // The sums and losses of 16 rows from their tiles' parts, 16 threads each
-__device__ __forceinline__ void join_rows(const HeadArgs &a, float *loss, int n0, int count, float2 (&part)[16][17]) {
+__device__ __forceinline__ void join_rows(const HeadArgs &a, float *loss, int n0, int count, Joined (&part)[16][17]) {
     const int r = threadIdx.x & 15, g = threadIdx.x >> 4, n = n0 + r;
-    float2 v = make_float2(-INFINITY, 0.0f);
+    Joined all{-INFINITY, 0.0};
     if (n < count)
-        for (int t = g; t < a.tiles_n; t += 16) v = joined(v, a.part[(int64_t)t * a.rows + n]);
-    part[g][r] = v;
+        for (int t = g; t < a.tiles_n; t += 16) {
+            const float2 tile = a.part[(int64_t)t * a.rows + n];
+            all = joined(all, tile.x, tile.y);
+        }
+    part[g][r] = all;
     __syncthreads();
     if (g == 0 && n < count) {
-        for (int k = 1; k < 16; ++k) v = joined(v, part[k][r]);
+        for (int k = 1; k < 16; ++k) all = joined(all, part[k][r].m, part[k][r].s);
+        const float2 v = make_float2(all.m, (float)all.s);
         a.sums[n] = v;
         const float l = logf(v.y) + LN2 * __builtin_fmaf(a.picked[n], -LOG2E, v.x);
         loss[a.reduction == HEAD_NONE ? a.kept[1 + n] : n] = word_of(a, n) == HEAD_BAD ? __builtin_nanf("") : l;
@@ -376,7 +390,7 @@ __device__ __forceinline__ void total_loss(const float *loss, int count, bool me
 }
 // total: the one work-group of a small call adds the losses up too
 __global__ __launch_bounds__(256) void join_kernel(HeadArgs a, float *loss, float *total) {
-    __shared__ float2 part[16][17];
+    __shared__ Joined part[16][17];
     const int count = kept_rows(a);
     for (int n0 = (int)blockIdx.x * 16; n0 < count; n0 += (int)gridDim.x * 16) join_rows(a, loss, n0, count, part);
     if (total) total_loss(loss, count, a.reduction == HEAD_MEAN, total);

@@ -511,3 +511,32 @@ def test_gradients_are_off_by_their_roundings_alone(rows, vocab, d, reduction):
     for got, want, model in ((dx[on], G @ W, own @ W), (dw, G.t() @ X, rounded.t() @ X)):
         want, error = c * want, torch.linalg.norm((c * model).to(BF16).double() - c * want)
         assert torch.linalg.norm(got.double() - want) <= 1.02 * error
+
+
+@pytest.mark.parametrize("rows,vocab", [(200, 9000), (300, 50000), (4096, 9000)])
+@pytest.mark.parametrize("size", [8.0, 40.0, 976.0])
+def test_nearly_sure_words_of_several_tiles(L, rows, vocab, size):
+    """Logits (exact in fp32) of `size` + 25 for the target, which lies in any of several tiles, and of `size` for the others, in more rows than G is
+    kept as two numbers for, and tiles of 64 to 256.  1 - p is (vocab - 1) exp(-25), 2 to 12 u, and a row's l has an ulp of 32 u and
+    more.  As in the test of a single tile 8 u bounds the loss and the target's element of G: the sum of the word's own tile may lose the tile's
+    others, 256 exp(-25) or 0.06 u, and the tiles' sums are joined in 64 bits (in 32 the other tiles, each less than half of 1's ulp, would leave
+    nothing: up to 12 u).  The others' elements of G are rounded to 2^-9 of themselves, all to the same side."""
+    words = torch.tensor([1, 63, 64, 300, 1111, 4095, 7000, vocab - 1], device=DEV)
+    k = torch.arange(rows, device=DEV) % 8
+    x = torch.zeros((rows, 16), dtype=BF16, device=DEV)
+    x[:, 0] = size
+    x[torch.arange(rows, device=DEV), 1 + k] = 25
+    w = torch.zeros((vocab, 16), dtype=BF16, device=DEV)
+    w[:, 0] = 1
+    w[words, 1 + torch.arange(8, device=DEV)] = 1
+    assert plan(L, rows, vocab, 16)[0] in ((64, 128) if rows < 300 else (256,))
+    loss, dx, _ = run(x, w, words[k], torch.ones(rows, device=DEV), "none")
+    one = math.exp(-25)
+    others = (vocab - 1) * one
+    assert ((loss.double() - math.log1p(others)).abs() <= 8 * U).all(), loss
+    assert (dx[:, 0].abs() <= 8 * U + H * others).all(), dx[:, 0]          # the sum of a row of G is 0
+    own = torch.zeros((rows, 8), dtype=torch.bool, device=DEV)
+    own[torch.arange(rows, device=DEV), k] = True
+    G = dx[:, 1:9].double()
+    assert ((G[own] + others / (1 + others)).abs() <= 8 * U + H * others).all(), G[own]
+    assert ((G[~own] - one / (1 + others)).abs() <= 2 * H * one).all()
