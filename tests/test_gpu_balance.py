@@ -190,3 +190,25 @@ def test_logits_far_from_zero_and_an_even_load(tokens, experts, offset):
     want = up.double() * p * (slope - dot)
     bound = up.double() * (ep * (slope - dot).abs() + p * (edot + 4 * U * slope)) + 4 * U * want.abs()
     assert ((d.double() - want).abs() <= bound).all()
+
+
+def test_more_than_2_31_elements():
+    """2.2 million tokens of 1024 experts: the counts are those of numpy, the last tokens' gradients those of the formula."""
+    tokens, experts = 2200000, 1024
+    g = gen(50)
+    logits = torch.randn((tokens, experts), generator=g, device=DEV, dtype=BF16)
+    ids = torch.randint(0, experts, (tokens, 1), generator=g, device=DEV)
+    loss, counts, d = run(logits, ids, None, torch.ones((), device=DEV))
+    assert torch.equal(counts.long(), torch.bincount(ids.flatten(), minlength=experts))
+    slope = counts.double() * experts / (float(tokens) * tokens)
+    total = sum((torch.softmax(part.double(), 1).sum(0) * slope).sum().item() for part in logits.split(50000))
+    # sums of tokens / 4096 probabilities in a lane, then of 16 waves' and of 256 work-groups'; a probability is off by 100 u of itself at most:
+    # 4 u (|x - max| + 1) for logits that are up to 11 apart, and 40 u for its sum and quotient
+    assert abs(loss.item() - total) <= (tokens / 4096 + 16 + 256 + 100) * U * total
+    p = torch.softmax(logits[-500:].double(), 1)
+    dot = (p * slope).sum(1, keepdim=True)
+    want = p * (slope - dot)
+    far = logits[-500:].double().amax(1, keepdim=True) - logits[-500:].double()
+    ep = p * (4 * U * (far + 1) + 40 * U)
+    bound = ep * (slope - dot).abs() + p * ((ep * slope).sum(1, keepdim=True) + 40 * U * dot + 4 * U * slope)
+    assert ((d[-500:].double() - want).abs() <= bound + UNIT[BF16] * (want.abs() + bound) + 2.0 ** -126).all()

@@ -307,3 +307,22 @@ def test_saved_tensors_of_a_shared_buffer():
     """Such hooks change no bit, and refuse nothing, with the accumulators and without."""
     test_saved_tensors(shifted)
     test_accumulators_under_saved_tensor_hooks(shifted)
+
+
+def test_transforms_and_forward_mode_are_refused():
+    """torch.func's transforms and forward-mode derivatives raise; none returns without a derivative."""
+    from torch.autograd import forward_ad
+    from muon_sr_amd import balance_loss, embedding, layer_norm, linear_cross_entropy
+    t = inputs(18)
+    chosen = torch.zeros((700, 2), dtype=torch.int64, device=DEV)
+    x = t["table"][t["ids"]]
+    calls = [(lambda v: linear_cross_entropy(v, t["head"], t["target"]), x), (lambda v: linear_cross_entropy(x, v, t["target"]), t["head"]),
+             (lambda v: layer_norm(v, t["w"], t["b"]), x), (lambda v: layer_norm(x, v, t["b"]), t["w"]), (lambda v: embedding(t["ids"], v), t["table"]),
+             (lambda v: balance_loss(v, chosen)[0], torch.zeros((700, 12), device=DEV))]
+    for f, v in calls:
+        for transform in (lambda: torch.func.grad(lambda z: f(z).float().sum())(v), lambda: torch.func.vmap(f)(torch.stack([v, v])),
+                          lambda: torch.func.jvp(f, (v,), (v,))):
+            with pytest.raises(RuntimeError, match="functorch"):
+                transform()
+        with forward_ad.dual_level(), pytest.raises(RuntimeError, match="jvp"):
+            f(forward_ad.make_dual(v, v))

@@ -247,3 +247,23 @@ def test_gradients_of_rows_far_from_zero(d):
     for got, want in zip(run(x, w, b, dy, 1e-6), exact_far(x, w, b, dy, 1e-6, depth)):
         near(got, want)
         assert torch.linalg.norm(want[1]) <= 3e-4 * torch.linalg.norm(want[0])
+
+
+@pytest.mark.parametrize("rows,d", [(600000, 4096), (120000, 20000)])
+def test_more_than_2_31_elements(rows, d):
+    """The last rows of y and dx are those of a call of them alone, bit for bit; dw and db are the sums over all rows."""
+    g = gen(50)
+    x, dy = (torch.randn((rows, d), generator=g, device=DEV, dtype=BF16) for _ in range(2))
+    _, w, b, _ = make(1, d, BF16, F32, 51)
+    y, dx, dw, db = run(x, w, b, dy)
+    last = slice(rows - 700, rows)
+    alone = run(x[last], w, b, dy[last])
+    assert torch.equal(y[last], alone[0]) and torch.equal(dx[last], alone[1])
+    del y, dx
+    sums = [torch.zeros(d, dtype=torch.float64, device=DEV) for _ in range(4)]
+    for i in range(0, rows, 10000):
+        _, _, (v, e), (u, f) = exact(x[i:i + 10000], w, b, dy[i:i + 10000])
+        for s, t in zip(sums, (v, e, u, f)):
+            s += t
+    near(dw, (sums[0], sums[1] * rows / 10000))      # (the bound of the sums is rows u times the terms')
+    near(db, (sums[2], sums[3] * rows / 10000))
