@@ -6,7 +6,7 @@
 // Both passes read the logits once; the probabilities are not stored, but each token's largest logit m and 1 / s, s = sum exp(logit - m), are:
 // both passes form p = exp(logit - m) / s by the same instructions.  (m + log s in one number is rounded at the size of the logits, and all p of a
 // token are off by a common factor, which u[e] - sum_j u[j] p[j] multiplies where the load is nearly even: 64 experts, u spread by 1 %,
-// logits of deviation 1 around 1000, dlogits off by 2e-3, and by 5e-6 so wherever they are.)  A token is held by
+// logits of deviation 1 around 1000, dlogits off by 2e-3, and by 8e-6 so wherever they are.)  A token is held by
 // L lanes, U cells of 16 bytes each, so that a wave sums the probabilities of 64 / L tokens at a time in registers, the next
 // tokens' logits on their way; the work-groups' sums (fp32) and counts are added in order by a second kernel.  Logits of -inf have probability 0, and a token that has no others counts with 0
 // everywhere.
@@ -88,7 +88,7 @@ __global__ __launch_bounds__(BAL_THREADS) void balance_kernel(BalanceArgs a, int
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             next[i][u].get(x[u]);
-            const int held = on ? a.experts - (u * L + l) * N : 0;   // (a select for each: a branch around them was compiled wrongly)
+            const int held = on ? a.experts - (u * L + l) * N : 0;   // (a select for each: with a branch around them clang 22.0.0 of ROCm 7.2.0 loses the -inf of element 0 in lanes whose first element is absent)
 #pragma unroll
             for (int e = 0; e < N; ++e) {
                 x[u][e] = e < held ? x[u][e] : -INFINITY;
