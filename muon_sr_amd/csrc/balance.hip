@@ -88,7 +88,9 @@ __global__ __launch_bounds__(BAL_THREADS) void balance_kernel(BalanceArgs a, int
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             next[i][u].get(x[u]);
-            const int held = on ? a.experts - (u * L + l) * N : 0;   // (a select for each: with a branch around them clang 22.0.0 of ROCm 7.2.0 loses the -inf of element 0 in lanes whose first element is absent)
+            // (a select for each element: with a branch around them clang 22.0.0 of ROCm 7.2.0 loses the -inf of element 0 in lanes whose first
+            // element is absent)
+            const int held = on ? a.experts - (u * L + l) * N : 0;
 #pragma unroll
             for (int e = 0; e < N; ++e) {
                 x[u][e] = e < held ? x[u][e] : -INFINITY;

@@ -544,7 +544,7 @@ __global__ __launch_bounds__(256) void dx_kernel(HeadArgs a, uint16_t *dx) {
         float f[8] = {};
         if (p >= 0) {
             const int word = word_of(a, p);
-            if (word != HEAD_BAD) {
+            if (word >= 0 && word < a.vocab) {         // (HEAD_BAD is not)
                 const float rest = a.rest[p];
                 float h[8];
                 unpack8(reinterpret_cast<const Bytes16 *>(a.w + (int64_t)word * d + c)->w, h);
